@@ -60,6 +60,12 @@ enum {
   RMSNORM_B200_F32 = 2
 };
 
+/* 8-bit output types of rmsnorm_b200_quant_fwd. */
+enum {
+  RMSNORM_B200_E4M3 = 3, /* 4 exponent and 3 mantissa bits, finite, largest value 448 */
+  RMSNORM_B200_I8 = 4    /* symmetric: -127 .. 127 */
+};
+
 /* status codes */
 enum {
   RMSNORM_B200_OK = 0,
@@ -237,6 +243,175 @@ typedef struct rmsnorm_b200_ln_fwd_args {
 } rmsnorm_b200_ln_fwd_args;
 
 int rmsnorm_b200_layernorm_fwd(const rmsnorm_b200_ln_fwd_args* args, void* stream);
+
+/* ---- Fused operators around the norm. No counterpart in the reference. ---- */
+
+/* Residual addition + RMSNorm with an 8-bit output and scales (the input of an 8-bit
+ * product). Per row: h = x (+ residual); y = h * rsqrt(mean(h^2) + eps) * weight (+ bias),
+ * all in fp32; then for the whole row (group = 0) or each group of `group` consecutive
+ * columns (the last one may be shorter)
+ *   scale = max(max |y| / Q, 2^-126), Q = 448 (E4M3) or 127 (I8)
+ *   q     = y / scale rounded to nearest, ties to even, never beyond +-Q.
+ * A NaN in a group makes its scale NaN; an infinity makes it infinite. residual_out
+ * receives h. */
+typedef struct rmsnorm_b200_quant_args {
+  int64_t rows;               /* >= 0 */
+  int64_t hidden;             /* >= 1 */
+  const void* x;              /* [rows, hidden] */
+  const void* residual;       /* nullable, [rows, hidden] */
+  const void* weight;         /* nullable (ones), [hidden] */
+  const void* bias;           /* nullable (zeros), [hidden] */
+  void* q;                    /* [rows, hidden], one byte each */
+  float* scales;              /* scale of (row r, group g) at r * scale_row_stride + g * scale_group_stride */
+  void* residual_out;         /* nullable, [rows, hidden] */
+  int64_t scale_row_stride;   /* in elements */
+  int64_t scale_group_stride;
+  int32_t x_dtype;
+  int32_t residual_dtype;
+  int32_t weight_dtype;
+  int32_t bias_dtype;
+  int32_t q_dtype;            /* RMSNORM_B200_E4M3 or RMSNORM_B200_I8 */
+  int32_t residual_out_dtype;
+  int32_t group;              /* 0 (one scale per row), 32, 64, 128 or 256 */
+  float eps;
+} rmsnorm_b200_quant_args;
+
+int rmsnorm_b200_quant_fwd(const rmsnorm_b200_quant_args* args, void* stream);
+
+/* A dropout mask that is never stored. The element in row i and column j is kept when word
+ * j % 4 of Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as
+ * 1, 2, 3, 2011) is at least floor(p * 2^32), where the key is `seed` and the counter is
+ * (j / 4, row_offset + i, o mod 2^32, o / 2^32) with o = offset + *step. */
+typedef struct rmsnorm_b200_dropout {
+  uint64_t seed;
+  uint64_t offset;
+  const int64_t* step;        /* nullable; device memory, read when the kernel runs */
+  int64_t row_offset;         /* row_offset + rows <= 2^32 */
+  double p;                   /* 0 <= p < 1 */
+} rmsnorm_b200_dropout;
+
+/* Dropout + residual addition + RMSNorm. Per row, in fp32:
+ *   h = (kept ? x / (1 - p) : 0) (+ residual); rstd = rsqrt(mean(h^2) + eps);
+ *   out = h * rstd * weight (+ bias); residual_out = h. */
+typedef struct rmsnorm_b200_dropout_fwd_args {
+  int64_t rows;
+  int64_t hidden;
+  const void* x;              /* [rows, hidden] */
+  const void* residual;       /* nullable, [rows, hidden] */
+  const void* weight;         /* nullable (ones), [hidden] */
+  const void* bias;           /* nullable (zeros), [hidden] */
+  void* out;                  /* [rows, hidden] */
+  void* residual_out;         /* nullable, [rows, hidden] */
+  float* rstd;                /* nullable, [rows] */
+  rmsnorm_b200_dropout drop;
+  int32_t x_dtype;
+  int32_t residual_dtype;
+  int32_t weight_dtype;
+  int32_t bias_dtype;
+  int32_t out_dtype;
+  int32_t residual_out_dtype;
+  float eps;
+  int32_t reserved0;
+} rmsnorm_b200_dropout_fwd_args;
+
+int rmsnorm_b200_dropout_rmsnorm_fwd(const rmsnorm_b200_dropout_fwd_args* args, void* stream);
+
+/* Its backward, from the saved h (residual_out) and rstd:
+ *   dh = (dout * weight - xhat * mean(xhat * dout * weight)) * rstd (+ dresidual_out),
+ *   xhat = h * rstd; dresidual = dh; dx = kept ? dh / (1 - p) : 0;
+ *   dweight = sum_rows(dout * xhat); dbias = sum_rows(dout), in a fixed order. */
+typedef struct rmsnorm_b200_dropout_bwd_args {
+  int64_t rows;
+  int64_t hidden;
+  const void* h;              /* [rows, hidden] */
+  const void* dout;           /* [rows, hidden] */
+  const float* rstd;          /* [rows] */
+  const void* weight;         /* nullable, [hidden] */
+  const void* dresidual_out;  /* nullable, [rows, hidden] */
+  void* dx;                   /* [rows, hidden] */
+  void* dresidual;            /* nullable, [rows, hidden] */
+  void* dweight;              /* nullable, [hidden] */
+  void* dbias;                /* nullable, [hidden] */
+  rmsnorm_b200_dropout drop;
+  int32_t h_dtype;
+  int32_t dout_dtype;
+  int32_t weight_dtype;
+  int32_t dresidual_out_dtype;
+  int32_t dx_dtype;
+  int32_t dresidual_dtype;
+  int32_t dweight_dtype;
+  int32_t dbias_dtype;
+} rmsnorm_b200_dropout_bwd_args;
+
+/* Bytes of device workspace the backward needs on the current device. */
+int rmsnorm_b200_dropout_rmsnorm_bwd_workspace_size(const rmsnorm_b200_dropout_bwd_args* args, size_t* bytes);
+
+/* `workspace`: as for rmsnorm_b200_bwd. */
+int rmsnorm_b200_dropout_rmsnorm_bwd(const rmsnorm_b200_dropout_bwd_args* args, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
+/* Per-head RMSNorm of q and k followed by rotary positions with one to four axes. For each
+ * token and head: y = x * rsqrt(mean(x^2) + eps) * weight (y = x when norm is 0), in fp32.
+ * Pair i < rotary_dim / 2 is the columns (i, i + rotary_dim / 2), or (2i, 2i + 1) when
+ * interleaved; with position t = positions[axis(i)][token], c = table[t][i] and
+ * s = table[t][rotary_dim / 2 + i] it becomes (y_a c - y_b s, y_b c + y_a s). Columns from
+ * rotary_dim on are not turned. A position outside the table makes the token's turned
+ * columns NaN and records RMSNORM_B200_ERR_INVALID_ARGUMENT (site 10) in the device status
+ * word. Only the last dimension of a tensor has to be contiguous. */
+#define RMSNORM_B200_ROPE_MAX_HEAD_DIM 256
+typedef struct rmsnorm_b200_rope_tensor {
+  void* data;                 /* [tokens, heads, head_dim] */
+  int64_t token_stride;       /* in elements */
+  int64_t head_stride;
+} rmsnorm_b200_rope_tensor;
+
+typedef struct rmsnorm_b200_rope_args {
+  int64_t tokens;             /* >= 0 */
+  int64_t table_rows;
+  const void* positions;      /* axis a, token t at a * position_axis_stride + t; int32 or int64 */
+  int64_t position_axis_stride;
+  const float* table;         /* [table_rows, rotary_dim]: cosines, then sines */
+  const void* q_weight;       /* nullable (ones), [q_weight_heads, head_dim] */
+  const void* k_weight;       /* nullable (ones), [k_weight_heads, head_dim] */
+  rmsnorm_b200_rope_tensor q; /* inputs; k_heads may be 0 */
+  rmsnorm_b200_rope_tensor k;
+  uint64_t axis_of_pair[4];   /* two bits per pair: pair i in word i / 32 at bit 2 * (i % 32) */
+  int32_t q_heads;
+  int32_t k_heads;
+  int32_t head_dim;           /* 1 .. RMSNORM_B200_ROPE_MAX_HEAD_DIM */
+  int32_t rotary_dim;         /* even, 0 .. head_dim */
+  int32_t axes;               /* 1 .. 4 */
+  int32_t interleaved;
+  int32_t norm;
+  int32_t positions_64bit;
+  int32_t dtype;              /* of q, k, their outputs and gradients */
+  int32_t weight_dtype;       /* of both weights */
+  int32_t q_weight_heads;     /* 1 or q_heads */
+  int32_t k_weight_heads;     /* 1 or k_heads */
+  float eps;
+  int32_t reserved0;
+} rmsnorm_b200_rope_args;
+
+/* q_out / k_out may be the inputs themselves. */
+int rmsnorm_b200_rope_fwd(const rmsnorm_b200_rope_args* args, const rmsnorm_b200_rope_tensor* q_out,
+                          const rmsnorm_b200_rope_tensor* k_out, void* stream);
+
+/* Backward: g = the inverse turn of dout; dx = (g * weight - xhat * mean(xhat * g * weight)) * rstd;
+ * dweight = the sum of g * xhat over tokens (and heads, for a weight shared by them), in a
+ * fixed order. dq_weight / dk_weight: nullable, of the weights' shapes and dtype. */
+typedef struct rmsnorm_b200_rope_grads {
+  rmsnorm_b200_rope_tensor dq_out;
+  rmsnorm_b200_rope_tensor dk_out;
+  rmsnorm_b200_rope_tensor dq;
+  rmsnorm_b200_rope_tensor dk;
+  void* dq_weight;
+  void* dk_weight;
+} rmsnorm_b200_rope_grads;
+
+int rmsnorm_b200_rope_bwd_workspace_size(const rmsnorm_b200_rope_args* args, const rmsnorm_b200_rope_grads* grads,
+                                         size_t* bytes);
+int rmsnorm_b200_rope_bwd(const rmsnorm_b200_rope_args* args, const rmsnorm_b200_rope_grads* grads, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 /* Static, human-readable message for a status code. */
 const char* rmsnorm_b200_strerror(int status);

@@ -1,0 +1,148 @@
+// fused_bwd.cu -- rmsnorm_b200_dropout_rmsnorm_bwd: argument checks, plan and launch.
+#define RMSB_UNIT fused_bwd
+#include "unit_state.cuh"
+
+#include "fused_generic.cuh"
+
+namespace rmsb200 {
+namespace {
+
+struct Plan {
+  int64_t nparts = 0;      // partial rows of dweight / dbias
+  int64_t chunk_rows = 1;  // generic path: rows per partial row
+};
+
+int check(const rmsnorm_b200_dropout_bwd_args* a) {
+  if (!a || a->rows < 0 || a->hidden < 1) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if (!valid_dt(a->h_dtype) || !valid_dt(a->dout_dtype) || !valid_dt(a->dx_dtype))
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if ((a->weight && !valid_dt(a->weight_dtype)) || (a->dresidual_out && !valid_dt(a->dresidual_out_dtype)) ||
+      (a->dresidual && !valid_dt(a->dresidual_dtype)) || (a->dweight && !valid_dt(a->dweight_dtype)) ||
+      (a->dbias && !valid_dt(a->dbias_dtype)))
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if (!valid_drop(a->drop, a->rows)) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if (a->rows > 0 && (!a->h || !a->dout || !a->rstd || !a->dx)) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  return RMSNORM_B200_OK;
+}
+
+void make_plan(const UnitDevice* ud, const rmsnorm_b200_dropout_bwd_args* a, Plan* pl) {
+  if (!a->dweight && !a->dbias) return;
+  const int64_t col_blocks = (a->hidden + kGenericThreads - 1) / kGenericThreads;
+  const int64_t target = std::clamp<int64_t>((4 * ud->sm_count + col_blocks - 1) / col_blocks, 1, 1024);
+  // at most 256 rows are added one after the other (longer runs lose digits of the sum), and
+  // at most 65535 chunks fit a grid
+  pl->chunk_rows = std::clamp<int64_t>((a->rows + target - 1) / target, 1, 256);
+  pl->chunk_rows = std::max<int64_t>(pl->chunk_rows, (a->rows + 65534) / 65535);
+  pl->nparts = (a->rows + pl->chunk_rows - 1) / pl->chunk_rows;
+}
+
+size_t workspace(const rmsnorm_b200_dropout_bwd_args* a, const Plan& pl) {
+  const size_t per = static_cast<size_t>(pl.nparts) * static_cast<size_t>(a->hidden) * sizeof(float);
+  return (a->dweight ? per : 0) + (a->dbias ? per : 0);
+}
+
+int launch_generic(const FusedBwdParams& p, const Plan& pl, UnitDevice* ud, cudaStream_t stream, const char* why) {
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(p.rows, int64_t{8} * ud->sm_count));
+  fused_bwd_generic_kernel<<<grid, kGenericThreads, 0, stream>>>(p);
+  int st = launched(std::string("fused_bwd_generic (") + why + ") grid=" + std::to_string(grid) +
+                    " chunks=" + std::to_string(pl.nparts));
+  if (st || (!p.dw_part && !p.db_part)) return st;
+  GenBwdParams g = {};
+  g.rows = p.rows; g.N = p.N; g.H = 1;
+  g.x = p.h; g.x_dt = p.h_dt; g.dy = p.dy; g.dy_dt = p.dy_dt; g.rstd = p.rstd;
+  const dim3 pg(static_cast<unsigned>((p.N + kGenericThreads - 1) / kGenericThreads),
+                static_cast<unsigned>(pl.nparts));
+  bwd_generic_partials_kernel<<<pg, kGenericThreads, 0, stream>>>(g, pl.chunk_rows, p.dw_part, p.db_part);
+  return launched("");
+}
+
+int run(const rmsnorm_b200_dropout_bwd_args* a, void* ws, size_t ws_bytes, cudaStream_t stream) {
+  int st = check(a);
+  if (st) return st;
+  UnitDevice* ud = nullptr;
+  st = unit_device(&ud);
+  if (st) return st;
+  Plan pl;
+  make_plan(ud, a, &pl);
+  const size_t need = workspace(a, pl);
+  if (need > ws_bytes || (need > 0 && (!ws || !aligned_to(ws, 16)))) return RMSNORM_B200_ERR_WORKSPACE;
+  Ranges ranges;
+  const size_t n = static_cast<size_t>(a->rows) * static_cast<size_t>(a->hidden);
+  ranges.add(a->h, n * elem_bytes(a->h_dtype));
+  ranges.add(a->dout, n * elem_bytes(a->dout_dtype));
+  ranges.add(a->rstd, static_cast<size_t>(a->rows) * 4);
+  if (a->weight) ranges.add(a->weight, a->hidden * elem_bytes(a->weight_dtype));
+  if (a->dresidual_out) ranges.add(a->dresidual_out, n * elem_bytes(a->dresidual_out_dtype));
+  ranges.add(a->dx, n * elem_bytes(a->dx_dtype));
+  if (a->dresidual) ranges.add(a->dresidual, n * elem_bytes(a->dresidual_dtype));
+  if (a->dweight) ranges.add(a->dweight, a->hidden * elem_bytes(a->dweight_dtype));
+  if (a->dbias) ranges.add(a->dbias, a->hidden * elem_bytes(a->dbias_dtype));
+  if (a->drop.step) ranges.add(a->drop.step, 8);
+  ranges.add(ws, need);
+  st = ranges.send(stream);
+  if (st) return st;
+
+  FusedBwdParams p = {};
+  p.h = a->h; p.dy = a->dout; p.rstd = a->rstd; p.w = a->weight; p.dro = a->dresidual_out;
+  p.dx = a->dx; p.dres = a->dresidual;
+  p.rows = a->rows; p.N = a->hidden;
+  p.h_dt = a->h_dtype; p.dy_dt = a->dout_dtype; p.w_dt = a->weight_dtype; p.dro_dt = a->dresidual_out_dtype;
+  p.dx_dt = a->dx_dtype; p.dres_dt = a->dresidual_dtype;
+  p.dw_part = a->dweight ? static_cast<float*>(ws) : nullptr;
+  p.db_part = a->dbias ? static_cast<float*>(ws) + (a->dweight ? pl.nparts * a->hidden : 0) : nullptr;
+  expand_drop(a->drop, &p.drop);
+  if (a->rows > 0) {
+    st = launch_generic(p, pl, ud, stream, "plain");
+    if (st) return st;
+  } else {
+    rmsb_units::set_last_plan("dropout bwd empty");
+  }
+  // dweight and dbias: fixed-order column sums of the partial rows, one launch for both
+  ReduceParams rp = {};
+  rp.C = a->rows > 0 ? pl.nparts : 0;
+  rp.W = a->hidden;
+  rp.N = a->hidden;
+  int njobs = 0;
+  int64_t blocks = 0;
+  auto add_job = [&](const float* part, void* out, int dt) {
+    ReduceJob& jb = rp.job[njobs++];
+    jb.part = part;
+    jb.out = out;
+    jb.wout = a->hidden;
+    jb.fold = 1;
+    jb.out_dt = dt;
+    const int64_t cols = reduce_vectorised(jb, rp.W) ? kReduceVCols : kReduceCols;
+    blocks = std::max(blocks, (jb.wout + cols - 1) / cols);
+  };
+  if (a->dweight) add_job(p.dw_part, a->dweight, a->dweight_dtype);
+  if (a->dbias) add_job(p.db_part, a->dbias, a->dbias_dtype);
+  if (njobs == 0) return RMSNORM_B200_OK;
+  reduce_partials_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(njobs)), kReduceThreads, 0,
+                           stream>>>(rp);
+  return launched("");
+}
+
+}  // namespace
+}  // namespace rmsb200
+
+using namespace rmsb200;
+
+extern "C" int rmsnorm_b200_dropout_rmsnorm_bwd_workspace_size(const rmsnorm_b200_dropout_bwd_args* a,
+                                                               size_t* bytes) {
+  if (!bytes) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  *bytes = 0;
+  int st = check(a);
+  if (st) return st;
+  UnitDevice* ud = nullptr;
+  st = unit_device(&ud);
+  if (st) return st;
+  Plan pl;
+  make_plan(ud, a, &pl);
+  *bytes = workspace(a, pl);
+  return RMSNORM_B200_OK;
+}
+
+extern "C" int rmsnorm_b200_dropout_rmsnorm_bwd(const rmsnorm_b200_dropout_bwd_args* a, void* workspace,
+                                                size_t workspace_bytes, void* stream) {
+  return run(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}

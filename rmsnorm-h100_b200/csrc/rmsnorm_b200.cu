@@ -24,6 +24,7 @@
 #include "generic_kernels.cuh"
 #include "peer_allreduce.cuh"
 #include "stream_kernels.cuh"
+#include "translation_units.h"
 
 // One rank's member of a peer group (opaque in the C ABI): the exchange buffers of the
 // fused dweight / dbias all-reduce (peer_allreduce.cuh).
@@ -1228,8 +1229,18 @@ int do_bwd(const rmsnorm_b200_bwd_args* a, void* ws, size_t ws_bytes, cudaStream
   return RMSNORM_B200_OK;
 }
 
+// The library's other translation units (each has device-side state of its own).
+const rmsb_units::UnitHooks* const kUnitHooks[] = {&rmsb_units::fused_fwd_unit, &rmsb_units::fused_bwd_unit,
+                                                   &rmsb_units::rope_unit};
+constexpr int kUnits = static_cast<int>(sizeof(kUnitHooks) / sizeof(kUnitHooks[0]));
+
 }  // namespace
 }  // namespace rmsb200
+
+namespace rmsb_units {
+void count_launches(uint64_t n) { rmsb200::g_launches.fetch_add(n, std::memory_order_relaxed); }
+void set_last_plan(std::string plan) { rmsb200::t_last_plan = std::move(plan); }
+}  // namespace rmsb_units
 
 // =========================================================================================
 // C ABI
@@ -1418,7 +1429,14 @@ extern "C" int rmsnorm_b200_device_status(void* stream, int32_t* status, int32_t
         cudaMemcpyToSymbolAsync(g_status_where, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s) != cudaSuccess)
       return RMSNORM_B200_ERR_CUDA;
   }
+  int unit_st[kUnits] = {}, unit_wh[kUnits] = {};
+  for (int i = 0; i < kUnits; ++i)
+    if (const int err = kUnitHooks[i]->status(s, &unit_st[i], &unit_wh[i], clear != 0)) return err;
   if (cudaStreamSynchronize(s) != cudaSuccess) return RMSNORM_B200_ERR_CUDA;
+  for (int i = 0; i < kUnits && st == 0; ++i) {
+    st = unit_st[i];
+    wh = unit_wh[i];
+  }
   if (status) *status = st;
   if (where) *where = wh;
   return RMSNORM_B200_OK;
@@ -1428,6 +1446,8 @@ extern "C" int rmsnorm_b200_set_wait_timeout_ns(uint64_t timeout_ns) {
   if (timeout_ns < kMinWaitTimeoutNs) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
   unsigned long long v = timeout_ns;
   if (cudaMemcpyToSymbol(g_wait_timeout_ns, &v, sizeof(v)) != cudaSuccess) return RMSNORM_B200_ERR_CUDA;
+  for (const auto* unit : kUnitHooks)
+    if (const int err = unit->set_wait_timeout(v)) return err;
   return RMSNORM_B200_OK;
 }
 
@@ -1465,6 +1485,13 @@ extern "C" int rmsnorm_b200_debug_report(void* stream, uint64_t* violations, int
   if (cudaStreamSynchronize(static_cast<cudaStream_t>(stream)) != cudaSuccess) return RMSNORM_B200_ERR_CUDA;
   unsigned long long rep[4] = {0, 0, 0, 0};
   if (cudaMemcpyFromSymbol(rep, g_dbg_report, sizeof(rep)) != cudaSuccess) return RMSNORM_B200_ERR_CUDA;
+  for (const auto* unit : kUnitHooks) {  // counts add up; the first failure found is described
+    unsigned long long more[4] = {0, 0, 0, 0};
+    if (const int err = unit->report(more, clear != 0)) return err;
+    if (rep[0] == 0)
+      for (int i = 1; i < 4; ++i) rep[i] = more[i];
+    rep[0] += more[0];
+  }
   if (violations) *violations = rep[0];
   if (site) *site = static_cast<int32_t>(rep[1]);
   if (address) *address = rep[2];

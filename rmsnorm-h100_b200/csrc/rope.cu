@@ -1,0 +1,219 @@
+// rope.cu -- rmsnorm_b200_rope_fwd and rmsnorm_b200_rope_bwd: argument checks, plan and launch.
+#define RMSB_UNIT rope
+#include "unit_state.cuh"
+
+#include "rope_kernels.cuh"
+
+namespace rmsb200 {
+namespace {
+
+bool valid_tensor(const rmsnorm_b200_rope_tensor& t, int64_t tokens, int heads) {
+  return heads == 0 || tokens == 0 || (t.data && t.token_stride >= 0 && t.head_stride >= 0);
+}
+
+int check(const rmsnorm_b200_rope_args* a) {
+  if (!a || a->tokens < 0 || a->q_heads < 1 || a->k_heads < 0) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if (a->head_dim < 1 || a->head_dim > kRopeMaxDim || a->rotary_dim < 0 || a->rotary_dim > a->head_dim ||
+      (a->rotary_dim & 1))
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if (a->axes < 1 || a->axes > 4 || !valid_dt(a->dtype)) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  for (int i = 0; i < a->rotary_dim / 2; ++i)
+    if (static_cast<int>(a->axis_of_pair[i >> 5] >> (2 * (i & 31)) & 3) >= a->axes)
+      return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if ((a->q_weight || a->k_weight) && !valid_dt(a->weight_dtype)) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if (a->q_weight && a->q_weight_heads != 1 && a->q_weight_heads != a->q_heads)
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if (a->k_weight && a->k_weight_heads != 1 && a->k_weight_heads != a->k_heads)
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if (!valid_tensor(a->q, a->tokens, a->q_heads) || !valid_tensor(a->k, a->tokens, a->k_heads))
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if (a->tokens > 0 && a->rotary_dim > 0 &&
+      (!a->positions || !a->table || a->table_rows < 0 || a->position_axis_stride < 0))
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  return RMSNORM_B200_OK;
+}
+
+void add_tensor(Ranges& r, const rmsnorm_b200_rope_tensor& t, const rmsnorm_b200_rope_args* a, int heads) {
+  if (heads == 0) return;
+  r.add(t.data, ((a->tokens - 1) * t.token_stride + (heads - 1) * t.head_stride + a->head_dim) *
+                    elem_bytes(a->dtype));
+}
+
+void add_ranges(Ranges& r, const rmsnorm_b200_rope_args* a) {
+  add_tensor(r, a->q, a, a->q_heads);
+  add_tensor(r, a->k, a, a->k_heads);
+  const size_t wb = static_cast<size_t>(a->head_dim) * elem_bytes(a->weight_dtype);
+  if (a->q_weight) r.add(a->q_weight, a->q_weight_heads * wb);
+  if (a->k_weight) r.add(a->k_weight, a->k_weight_heads * wb);
+  if (a->rotary_dim == 0) return;
+  r.add(a->positions, ((a->axes - 1) * a->position_axis_stride + a->tokens) * (a->positions_64bit ? 8 : 4));
+  r.add(a->table, static_cast<size_t>(a->table_rows) * a->rotary_dim * 4);
+}
+
+RopeTensor tensor(const rmsnorm_b200_rope_tensor& t) { return {t.data, t.token_stride, t.head_stride}; }
+
+RopeParams params(const rmsnorm_b200_rope_args* a) {
+  RopeParams p = {};
+  p.tokens = a->tokens; p.table_rows = a->table_rows;
+  p.pos = a->positions; p.pos_axis = a->position_axis_stride; p.table = a->table;
+  p.w[0] = a->q_weight; p.w[1] = a->k_weight;
+  p.x[0] = tensor(a->q); p.x[1] = tensor(a->k);
+  for (int i = 0; i < 4; ++i) p.axis_of[i] = a->axis_of_pair[i];
+  p.heads[0] = a->q_heads; p.heads[1] = a->k_heads;
+  p.w_per_head[0] = a->q_weight && a->q_weight_heads > 1;
+  p.w_per_head[1] = a->k_weight && a->k_weight_heads > 1;
+  p.D = a->head_dim; p.rd = a->rotary_dim; p.axes = a->axes; p.interleaved = a->interleaved != 0;
+  p.norm = a->norm != 0; p.pos64 = a->positions_64bit != 0; p.dt = a->dtype; p.w_dt = a->weight_dtype;
+  p.eps = a->eps;
+  return p;
+}
+
+int run_fwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_tensor* qo, const rmsnorm_b200_rope_tensor* ko,
+            cudaStream_t stream) {
+  int st = check(a);
+  if (st) return st;
+  if (!qo || !valid_tensor(*qo, a->tokens, a->q_heads) || (a->k_heads > 0 && (!ko || !valid_tensor(*ko, a->tokens, a->k_heads))))
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if (a->tokens == 0) {
+    rmsb_units::set_last_plan("rope fwd empty");
+    return RMSNORM_B200_OK;
+  }
+  UnitDevice* ud = nullptr;
+  st = unit_device(&ud);
+  if (st) return st;
+  Ranges ranges;
+  add_ranges(ranges, a);
+  add_tensor(ranges, *qo, a, a->q_heads);
+  if (ko) add_tensor(ranges, *ko, a, a->k_heads);
+  st = ranges.send(stream);
+  if (st) return st;
+  RopeParams p = params(a);
+  p.out[0] = tensor(*qo);
+  if (ko) p.out[1] = tensor(*ko);
+  const int64_t work = a->tokens * (a->q_heads + a->k_heads);
+  const int64_t warps = kGenericThreads / 32;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((work + warps - 1) / warps, int64_t{16} * ud->sm_count));
+  rope_fwd_generic_kernel<<<grid, kGenericThreads, 0, stream>>>(p);
+  return launched("rope_fwd_generic grid=" + std::to_string(grid));
+}
+
+struct BwdPlan {
+  int64_t chunk = 1, chunks = 1;
+};
+
+int check_bwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g) {
+  int st = check(a);
+  if (st) return st;
+  if (!g || !valid_tensor(g->dq_out, a->tokens, a->q_heads) || !valid_tensor(g->dk_out, a->tokens, a->k_heads) ||
+      !valid_tensor(g->dq, a->tokens, a->q_heads) || !valid_tensor(g->dk, a->tokens, a->k_heads))
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if ((g->dq_weight && !a->q_weight) || (g->dk_weight && !a->k_weight)) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  return RMSNORM_B200_OK;
+}
+
+BwdPlan plan_bwd(const UnitDevice* ud, const rmsnorm_b200_rope_args* a) {
+  BwdPlan pl;
+  const int64_t heads = a->q_heads + a->k_heads;
+  const int64_t target = std::max<int64_t>(1, (int64_t{16} * ud->sm_count + heads - 1) / heads);
+  // at most 256 tokens per warp are added one after the other, at most 65535 chunks fit a grid
+  pl.chunk = std::clamp<int64_t>((a->tokens + target - 1) / target, kGenericThreads / 32, 256 * (kGenericThreads / 32));
+  pl.chunk = std::max<int64_t>(pl.chunk, (a->tokens + 65534) / 65535);
+  pl.chunks = (a->tokens + pl.chunk - 1) / pl.chunk;
+  return pl;
+}
+
+size_t workspace(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g, const BwdPlan& pl) {
+  if (!g->dq_weight && !g->dk_weight) return 0;
+  return static_cast<size_t>(pl.chunks) * (a->q_heads + a->k_heads) * a->head_dim * sizeof(float);
+}
+
+int run_bwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g, void* ws, size_t ws_bytes,
+            cudaStream_t stream) {
+  int st = check_bwd(a, g);
+  if (st) return st;
+  UnitDevice* ud = nullptr;
+  st = unit_device(&ud);
+  if (st) return st;
+  const BwdPlan pl = plan_bwd(ud, a);
+  const size_t need = workspace(a, g, pl);
+  if (need > ws_bytes || (need > 0 && (!ws || !aligned_to(ws, 16)))) return RMSNORM_B200_ERR_WORKSPACE;
+  const int heads = a->q_heads + a->k_heads;
+  Ranges ranges;
+  if (a->tokens > 0) {
+    add_ranges(ranges, a);
+    add_tensor(ranges, g->dq_out, a, a->q_heads);
+    add_tensor(ranges, g->dk_out, a, a->k_heads);
+    add_tensor(ranges, g->dq, a, a->q_heads);
+    add_tensor(ranges, g->dk, a, a->k_heads);
+  }
+  ranges.add(ws, need);
+  const size_t wb = static_cast<size_t>(a->head_dim) * elem_bytes(a->weight_dtype);
+  if (g->dq_weight) ranges.add(g->dq_weight, a->q_weight_heads * wb);
+  if (g->dk_weight) ranges.add(g->dk_weight, a->k_weight_heads * wb);
+  st = ranges.send(stream);
+  if (st) return st;
+  RopeParams p = params(a);
+  p.dy[0] = tensor(g->dq_out); p.dy[1] = tensor(g->dk_out);
+  p.out[0] = tensor(g->dq); p.out[1] = tensor(g->dk);
+  p.part = need ? static_cast<float*>(ws) : nullptr;
+  if (a->tokens > 0) {
+    const dim3 grid(static_cast<unsigned>(heads), static_cast<unsigned>(pl.chunks));
+    rope_bwd_generic_kernel<<<grid, kGenericThreads, 0, stream>>>(p, pl.chunk);
+    st = launched("rope_bwd_generic chunks=" + std::to_string(pl.chunks));
+    if (st) return st;
+  } else {
+    rmsb_units::set_last_plan("rope bwd empty");
+  }
+  // the weights' gradients: fixed-order sums over the chunks (and over the heads that share
+  // a weight), one launch for both
+  ReduceParams rp = {};
+  rp.C = a->tokens > 0 ? pl.chunks : 0;
+  rp.W = static_cast<int64_t>(heads) * a->head_dim;
+  rp.N = a->head_dim;
+  int njobs = 0;
+  int64_t blocks = 0;
+  auto add_job = [&](int64_t first_head, void* out, int nheads, int w_heads) {
+    ReduceJob& jb = rp.job[njobs++];
+    jb.part = static_cast<const float*>(ws) + first_head * a->head_dim;
+    jb.out = out;
+    jb.fold = w_heads == 1 ? nheads : 1;
+    jb.wout = jb.fold > 1 ? a->head_dim : static_cast<int64_t>(nheads) * a->head_dim;
+    jb.out_dt = a->weight_dtype;
+    const int64_t cols = reduce_vectorised(jb, rp.W) ? kReduceVCols : kReduceCols;
+    blocks = std::max(blocks, (jb.wout + cols - 1) / cols);
+  };
+  if (g->dq_weight) add_job(0, g->dq_weight, a->q_heads, a->q_weight_heads);
+  if (g->dk_weight) add_job(a->q_heads, g->dk_weight, a->k_heads, a->k_weight_heads);
+  if (njobs == 0) return RMSNORM_B200_OK;
+  reduce_partials_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(njobs)), kReduceThreads, 0,
+                           stream>>>(rp);
+  return launched("");
+}
+
+}  // namespace
+}  // namespace rmsb200
+
+using namespace rmsb200;
+
+extern "C" int rmsnorm_b200_rope_fwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_tensor* q_out,
+                                     const rmsnorm_b200_rope_tensor* k_out, void* stream) {
+  return run_fwd(a, q_out, k_out, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int rmsnorm_b200_rope_bwd_workspace_size(const rmsnorm_b200_rope_args* a,
+                                                    const rmsnorm_b200_rope_grads* g, size_t* bytes) {
+  if (!bytes) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  *bytes = 0;
+  int st = check_bwd(a, g);
+  if (st) return st;
+  UnitDevice* ud = nullptr;
+  st = unit_device(&ud);
+  if (st) return st;
+  *bytes = workspace(a, g, plan_bwd(ud, a));
+  return RMSNORM_B200_OK;
+}
+
+extern "C" int rmsnorm_b200_rope_bwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  return run_bwd(a, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}

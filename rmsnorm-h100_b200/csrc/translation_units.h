@@ -1,0 +1,32 @@
+// translation_units.h -- what the library's translation units share on the host.
+//
+// The library is compiled from several translation units without relocatable device code,
+// so each has its own copy of the device-side state that device_common.cuh defines (status
+// word, wait limit, bounds-check report). The main unit (rmsnorm_b200.cu) owns the C entry
+// points that read and set that state; every other unit hands it a UnitHooks.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <string>
+
+namespace rmsb_units {
+
+struct UnitHooks {
+  // Enqueues the read (and clear) of the unit's status word; the caller synchronises.
+  int (*status)(cudaStream_t stream, int* status, int* where, bool clear);
+  int (*set_wait_timeout)(unsigned long long ns);
+  // The four words of the unit's bounds-check report (bounds-checked build only).
+  int (*report)(unsigned long long (&words)[4], bool clear);
+};
+
+extern const UnitHooks fused_fwd_unit;
+extern const UnitHooks fused_bwd_unit;
+extern const UnitHooks rope_unit;
+
+// Bookkeeping of the main unit: rmsnorm_b200_launch_count and rmsnorm_b200_last_plan.
+void count_launches(uint64_t n);
+void set_last_plan(std::string plan);
+
+}  // namespace rmsb_units

@@ -20,7 +20,9 @@ import torch
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "librmsnorm_b200.so"
 
 F16, BF16, F32 = 0, 1, 2
+E4M3, I8 = 3, 4
 _DTYPE_CODES = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
+_QUANT_CODES = {torch.float8_e4m3fn: E4M3, torch.int8: I8}
 
 OK = 0
 ERR_DEVICE_TIMEOUT = 5
@@ -101,7 +103,159 @@ class LnFwdArgs(ctypes.Structure):
     ]
 
 
+class QuantArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("hidden", ctypes.c_int64),
+        ("x", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("residual_out", ctypes.c_void_p),
+        ("scale_row_stride", ctypes.c_int64),
+        ("scale_group_stride", ctypes.c_int64),
+        ("x_dtype", ctypes.c_int32),
+        ("residual_dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("q_dtype", ctypes.c_int32),
+        ("residual_out_dtype", ctypes.c_int32),
+        ("group", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class Dropout(ctypes.Structure):
+    _fields_ = [
+        ("seed", ctypes.c_uint64),
+        ("offset", ctypes.c_uint64),
+        ("step", ctypes.c_void_p),
+        ("row_offset", ctypes.c_int64),
+        ("p", ctypes.c_double),
+    ]
+
+
+class DropoutFwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("hidden", ctypes.c_int64),
+        ("x", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("residual_out", ctypes.c_void_p),
+        ("rstd", ctypes.c_void_p),
+        ("drop", Dropout),
+        ("x_dtype", ctypes.c_int32),
+        ("residual_dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("residual_out_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
+class DropoutBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("hidden", ctypes.c_int64),
+        ("h", ctypes.c_void_p),
+        ("dout", ctypes.c_void_p),
+        ("rstd", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("dresidual_out", ctypes.c_void_p),
+        ("dx", ctypes.c_void_p),
+        ("dresidual", ctypes.c_void_p),
+        ("dweight", ctypes.c_void_p),
+        ("dbias", ctypes.c_void_p),
+        ("drop", Dropout),
+        ("h_dtype", ctypes.c_int32),
+        ("dout_dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("dresidual_out_dtype", ctypes.c_int32),
+        ("dx_dtype", ctypes.c_int32),
+        ("dresidual_dtype", ctypes.c_int32),
+        ("dweight_dtype", ctypes.c_int32),
+        ("dbias_dtype", ctypes.c_int32),
+    ]
+
+
+class RopeTensor(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class RopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("table_rows", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("position_axis_stride", ctypes.c_int64),
+        ("table", ctypes.c_void_p),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("q", RopeTensor),
+        ("k", RopeTensor),
+        ("axis_of_pair", ctypes.c_uint64 * 4),
+        ("q_heads", ctypes.c_int32),
+        ("k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("axes", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("positions_64bit", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("q_weight_heads", ctypes.c_int32),
+        ("k_weight_heads", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
+class RopeGrads(ctypes.Structure):
+    _fields_ = [
+        ("dq_out", RopeTensor),
+        ("dk_out", RopeTensor),
+        ("dq", RopeTensor),
+        ("dk", RopeTensor),
+        ("dq_weight", ctypes.c_void_p),
+        ("dk_weight", ctypes.c_void_p),
+    ]
+
+
 SIGNATURES = {
+    "rmsnorm_b200_quant_fwd": (ctypes.c_int, [ctypes.POINTER(QuantArgs), ctypes.c_void_p]),
+    "rmsnorm_b200_dropout_rmsnorm_fwd": (ctypes.c_int, [ctypes.POINTER(DropoutFwdArgs), ctypes.c_void_p]),
+    "rmsnorm_b200_dropout_rmsnorm_bwd_workspace_size": (
+        ctypes.c_int,
+        [ctypes.POINTER(DropoutBwdArgs), ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "rmsnorm_b200_dropout_rmsnorm_bwd": (
+        ctypes.c_int,
+        [ctypes.POINTER(DropoutBwdArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "rmsnorm_b200_rope_fwd": (
+        ctypes.c_int,
+        [ctypes.POINTER(RopeArgs), ctypes.POINTER(RopeTensor), ctypes.POINTER(RopeTensor), ctypes.c_void_p],
+    ),
+    "rmsnorm_b200_rope_bwd_workspace_size": (
+        ctypes.c_int,
+        [ctypes.POINTER(RopeArgs), ctypes.POINTER(RopeGrads), ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "rmsnorm_b200_rope_bwd": (
+        ctypes.c_int,
+        [ctypes.POINTER(RopeArgs), ctypes.POINTER(RopeGrads), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    ),
     "rmsnorm_b200_fwd": (ctypes.c_int, [ctypes.POINTER(FwdArgs), ctypes.c_void_p]),
     "rmsnorm_b200_layernorm_fwd": (ctypes.c_int, [ctypes.POINTER(LnFwdArgs), ctypes.c_void_p]),
     "rmsnorm_b200_bwd_workspace_size": (
@@ -206,6 +360,26 @@ def _check(status: int, what: str) -> None:
 
 def _stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def enqueue(name: str, device: torch.device, *args) -> None:
+    """Calls the entry point `name` with `args` and the current stream of `device`."""
+    fn = getattr(load_library(), name)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    _check(status, name)
+
+
+def workspace_bytes(name: str, device: torch.device, *args) -> int:
+    """Answer of the workspace-size entry point `name`."""
+    n = ctypes.c_size_t(0)
+    with torch.cuda.device(device):
+        _check(getattr(load_library(), name)(*args, ctypes.byref(n)), name)
+    return n.value
 
 
 def fwd(
