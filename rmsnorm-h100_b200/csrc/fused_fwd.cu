@@ -3,10 +3,38 @@
 #define RMSB_UNIT fused_fwd
 #include "unit_state.cuh"
 
-#include "fused_generic.cuh"
+#include "fused_fwd_kernels.cuh"
+#include "row_plan.h"
 
 namespace rmsb200 {
 namespace {
+
+using FwdKernel = void (*)(const FusedFwdParams, const RowPlan);
+constexpr int kNone = -1;
+
+template <typename X, typename RT>
+FwdKernel pick_steps(int k, bool drop) {
+  switch (k) {
+    case 1: return drop ? fused_fwd_kernel<X, RT, 1, true> : fused_fwd_kernel<X, RT, 1, false>;
+    case 2: return drop ? fused_fwd_kernel<X, RT, 2, true> : fused_fwd_kernel<X, RT, 2, false>;
+    default: return drop ? fused_fwd_kernel<X, RT, 4, true> : fused_fwd_kernel<X, RT, 4, false>;
+  }
+}
+
+FwdKernel pick(int x, int res, int k, bool drop) {
+  constexpr int H = RMSNORM_B200_F16, B = RMSNORM_B200_BF16, F = RMSNORM_B200_F32;
+  using h16 = __half;
+  using b16 = __nv_bfloat16;
+  if (x == B && res == kNone) return pick_steps<b16, NoT>(k, drop);
+  if (x == H && res == kNone) return pick_steps<h16, NoT>(k, drop);
+  if (x == F && res == kNone) return pick_steps<float, NoT>(k, drop);
+  if (x == B && res == B) return pick_steps<b16, b16>(k, drop);
+  if (x == H && res == H) return pick_steps<h16, h16>(k, drop);
+  if (x == F && res == F) return pick_steps<float, float>(k, drop);
+  if (x == B && res == F) return pick_steps<b16, float>(k, drop);
+  if (x == H && res == F) return pick_steps<h16, float>(k, drop);
+  return nullptr;
+}
 
 int launch_generic(const FusedFwdParams& p, bool drop, UnitDevice* ud, cudaStream_t stream, const char* why) {
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(p.rows, int64_t{8} * ud->sm_count));
@@ -37,7 +65,27 @@ int run(const FusedFwdParams& p, bool drop, cudaStream_t stream) {
   if (p.drop.step) ranges.add(p.drop.step, 8);
   st = ranges.send(stream);
   if (st) return st;
-  return launch_generic(p, drop, ud, stream, "plain");
+  const void* ptrs[] = {p.x, p.res, p.out, p.ro};
+  const char* why = p.N % 8 ? "hidden % 8" : nullptr;
+  for (const void* ptr : ptrs)
+    if (!aligned_to(ptr, ptr == p.out && p.scales ? 8 : 16)) why = "unaligned pointer";
+  if (!why) {
+    const int bytes[3] = {elem_bytes(p.x_dt), p.res ? elem_bytes(p.res_dt) : 0, 0};
+    RowPlan pl;
+    int k = 0, smem = 0;
+    why = plan_rows(p.rows, p.N, bytes, p.b != nullptr, kRowMaxVecs, ud->sm_count, &pl, &k, &smem);
+    if (!why) {
+      FwdKernel kernel = pick(p.x_dt, p.res ? p.res_dt : kNone, k, drop);
+      if (kernel) {
+        st = launch_rows(ud, kernel, p, pl, smem, stream, drop ? "dropout_fwd" : "quant_fwd", k);
+        if (st != RMSNORM_B200_ERR_UNSUPPORTED) return st;
+        why = "cluster not schedulable";
+      } else {
+        why = "dtype combination";
+      }
+    }
+  }
+  return launch_generic(p, drop, ud, stream, why);
 }
 
 }  // namespace

@@ -1,0 +1,117 @@
+// row_plan.h -- launch plan of the fused row kernels (row_ring.cuh has the vocabulary).
+#pragma once
+
+#include "row_ring.cuh"
+
+namespace rmsb200 {
+namespace {
+
+inline int pow2_ceil(int64_t v) {
+  int p = 1;
+  while (p < v) p <<= 1;
+  return p;
+}
+
+// Plans rows of N columns (a multiple of 8) whose tensors have elements of bytes[i] (0: absent).
+// max_steps: vector steps a thread can hold. Returns why there is no plan, or null.
+inline const char* plan_rows(int64_t rows, int64_t N, const int (&bytes)[3], bool bias, int max_steps, int sms,
+                             RowPlan* pl, int* k, int* smem) {
+  const int64_t cta_cols = static_cast<int64_t>(kRowThreads) * 8 * max_steps;
+  if (N > cta_cols * kMaxRowCtas) return "rows wider than a cluster holds";
+  pl->C = N > cta_cols ? pow2_ceil((N + cta_cols - 1) / cta_cols) : 1;
+  pl->slice = static_cast<int>(N);
+  if (pl->C > 1) {
+    const int64_t per = (N + pl->C - 1) / pl->C;
+    pl->slice = static_cast<int>((per + kScaleAlign - 1) / kScaleAlign * kScaleAlign);
+  }
+  const int vecs = (pl->slice + 7) / 8;
+  // Few rows: as many threads to a row as it has vectors, for the latency. Otherwise as few as
+  // hold it, so that a CTA works on several rows at once and their totals overlap.
+  const int steps = rows <= sms ? 1 : max_steps;
+  pl->G = std::clamp(pow2_ceil((vecs + steps - 1) / steps), 32, kRowThreads);
+  *k = pow2_ceil((vecs + pl->G - 1) / pl->G);
+  pl->groups = pl->C > 1 ? 1 : kRowThreads / pl->G;
+  const int elem = bytes[0] + bytes[1] + bytes[2];
+  pl->KC = *k;
+  while (pl->KC > 1 && pl->KC * pl->G * 8 * elem > 32768) pl->KC >>= 1;
+  pl->unit_shift = 0;
+  while ((pl->KC << pl->unit_shift) < *k) ++pl->unit_shift;
+  // Short rows go several to a unit: a copy of about 4 KB at least, but no fewer tiles than groups.
+  pl->R = 1;
+  if (pl->C == 1 && pl->KC == *k) {
+    const int64_t fair = rows / (static_cast<int64_t>(sms) * pl->groups);
+    pl->R = static_cast<int>(std::clamp<int64_t>(std::min<int64_t>(4096 / (N * elem), fair), 1, 8));
+  }
+  const int unit_cols = pl->R > 1 ? pl->R * pl->slice : std::min(pl->slice, pl->KC * pl->G * 8);
+  uint32_t off = 0;
+  for (int i = 0; i < 3; ++i) {
+    pl->off[i] = off;
+    off += static_cast<uint32_t>(unit_cols) * bytes[i];
+  }
+  pl->unit_bytes = (off + 127u) & ~127u;
+  pl->bias = bias;
+  pl->tiles = (rows + pl->R - 1) / pl->R;
+  const int affine = pl->slice * 4 * (bias ? 2 : 1);
+  const int fixed = affine + static_cast<int>(sizeof(RowBars)) + 16;
+  const int unit = pl->groups * static_cast<int>(pl->unit_bytes);
+  const int64_t per_group = (pl->tiles * pl->C + static_cast<int64_t>(sms) * pl->groups - 1) /
+                            (static_cast<int64_t>(sms) * pl->groups);
+  pl->S = std::min({16, kMaxUnits / pl->groups, (kSmemOptIn - fixed) / unit});
+  pl->S = static_cast<int>(std::min<int64_t>(pl->S, std::max<int64_t>(1, per_group << pl->unit_shift)));
+  if (pl->S < 1) return "rows too wide for shared memory";
+  *smem = pl->S * unit + fixed;
+  return nullptr;
+}
+
+// Launches a persistent grid: one CTA per SM (as many clusters as fit), at most one row group per
+// tile. Returns UNSUPPORTED when no cluster of this shape fits.
+template <typename Kernel, typename Params>
+int launch_rows(UnitDevice* ud, Kernel kernel, const Params& p, const RowPlan& pl, int smem, cudaStream_t stream,
+                const char* kind, int k, int* grid_out = nullptr, bool dry_run = false) {
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  int clusters = ud->sm_count;
+  {
+    std::lock_guard<std::mutex> lock(ud->mu);
+    if (!ud->attrs_done.count(fn)) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemOptIn) != cudaSuccess ||
+          cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return RMSNORM_B200_ERR_CUDA;
+      ud->attrs_done.insert(fn);
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.blockDim = dim3(pl.G * pl.groups);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (pl.C > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = pl.C;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(pl.C * ud->sm_count);
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) clusters = 0;
+    cudaGetLastError();
+    if (clusters < 1) return RMSNORM_B200_ERR_UNSUPPORTED;
+  } else {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+  }
+  const int64_t grid = std::min<int64_t>(pl.tiles, clusters) * pl.C;
+  if (grid_out) *grid_out = static_cast<int>(grid);
+  if (dry_run) return RMSNORM_B200_OK;
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  if (cudaLaunchKernelEx(&cfg, kernel, p, pl) != cudaSuccess) {
+    cudaGetLastError();
+    return RMSNORM_B200_ERR_CUDA;
+  }
+  char buf[160];
+  std::snprintf(buf, sizeof(buf), "%s grid=%d G=%d groups=%d K=%d KC=%d R=%d S=%d C=%d slice=%d unit=%u smem=%d", kind,
+                static_cast<int>(grid), pl.G, pl.groups, k, pl.KC, pl.R, pl.S, pl.C, pl.slice, pl.unit_bytes, smem);
+  return launched(buf);
+}
+
+}  // namespace
+}  // namespace rmsb200
