@@ -2,15 +2,43 @@
 #define RMSB_UNIT fused_bwd
 #include "unit_state.cuh"
 
-#include "fused_generic.cuh"
+#include "fused_bwd_kernels.cuh"
+#include "row_plan.h"
 
 namespace rmsb200 {
 namespace {
 
+using BwdKernel = void (*)(const FusedBwdParams, const RowPlan);
+constexpr int kNone = -1;
+
 struct Plan {
   int64_t nparts = 0;      // partial rows of dweight / dbias
   int64_t chunk_rows = 1;  // generic path: rows per partial row
+  BwdKernel kernel = nullptr;
+  RowPlan rows;
+  int k = 0, smem = 0;
+  const char* why = nullptr;  // why the generic path is taken
 };
+
+template <typename H, typename DY, typename DRO>
+BwdKernel pick_steps(int k) {
+  return k == 1 ? fused_bwd_kernel<H, DY, DRO, 1> : fused_bwd_kernel<H, DY, DRO, 2>;
+}
+
+// (h, dout, dresidual_out): the saved input in dout's type or in fp32, its gradient in its own.
+BwdKernel pick(int h, int dy, int dro, int k) {
+  constexpr int H = RMSNORM_B200_F16, B = RMSNORM_B200_BF16, F = RMSNORM_B200_F32;
+  using h16 = __half;
+  using b16 = __nv_bfloat16;
+  if (dro != kNone && dro != h) return nullptr;
+  const bool none = dro == kNone;
+  if (h == B && dy == B) return none ? pick_steps<b16, b16, NoT>(k) : pick_steps<b16, b16, b16>(k);
+  if (h == H && dy == H) return none ? pick_steps<h16, h16, NoT>(k) : pick_steps<h16, h16, h16>(k);
+  if (h == F && dy == F) return none ? pick_steps<float, float, NoT>(k) : pick_steps<float, float, float>(k);
+  if (h == F && dy == B) return none ? pick_steps<float, b16, NoT>(k) : pick_steps<float, b16, float>(k);
+  if (h == F && dy == H) return none ? pick_steps<float, h16, NoT>(k) : pick_steps<float, h16, float>(k);
+  return nullptr;
+}
 
 int check(const rmsnorm_b200_dropout_bwd_args* a) {
   if (!a || a->rows < 0 || a->hidden < 1) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
@@ -25,8 +53,34 @@ int check(const rmsnorm_b200_dropout_bwd_args* a) {
   return RMSNORM_B200_OK;
 }
 
-void make_plan(const UnitDevice* ud, const rmsnorm_b200_dropout_bwd_args* a, Plan* pl) {
-  if (!a->dweight && !a->dbias) return;
+int make_plan(UnitDevice* ud, const rmsnorm_b200_dropout_bwd_args* a, Plan* pl) {
+  const void* ptrs[] = {a->h, a->dout, a->dresidual_out, a->dx, a->dresidual};
+  pl->why = a->hidden % 8 ? "hidden % 8" : nullptr;
+  for (const void* ptr : ptrs)
+    if (!aligned_to(ptr, 16)) pl->why = "unaligned pointer";
+  if (!pl->why) {
+    const int bytes[3] = {elem_bytes(a->h_dtype), elem_bytes(a->dout_dtype),
+                          a->dresidual_out ? elem_bytes(a->dresidual_out_dtype) : 0};
+    pl->why = plan_rows(a->rows, a->hidden, bytes, false, kBwdSteps, ud->sm_count, &pl->rows, &pl->k, &pl->smem);
+  }
+  if (!pl->why) {
+    pl->kernel = pick(a->h_dtype, a->dout_dtype, a->dresidual_out ? a->dresidual_out_dtype : kNone, pl->k);
+    if (!pl->kernel) pl->why = "dtype combination";
+  }
+  if (pl->kernel) {
+    // the groups' sums pass through the rings
+    pl->smem = std::max(pl->smem, pl->rows.groups * pl->rows.slice * 4);
+    int grid = 0;
+    const int st = launch_rows(ud, pl->kernel, FusedBwdParams{}, pl->rows, pl->smem, nullptr, "", pl->k, &grid, true);
+    if (st == RMSNORM_B200_OK) {
+      pl->nparts = a->dweight || a->dbias ? grid / pl->rows.C : 0;
+      return st;
+    }
+    if (st != RMSNORM_B200_ERR_UNSUPPORTED) return st;
+    pl->kernel = nullptr;
+    pl->why = "cluster not schedulable";
+  }
+  if (!a->dweight && !a->dbias) return RMSNORM_B200_OK;
   const int64_t col_blocks = (a->hidden + kGenericThreads - 1) / kGenericThreads;
   const int64_t target = std::clamp<int64_t>((4 * ud->sm_count + col_blocks - 1) / col_blocks, 1, 1024);
   // at most 256 rows are added one after the other (longer runs lose digits of the sum), and
@@ -34,6 +88,7 @@ void make_plan(const UnitDevice* ud, const rmsnorm_b200_dropout_bwd_args* a, Pla
   pl->chunk_rows = std::clamp<int64_t>((a->rows + target - 1) / target, 1, 256);
   pl->chunk_rows = std::max<int64_t>(pl->chunk_rows, (a->rows + 65534) / 65535);
   pl->nparts = (a->rows + pl->chunk_rows - 1) / pl->chunk_rows;
+  return RMSNORM_B200_OK;
 }
 
 size_t workspace(const rmsnorm_b200_dropout_bwd_args* a, const Plan& pl) {
@@ -63,7 +118,8 @@ int run(const rmsnorm_b200_dropout_bwd_args* a, void* ws, size_t ws_bytes, cudaS
   st = unit_device(&ud);
   if (st) return st;
   Plan pl;
-  make_plan(ud, a, &pl);
+  st = make_plan(ud, a, &pl);
+  if (st) return st;
   const size_t need = workspace(a, pl);
   if (need > ws_bytes || (need > 0 && (!ws || !aligned_to(ws, 16)))) return RMSNORM_B200_ERR_WORKSPACE;
   Ranges ranges;
@@ -92,7 +148,8 @@ int run(const rmsnorm_b200_dropout_bwd_args* a, void* ws, size_t ws_bytes, cudaS
   p.db_part = a->dbias ? static_cast<float*>(ws) + (a->dweight ? pl.nparts * a->hidden : 0) : nullptr;
   expand_drop(a->drop, &p.drop);
   if (a->rows > 0) {
-    st = launch_generic(p, pl, ud, stream, "plain");
+    st = pl.kernel ? launch_rows(ud, pl.kernel, p, pl.rows, pl.smem, stream, "dropout_bwd", pl.k)
+                   : launch_generic(p, pl, ud, stream, pl.why);
     if (st) return st;
   } else {
     rmsb_units::set_last_plan("dropout bwd empty");
@@ -137,7 +194,8 @@ extern "C" int rmsnorm_b200_dropout_rmsnorm_bwd_workspace_size(const rmsnorm_b20
   st = unit_device(&ud);
   if (st) return st;
   Plan pl;
-  make_plan(ud, a, &pl);
+  st = make_plan(ud, a, &pl);
+  if (st) return st;
   *bytes = workspace(a, pl);
   return RMSNORM_B200_OK;
 }
