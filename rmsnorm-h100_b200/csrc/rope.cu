@@ -68,6 +68,64 @@ RopeParams params(const rmsnorm_b200_rope_args* a) {
   return p;
 }
 
+// Whether the vectorised kernels take these tensors; nothing but whole chunks of 4 elements.
+bool vectorised(const rmsnorm_b200_rope_args* a, std::initializer_list<const rmsnorm_b200_rope_tensor*> tensors) {
+  if (a->head_dim % 8 || a->rotary_dim % 8 || !aligned_to(a->table, 16)) return false;
+  const uintptr_t chunk = 4 * elem_bytes(a->dtype);
+  for (const auto* t : tensors)
+    if (t && (!aligned_to(t->data, chunk) || t->token_stride % 4 || t->head_stride % 4)) return false;
+  return true;
+}
+
+// U: heads a lane works on at a time.
+RopePlan plan(const rmsnorm_b200_rope_args* a, int u) {
+  RopePlan pl = {};
+  while ((8 << pl.lanes_shift) < a->head_dim) ++pl.lanes_shift;
+  const int heads = u * (32 >> pl.lanes_shift);  // of a job
+  pl.jobs[0] = (a->q_heads + heads - 1) / heads;
+  pl.jobs[1] = (a->k_heads + heads - 1) / heads;
+  pl.turned_lanes = a->rotary_dim / 8;
+  return pl;
+}
+
+// Launches with programmatic dependent launch: the kernels wait for the one before them
+// before their first global access.
+template <typename Kernel>
+int launch(Kernel kernel, dim3 grid, int threads, cudaStream_t stream, const RopeParams& p, const RopePlan& pl,
+           const char* kind) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, p, pl) != cudaSuccess) {
+    cudaGetLastError();
+    return RMSNORM_B200_ERR_CUDA;
+  }
+  char buf[128];
+  std::snprintf(buf, sizeof(buf), "%s grid=%ux%u threads=%d lanes=%d jobs=%d+%d", kind, grid.x, grid.y, threads,
+                1 << pl.lanes_shift, pl.jobs[0], pl.jobs[1]);
+  return launched(buf);
+}
+
+using RopeKernel = void (*)(const RopeParams, const RopePlan);
+
+template <int U>
+RopeKernel pick_fwd(int dt) {
+  return dt == RMSNORM_B200_BF16 ? rope_fwd_kernel<__nv_bfloat16, U>
+         : dt == RMSNORM_B200_F16 ? rope_fwd_kernel<__half, U> : rope_fwd_kernel<float, U>;
+}
+
+template <bool kPerHead>
+RopeKernel pick_bwd(int dt) {
+  return dt == RMSNORM_B200_BF16 ? rope_bwd_kernel<__nv_bfloat16, 4, kPerHead>
+         : dt == RMSNORM_B200_F16 ? rope_bwd_kernel<__half, 4, kPerHead> : rope_bwd_kernel<float, 2, kPerHead>;
+}
+
 int run_fwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_tensor* qo, const rmsnorm_b200_rope_tensor* ko,
             cudaStream_t stream) {
   int st = check(a);
@@ -90,6 +148,16 @@ int run_fwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_tensor* qo,
   RopeParams p = params(a);
   p.out[0] = tensor(*qo);
   if (ko) p.out[1] = tensor(*ko);
+  if (vectorised(a, {&a->q, &a->k, qo, ko})) {
+    // Four heads a lane where that leaves every SM eight warps to run; single heads below.
+    constexpr int kWarps = kRopeThreads / 32;
+    RopePlan pl = plan(a, 4);
+    const bool wide = a->tokens * (pl.jobs[0] + pl.jobs[1]) >= int64_t{kWarps} * ud->sm_count;
+    if (!wide) pl = plan(a, 1);
+    const int64_t ctas = (a->tokens * (pl.jobs[0] + pl.jobs[1]) + kWarps - 1) / kWarps;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(ctas, int64_t{8} * ud->sm_count)));
+    return launch(wide ? pick_fwd<4>(a->dtype) : pick_fwd<1>(a->dtype), grid, kRopeThreads, stream, p, pl, "rope_fwd");
+  }
   const int64_t work = a->tokens * (a->q_heads + a->k_heads);
   const int64_t warps = kGenericThreads / 32;
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>((work + warps - 1) / warps, int64_t{16} * ud->sm_count));
@@ -98,7 +166,13 @@ int run_fwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_tensor* qo,
 }
 
 struct BwdPlan {
-  int64_t chunk = 1, chunks = 1;
+  int64_t chunk = 1, chunks = 1;  // scalar kernel
+  bool vec = false;
+  bool per_head = false;          // partial rows of every head
+  int threads = 0;
+  dim3 grid;
+  RopePlan rope;
+  int64_t rows = 0, width = 0;    // partial rows of dweight
 };
 
 int check_bwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g) {
@@ -111,20 +185,39 @@ int check_bwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g)
   return RMSNORM_B200_OK;
 }
 
-BwdPlan plan_bwd(const UnitDevice* ud, const rmsnorm_b200_rope_args* a) {
+BwdPlan plan_bwd(const UnitDevice* ud, const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g) {
   BwdPlan pl;
   const int64_t heads = a->q_heads + a->k_heads;
+  pl.per_head = (a->q_weight && a->q_weight_heads > 1) || (a->k_weight && a->k_weight_heads > 1);
+  pl.vec = vectorised(a, {&a->q, &a->k, &g->dq_out, &g->dk_out, &g->dq, &g->dk});
+  if (pl.vec) {
+    pl.rope = plan(a, a->dtype == RMSNORM_B200_F32 ? 2 : 4);
+    const int jobs = pl.rope.jobs[0] + pl.rope.jobs[1];
+    pl.rope.cta_jobs = std::min(jobs, kRopeBwdWarps);
+    const int at_once = kRopeBwdWarps / pl.rope.cta_jobs;
+    pl.threads = at_once * pl.rope.cta_jobs * 32;
+    const int64_t across = (jobs + pl.rope.cta_jobs - 1) / pl.rope.cta_jobs;
+    const int64_t most = std::max<int64_t>(1, int64_t{2} * ud->sm_count / across);
+    const int64_t along = std::clamp<int64_t>((a->tokens + at_once - 1) / at_once, 1, most);
+    pl.grid = dim3(static_cast<unsigned>(along), static_cast<unsigned>(across));
+    pl.rows = pl.per_head ? along : along * across;
+    pl.width = (pl.per_head ? heads : 2) * a->head_dim;
+    return pl;
+  }
+  pl.per_head = true;
   const int64_t target = std::max<int64_t>(1, (int64_t{16} * ud->sm_count + heads - 1) / heads);
   // at most 256 tokens per warp are added one after the other, at most 65535 chunks fit a grid
   pl.chunk = std::clamp<int64_t>((a->tokens + target - 1) / target, kGenericThreads / 32, 256 * (kGenericThreads / 32));
   pl.chunk = std::max<int64_t>(pl.chunk, (a->tokens + 65534) / 65535);
   pl.chunks = (a->tokens + pl.chunk - 1) / pl.chunk;
+  pl.rows = pl.chunks;
+  pl.width = heads * a->head_dim;
   return pl;
 }
 
-size_t workspace(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g, const BwdPlan& pl) {
+size_t workspace(const rmsnorm_b200_rope_grads* g, const BwdPlan& pl) {
   if (!g->dq_weight && !g->dk_weight) return 0;
-  return static_cast<size_t>(pl.chunks) * (a->q_heads + a->k_heads) * a->head_dim * sizeof(float);
+  return static_cast<size_t>(pl.rows) * pl.width * sizeof(float);
 }
 
 int run_bwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g, void* ws, size_t ws_bytes,
@@ -134,8 +227,8 @@ int run_bwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g, v
   UnitDevice* ud = nullptr;
   st = unit_device(&ud);
   if (st) return st;
-  const BwdPlan pl = plan_bwd(ud, a);
-  const size_t need = workspace(a, g, pl);
+  const BwdPlan pl = plan_bwd(ud, a, g);
+  const size_t need = workspace(g, pl);
   if (need > ws_bytes || (need > 0 && (!ws || !aligned_to(ws, 16)))) return RMSNORM_B200_ERR_WORKSPACE;
   const int heads = a->q_heads + a->k_heads;
   Ranges ranges;
@@ -157,9 +250,14 @@ int run_bwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g, v
   p.out[0] = tensor(g->dq); p.out[1] = tensor(g->dk);
   p.part = need ? static_cast<float*>(ws) : nullptr;
   if (a->tokens > 0) {
-    const dim3 grid(static_cast<unsigned>(heads), static_cast<unsigned>(pl.chunks));
-    rope_bwd_generic_kernel<<<grid, kGenericThreads, 0, stream>>>(p, pl.chunk);
-    st = launched("rope_bwd_generic chunks=" + std::to_string(pl.chunks));
+    if (pl.vec) {
+      st = launch(pl.per_head ? pick_bwd<true>(a->dtype) : pick_bwd<false>(a->dtype), pl.grid, pl.threads, stream, p,
+                  pl.rope, "rope_bwd");
+    } else {
+      const dim3 grid(static_cast<unsigned>(heads), static_cast<unsigned>(pl.chunks));
+      rope_bwd_generic_kernel<<<grid, kGenericThreads, 0, stream>>>(p, pl.chunk);
+      st = launched("rope_bwd_generic chunks=" + std::to_string(pl.chunks));
+    }
     if (st) return st;
   } else {
     rmsb_units::set_last_plan("rope bwd empty");
@@ -167,17 +265,17 @@ int run_bwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g, v
   // the weights' gradients: fixed-order sums over the chunks (and over the heads that share
   // a weight), one launch for both
   ReduceParams rp = {};
-  rp.C = a->tokens > 0 ? pl.chunks : 0;
-  rp.W = static_cast<int64_t>(heads) * a->head_dim;
+  rp.C = a->tokens > 0 ? pl.rows : 0;
+  rp.W = pl.width;
   rp.N = a->head_dim;
   int njobs = 0;
   int64_t blocks = 0;
   auto add_job = [&](int64_t first_head, void* out, int nheads, int w_heads) {
     ReduceJob& jb = rp.job[njobs++];
-    jb.part = static_cast<const float*>(ws) + first_head * a->head_dim;
+    jb.part = static_cast<const float*>(ws) + (pl.per_head ? first_head : first_head > 0) * a->head_dim;
     jb.out = out;
-    jb.fold = w_heads == 1 ? nheads : 1;
-    jb.wout = jb.fold > 1 ? a->head_dim : static_cast<int64_t>(nheads) * a->head_dim;
+    jb.fold = pl.per_head && w_heads == 1 ? nheads : 1;
+    jb.wout = static_cast<int64_t>(w_heads) * a->head_dim;
     jb.out_dt = a->weight_dtype;
     const int64_t cols = reduce_vectorised(jb, rp.W) ? kReduceVCols : kReduceCols;
     blocks = std::max(blocks, (jb.wout + cols - 1) / cols);
@@ -209,7 +307,7 @@ extern "C" int rmsnorm_b200_rope_bwd_workspace_size(const rmsnorm_b200_rope_args
   UnitDevice* ud = nullptr;
   st = unit_device(&ud);
   if (st) return st;
-  *bytes = workspace(a, g, plan_bwd(ud, a));
+  *bytes = workspace(g, plan_bwd(ud, a, g));
   return RMSNORM_B200_OK;
 }
 
