@@ -45,7 +45,27 @@ namespace rmsb200 {
 namespace {
 
 std::atomic<uint64_t> g_launches{0};
-thread_local std::string t_last_plan;
+// The plan of the last call on this thread: a text, or (the fused operators, whose smallest
+// calls take a few microseconds) what a text is made of when somebody asks for it.
+struct LastPlan {
+  std::string text;
+  rmsb_units::PlanText make = nullptr;
+  alignas(8) unsigned char data[rmsb_units::kPlanBytes];
+  LastPlan& operator=(std::string s) {
+    text = std::move(s);
+    make = nullptr;
+    return *this;
+  }
+  LastPlan& operator+=(const std::string& s) {
+    text += s;
+    return *this;
+  }
+  const std::string& get() {
+    if (make) *this = make(data);
+    return text;
+  }
+};
+thread_local LastPlan t_last_plan;
 
 // Shared memory an SM offers (228 KB), the opt-in maximum per CTA (227 KB), and the
 // 1 KB the runtime reserves per resident CTA.
@@ -1240,6 +1260,10 @@ constexpr int kUnits = static_cast<int>(sizeof(kUnitHooks) / sizeof(kUnitHooks[0
 namespace rmsb_units {
 void count_launches(uint64_t n) { rmsb200::g_launches.fetch_add(n, std::memory_order_relaxed); }
 void set_last_plan(std::string plan) { rmsb200::t_last_plan = std::move(plan); }
+void set_last_plan(PlanText make, const void* data, size_t bytes) {
+  rmsb200::t_last_plan.make = make;
+  std::memcpy(rmsb200::t_last_plan.data, data, bytes);
+}
 }  // namespace rmsb_units
 
 // =========================================================================================
@@ -1510,7 +1534,7 @@ extern "C" int rmsnorm_b200_debug_report(void* stream, uint64_t* violations, int
 extern "C" uint64_t rmsnorm_b200_launch_count(void) { return g_launches.load(); }
 
 extern "C" int rmsnorm_b200_last_plan(char* buf, size_t len) {
-  const std::string& s = t_last_plan;
+  const std::string& s = t_last_plan.get();
   if (buf && len > 0) {
     const size_t n = std::min(len - 1, s.size());
     std::memcpy(buf, s.data(), n);

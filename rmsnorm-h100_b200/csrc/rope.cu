@@ -2,6 +2,8 @@
 #define RMSB_UNIT rope
 #include "unit_state.cuh"
 
+#include <cstring>
+
 #include "rope_kernels.cuh"
 
 namespace rmsb200 {
@@ -88,6 +90,21 @@ RopePlan plan(const rmsnorm_b200_rope_args* a, int u) {
   return pl;
 }
 
+struct RopeLaunch {  // for rmsnorm_b200_last_plan
+  RopePlan pl;
+  char kind[16];
+  unsigned x, y;
+  int threads;
+};
+
+std::string describe_rope(const void* data) {
+  const RopeLaunch& l = *static_cast<const RopeLaunch*>(data);
+  char buf[128];
+  std::snprintf(buf, sizeof(buf), "%s grid=%ux%u threads=%d lanes=%d jobs=%d+%d", l.kind, l.x, l.y, l.threads,
+                1 << l.pl.lanes_shift, l.pl.jobs[0], l.pl.jobs[1]);
+  return buf;
+}
+
 // Launches with programmatic dependent launch: the kernels wait for the one before them
 // before their first global access.
 template <typename Kernel>
@@ -106,10 +123,9 @@ int launch(Kernel kernel, dim3 grid, int threads, cudaStream_t stream, const Rop
     cudaGetLastError();
     return RMSNORM_B200_ERR_CUDA;
   }
-  char buf[128];
-  std::snprintf(buf, sizeof(buf), "%s grid=%ux%u threads=%d lanes=%d jobs=%d+%d", kind, grid.x, grid.y, threads,
-                1 << pl.lanes_shift, pl.jobs[0], pl.jobs[1]);
-  return launched(buf);
+  RopeLaunch l = {pl, {}, grid.x, grid.y, threads};
+  std::strncpy(l.kind, kind, sizeof(l.kind) - 1);
+  return launched(describe_rope, l);
 }
 
 using RopeKernel = void (*)(const RopeParams, const RopePlan);

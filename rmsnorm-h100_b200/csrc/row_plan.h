@@ -1,6 +1,8 @@
 // row_plan.h -- launch plan of the fused row kernels (row_ring.cuh has the vocabulary).
 #pragma once
 
+#include <cstring>
+
 #include "row_ring.cuh"
 
 namespace rmsb200 {
@@ -63,54 +65,92 @@ inline const char* plan_rows(int64_t rows, int64_t N, const int (&bytes)[3], boo
   return nullptr;
 }
 
+struct RowLaunch {  // for rmsnorm_b200_last_plan
+  RowPlan pl;
+  char kind[16];
+  int grid, k, smem;
+};
+
+inline std::string describe_rows(const void* data) {
+  const RowLaunch& l = *static_cast<const RowLaunch*>(data);
+  char buf[192];
+  std::snprintf(buf, sizeof(buf), "%s grid=%d G=%d groups=%d K=%d KC=%d R=%d S=%d C=%d slice=%d unit=%u smem=%d", l.kind,
+                l.grid, l.pl.G, l.pl.groups, l.k, l.pl.KC, l.pl.R, l.pl.S, l.pl.C, l.pl.slice, l.pl.unit_bytes, l.smem);
+  return buf;
+}
+
+// Clusters of the plan's shape (CTAs, without a split) that can be resident at once.
+template <typename Kernel>
+int resident_clusters(UnitDevice* ud, Kernel kernel, const RowPlan& pl, int smem, int* clusters) {
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  std::lock_guard<std::mutex> lock(ud->mu);
+  if (!ud->attrs_done.count(fn)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemOptIn) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return RMSNORM_B200_ERR_CUDA;
+    ud->attrs_done.insert(fn);
+  }
+  *clusters = ud->sm_count;
+  if (pl.C == 1) return RMSNORM_B200_OK;
+  const auto key = std::make_tuple(fn, pl.C, smem);
+  const auto it = ud->clusters.find(key);
+  if (it != ud->clusters.end()) {
+    *clusters = it->second;
+    return RMSNORM_B200_OK;
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = pl.C;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(pl.C * ud->sm_count);
+  cfg.blockDim = dim3(pl.G * pl.groups);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(clusters, kernel, &cfg) != cudaSuccess) *clusters = 0;
+  cudaGetLastError();
+  ud->clusters[key] = *clusters;
+  return RMSNORM_B200_OK;
+}
+
 // Launches a persistent grid: one CTA per SM (as many clusters as fit), at most one row group per
 // tile. Returns UNSUPPORTED when no cluster of this shape fits.
 template <typename Kernel, typename Params>
 int launch_rows(UnitDevice* ud, Kernel kernel, const Params& p, const RowPlan& pl, int smem, cudaStream_t stream,
                 const char* kind, int k, int* grid_out = nullptr, bool dry_run = false) {
-  const void* fn = reinterpret_cast<const void*>(kernel);
-  int clusters = ud->sm_count;
-  {
-    std::lock_guard<std::mutex> lock(ud->mu);
-    if (!ud->attrs_done.count(fn)) {
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemOptIn) != cudaSuccess ||
-          cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-        return RMSNORM_B200_ERR_CUDA;
-      ud->attrs_done.insert(fn);
-    }
-  }
-  cudaLaunchConfig_t cfg = {};
+  int clusters = 0;
+  const int st = resident_clusters(ud, kernel, pl, smem, &clusters);
+  if (st) return st;
+  if (clusters < 1) return RMSNORM_B200_ERR_UNSUPPORTED;
+  const int64_t grid = std::min<int64_t>(pl.tiles, clusters) * pl.C;
+  if (grid_out) *grid_out = static_cast<int>(grid);
+  if (dry_run) return RMSNORM_B200_OK;
   cudaLaunchAttribute attr[1];
-  cfg.blockDim = dim3(pl.G * pl.groups);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   if (pl.C > 1) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = pl.C;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(pl.C * ud->sm_count);
-    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) clusters = 0;
-    cudaGetLastError();
-    if (clusters < 1) return RMSNORM_B200_ERR_UNSUPPORTED;
   } else {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
   }
-  const int64_t grid = std::min<int64_t>(pl.tiles, clusters) * pl.C;
-  if (grid_out) *grid_out = static_cast<int>(grid);
-  if (dry_run) return RMSNORM_B200_OK;
+  cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(pl.G * pl.groups);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, kernel, p, pl) != cudaSuccess) {
     cudaGetLastError();
     return RMSNORM_B200_ERR_CUDA;
   }
-  char buf[160];
-  std::snprintf(buf, sizeof(buf), "%s grid=%d G=%d groups=%d K=%d KC=%d R=%d S=%d C=%d slice=%d unit=%u smem=%d", kind,
-                static_cast<int>(grid), pl.G, pl.groups, k, pl.KC, pl.R, pl.S, pl.C, pl.slice, pl.unit_bytes, smem);
-  return launched(buf);
+  RowLaunch l = {pl, {}, static_cast<int>(grid), k, smem};
+  std::strncpy(l.kind, kind, sizeof(l.kind) - 1);
+  return launched(describe_rows, l);
 }
 
 }  // namespace

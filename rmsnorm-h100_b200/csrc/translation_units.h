@@ -8,6 +8,7 @@
 
 #include <cuda_runtime.h>
 
+#include <cstddef>
 #include <cstdint>
 #include <string>
 
@@ -28,5 +29,10 @@ extern const UnitHooks rope_unit;
 // Bookkeeping of the main unit: rmsnorm_b200_launch_count and rmsnorm_b200_last_plan.
 void count_launches(uint64_t n);
 void set_last_plan(std::string plan);
+
+// The same, as the function that makes the text from a copy of `data` (at most kPlanBytes).
+using PlanText = std::string (*)(const void* data);
+constexpr size_t kPlanBytes = 256;
+void set_last_plan(PlanText make, const void* data, size_t bytes);
 
 }  // namespace rmsb_units

@@ -16,9 +16,11 @@
 
 #include <algorithm>
 #include <cstdio>
+#include <map>
 #include <memory>
 #include <mutex>
 #include <string>
+#include <tuple>
 #include <unordered_set>
 #include <vector>
 
@@ -39,6 +41,7 @@ struct UnitDevice {
   int sm_count = 0;
   std::mutex mu;
   std::unordered_set<const void*> attrs_done;
+  std::map<std::tuple<const void*, int, int>, int> clusters;  // that fit, by kernel, CTAs and shared memory
 };
 
 std::mutex g_unit_mu;
@@ -120,6 +123,16 @@ int launched(std::string plan, uint64_t n = 1) {
   if (cudaGetLastError() != cudaSuccess) return RMSNORM_B200_ERR_CUDA;
   rmsb_units::count_launches(n);
   if (!plan.empty()) rmsb_units::set_last_plan(std::move(plan));
+  return RMSNORM_B200_OK;
+}
+
+// The same with a plan whose text is made on demand.
+template <typename Plan>
+int launched(rmsb_units::PlanText make, const Plan& plan) {
+  static_assert(sizeof(Plan) <= rmsb_units::kPlanBytes, "plan size");
+  if (cudaGetLastError() != cudaSuccess) return RMSNORM_B200_ERR_CUDA;
+  rmsb_units::count_launches(1);
+  rmsb_units::set_last_plan(make, &plan, sizeof(plan));
   return RMSNORM_B200_OK;
 }
 

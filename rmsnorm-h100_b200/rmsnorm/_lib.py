@@ -362,23 +362,39 @@ def _stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def enqueue(name: str, device: torch.device, *args) -> None:
-    """Calls the entry point `name` with `args` and the current stream of `device`."""
-    fn = getattr(load_library(), name)
-    index = device.index
+_PACKED = {}
+
+
+def packed_entry(name: str, *argtypes):
+    """The entry point `name` as a function of other ctypes argument types than SIGNATURES
+    gives it: argument structs as packed bytes (c_char_p) cost a fraction of a Structure."""
+    fn = _PACKED.get(name)
+    if fn is None:
+        fn = _PACKED[name] = ctypes.CFUNCTYPE(ctypes.c_int, *argtypes)((name, load_library()))
+    return fn
+
+
+def enqueue(fn, name: str, index: int, *args) -> None:
+    """Calls a packed entry point with `args` and the current stream of CUDA device `index`."""
     if index == torch._C._cuda_getDevice():
         status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
             status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    _check(status, name)
+    if status:
+        _check(status, name)
 
 
-def workspace_bytes(name: str, device: torch.device, *args) -> int:
-    """Answer of the workspace-size entry point `name`."""
+def workspace_bytes(fn, name: str, index: int, *args) -> int:
+    """Answer of a packed workspace-size entry point."""
     n = ctypes.c_size_t(0)
-    with torch.cuda.device(device):
-        _check(getattr(load_library(), name)(*args, ctypes.byref(n)), name)
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, ctypes.byref(n))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, ctypes.byref(n))
+    if status:
+        _check(status, name)
     return n.value
 
 

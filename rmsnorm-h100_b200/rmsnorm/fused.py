@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -29,7 +30,6 @@ from .rmsnorm import (
     _check_tensor_dtype,
     _check_x_shape,
     _contig,
-    _SUPPORTED_DTYPES,
 )
 
 __all__ = [
@@ -49,52 +49,74 @@ __all__ = [
 
 _CODE = _lib._DTYPE_CODES
 _GROUP_SIZES = (None, 32, 64, 128, 256)
+_is_compiling = torch.compiler.is_compiling
+
+# The C argument structs as packed bytes, field by field as _lib declares them (null pointers
+# are 0). A decoding step calls these operators with microseconds of work, so the checks and
+# the call are kept short.
+_QUANT = struct.Struct("2q7Q2q7if")
+_DROP_FWD = struct.Struct("2q7Q3Qqd6ifi")
+_DROP_BWD = struct.Struct("2q9Q3Qqd8i")
+_ROPE_TENSOR = struct.Struct("Q2q")
+_ROPE = struct.Struct("2qQq3QQ2qQ2q4Q12ifi")
+_ROPE_GRADS = struct.Struct("Q2qQ2qQ2qQ2q2Q")
+for _s, _c in ((_QUANT, _lib.QuantArgs), (_DROP_FWD, _lib.DropoutFwdArgs), (_DROP_BWD, _lib.DropoutBwdArgs),
+               (_ROPE_TENSOR, _lib.RopeTensor), (_ROPE, _lib.RopeArgs), (_ROPE_GRADS, _lib.RopeGrads)):
+    assert _s.size == ctypes.sizeof(_c), _c.__name__
+
+_BYTES, _STREAM, _SIZE, _OUT = ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.POINTER(ctypes.c_size_t)
 
 
-def _ptr(t: Optional[Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
-
-
-def _code(t: Optional[Tensor]) -> int:
-    return 0 if t is None else _CODE[t.dtype]
-
-
-def _check_affine(name: str, t: Optional[Tensor], n: int, device: torch.device) -> None:
+def _affine_code(name: str, t: Optional[Tensor], n: int, device: torch.device) -> int:
     if t is None:
-        return
-    if t.dtype not in _SUPPORTED_DTYPES:
+        return 0
+    code = _CODE.get(t.dtype)
+    if code is None:
         _check_tensor_dtype(name.capitalize(), t)
-    if t.dim() != 1 or t.shape[0] != n:
+    if t.shape != (n,):
         raise ValueError(f"{name} shape must be (N,) with N={n}, got {tuple(t.shape)}")
     if t.device != device:
         _check_same_device(name, t, device)
+    return code
 
 
-def _check_like(name: str, t: Optional[Tensor], x: Tensor) -> None:
+def _like_code(name: str, t: Optional[Tensor], x: Tensor, shape, device: torch.device) -> int:
     if t is None:
-        return
-    if t.dtype not in _SUPPORTED_DTYPES:
+        return 0
+    code = _CODE.get(t.dtype)
+    if code is None:
         _check_tensor_dtype(name.capitalize(), t)
-    if t.shape != x.shape:
-        raise ValueError(f"{name} shape must match x shape {tuple(x.shape)}, got {tuple(t.shape)}")
-    if t.device != x.device:
-        _check_same_device(name, t, x.device)
+    if t.shape != shape:
+        raise ValueError(f"{name} shape must match x shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        _check_same_device(name, t, device)
+    return code
 
 
-def _check_row_input(x: Tensor, weight, bias, residual) -> None:
-    if x.dtype not in _SUPPORTED_DTYPES:
+def _dtype_code(name: str, dtype: torch.dtype) -> int:
+    code = _CODE.get(dtype)
+    if code is None:
+        _check_optional_dtype(name, dtype)
+    return code
+
+
+def _row_codes(x: Tensor, weight, bias, residual):
+    """Checks the inputs of a row operator; (shape, hidden, device, their dtype codes)."""
+    code = _CODE.get(x.dtype)
+    if code is None:
         raise AssertionError("Unsupported dtype")
-    _check_x_shape(x.shape)
-    n = x.shape[-1]
-    _check_affine("weight", weight, n, x.device)
-    _check_affine("bias", bias, n, x.device)
-    _check_like("residual", residual, x)
+    shape = x.shape
+    if not shape or not shape[-1]:
+        _check_x_shape(shape)
+    n = shape[-1]
+    device = x.device
+    return (shape, n, device, code, _affine_code("weight", weight, n, device), _affine_code("bias", bias, n, device),
+            _like_code("residual", residual, x, shape, device))
 
 
 # ---------------------------------------------------------------------------------------
 # Residual addition + RMSNorm with an 8-bit output
 # ---------------------------------------------------------------------------------------
-@torch.compiler.disable
 def rmsnorm_quant_fwd(
     x: Tensor,
     weight: Optional[Tensor] = None,
@@ -115,26 +137,28 @@ def rmsnorm_quant_fwd(
     even. NaN in a group makes its scale NaN. `scales_column_major` lays grouped scales out
     column by column (the strides of a transposed tensor), as block-scaled products take
     them. residual_out as in `rmsnorm_fwd`."""
-    _check_row_input(x, weight, bias, residual)
-    if residual_dtype is not None:
-        _check_optional_dtype("residual_dtype", residual_dtype)
-    if quant_dtype not in _lib._QUANT_CODES:
+    if _is_compiling():
+        return _outside_graph(rmsnorm_quant_fwd)(
+            x, weight, bias, residual, quant_dtype, group_size, residual_dtype, eps, scales_column_major)
+    shape, n, device, xc, wc, bc, rc = _row_codes(x, weight, bias, residual)
+    roc = 0 if residual_dtype is None else _dtype_code("residual_dtype", residual_dtype)
+    qc = _lib._QUANT_CODES.get(quant_dtype)
+    if qc is None:
         raise AssertionError("quant_dtype must be float8_e4m3fn or int8")
     if group_size not in _GROUP_SIZES:
         raise ValueError(f"group_size must be None, 32, 64, 128 or 256, got {group_size}")
-    shape = x.shape
-    n = shape[-1]
     rows = x.numel() // n
     row_stride, group_stride = 1, 0
     if group_size is None:
-        scales = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+        scales = torch.empty(*shape[:-1], dtype=torch.float32, device=device) if len(shape) > 1 else torch.empty(
+            (), dtype=torch.float32, device=device)
     else:
         groups = -(-n // group_size)
         if scales_column_major:
-            scales = torch.empty((groups, *shape[:-1]), dtype=torch.float32, device=x.device).movedim(0, -1)
+            scales = torch.empty(groups, *shape[:-1], dtype=torch.float32, device=device).movedim(0, -1)
             row_stride, group_stride = 1, rows
         else:
-            scales = torch.empty((*shape[:-1], groups), dtype=torch.float32, device=x.device)
+            scales = torch.empty(*shape[:-1], groups, dtype=torch.float32, device=device)
             row_stride, group_stride = groups, 1
     if not x.is_cuda:
         q, residual_out = _host.rmsnorm_quant_fwd(
@@ -144,18 +168,29 @@ def rmsnorm_quant_fwd(
     residual = _contig(residual)
     weight = _contig(weight)
     bias = _contig(bias)
-    q = torch.empty(shape, dtype=quant_dtype, device=x.device)
+    q = torch.empty_like(x, dtype=quant_dtype)
     residual_out = None
     if residual is not None:
-        residual_out = torch.empty(shape, dtype=residual_dtype or residual.dtype, device=x.device)
+        if residual_dtype is None:
+            residual_out, roc = torch.empty_like(residual), rc
+        else:
+            residual_out = torch.empty_like(x, dtype=residual_dtype)
     elif residual_dtype is not None and residual_dtype != x.dtype:
-        residual_out = torch.empty(shape, dtype=residual_dtype, device=x.device)
-    args = _lib.QuantArgs(
-        rows, n, x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), q.data_ptr(), scales.data_ptr(),
-        _ptr(residual_out), row_stride, group_stride, _CODE[x.dtype], _code(residual), _code(weight), _code(bias),
-        _lib._QUANT_CODES[quant_dtype], _code(residual_out), group_size or 0, eps)
-    _lib.enqueue("rmsnorm_b200_quant_fwd", x.device, ctypes.byref(args))
+        residual_out = torch.empty_like(x, dtype=residual_dtype)
+    args = _QUANT.pack(
+        rows, n, x.data_ptr(), 0 if residual is None else residual.data_ptr(),
+        0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(), q.data_ptr(),
+        scales.data_ptr(), 0 if residual_out is None else residual_out.data_ptr(), row_stride, group_stride, xc, rc, wc,
+        bc, qc, roc, group_size or 0, eps)
+    name = "rmsnorm_b200_quant_fwd"
+    _lib.enqueue(_lib.packed_entry(name, _BYTES, _STREAM), name, device.index, args)
     return q, scales, x if residual_out is None else residual_out
+
+
+@functools.lru_cache(maxsize=None)
+def _outside_graph(fn):
+    """`fn` as torch.compile calls it: untraced."""
+    return torch.compiler.disable(fn)
 
 
 # ---------------------------------------------------------------------------------------
@@ -194,7 +229,6 @@ def _with_step(offset: int, step: Optional[Tensor]) -> int:
     return offset if step is None else (offset + int(step)) % (1 << 64)
 
 
-@torch.compiler.disable
 def dropout_add_rmsnorm_fwd(
     x: Tensor,
     weight: Optional[Tensor] = None,
@@ -218,18 +252,20 @@ def dropout_add_rmsnorm_fwd(
     tensor of one element, is added to the offset when the kernel runs, so that replays of a
     CUDA graph can draw new masks. `row_offset` is the row of the whole tensor's mask that x
     begins with, for tensors whose rows are spread over ranks."""
-    _check_row_input(x, weight, bias, residual)
-    if out_dtype is not None:
-        _check_optional_dtype("out_dtype", out_dtype)
-    if residual_dtype is not None:
-        _check_optional_dtype("residual_dtype", residual_dtype)
-    shape = x.shape
-    n = shape[-1]
+    if _is_compiling():
+        return _outside_graph(dropout_add_rmsnorm_fwd)(
+            x, weight, bias, residual, p, rng, out_dtype, residual_dtype, eps, store_rstd, rng_step, row_offset)
+    shape, n, device, xc, wc, bc, rc = _row_codes(x, weight, bias, residual)
+    if out_dtype is None:
+        out_dtype, oc = x.dtype, xc
+    else:
+        oc = _dtype_code("out_dtype", out_dtype)
+    if residual_dtype is None:
+        residual_dtype, roc = (x.dtype, xc) if residual is None else (residual.dtype, rc)
+    else:
+        roc = _dtype_code("residual_dtype", residual_dtype)
     rows = x.numel() // n
-    device = x.device
     seed, offset = _check_dropout(p, rng, rng_step, row_offset, rows, device)
-    out_dtype = out_dtype or x.dtype
-    residual_dtype = residual_dtype or (x.dtype if residual is None else residual.dtype)
     if not x.is_cuda:
         mask = _host.dropout_mask(shape, p, seed, _with_step(offset, rng_step), row_offset, device)
         return _host.dropout_add_rmsnorm_fwd(
@@ -238,18 +274,19 @@ def dropout_add_rmsnorm_fwd(
     residual = _contig(residual)
     weight = _contig(weight)
     bias = _contig(bias)
-    out = torch.empty(shape, dtype=out_dtype, device=device)
-    residual_out = torch.empty(shape, dtype=residual_dtype, device=device)
+    out = torch.empty_like(x, dtype=out_dtype)
+    residual_out = torch.empty_like(x, dtype=residual_dtype)
     rstd = torch.empty(shape[:-1], dtype=torch.float32, device=device) if store_rstd else None
-    args = _lib.DropoutFwdArgs(
-        rows, n, x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), out.data_ptr(), residual_out.data_ptr(),
-        _ptr(rstd), _lib.Dropout(seed, offset, _ptr(rng_step), row_offset, p), _CODE[x.dtype], _code(residual),
-        _code(weight), _code(bias), _CODE[out_dtype], _CODE[residual_dtype], eps, 0)
-    _lib.enqueue("rmsnorm_b200_dropout_rmsnorm_fwd", device, ctypes.byref(args))
+    args = _DROP_FWD.pack(
+        rows, n, x.data_ptr(), 0 if residual is None else residual.data_ptr(),
+        0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(),
+        residual_out.data_ptr(), 0 if rstd is None else rstd.data_ptr(), seed, offset,
+        0 if rng_step is None else rng_step.data_ptr(), row_offset, p, xc, rc, wc, bc, oc, roc, eps, 0)
+    name = "rmsnorm_b200_dropout_rmsnorm_fwd"
+    _lib.enqueue(_lib.packed_entry(name, _BYTES, _STREAM), name, device.index, args)
     return out, residual_out, rstd
 
 
-@torch.compiler.disable
 def dropout_add_rmsnorm_bwd(
     residual_out: Tensor,
     weight: Optional[Tensor],
@@ -270,22 +307,23 @@ def dropout_add_rmsnorm_bwd(
     rng_step and row_offset as in the forward. dx is in dx_dtype (default: dout's), dresidual
     (None unless has_residual) in dresidual_dtype (default: residual_out's); dweight and dbias
     follow the affine tensors (dbias without a bias tensor: weight's dtype, else dout's)."""
+    if _is_compiling():
+        return _outside_graph(dropout_add_rmsnorm_bwd)(
+            residual_out, weight, dout, rstd, dresidual_out, p, rng, has_bias, has_residual, bias, dx_dtype,
+            dresidual_dtype, rng_step, row_offset)
     h = residual_out
-    if h.dtype not in _SUPPORTED_DTYPES:
-        raise AssertionError("Unsupported dtype")
-    _check_x_shape(h.shape)
-    shape = h.shape
-    n = shape[-1]
+    shape, n, device, hc, wc, bc, _ = _row_codes(h, weight, bias, None)
+    yc = _like_code("dout", dout, h, shape, device)
+    doc = _like_code("dresidual_out", dresidual_out, h, shape, device)
+    if dx_dtype is None:
+        dx_dtype, dxc = dout.dtype, yc
+    else:
+        dxc = _dtype_code("dx_dtype", dx_dtype)
+    if dresidual_dtype is None:
+        dresidual_dtype, dresc = h.dtype, hc
+    else:
+        dresc = _dtype_code("dresidual_dtype", dresidual_dtype)
     rows = h.numel() // n
-    device = h.device
-    _check_affine("weight", weight, n, device)
-    _check_affine("bias", bias, n, device)
-    _check_like("dout", dout, h)
-    _check_like("dresidual_out", dresidual_out, h)
-    if dx_dtype is not None:
-        _check_optional_dtype("dx_dtype", dx_dtype)
-    if dresidual_dtype is not None:
-        _check_optional_dtype("dresidual_dtype", dresidual_dtype)
     if rstd.dtype != torch.float32:
         raise ValueError("rstd must be float32")
     if rstd.numel() != rows:
@@ -293,8 +331,6 @@ def dropout_add_rmsnorm_bwd(
     if rstd.device != device:
         _check_same_device("rstd", rstd, device)
     seed, offset = _check_dropout(p, rng, rng_step, row_offset, rows, device)
-    dx_dtype = dx_dtype or dout.dtype
-    dresidual_dtype = dresidual_dtype or h.dtype
     if not h.is_cuda:
         mask = _host.dropout_mask(shape, p, seed, _with_step(offset, rng_step), row_offset, device)
         dx, dw, db, dh = _host.dropout_add_rmsnorm_bwd(
@@ -302,25 +338,33 @@ def dropout_add_rmsnorm_bwd(
         return dx, dw, db, dh.to(dresidual_dtype) if has_residual else None
     h = _contig(h)
     dout = _contig(dout)
-    rstd = rstd.contiguous()
+    rstd = _contig(rstd)
     weight = _contig(weight)
     dresidual_out = _contig(dresidual_out)
-    dx = torch.empty(shape, dtype=dx_dtype, device=device)
-    dresidual = torch.empty(shape, dtype=dresidual_dtype, device=device) if has_residual else None
+    dx = torch.empty_like(h, dtype=dx_dtype)
+    dresidual = torch.empty_like(h, dtype=dresidual_dtype) if has_residual else None
     dw = torch.empty_like(weight) if weight is not None else None
     db = None
     if has_bias:
-        like = bias if bias is not None else weight
-        db = torch.empty((n,), dtype=like.dtype if like is not None else dout.dtype, device=device)
-    args = _lib.DropoutBwdArgs(
-        rows, n, h.data_ptr(), dout.data_ptr(), rstd.data_ptr(), _ptr(weight), _ptr(dresidual_out), dx.data_ptr(),
-        _ptr(dresidual), _ptr(dw), _ptr(db), _lib.Dropout(seed, offset, _ptr(rng_step), row_offset, p),
-        _CODE[h.dtype], _CODE[dout.dtype], _code(weight), _code(dresidual_out), _CODE[dx_dtype],
-        _CODE[dresidual_dtype], _code(dw), _code(db))
-    a = ctypes.byref(args)
-    nbytes = _lib.workspace_bytes("rmsnorm_b200_dropout_rmsnorm_bwd_workspace_size", device, a)
+        if bias is None:
+            db = torch.empty(n, dtype=dout.dtype, device=device) if weight is None else torch.empty_like(weight)
+            bc = yc if weight is None else wc
+        else:
+            db = torch.empty_like(bias, memory_format=torch.contiguous_format)
+    args = _DROP_BWD.pack(
+        rows, n, h.data_ptr(), dout.data_ptr(), rstd.data_ptr(), 0 if weight is None else weight.data_ptr(),
+        0 if dresidual_out is None else dresidual_out.data_ptr(), dx.data_ptr(),
+        0 if dresidual is None else dresidual.data_ptr(), 0 if dw is None else dw.data_ptr(),
+        0 if db is None else db.data_ptr(), seed, offset, 0 if rng_step is None else rng_step.data_ptr(), row_offset, p,
+        hc, yc, wc, doc, dxc, dresc, wc, bc)
+    nbytes = 0
+    if dw is not None or db is not None:
+        name = "rmsnorm_b200_dropout_rmsnorm_bwd_workspace_size"
+        nbytes = _lib.workspace_bytes(_lib.packed_entry(name, _BYTES, _OUT), name, device.index, args)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    _lib.enqueue("rmsnorm_b200_dropout_rmsnorm_bwd", device, a, _ptr(ws), nbytes)
+    name = "rmsnorm_b200_dropout_rmsnorm_bwd"
+    _lib.enqueue(_lib.packed_entry(name, _BYTES, _STREAM, _SIZE, _STREAM), name, device.index, args,
+                 None if ws is None else ws.data_ptr(), nbytes)
     return dx, dw, db, dresidual
 
 
@@ -348,7 +392,6 @@ class DropoutAddRMSNormFunction(torch.autograd.Function):
         return dx, dw, db, dresidual, *([None] * 8)
 
 
-@torch.compiler.disable
 def dropout_add_rmsnorm(
     x: Tensor,
     weight: Optional[Tensor] = None,
@@ -364,6 +407,9 @@ def dropout_add_rmsnorm(
     row_offset: int = 0,
 ):
     """`dropout_add_rmsnorm_fwd` with autograd: out, or (out, residual_out) when prenorm."""
+    if _is_compiling():
+        return _outside_graph(dropout_add_rmsnorm)(
+            x, weight, bias, residual, p, rng, out_dtype, residual_dtype, eps, prenorm, rng_step, row_offset)
     return DropoutAddRMSNormFunction.apply(
         x, weight, bias, residual, p, tuple(rng), out_dtype, residual_dtype, eps, prenorm, rng_step, row_offset)
 
@@ -398,67 +444,86 @@ def rope_axes(sections: Sequence[int], interleaved: bool = False) -> Tuple[int, 
     return tuple(out)
 
 
-@functools.lru_cache(maxsize=64)
-def _axis_words(axes: Tuple[int, ...]) -> Tuple[int, ...]:
+@functools.lru_cache(maxsize=256)
+def _axis_words(axes: Optional[Tuple[int, ...]], pairs: int, naxes: int):
+    """(axes, two bits per pair in four words), checked."""
+    if axes is None:
+        axes = (0,) * pairs
+    if len(axes) != pairs or (axes and not 0 <= min(axes) <= max(axes) < naxes):
+        raise ValueError(f"axes must name one of the {naxes} position axes for each of the {pairs} pairs")
     words = [0, 0, 0, 0]
     for i, a in enumerate(axes):
         words[i // 32] |= a << (2 * (i % 32))
-    return tuple(words)
+    return axes, tuple(words)
 
 
-def _check_rope(q, k, positions, table, q_weight, k_weight, axes) -> Tuple[Tuple[int, ...], int]:
-    """(axis of each pair, number of axes)."""
-    if q.dtype not in _SUPPORTED_DTYPES:
+def _rope_weight_code(name: str, w: Optional[Tensor], heads: int, d: int, device: torch.device) -> Tuple[int, int]:
+    """(dtype code, heads) of a weight."""
+    if w is None:
+        return 0, 1
+    code = _CODE.get(w.dtype)
+    if code is None:
+        _check_tensor_dtype(name, w)
+    shape = w.shape
+    if shape != (d,) and (heads < 1 or shape != (heads, d)):
+        raise ValueError(f"{name} shape must be ({d},) or ({heads}, {d}), got {tuple(shape)}")
+    if w.device != device:
+        raise ValueError(f"{name} must be on the same device as q")
+    return code, 1 if len(shape) == 1 else heads
+
+
+def _check_rope(q, k, positions, table, q_weight, k_weight, axes):
+    """(axis of each pair, packed axes, number of axes, device, dtype code, weights' dtype
+    code, q's and k's weight heads)."""
+    dt = q.dtype
+    code = _CODE.get(dt)
+    if code is None:
         raise AssertionError("Unsupported dtype")
-    if q.dim() < 2:
+    shape = q.shape
+    if len(shape) < 2:
         raise ValueError("q must have at least two dimensions (heads, head_dim)")
-    d = q.shape[-1]
+    d = shape[-1]
     device = q.device
     if not 1 <= d <= 256:
         raise ValueError(f"head_dim must be 1 to 256, got {d}")
-    if q.shape[-2] < 1:
+    if shape[-2] < 1:
         raise ValueError("q must have at least one head")
+    tokens = shape[:-2]
+    k_heads = 0
     if k is not None:
-        if k.dtype != q.dtype:
+        if k.dtype != dt:
             raise AssertionError("q and k must have the same dtype")
-        if k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != d:
-            raise ValueError(f"k must have q's shape apart from the heads, got {tuple(k.shape)} for {tuple(q.shape)}")
+        kshape = k.shape
+        if len(kshape) != len(shape) or kshape[:-2] != tokens or kshape[-1] != d:
+            raise ValueError(f"k must have q's shape apart from the heads, got {tuple(kshape)} for {tuple(shape)}")
         if k.device != device:
             raise ValueError("k must be on the same device as q")
-    if table.dtype != torch.float32 or table.dim() != 2 or table.shape[1] % 2 or table.shape[1] > d:
+        k_heads = kshape[-2]
+    elif k_weight is not None:
+        raise ValueError("k_weight needs k")
+    tshape = table.shape
+    if table.dtype != torch.float32 or len(tshape) != 2 or tshape[1] % 2 or tshape[1] > d:
         raise ValueError(f"table must be float32 [positions, rotary_dim] with an even rotary_dim of at most {d}")
-    tokens = q.shape[:-2]
-    pairs = table.shape[1] // 2
-    if positions.dtype not in (torch.int32, torch.int64):
+    if positions.dtype != torch.int64 and positions.dtype != torch.int32:
         raise ValueError("positions must be int32 or int64")
-    if positions.shape == tokens:
+    pshape = positions.shape
+    if pshape == tokens:
         naxes = 1
-    elif positions.dim() == len(tokens) + 1 and positions.shape[1:] == tokens and 1 <= positions.shape[0] <= 4:
-        naxes = positions.shape[0]
+    elif len(pshape) == len(tokens) + 1 and pshape[1:] == tokens and 1 <= pshape[0] <= 4:
+        naxes = pshape[0]
     else:
         raise ValueError(f"positions must be q's leading shape {tuple(tokens)}, or 1 to 4 axes of it, got "
-                         f"{tuple(positions.shape)}")
-    for name, t in (("positions", positions), ("table", table)):
-        if t.device != device:
-            raise ValueError(f"{name} must be on the same device as q")
-    for name, w, heads in (("q_weight", q_weight, q.shape[-2]), ("k_weight", k_weight, k.shape[-2] if k is not None else 0)):
-        if w is None:
-            continue
-        if name == "k_weight" and k is None:
-            raise ValueError("k_weight needs k")
-        _check_tensor_dtype(name, w)
-        if tuple(w.shape) != (d,) and tuple(w.shape) != (heads, d):
-            raise ValueError(f"{name} shape must be ({d},) or ({heads}, {d}), got {tuple(w.shape)}")
-        if w.device != device:
-            raise ValueError(f"{name} must be on the same device as q")
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+                         f"{tuple(pshape)}")
+    if positions.device != device:
+        raise ValueError("positions must be on the same device as q")
+    if table.device != device:
+        raise ValueError("table must be on the same device as q")
+    qwc, qwh = _rope_weight_code("q_weight", q_weight, shape[-2], d, device)
+    kwc, kwh = _rope_weight_code("k_weight", k_weight, k_heads, d, device)
+    if q_weight is not None and k_weight is not None and qwc != kwc:
         raise AssertionError("q_weight and k_weight must have the same dtype")
-    if axes is None:
-        axes = (0,) * pairs
-    axes = tuple(axes)
-    if len(axes) != pairs or (axes and not 0 <= min(axes) <= max(axes) < naxes):
-        raise ValueError(f"axes must name one of the {naxes} position axes for each of the {pairs} pairs")
-    return axes, naxes
+    axes, words = _axis_words(None if axes is None else tuple(axes), tshape[1] // 2, naxes)
+    return axes, words, naxes, device, code, kwc if q_weight is None else qwc, qwh, kwh
 
 
 def _flat(t: Tensor) -> Tensor:
@@ -469,29 +534,23 @@ def _flat(t: Tensor) -> Tensor:
     return t if t.dim() == 3 else t.reshape(-1, t.shape[-2], t.shape[-1])
 
 
-def _tensor(t: Optional[Tensor]) -> _lib.RopeTensor:
+def _place(t: Optional[Tensor]) -> Tuple[int, int, int]:
+    """Address, token stride and head stride of a _flat tensor."""
     if t is None:
-        return _lib.RopeTensor(None, 0, 0)
-    s = t.stride()
-    return _lib.RopeTensor(t.data_ptr(), s[0], s[1])
+        return 0, 0, 0
+    return t.data_ptr(), t.stride(0), t.stride(1)
 
 
-def _weight_heads(w: Optional[Tensor]) -> int:
-    return w.shape[0] if (w is not None and w.dim() == 2) else 1
+def _rope_args(q, k, positions, table, q_weight, k_weight, checked, interleaved, norm, eps) -> bytes:
+    _, words, naxes, _, code, wc, qwh, kwh = checked
+    tokens, heads, d = q.shape
+    return _ROPE.pack(
+        tokens, table.shape[0], positions.data_ptr(), tokens, table.data_ptr(),
+        0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), *_place(q),
+        *_place(k), *words, heads, 0 if k is None else k.shape[1], d, table.shape[1], naxes, bool(interleaved),
+        bool(norm), positions.dtype == torch.int64, code, wc, qwh, kwh, eps, 0)
 
 
-def _rope_args(q, k, positions, table, q_weight, k_weight, axes, naxes, interleaved, norm, eps):
-    words = (ctypes.c_uint64 * 4)(*_axis_words(axes))
-    tokens = q.shape[0]
-    w = q_weight if q_weight is not None else k_weight
-    return _lib.RopeArgs(
-        tokens, table.shape[0], positions.data_ptr(), tokens, table.data_ptr(), _ptr(q_weight), _ptr(k_weight),
-        _tensor(q), _tensor(k), words, q.shape[1], 0 if k is None else k.shape[1], q.shape[2], table.shape[1], naxes,
-        bool(interleaved), bool(norm), positions.dtype == torch.int64, _CODE[q.dtype], _code(w),
-        _weight_heads(q_weight), _weight_heads(k_weight), eps, 0)
-
-
-@torch.compiler.disable
 def qk_norm_rope_fwd(
     q: Tensor,
     k: Optional[Tensor],
@@ -516,10 +575,12 @@ def qk_norm_rope_fwd(
     columns (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when `interleaved`. `table` is
     `rope_table`'s. A position outside the table gives NaN columns, and on CUDA an
     invalid-argument entry in the device status word."""
-    axes, naxes = _check_rope(q, k, positions, table, q_weight, k_weight, axes)
+    if _is_compiling():
+        return _outside_graph(qk_norm_rope_fwd)(
+            q, k, positions, table, q_weight, k_weight, axes, interleaved, norm, eps, inplace)
+    checked = _check_rope(q, k, positions, table, q_weight, k_weight, axes)
     if not q.is_cuda:
-        pos = positions.reshape(naxes, *q.shape[:-2])
-        cos, sin = _host.rope_cos_sin(pos, table, axes)
+        cos, sin = _host.rope_cos_sin(positions.reshape(checked[2], *q.shape[:-2]), table, checked[0])
         outs = [t if t is None else _host.qk_norm_rope_fwd(t, w, cos, sin, interleaved, norm, eps)
                 for t, w in ((q, q_weight), (k, k_weight))]
         if inplace:
@@ -537,11 +598,10 @@ def qk_norm_rope_fwd(
                 raise ValueError("inplace needs q and k whose leading dimensions collapse to one stride")
         qo, ko = qf, kf
     else:
-        q_out = qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ko = None
         if k is not None:
-            k_out = ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        else:
-            ko = None
+            k_out = ko = torch.empty_like(k, memory_format=torch.contiguous_format)
         if q.dim() != 3:
             qo = qo.view(qf.shape)
             ko = None if ko is None else ko.view(kf.shape)
@@ -549,13 +609,13 @@ def qk_norm_rope_fwd(
     table = table.contiguous()
     q_weight = _contig(q_weight)
     k_weight = _contig(k_weight)
-    args = _rope_args(qf, kf, positions, table, q_weight, k_weight, axes, naxes, interleaved, norm, eps)
-    _lib.enqueue("rmsnorm_b200_rope_fwd", q.device, ctypes.byref(args), ctypes.byref(_tensor(qo)),
-                 ctypes.byref(_tensor(ko)))
+    args = _rope_args(qf, kf, positions, table, q_weight, k_weight, checked, interleaved, norm, eps)
+    name = "rmsnorm_b200_rope_fwd"
+    _lib.enqueue(_lib.packed_entry(name, _BYTES, _BYTES, _BYTES, _STREAM), name, checked[3].index, args,
+                 _ROPE_TENSOR.pack(*_place(qo)), _ROPE_TENSOR.pack(*_place(ko)))
     return q_out, k_out
 
 
-@torch.compiler.disable
 def qk_norm_rope_bwd(
     q: Tensor,
     k: Optional[Tensor],
@@ -572,25 +632,27 @@ def qk_norm_rope_bwd(
 ) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
     """(dq, dk, dq_weight, dk_weight) from the forward's inputs and the gradients of its
     outputs; the weights' gradients (None without a weight) are summed in a fixed order."""
-    axes, naxes = _check_rope(q, k, positions, table, q_weight, k_weight, axes)
+    if _is_compiling():
+        return _outside_graph(qk_norm_rope_bwd)(
+            q, k, positions, table, dq_out, dk_out, q_weight, k_weight, axes, interleaved, norm, eps)
+    checked = _check_rope(q, k, positions, table, q_weight, k_weight, axes)
     for name, g, t in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
         if (g is None) != (t is None):
             raise ValueError(f"{name} is needed exactly when its input is given")
         if g is not None and (g.shape != t.shape or g.dtype != q.dtype or g.device != q.device):
             raise ValueError(f"{name} must have its input's shape, dtype and device")
     if not q.is_cuda:
-        pos = positions.reshape(naxes, *q.shape[:-2])
-        cos, sin = _host.rope_cos_sin(pos, table, axes)
+        cos, sin = _host.rope_cos_sin(positions.reshape(checked[2], *q.shape[:-2]), table, checked[0])
         dq, dqw = _host.qk_norm_rope_bwd(q, q_weight, dq_out, cos, sin, interleaved, norm, eps)
         dk = dkw = None
         if k is not None:
             dk, dkw = _host.qk_norm_rope_bwd(k, k_weight, dk_out, cos, sin, interleaved, norm, eps)
         return dq, dk, dqw, dkw
-    device = q.device
+    device = checked[3]
     qf = _flat(q)
     kf = None if k is None else _flat(k)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=device)
-    dk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=device)
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     q_weight = _contig(q_weight)
     k_weight = _contig(k_weight)
     dqw = None if q_weight is None else torch.empty_like(q_weight)
@@ -599,13 +661,19 @@ def qk_norm_rope_bwd(
     table = table.contiguous()
     dqo = _flat(dq_out)
     dko = None if k is None else _flat(dk_out)
-    args = _rope_args(qf, kf, positions, table, q_weight, k_weight, axes, naxes, interleaved, norm, eps)
-    grads = _lib.RopeGrads(_tensor(dqo), _tensor(dko), _tensor(dq.view(qf.shape)),
-                           _tensor(None if k is None else dk.view(kf.shape)), _ptr(dqw), _ptr(dkw))
-    a, g = ctypes.byref(args), ctypes.byref(grads)
-    nbytes = _lib.workspace_bytes("rmsnorm_b200_rope_bwd_workspace_size", device, a, g)
+    args = _rope_args(qf, kf, positions, table, q_weight, k_weight, checked, interleaved, norm, eps)
+    grads = _ROPE_GRADS.pack(
+        *_place(dqo), *_place(dko), dq.data_ptr(), dq.stride(-2) * q.shape[-2], dq.stride(-2),
+        *((0, 0, 0) if k is None else (dk.data_ptr(), dk.stride(-2) * k.shape[-2], dk.stride(-2))),
+        0 if dqw is None else dqw.data_ptr(), 0 if dkw is None else dkw.data_ptr())
+    nbytes = 0
+    if dqw is not None or dkw is not None:
+        name = "rmsnorm_b200_rope_bwd_workspace_size"
+        nbytes = _lib.workspace_bytes(_lib.packed_entry(name, _BYTES, _BYTES, _OUT), name, device.index, args, grads)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    _lib.enqueue("rmsnorm_b200_rope_bwd", device, a, g, _ptr(ws), nbytes)
+    name = "rmsnorm_b200_rope_bwd"
+    _lib.enqueue(_lib.packed_entry(name, _BYTES, _BYTES, _STREAM, _SIZE, _STREAM), name, device.index, args, grads,
+                 None if ws is None else ws.data_ptr(), nbytes)
     return dq, dk, dqw, dkw
 
 
@@ -623,7 +691,6 @@ class QKNormRopeFunction(torch.autograd.Function):
         return dq, dk, None, None, dqw, dkw, None, None, None, None
 
 
-@torch.compiler.disable
 def qk_norm_rope(
     q: Tensor,
     k: Optional[Tensor],
@@ -637,5 +704,8 @@ def qk_norm_rope(
     eps: float = 1e-6,
 ) -> Tuple[Tensor, Optional[Tensor]]:
     """`qk_norm_rope_fwd` with autograd (for q, k and the weights)."""
+    if _is_compiling():
+        return _outside_graph(qk_norm_rope)(
+            q, k, positions, table, q_weight, k_weight, axes, interleaved, norm, eps)
     return QKNormRopeFunction.apply(
         q, k, positions, table, q_weight, k_weight, None if axes is None else tuple(axes), interleaved, norm, eps)
