@@ -9,7 +9,6 @@ namespace rmsb200 {
 namespace {
 
 using BwdKernel = void (*)(const FusedBwdParams, const RowPlan);
-constexpr int kNone = -1;
 
 struct Plan {
   int64_t nparts = 0;      // partial rows of dweight / dbias
@@ -20,23 +19,35 @@ struct Plan {
   const char* why = nullptr;  // why the generic path is taken
 };
 
-template <typename H, typename DY, typename DRO>
+template <typename H, typename DY, typename DRO, typename DRES>
 BwdKernel pick_steps(int k) {
-  return k == 1 ? fused_bwd_kernel<H, DY, DRO, 1> : fused_bwd_kernel<H, DY, DRO, 2>;
+  if (k == 1) return fused_bwd_kernel<H, DY, DRO, DRES, 1>;
+  if (k == 2) return fused_bwd_kernel<H, DY, DRO, DRES, 2>;
+  // four steps hold a row of 16-bit values only
+  if constexpr (sizeof(H) == 2 && sizeof(DY) == 2) return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps>;
+  return nullptr;
 }
 
-// (h, dout, dresidual_out): the saved input in dout's type or in fp32, its gradient in its own.
-BwdKernel pick(int h, int dy, int dro, int k) {
+template <typename H, typename DY>
+BwdKernel pick_residual(bool dro, bool dres, int k) {
+  if (dro) return dres ? pick_steps<H, DY, H, H>(k) : pick_steps<H, DY, H, NoT>(k);
+  return dres ? pick_steps<H, DY, NoT, H>(k) : pick_steps<H, DY, NoT, NoT>(k);
+}
+
+// The saved input in dout's type or in fp32; dresidual_out and dresidual have its type, dx has
+// dout's.
+BwdKernel pick(const rmsnorm_b200_dropout_bwd_args* a, int k) {
   constexpr int H = RMSNORM_B200_F16, B = RMSNORM_B200_BF16, F = RMSNORM_B200_F32;
   using h16 = __half;
   using b16 = __nv_bfloat16;
-  if (dro != kNone && dro != h) return nullptr;
-  const bool none = dro == kNone;
-  if (h == B && dy == B) return none ? pick_steps<b16, b16, NoT>(k) : pick_steps<b16, b16, b16>(k);
-  if (h == H && dy == H) return none ? pick_steps<h16, h16, NoT>(k) : pick_steps<h16, h16, h16>(k);
-  if (h == F && dy == F) return none ? pick_steps<float, float, NoT>(k) : pick_steps<float, float, float>(k);
-  if (h == F && dy == B) return none ? pick_steps<float, b16, NoT>(k) : pick_steps<float, b16, float>(k);
-  if (h == F && dy == H) return none ? pick_steps<float, h16, NoT>(k) : pick_steps<float, h16, float>(k);
+  const int h = a->h_dtype, dy = a->dout_dtype;
+  const bool dro = a->dresidual_out, dres = a->dresidual;
+  if (a->dx_dtype != dy || (dro && a->dresidual_out_dtype != h) || (dres && a->dresidual_dtype != h)) return nullptr;
+  if (h == B && dy == B) return pick_residual<b16, b16>(dro, dres, k);
+  if (h == H && dy == H) return pick_residual<h16, h16>(dro, dres, k);
+  if (h == F && dy == F) return pick_residual<float, float>(dro, dres, k);
+  if (h == F && dy == B) return pick_residual<float, b16>(dro, dres, k);
+  if (h == F && dy == H) return pick_residual<float, h16>(dro, dres, k);
   return nullptr;
 }
 
@@ -61,15 +72,17 @@ int make_plan(UnitDevice* ud, const rmsnorm_b200_dropout_bwd_args* a, Plan* pl) 
   if (!pl->why) {
     const int bytes[3] = {elem_bytes(a->h_dtype), elem_bytes(a->dout_dtype),
                           a->dresidual_out ? elem_bytes(a->dresidual_out_dtype) : 0};
-    pl->why = plan_rows(a->rows, a->hidden, bytes, false, kBwdSteps, ud->sm_count, &pl->rows, &pl->k, &pl->smem);
+    const int64_t in_registers = kBwdThreads * 8 * kBwdRegSteps;
+    const int steps = a->h_dtype == RMSNORM_B200_F32 || a->hidden <= in_registers ? kBwdRegSteps : kBwdTmemSteps;
+    pl->why = plan_rows(a->rows, a->hidden, bytes, false, kBwdThreads, steps, ud->sm_count, &pl->rows, &pl->k, &pl->smem);
   }
   if (!pl->why) {
-    pl->kernel = pick(a->h_dtype, a->dout_dtype, a->dresidual_out ? a->dresidual_out_dtype : kNone, pl->k);
+    pl->kernel = pick(a, pl->k);
     if (!pl->kernel) pl->why = "dtype combination";
   }
   if (pl->kernel) {
-    // the groups' sums pass through the rings
-    pl->smem = std::max(pl->smem, pl->rows.groups * pl->rows.slice * 4);
+    // the groups' sums of a vector step pass through the rings
+    if (pl->rows.groups > 1) pl->smem = std::max(pl->smem, kBwdThreads * 64);
     int grid = 0;
     const int st = launch_rows(ud, pl->kernel, FusedBwdParams{}, pl->rows, pl->smem, nullptr, "", pl->k, &grid, true);
     if (st == RMSNORM_B200_OK) {

@@ -6,9 +6,13 @@
 
 namespace rmsb200 {
 
-constexpr int kBwdSteps = 2;  // vector steps a thread: its dweight and dbias sums take 16 registers each
+constexpr int kBwdThreads = 512;
+constexpr int kBwdRegSteps = 2;    // vector steps a thread whose sums stay in registers
+constexpr int kBwdTmemSteps = 4;   // in tensor memory
+constexpr uint32_t kTmemCols = 256;
 
-// One row's values of one tensor as loaded: 4 registers a vector, 8 for fp32.
+// One vector of a tensor as loaded: 4 registers, 8 for fp32. A row is held like this from the
+// first pass to the second, so its slot loads again in between.
 template <typename T>
 struct Raw8 {
   static constexpr int kWords = Vec8<T>::kBytes / 16;
@@ -23,32 +27,42 @@ struct Raw8 {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) v[i] = make_uint4(0, 0, 0, 0);
   }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
+  __device__ __forceinline__ void get(float2 (&f)[4]) const {
     if constexpr (kWords == 2) {
-      f[0] = __uint_as_float(v[0].x); f[1] = __uint_as_float(v[0].y);
-      f[2] = __uint_as_float(v[0].z); f[3] = __uint_as_float(v[0].w);
-      f[4] = __uint_as_float(v[1].x); f[5] = __uint_as_float(v[1].y);
-      f[6] = __uint_as_float(v[1].z); f[7] = __uint_as_float(v[1].w);
+      f[0] = make_float2(__uint_as_float(v[0].x), __uint_as_float(v[0].y));
+      f[1] = make_float2(__uint_as_float(v[0].z), __uint_as_float(v[0].w));
+      f[2] = make_float2(__uint_as_float(v[1].x), __uint_as_float(v[1].y));
+      f[3] = make_float2(__uint_as_float(v[1].z), __uint_as_float(v[1].w));
     } else {
-      Vec8<T>::unpack(v[0], f);
+      Pair8<T>::unpack(v[0], f);
     }
   }
 };
 
-// H: type of h, DY: of dout, DRO: of dresidual_out (NoT without one).
-template <typename H, typename DY, typename DRO, int K>
-__global__ void __launch_bounds__(kRowThreads, 1) fused_bwd_kernel(const FusedBwdParams p, const RowPlan pl) {
-  constexpr bool kDro = Present<DRO>::value;
+// H: type of h (and of dresidual), DY: of dout (and of dx), DRO: of dresidual_out, DRES: of
+// dresidual (NoT: absent).
+//   dh = rs dy w - h rs^3 mean(h dy w) (+ dresidual_out)
+// dweight and dbias are summed over a thread's rows in registers, 16 a vector step; with four
+// steps (rows of up to 16384 columns) in tensor memory, which this kernel has no other use
+// for: 16 columns of the thread's lane a step, read and written once a row. (Four steps in
+// registers leave no room for the row itself.)
+template <typename H, typename DY, typename DRO, typename DRES, int K>
+__global__ void __launch_bounds__(kBwdThreads, 1) fused_bwd_kernel(const FusedBwdParams p, const RowPlan pl) {
+  constexpr bool kDro = Present<DRO>::value, kDres = Present<DRES>::value, kTmem = K > kBwdRegSteps;
   constexpr int kStreams = kDro ? 3 : 2;
+  constexpr int kH = Vec8<H>::kBytes / 8, kDy = Vec8<DY>::kBytes / 8;
   RowCtx c = row_begin(pl, p.N);
   pdl_launch_dependents();
+  if constexpr (kTmem) {
+    if (c.warp == 0) tmem_alloc_warp(&c.bars->tmem, kTmemCols);
+  }
   pdl_wait();
   const void* src[kStreams];
   int bytes[kStreams];
   src[0] = p.h;
-  bytes[0] = Vec8<H>::kBytes / 8;
+  bytes[0] = kH;
   src[1] = p.dy;
-  bytes[1] = Vec8<DY>::kBytes / 8;
+  bytes[1] = kDy;
   if constexpr (kDro) {
     src[2] = p.dro;
     bytes[2] = Vec8<DRO>::kBytes / 8;
@@ -56,15 +70,26 @@ __global__ void __launch_bounds__(kRowThreads, 1) fused_bwd_kernel(const FusedBw
   const uint64_t policy = l2_policy_evict_first();
   if (c.gl == 0)
     for (int u = 0; u < pl.S && u < c.units; ++u) issue_unit(pl, c, u, u, p.rows, p.N, src, bytes, policy);
+  if constexpr (kTmem) tmem_fence_before_sync();
   load_affine(pl, c, p.w, p.w_dt, nullptr, 0);
+  uint32_t tmem_base = 0, sums_at = 0;  // a warp reaches the 32 lanes of its quarter: the warps of a quarter side by side
+  if constexpr (kTmem) {
+    tmem_fence_after_sync();
+    tmem_base = c.bars->tmem;
+    sums_at = tmem_base + (static_cast<uint32_t>(c.warp & 3) << 21) + static_cast<uint32_t>(c.warp >> 2) * (K * 16);
+  }
   const uint64_t offset = drop_offset(p.drop);
   const float inv_n = 1.f / static_cast<float>(p.N);
 
-  float dw[K][8], db[K][8];
+  float2 sums[kTmem ? 1 : K][8];  // dweight, then dbias, of eight columns
 #pragma unroll
-  for (int j = 0; j < K; ++j)
+  for (int j = 0; j < (kTmem ? 1 : K); ++j)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dw[j][i] = db[j][i] = 0.f;
+    for (int i = 0; i < 8; ++i) sums[j][i] = make_float2(0.f, 0.f);
+  if constexpr (kTmem) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) tmem_st16(sums_at + j * 16, sums[0]);
+  }
 
   int slot = 0;
   uint32_t phase = 0;
@@ -79,33 +104,51 @@ __global__ void __launch_bounds__(kRowThreads, 1) fused_bwd_kernel(const FusedBw
       Raw8<H> h[K];
       Raw8<DY> dy[K];
       Raw8<std::conditional_t<kDro, DRO, __half>> dro[kDro ? K : 1];
-      float s = 0.f;
+      float2 s2 = make_float2(0.f, 0.f);
+      if constexpr (kTmem) tmem_wait_st();  // of the row before
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         const int first_step = j & ~(pl.KC - 1);
-        if (r == 0 && j == first_step) mbar_wait(&c.full[slot], phase, kSiteBwdFull);
         const int col = (j * pl.G + c.gl) * 8;
+        float2(&sum)[8] = sums[kTmem ? 0 : j];
+        if constexpr (kTmem) tmem_ld16(sums_at + j * 16, sum);
+        if (r == 0 && j == first_step) mbar_wait(&c.full[slot], phase, kSiteBwdFull);
+        float2 hg[4], g[4];
         if (col < c.ncols) {
           const unsigned char* base = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;
           const int at = r * static_cast<int>(p.N) + col - first_step * pl.G * 8;
-          h[j].load(base + at * (Vec8<H>::kBytes / 8));
-          dy[j].load(base + pl.off[1] + at * (Vec8<DY>::kBytes / 8));
+          h[j].load(base + at * kH);
+          dy[j].load(base + pl.off[1] + at * kDy);
           if constexpr (kDro) dro[j].load(base + pl.off[2] + at * (Vec8<DRO>::kBytes / 8));
-          float hv[8], g[8], w[8];
-          h[j].get(hv);
+          float2 w[4];
+          h[j].get(hg);
           dy[j].get(g);
-          lds8(c.w + col, w);
+          affine8(pl, c.w, col, w);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float hg = hv[i] * g[i];
-            s = fmaf(hg, w[i], s);
-            dw[j][i] = fmaf(hg, rs, dw[j][i]);
-            db[j][i] += g[i];
+          for (int i = 0; i < 4; ++i) {
+            hg[i] = mul2(hg[i], g[i]);
+            s2 = fma2(hg[i], w[i], s2);
           }
+        } else {
+          h[j].zero();
+          dy[j].zero();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) hg[i] = g[i] = make_float2(0.f, 0.f);
         }
+        if constexpr (kTmem) {
+          __syncwarp();
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sum[i] = fma2(hg[i], splat2(rs), sum[i]);
+          sum[4 + i] = add2(g[i], sum[4 + i]);
+        }
+        if constexpr (kTmem) tmem_st16(sums_at + j * 16, sum);
         if (r == nrows - 1 && ((j + 1) & (pl.KC - 1)) == 0) {
           if (release_unit(c, slot) && unit + pl.S < c.units)
             issue_unit(pl, c, unit + pl.S, slot, p.rows, p.N, src, bytes, policy);
+          __syncwarp();
           ++unit;
           if (++slot == pl.S) {
             slot = 0;
@@ -113,68 +156,92 @@ __global__ void __launch_bounds__(kRowThreads, 1) fused_bwd_kernel(const FusedBw
           }
         }
       }
+      float s = s2.x + s2.y;
       uint32_t unused = 0;
       row_total<true, false>(pl, c, s, unused, kSiteBwdCluster);
-      const float t = rs * rs * rs * (s * inv_n);  // dh = rs dy w - h rs^3 mean(h dy w)
+      const float t = -(rs * rs * rs * (s * inv_n));
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         const int col = (j * pl.G + c.gl) * 8;
         if (col >= c.ncols) continue;
-        float hv[8], g[8], w[8], d[8];
-        h[j].get(hv);
+        float2 d[4], g[4], w[4];
+        h[j].get(d);
         dy[j].get(g);
-        lds8(c.w + col, w);
+        affine8(pl, c.w, col, w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = fma2(mul2(g[i], w[i]), splat2(rs), mul2(d[i], splat2(t)));
         if constexpr (kDro) {
-          dro[j].get(d);
+          dro[j].get(g);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) d[i] += fmaf(-hv[i], t, g[i] * w[i] * rs);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) d[i] = fmaf(-hv[i], t, g[i] * w[i] * rs);
+          for (int i = 0; i < 4; ++i) d[i] = add2(d[i], g[i]);
         }
-        if (p.dres) store8_rt(p.dres, p.dres_dt, e0 + col, d);
-        const uint32_t keep = keep8(p.drop, c.slice0 + col, row, offset);
+        if constexpr (kDres)
+          Pair8<DRES>::store(static_cast<unsigned char*>(p.dres) + (e0 + col) * (Vec8<DRES>::kBytes / 8), d);
+        float2 zero[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = keep >> i & 1u ? d[i] * p.drop.scale : 0.f;
-        store8_rt(p.dx, p.dx_dt, e0 + col, d);
+        for (int i = 0; i < 4; ++i) {
+          d[i] = mul2(d[i], splat2(p.drop.scale));
+          zero[i] = make_float2(0.f, 0.f);
+        }
+        select8(p.drop, c.slice0 + col, row, offset, d, zero, g);
+        Pair8<DY>::store(static_cast<unsigned char*>(p.dx) + (e0 + col) * kDy, g);
       }
+      if constexpr (kTmem) __syncwarp();  // together again for the next row's tensor memory accesses
     }
   }
   row_end(pl, c);
-  // The groups' sums, one partial row per cluster: through the rings (every copy has landed
-  // and been read), added in group order.
-  if (!p.dw_part && !p.db_part) return;
-  float* sums = reinterpret_cast<float*>(rmsb_dyn_smem);
+  // One partial row of dweight and of dbias per cluster. Several groups add theirs in group
+  // order through the rings, whose every copy has landed and been read.
+  if constexpr (kTmem) tmem_wait_st();
+  float* staged = reinterpret_cast<float*>(rmsb_dyn_smem);
   const int64_t part = blockIdx.x / pl.C;
+  const bool want = p.dw_part || p.db_part;
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    float* out = which == 0 ? p.dw_part : p.db_part;
-    if (!out) continue;
-    float* dst = out + part * p.N + c.slice0;
+  for (int j = 0; j < K; ++j) {
+    if (!want) break;
+    const int col = (j * pl.G + c.gl) * 8;
+    float2(&sum)[8] = sums[kTmem ? 0 : j];
+    if constexpr (kTmem) {
+      __syncwarp();
+      tmem_ld16(sums_at + j * 16, sum);
+      tmem_wait_ld();
+    }
+    const float2 dw[4] = {sum[0], sum[1], sum[2], sum[3]}, db[4] = {sum[4], sum[5], sum[6], sum[7]};
     if (pl.groups == 1) {
-#pragma unroll
-      for (int j = 0; j < K; ++j) {
-        const int col = (j * pl.G + c.gl) * 8;
-        if (col < c.ncols) Vec8<float>::store(dst + col, which == 0 ? dw[j] : db[j]);
+      if (col < c.ncols) {
+        float* dst = p.dw_part + part * p.N + c.slice0 + col;
+        if (p.dw_part) Pair8<float>::store(dst, dw);
+        dst = p.db_part + part * p.N + c.slice0 + col;
+        if (p.db_part) Pair8<float>::store(dst, db);
       }
       continue;
     }
     __syncthreads();
+    if (col < c.ncols) {
+      float2* q = reinterpret_cast<float2*>(staged + (2 * c.gid) * pl.G * 8 + c.gl * 8);
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-      const int col = (j * pl.G + c.gl) * 8;
-      if (col < c.ncols) {
-        float* q = sums + c.gid * pl.slice + col;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = which == 0 ? dw[j][i] : db[j][i];
+      for (int i = 0; i < 4; ++i) {
+        q[i] = dw[i];
+        q[pl.G * 4 + i] = db[i];
       }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < c.ncols; i += blockDim.x) {
-      float v = 0.f;
-      for (int g = 0; g < pl.groups; ++g) v += sums[g * pl.slice + i];
-      st1(&dst[i], v);
+    const int first = j * pl.G * 8;  // columns of this step
+    for (int i = threadIdx.x; i < pl.G * 8 && first + i < c.ncols; i += blockDim.x) {
+      float v = 0.f, u = 0.f;
+      for (int g = 0; g < pl.groups; ++g) {
+        v += staged[(2 * g) * pl.G * 8 + i];
+        u += staged[(2 * g + 1) * pl.G * 8 + i];
+      }
+      if (p.dw_part) st1(p.dw_part + part * p.N + c.slice0 + first + i, v);
+      if (p.db_part) st1(p.db_part + part * p.N + c.slice0 + first + i, u);
     }
+  }
+  if constexpr (kTmem) {
+    tmem_fence_before_sync();
+    __syncthreads();
+    tmem_fence_after_sync();
+    if (c.warp == 0) tmem_dealloc_warp(tmem_base, kTmemCols);
   }
 }
 

@@ -80,10 +80,23 @@ __device__ __forceinline__ bool keep1(const DropParams& d, int64_t col, int64_t 
 }
 
 // ---------------------------------------------------------------------------------------
-// 8-bit values. The largest magnitude of a group travels as the bits of |y|: as unsigned
-// integers these order every magnitude below infinity and infinity below NaN, so a NaN
-// reaches the scale (a floating maximum would lose it).
+// 8-bit values. The largest magnitude of a group is found with sm_100's three-input maximum
+// of absolute values, in the form that keeps NaN; across lanes and warps it travels as its
+// bits, which order as unsigned integers: below infinity, infinity below NaN.
 // ---------------------------------------------------------------------------------------
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+__device__ __forceinline__ float largest8(float most, const float2 (&y)[4]) {
+  most = max3_abs(most, y[0].x, y[0].y);
+  most = max3_abs(most, y[1].x, y[1].y);
+  most = max3_abs(most, y[2].x, y[2].y);
+  return max3_abs(most, y[3].x, y[3].y);
+}
+
 __device__ __forceinline__ uint32_t magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
 
 // scale = max(largest / Q, 2^-126), NaN kept: the floor keeps 1 / scale finite where the
@@ -93,22 +106,39 @@ __device__ __forceinline__ float scale_of(float largest, float inv_q) {
   return s < 1.17549435e-38f ? 1.17549435e-38f : s;
 }
 
-constexpr float kInvE4M3 = 1.f / 448.f;
-constexpr float kInvI8 = 1.f / 127.f;
-
-__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+// 1 / scale to the last place or the one before: a q that lies between two of its values
+// within that error may take either.
+__device__ __forceinline__ float inverse(float scale) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));
+  return r;
 }
 
-// Round to nearest even, held within +-127 (NaN gives 0: its scale is NaN).
-__device__ __forceinline__ uint32_t to_i8(float v) {
-  const int i = __float2int_rn(fminf(fmaxf(v, -127.f), 127.f));
-  return static_cast<uint32_t>(v == v ? i : 0) & 0xffu;
+// The 8-bit types. largest * inverse(scale) is Q within two places, so an int8 never rounds to
+// -128; e4m3 saturates. NaN becomes e4m3's NaN, or int8's 0 (its scale is NaN).
+struct E4M3 {
+  static constexpr float kInvQ = 1.f / 448.f;
+  __device__ __forceinline__ static uint32_t pack4(float2 a, float2 b) {
+    return __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
+           static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3)) << 16;
+  }
+};
+struct I8 {
+  static constexpr float kInvQ = 1.f / 127.f;
+  __device__ __forceinline__ static uint32_t pack4(float2 a, float2 b) {
+    const uint32_t lo = __byte_perm(__float2int_rn(a.x), __float2int_rn(a.y), 0x0040);
+    const uint32_t hi = __byte_perm(__float2int_rn(b.x), __float2int_rn(b.y), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+  }
+};
+
+__device__ __forceinline__ uint8_t q1(int dt, float v) {
+  const float2 p = make_float2(v, 0.f);
+  return static_cast<uint8_t>(dt == RMSNORM_B200_I8 ? I8::pack4(p, p) : E4M3::pack4(p, p));
 }
 
 __device__ __forceinline__ void store1_q(void* base, int dt, int64_t e, float v) {
-  const uint32_t q = dt == RMSNORM_B200_I8 ? to_i8(v) : (to_e4m3x2(v, 0.f) & 0xffu);
-  st1(static_cast<uint8_t*>(base) + e, static_cast<uint8_t>(q));
+  st1(static_cast<uint8_t*>(base) + e, q1(dt, v));
 }
 
 }  // namespace rmsb200

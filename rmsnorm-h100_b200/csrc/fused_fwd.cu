@@ -12,27 +12,60 @@ namespace {
 using FwdKernel = void (*)(const FusedFwdParams, const RowPlan);
 constexpr int kNone = -1;
 
-template <typename X, typename RT>
-FwdKernel pick_steps(int k, bool drop) {
+// What a row ends as: dropout, or an 8-bit type with one scale per row or per group.
+enum End { kDropped, kE4M3Row, kE4M3Group, kI8Row, kI8Group };
+
+template <typename X, typename RT, typename ROT, typename E>
+FwdKernel pick_steps(int k) {
   switch (k) {
-    case 1: return drop ? fused_fwd_kernel<X, RT, 1, true> : fused_fwd_kernel<X, RT, 1, false>;
-    case 2: return drop ? fused_fwd_kernel<X, RT, 2, true> : fused_fwd_kernel<X, RT, 2, false>;
-    default: return drop ? fused_fwd_kernel<X, RT, 4, true> : fused_fwd_kernel<X, RT, 4, false>;
+    case 1: return fused_fwd_kernel<X, RT, ROT, E, 1>;
+    case 2: return fused_fwd_kernel<X, RT, ROT, E, 2>;
+    default: return fused_fwd_kernel<X, RT, ROT, E, 4>;
   }
 }
 
-FwdKernel pick(int x, int res, int k, bool drop) {
+template <typename X, typename RT, typename ROT>
+FwdKernel pick_quant(int end, int k) {
+  switch (end) {
+    case kE4M3Row: return pick_steps<X, RT, ROT, Scaled<E4M3, true>>(k);
+    case kE4M3Group: return pick_steps<X, RT, ROT, Scaled<E4M3, false>>(k);
+    case kI8Row: return pick_steps<X, RT, ROT, Scaled<I8, true>>(k);
+    case kI8Group: return pick_steps<X, RT, ROT, Scaled<I8, false>>(k);
+    default: return nullptr;
+  }
+}
+
+// Types of x, residual and residual_out: the residual stream in x's type, in fp32, or turned
+// from x's type into fp32. The output of dropout has x's type.
+FwdKernel pick(int x, int res, int ro, int end, int k) {
   constexpr int H = RMSNORM_B200_F16, B = RMSNORM_B200_BF16, F = RMSNORM_B200_F32;
   using h16 = __half;
   using b16 = __nv_bfloat16;
-  if (x == B && res == kNone) return pick_steps<b16, NoT>(k, drop);
-  if (x == H && res == kNone) return pick_steps<h16, NoT>(k, drop);
-  if (x == F && res == kNone) return pick_steps<float, NoT>(k, drop);
-  if (x == B && res == B) return pick_steps<b16, b16>(k, drop);
-  if (x == H && res == H) return pick_steps<h16, h16>(k, drop);
-  if (x == F && res == F) return pick_steps<float, float>(k, drop);
-  if (x == B && res == F) return pick_steps<b16, float>(k, drop);
-  if (x == H && res == F) return pick_steps<h16, float>(k, drop);
+#define RMSB_FUSED(XC, RC, ROC, X, RT, ROT)  \
+  if (x == XC && res == RC && ro == ROC)     \
+    return end == kDropped ? pick_steps<X, RT, ROT, Dropped>(k) : pick_quant<X, RT, ROT>(end, k);
+#define RMSB_QUANT(XC, X) \
+  if (x == XC && res == kNone && ro == kNone) return pick_quant<X, NoT, NoT>(end, k);
+#define RMSB_DROP(XC, ROC, X, ROT) \
+  if (x == XC && res == kNone && ro == ROC && end == kDropped) return pick_steps<X, NoT, ROT, Dropped>(k);
+  RMSB_FUSED(B, B, B, b16, b16, b16)
+  RMSB_FUSED(H, H, H, h16, h16, h16)
+  RMSB_FUSED(F, F, F, float, float, float)
+  RMSB_FUSED(B, B, F, b16, b16, float)
+  RMSB_FUSED(H, H, F, h16, h16, float)
+  RMSB_FUSED(B, F, F, b16, float, float)
+  RMSB_FUSED(H, F, F, h16, float, float)
+  RMSB_QUANT(B, b16)
+  RMSB_QUANT(H, h16)
+  RMSB_QUANT(F, float)
+  RMSB_DROP(B, B, b16, b16)
+  RMSB_DROP(H, H, h16, h16)
+  RMSB_DROP(F, F, float, float)
+  RMSB_DROP(B, F, b16, float)
+  RMSB_DROP(H, F, h16, float)
+#undef RMSB_FUSED
+#undef RMSB_QUANT
+#undef RMSB_DROP
   return nullptr;
 }
 
@@ -73,9 +106,13 @@ int run(const FusedFwdParams& p, bool drop, cudaStream_t stream) {
     const int bytes[3] = {elem_bytes(p.x_dt), p.res ? elem_bytes(p.res_dt) : 0, 0};
     RowPlan pl;
     int k = 0, smem = 0;
-    why = plan_rows(p.rows, p.N, bytes, p.b != nullptr, kRowMaxVecs, ud->sm_count, &pl, &k, &smem);
-    if (!why) {
-      FwdKernel kernel = pick(p.x_dt, p.res ? p.res_dt : kNone, k, drop);
+    const bool few = p.rows <= ud->sm_count && p.N <= kFwdFewThreads * 8;
+    why = plan_rows(p.rows, p.N, bytes, p.b != nullptr, few ? kFwdFewThreads : kFwdThreads, few ? 1 : kFwdSteps,
+                    ud->sm_count, &pl, &k, &smem);
+    if (!why && (!drop || p.out_dt == p.x_dt)) {
+      const bool i8 = p.out_dt == RMSNORM_B200_I8;
+      const int end = drop ? kDropped : p.group ? (i8 ? kI8Group : kE4M3Group) : (i8 ? kI8Row : kE4M3Row);
+      FwdKernel kernel = pick(p.x_dt, p.res ? p.res_dt : kNone, p.ro ? p.ro_dt : kNone, end, k);
       if (kernel) {
         st = launch_rows(ud, kernel, p, pl, smem, stream, drop ? "dropout_fwd" : "quant_fwd", k);
         if (st != RMSNORM_B200_ERR_UNSUPPORTED) return st;
@@ -83,6 +120,8 @@ int run(const FusedFwdParams& p, bool drop, cudaStream_t stream) {
       } else {
         why = "dtype combination";
       }
+    } else if (!why) {
+      why = "dtype combination";
     }
   }
   return launch_generic(p, drop, ud, stream, why);
@@ -116,6 +155,7 @@ extern "C" int rmsnorm_b200_quant_fwd(const rmsnorm_b200_quant_args* a, void* st
   p.x_dt = a->x_dtype; p.res_dt = a->residual_dtype; p.w_dt = a->weight_dtype; p.b_dt = a->bias_dtype;
   p.out_dt = a->q_dtype; p.ro_dt = a->residual_out_dtype;
   p.group = a->group; p.eps = a->eps;
+  while (p.group >> p.group_shift > 1) ++p.group_shift;
   return run(p, false, static_cast<cudaStream_t>(stream));
 }
 

@@ -6,19 +6,39 @@
 
 namespace rmsb200 {
 
-// RT is NoT without a residual. kDrop: dropout, floating output; otherwise an 8-bit output.
-template <typename X, typename RT, int K, bool kDrop>
-__global__ void __launch_bounds__(kRowThreads, 1) fused_fwd_kernel(const FusedFwdParams p, const RowPlan pl) {
-  constexpr bool kRes = Present<RT>::value;
-  constexpr bool kQuant = !kDrop;
+// Vector steps a thread at most, and threads of a CTA. Four steps in 512 threads (128 registers
+// each) beat two in 1024 for many rows: 8192 x 4096 bf16 + residual with 8-bit groups 43.8
+// against 50.0 us, dropout 32768 x 4096 234 against 269 us. Few rows, a CTA each, take single
+// steps in up to 1024 threads: 64 x 8192 5.7 against 6.7 us.
+constexpr int kFwdSteps = 4;
+constexpr int kFwdThreads = 512;
+constexpr int kFwdFewThreads = 1024;
+
+// What a row ends as.
+struct Dropped {  // dropout; a floating output of x's type
+  static constexpr bool kQuant = false, kRowScale = false;
+};
+template <typename Q, bool kRow>
+struct Scaled {  // 8-bit values Q; one scale per row, or one per group of columns
+  static constexpr bool kQuant = true, kRowScale = kRow;
+  using Type = Q;
+};
+
+// X, RT, ROT: types of x, of the residual and of residual_out (NoT: absent).
+// Per element 5 (8-bit) to 12 (dropout) bytes cross HBM, which bounds the kernel.
+template <typename X, typename RT, typename ROT, typename End, int K>
+__global__ void __launch_bounds__(K == 1 ? kFwdFewThreads : kFwdThreads, 1) fused_fwd_kernel(const FusedFwdParams p, const RowPlan pl) {
+  constexpr bool kRes = Present<RT>::value, kRo = Present<ROT>::value;
+  constexpr bool kQuant = End::kQuant, kRowScale = End::kRowScale;
   constexpr int kStreams = kRes ? 2 : 1;
+  constexpr int kX = Vec8<X>::kBytes / 8;
   RowCtx c = row_begin(pl, p.N);
   pdl_launch_dependents();
   pdl_wait();
   const void* src[kStreams];
   int bytes[kStreams];
   src[0] = p.x;
-  bytes[0] = Vec8<X>::kBytes / 8;
+  bytes[0] = kX;
   if constexpr (kRes) {
     src[1] = p.res;
     bytes[1] = Vec8<RT>::kBytes / 8;
@@ -27,12 +47,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) fused_fwd_kernel(const FusedFw
   if (c.gl == 0)
     for (int u = 0; u < pl.S && u < c.units; ++u) issue_unit(pl, c, u, u, p.rows, p.N, src, bytes, policy);
   load_affine(pl, c, p.w, p.w_dt, p.b, p.b_dt);
-  const uint64_t offset = kDrop ? drop_offset(p.drop) : 0ull;
+  const uint64_t offset = kQuant ? 0ull : drop_offset(p.drop);
   const float inv_n = 1.f / static_cast<float>(p.N);
-  const bool i8 = p.out_dt == RMSNORM_B200_I8;
-  const float inv_q = i8 ? kInvI8 : kInvE4M3;
-  const bool row_scale = kQuant && p.group == 0;
-  const int scale_shift = kQuant && p.group ? 31 - __clz(p.group) : 0;
 
   int slot = 0;
   uint32_t phase = 0;
@@ -43,9 +59,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) fused_fwd_kernel(const FusedFw
     for (int r = 0; r < nrows; ++r) {
       const int64_t row = row0 + r;
       const int64_t e0 = row * p.N + c.slice0;
-      float h[K][8];
-      float ss = 0.f;
-      uint32_t most = 0;
+      float2 h[K][4];  // h; with a row's scale and no bias, h w
+      float2 ss = make_float2(0.f, 0.f);
+      float most = 0.f;
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         const int first_step = j & ~(pl.KC - 1);  // of this unit
@@ -54,33 +70,35 @@ __global__ void __launch_bounds__(kRowThreads, 1) fused_fwd_kernel(const FusedFw
         if (col < c.ncols) {
           const unsigned char* base = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;
           const int at = r * static_cast<int>(p.N) + col - first_step * pl.G * 8;
-          Vec8<X>::load(base + at * (Vec8<X>::kBytes / 8), h[j]);
-          float res[8];
-          if constexpr (kRes) Vec8<RT>::load(base + pl.off[1] + at * (Vec8<RT>::kBytes / 8), res);
-          if constexpr (kDrop) {
-            const uint32_t keep = keep8(p.drop, c.slice0 + col, row, offset);
+          Pair8<X>::load(base + at * kX, h[j]);
+          float2 res[4];
+          if constexpr (kRes) Pair8<RT>::load(base + pl.off[1] + at * (Vec8<RT>::kBytes / 8), res);
+          if constexpr (!kQuant) {
+            if constexpr (!kRes)
+              for (float2& v : res) v = make_float2(0.f, 0.f);
+            float2 kept[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float base_v = kRes ? res[i] : 0.f;
-              h[j][i] = keep >> i & 1u ? fmaf(h[j][i], p.drop.scale, base_v) : base_v;
-            }
+            for (int i = 0; i < 4; ++i) kept[i] = fma2(h[j][i], splat2(p.drop.scale), res[i]);
+            select8(p.drop, c.slice0 + col, row, offset, kept, res, h[j]);
           } else if constexpr (kRes) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[j][i] += res[i];
+            for (int i = 0; i < 4; ++i) h[j][i] = add2(h[j][i], res[i]);
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) ss = fmaf(h[j][i], h[j][i], ss);
-          if (p.ro) store8_rt(p.ro, p.ro_dt, e0 + col, h[j]);
-          if (row_scale && !pl.bias) {
+          for (int i = 0; i < 4; ++i) ss = fma2(h[j][i], h[j][i], ss);
+          if constexpr (kRo)
+            Pair8<ROT>::store(static_cast<unsigned char*>(p.ro) + (e0 + col) * (Vec8<ROT>::kBytes / 8), h[j]);
+          if (kRowScale && !pl.bias) {
             // max |y| = rstd * max |h w|: found along with the sum, one exchange for both
-            float w[8];
-            lds8(c.w + col, w);
+            float2 w[4];
+            affine8(pl, c.w, col, w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) most = max(most, magnitude(h[j][i] * w[i]));
+            for (int i = 0; i < 4; ++i) h[j][i] = mul2(h[j][i], w[i]);
+            most = largest8(most, h[j]);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) h[j][i] = 0.f;
+          for (int i = 0; i < 4; ++i) h[j][i] = make_float2(0.f, 0.f);
         }
         if (r == nrows - 1 && ((j + 1) & (pl.KC - 1)) == 0) {
           if (release_unit(c, slot) && unit + pl.S < c.units)
@@ -92,99 +110,80 @@ __global__ void __launch_bounds__(kRowThreads, 1) fused_fwd_kernel(const FusedFw
           }
         }
       }
-      if (row_scale && !pl.bias)
-        row_total<true, true>(pl, c, ss, most, kSiteFwdCluster);
+      float sum = ss.x + ss.y;
+      uint32_t bits = magnitude(most);
+      if (kRowScale && !pl.bias)
+        row_total<true, true>(pl, c, sum, bits, kSiteFwdCluster);
       else
-        row_total<true, false>(pl, c, ss, most, kSiteFwdCluster);
-      const float rs = rsqrtf(ss * inv_n + p.eps);
+        row_total<true, false>(pl, c, sum, bits, kSiteFwdCluster);
+      const float rs = rsqrtf(sum * inv_n + p.eps);
       if (p.rstd && c.gl == 0 && c.rank == 0) st1(&p.rstd[row], rs);
-      float inv = 1.f;     // of the row's scale: kept apart from rs, their product may overflow
-      if (row_scale) {
-        float largest;
-        if (!pl.bias) {
-          largest = __uint_as_float(most) * rs;
-        } else {
-#pragma unroll
-          for (int j = 0; j < K; ++j) {
-            const int col = (j * pl.G + c.gl) * 8;
-            if (col < c.ncols) {
-              float w[8], b[8];
-              lds8(c.w + col, w);
-              lds8(c.b + col, b);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                h[j][i] = fmaf(h[j][i] * rs, w[i], b[i]);
-                most = max(most, magnitude(h[j][i]));
-              }
-            }
-          }
-          float unused = 0.f;
-          row_total<false, true>(pl, c, unused, most, kSiteFwdCluster);
-          largest = __uint_as_float(most);
-        }
-        const float s = scale_of(largest, inv_q);
-        if (c.gl == 0 && c.rank == 0) st1(&p.scales[row * p.scale_row], s);
-        inv = 1.f / s;
-      }
+      // y in the place of h
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         const int col = (j * pl.G + c.gl) * 8;
-        const bool in = col < c.ncols;
-        if (!__any_sync(0xffffffffu, in)) continue;
-        float y[8];
-        if (row_scale && pl.bias) {
+        if (col >= c.ncols) continue;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = h[j][i] * inv;
+        for (int i = 0; i < 4; ++i) h[j][i] = mul2(h[j][i], splat2(rs));
+        if (kRowScale && !pl.bias) continue;
+        float2 w[4];
+        affine8(pl, c.w, col, w);
+        if (pl.bias) {
+          float2 b[4];
+          affine8(pl, c.b, col, b);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) h[j][i] = fma2(h[j][i], w[i], b[i]);
         } else {
-          float w[8];
-          if (in) {
-            lds8(c.w + col, w);
-          } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = 0.f;
+          for (int i = 0; i < 4; ++i) h[j][i] = mul2(h[j][i], w[i]);
+        }
+        if constexpr (!kQuant)
+          Pair8<X>::store(static_cast<unsigned char*>(p.out) + (e0 + col) * kX, h[j]);
+      }
+      if constexpr (kQuant) {
+        using Q = typename End::Type;
+        float inv[K];
+        if constexpr (kRowScale) {
+          float largest = __uint_as_float(bits) * rs;
+          if (pl.bias) {
+            most = 0.f;
+#pragma unroll
+            for (int j = 0; j < K; ++j) most = largest8(most, h[j]);
+            bits = magnitude(most);
+            float unused = 0.f;
+            row_total<false, true>(pl, c, unused, bits, kSiteFwdCluster);
+            largest = __uint_as_float(bits);
           }
-          if (row_scale) {
+          const float s = scale_of(largest, Q::kInvQ);
+          if (c.gl == 0 && c.rank == 0) st1(&p.scales[row * p.scale_row], s);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = (h[j][i] * w[i]) * rs * inv;
-          } else {
+          for (int j = 0; j < K; ++j) inv[j] = inverse(s);
+        } else {  // a scale's columns lie in 4, 8, 16 or 32 neighbouring lanes
+          float m[K];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = (h[j][i] * rs) * w[i];
-            if (pl.bias && in) {
-              float b[8];
-              lds8(c.b + col, b);
+          for (int j = 0; j < K; ++j) m[j] = largest8(0.f, h[j]);
+          for (int o = p.group >> 4; o > 0; o >>= 1) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) y[i] = fmaf(h[j][i] * rs, w[i], b[i]);
-            }
+            for (int j = 0; j < K; ++j) m[j] = max3_abs(m[j], __shfl_xor_sync(0xffffffffu, m[j], o), 0.f);
+          }
+#pragma unroll
+          for (int j = 0; j < K; ++j) {
+            const int col = (j * pl.G + c.gl) * 8;
+            const float s = scale_of(m[j], Q::kInvQ);
+            inv[j] = inverse(s);
+            if (col < c.ncols && (col & (p.group - 1)) == 0)  // slices begin at whole groups
+              st1(&p.scales[row * p.scale_row + ((c.slice0 + col) >> p.group_shift) * p.scale_group], s);
           }
         }
-        if constexpr (kQuant) {
-          if (!row_scale) {  // a scale's columns lie in 4, 8, 16 or 32 neighbouring lanes
-            uint32_t m = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = max(m, magnitude(y[i]));
-            for (int o = p.group >> 4; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float s = scale_of(__uint_as_float(m), inv_q);
-            const float inv_g = 1.f / s;
+        for (int j = 0; j < K; ++j) {
+          const int col = (j * pl.G + c.gl) * 8;
+          if (col >= c.ncols) continue;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] *= inv_g;
-            const int64_t gcol = c.slice0 + col;
-            if (in && (gcol & (p.group - 1)) == 0)
-              st1(&p.scales[row * p.scale_row + (gcol >> scale_shift) * p.scale_group], s);
-          }
-          if (in) {
-            uint2 q;
-            if (i8) {
-              q.x = to_i8(y[0]) | to_i8(y[1]) << 8 | to_i8(y[2]) << 16 | to_i8(y[3]) << 24;
-              q.y = to_i8(y[4]) | to_i8(y[5]) << 8 | to_i8(y[6]) << 16 | to_i8(y[7]) << 24;
-            } else {
-              q.x = to_e4m3x2(y[0], y[1]) | to_e4m3x2(y[2], y[3]) << 16;
-              q.y = to_e4m3x2(y[4], y[5]) | to_e4m3x2(y[6], y[7]) << 16;
-            }
-            uint2* dst = reinterpret_cast<uint2*>(static_cast<unsigned char*>(p.out) + e0 + col);
-            if (RMSB_DBG_OK(dst, 8, kDbgVecStore)) __stcs(dst, q);
-          }
-        } else if (in) {
-          store8_rt(p.out, p.out_dt, e0 + col, y);
+          for (int i = 0; i < 4; ++i) h[j][i] = mul2(h[j][i], splat2(inv[j]));
+          uint2* dst = reinterpret_cast<uint2*>(static_cast<unsigned char*>(p.out) + e0 + col);
+          if (RMSB_DBG_OK(dst, 8, kDbgVecStore))
+            __stcs(dst, make_uint2(Q::pack4(h[j][0], h[j][1]), Q::pack4(h[j][2], h[j][3])));
         }
       }
     }

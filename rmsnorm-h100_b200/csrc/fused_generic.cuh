@@ -22,6 +22,7 @@ struct FusedFwdParams {
   int64_t scale_row, scale_group;
   int32_t x_dt, res_dt, w_dt, b_dt, out_dt, ro_dt;
   int32_t group;    // columns per scale (0 = the row)
+  int32_t group_shift;  // its logarithm
   float eps;
   DropParams drop;
 };
@@ -59,7 +60,7 @@ __global__ void __launch_bounds__(kGenericThreads) fused_fwd_generic_kernel(cons
   const int64_t N = p.N;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool i8 = p.out_dt == RMSNORM_B200_I8;
-  const float inv_q = i8 ? kInvI8 : kInvE4M3;
+  const float inv_q = i8 ? I8::kInvQ : E4M3::kInvQ;
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
     float acc = 0.f;
     for (int64_t n = threadIdx.x; n < N; n += blockDim.x) {
@@ -84,7 +85,7 @@ __global__ void __launch_bounds__(kGenericThreads) fused_fwd_generic_kernel(cons
         for (int64_t n = g * p.group + lane; n < end; n += 32) most = max(most, magnitude(y(n)));
         const float s = scale_of(__uint_as_float(__reduce_max_sync(0xffffffffu, most)), inv_q);
         if (lane == 0) st1(&p.scales[r * p.scale_row + g * p.scale_group], s);
-        for (int64_t n = g * p.group + lane; n < end; n += 32) store1_q(p.out, p.out_dt, r * N + n, y(n) * (1.f / s));
+        for (int64_t n = g * p.group + lane; n < end; n += 32) store1_q(p.out, p.out_dt, r * N + n, y(n) * inverse(s));
       }
     } else {
       uint32_t most = 0;
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(kGenericThreads) fused_fwd_generic_kernel(cons
       __syncthreads();
       const float s = scale_of(__uint_as_float(most), inv_q);
       if (threadIdx.x == 0) st1(&p.scales[r * p.scale_row], s);
-      for (int64_t n = threadIdx.x; n < N; n += blockDim.x) store1_q(p.out, p.out_dt, r * N + n, y(n) * (1.f / s));
+      for (int64_t n = threadIdx.x; n < N; n += blockDim.x) store1_q(p.out, p.out_dt, r * N + n, y(n) * inverse(s));
     }
   }
 }

@@ -15,10 +15,10 @@ inline int pow2_ceil(int64_t v) {
 }
 
 // Plans rows of N columns (a multiple of 8) whose tensors have elements of bytes[i] (0: absent).
-// max_steps: vector steps a thread can hold. Returns why there is no plan, or null.
-inline const char* plan_rows(int64_t rows, int64_t N, const int (&bytes)[3], bool bias, int max_steps, int sms,
-                             RowPlan* pl, int* k, int* smem) {
-  const int64_t cta_cols = static_cast<int64_t>(kRowThreads) * 8 * max_steps;
+// threads of a CTA, max_steps: vector steps a thread can hold. Returns why there is no plan, or null.
+inline const char* plan_rows(int64_t rows, int64_t N, const int (&bytes)[3], bool bias, int threads, int max_steps,
+                             int sms, RowPlan* pl, int* k, int* smem) {
+  const int64_t cta_cols = static_cast<int64_t>(threads) * 8 * max_steps;
   if (N > cta_cols * kMaxRowCtas) return "rows wider than a cluster holds";
   pl->C = N > cta_cols ? pow2_ceil((N + cta_cols - 1) / cta_cols) : 1;
   pl->slice = static_cast<int>(N);
@@ -30,9 +30,10 @@ inline const char* plan_rows(int64_t rows, int64_t N, const int (&bytes)[3], boo
   // Few rows: as many threads to a row as it has vectors, for the latency. Otherwise as few as
   // hold it, so that a CTA works on several rows at once and their totals overlap.
   const int steps = rows <= sms ? 1 : max_steps;
-  pl->G = std::clamp(pow2_ceil((vecs + steps - 1) / steps), 32, kRowThreads);
+  pl->G = std::clamp(pow2_ceil((vecs + steps - 1) / steps), 32, threads);
+  if (pl->G > 32 && threads / pl->G > 15) pl->G *= 2;  // a named barrier per group: 15 beside barrier 0
   *k = pow2_ceil((vecs + pl->G - 1) / pl->G);
-  pl->groups = pl->C > 1 ? 1 : kRowThreads / pl->G;
+  pl->groups = pl->C > 1 ? 1 : threads / pl->G;
   const int elem = bytes[0] + bytes[1] + bytes[2];
   pl->KC = *k;
   while (pl->KC > 1 && pl->KC * pl->G * 8 * elem > 32768) pl->KC >>= 1;

@@ -1,7 +1,7 @@
 // row_ring.cuh -- the skeleton of the fused row kernels: persistent row groups that stream
 // their rows through shared-memory rings, row totals within a group and across a cluster.
 //
-//   * A CTA of up to 512 threads holds `groups` row groups of G threads. A group owns a ring
+//   * A CTA of 512 or 1024 threads holds `groups` row groups of G threads. A group owns a ring
 //     of S units of its own and drifts freely: nothing but the total of a row ties its warps
 //     together, and nothing ties the groups of a CTA.
 //   * A unit is R whole rows, or KC of a row's K vector steps where a row would fill the
@@ -11,7 +11,9 @@
 //   * A vector step is 8 consecutive columns a thread, G threads side by side.
 //   * A row wider than a CTA holds is split over the C CTAs of a cluster; their totals go
 //     through distributed shared memory.
-//   * weight and bias are kept in shared memory in fp32, read once a kernel.
+//   * weight and bias are kept in shared memory in fp32, read once a kernel: the first and the
+//     last four columns of a vector in an array each, so that neighbouring lanes read
+//     neighbouring 16 bytes.
 // Every wait is bounded (device_common.cuh).
 #pragma once
 
@@ -19,11 +21,9 @@
 
 namespace rmsb200 {
 
-constexpr int kRowThreads = 512;
-constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kRowWarps = 32;     // of a CTA, at most
 constexpr int kMaxUnits = 128;    // ring units of a CTA
 constexpr int kMaxRowCtas = 16;   // CTAs of a cluster
-constexpr int kRowMaxVecs = 4;    // vector steps a thread
 constexpr int kScaleAlign = 256;  // slices are multiples of it, so that no group of a scale is split
 
 struct RowPlan {
@@ -43,6 +43,7 @@ struct RowBars {
   int done[kMaxUnits];
   float xpart[2][kMaxRowCtas][2];
   float red[2][kRowWarps][2];
+  uint32_t tmem;  // address of the CTA's tensor memory (backward)
 };
 
 struct RowCtx {
@@ -106,10 +107,19 @@ __device__ __forceinline__ void load_affine(const RowPlan& pl, const RowCtx& c, 
                                             int b_dt) {
   for (int i = threadIdx.x; i < pl.slice; i += blockDim.x) {
     const bool in = i < c.ncols;
-    c.w[i] = in ? (w ? load1_rt(w, w_dt, c.slice0 + i) : 1.f) : 0.f;
-    if (pl.bias) c.b[i] = in ? load1_rt(b, b_dt, c.slice0 + i) : 0.f;
+    const int at = (i & 4 ? pl.slice / 2 : 0) + (i >> 3) * 4 + (i & 3);
+    c.w[at] = in ? (w ? load1_rt(w, w_dt, c.slice0 + i) : 1.f) : 0.f;
+    if (pl.bias) c.b[at] = in ? load1_rt(b, b_dt, c.slice0 + i) : 0.f;
   }
   __syncthreads();
+}
+
+// Columns col .. col + 7 of an affine array (col a multiple of 8).
+__device__ __forceinline__ void affine8(const RowPlan& pl, const float* a, int col, float2 (&v)[4]) {
+  const float4 lo = reinterpret_cast<const float4*>(a)[col >> 3];
+  const float4 hi = reinterpret_cast<const float4*>(a + pl.slice / 2)[col >> 3];
+  v[0] = make_float2(lo.x, lo.y); v[1] = make_float2(lo.z, lo.w);
+  v[2] = make_float2(hi.x, hi.y); v[3] = make_float2(hi.z, hi.w);
 }
 
 // Copies unit u of this group into its slot: kStreams tensors with elements of bytes[i].
@@ -207,17 +217,19 @@ __device__ __forceinline__ void row_end(const RowPlan& pl, const RowCtx& c) {
   if (pl.C > 1) cluster_sync_all();
 }
 
-// The eight columns' keep decisions of a vector (columns col .. col + 7, col a multiple of 8).
-__device__ __forceinline__ uint32_t keep8(const DropParams& d, int64_t col, int64_t row, uint64_t offset) {
-  uint32_t a[4], b[4], bits = 0;
+// Columns col .. col + 7 (col a multiple of 8): kept values of `a`, `b` elsewhere.
+__device__ __forceinline__ void select8(const DropParams& d, int64_t col, int64_t row, uint64_t offset,
+                                        const float2 (&a)[4], const float2 (&b)[4], float2 (&v)[4]) {
   const uint32_t quad = static_cast<uint32_t>(col >> 2), mrow = static_cast<uint32_t>(d.row0 + row);
-  philox(d, quad, mrow, offset, a);
-  philox(d, quad + 1, mrow, offset, b);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bits |= (a[i] >= d.least ? 1u << i : 0u) | (b[i] >= d.least ? 16u << i : 0u);
-  return bits;
+  for (int i = 0; i < 2; ++i) {
+    uint32_t w[4];
+    philox(d, quad + i, mrow, offset, w);
+    v[2 * i].x = w[0] >= d.least ? a[2 * i].x : b[2 * i].x;
+    v[2 * i].y = w[1] >= d.least ? a[2 * i].y : b[2 * i].y;
+    v[2 * i + 1].x = w[2] >= d.least ? a[2 * i + 1].x : b[2 * i + 1].x;
+    v[2 * i + 1].y = w[3] >= d.least ? a[2 * i + 1].y : b[2 * i + 1].y;
+  }
 }
-
-__device__ __forceinline__ void lds8(const float* p, float (&v)[8]) { Vec8<float>::load(p, v); }
 
 }  // namespace rmsb200
