@@ -3,6 +3,7 @@
 #include "unit_state.cuh"
 
 #include "fused_bwd_kernels.cuh"
+#include "odd_kernels.cuh"
 #include "row_plan.h"
 
 namespace rmsb200 {
@@ -16,6 +17,7 @@ struct Plan {
   BwdKernel kernel = nullptr;
   RowPlan rows;
   int k = 0, smem = 0;
+  const char* kind = "";
   const char* why = nullptr;  // why the generic path is taken
 };
 
@@ -65,24 +67,31 @@ int check(const rmsnorm_b200_dropout_bwd_args* a) {
 }
 
 int make_plan(UnitDevice* ud, const rmsnorm_b200_dropout_bwd_args* a, Plan* pl) {
+  // Whole aligned vectors in a combination of types with a kernel of its own; else the odd
+  // rows' kernels; else (rows wider than a cluster holds) the generic ones.
+  const int bytes[3] = {elem_bytes(a->h_dtype), elem_bytes(a->dout_dtype),
+                        a->dresidual_out ? elem_bytes(a->dresidual_out_dtype) : 0};
   const void* ptrs[] = {a->h, a->dout, a->dresidual_out, a->dx, a->dresidual};
-  pl->why = a->hidden % 8 ? "hidden % 8" : nullptr;
-  for (const void* ptr : ptrs)
-    if (!aligned_to(ptr, 16)) pl->why = "unaligned pointer";
-  if (!pl->why) {
-    const int bytes[3] = {elem_bytes(a->h_dtype), elem_bytes(a->dout_dtype),
-                          a->dresidual_out ? elem_bytes(a->dresidual_out_dtype) : 0};
-    const int64_t in_registers = kBwdThreads * 8 * kBwdRegSteps;
-    const int steps = a->h_dtype == RMSNORM_B200_F32 || a->hidden <= in_registers ? kBwdRegSteps : kBwdTmemSteps;
-    pl->why = plan_rows(a->rows, a->hidden, bytes, false, kBwdThreads, steps, ud->sm_count, &pl->rows, &pl->k, &pl->smem);
-  }
-  if (!pl->why) {
-    pl->kernel = pick(a, pl->k);
-    if (!pl->kernel) pl->why = "dtype combination";
-  }
-  if (pl->kernel) {
+  bool vectors = a->hidden % 8 == 0;
+  for (const void* ptr : ptrs) vectors = vectors && aligned_to(ptr, 16);
+  for (const bool odd : {false, true}) {
+    if (!odd && !vectors) continue;
+    if (odd) {
+      pl->why = plan_rows(a->rows, a->hidden, bytes, false, kOddThreads, kOddBwdSteps, ud->sm_count, &pl->rows, &pl->k,
+                          &pl->smem, true);
+      pl->kernel = pl->k == 1 ? odd_bwd_kernel<1> : odd_bwd_kernel<2>;
+    } else {
+      const int64_t in_registers = kBwdThreads * 8 * kBwdRegSteps;
+      const int steps = a->h_dtype == RMSNORM_B200_F32 || a->hidden <= in_registers ? kBwdRegSteps : kBwdTmemSteps;
+      pl->why = plan_rows(a->rows, a->hidden, bytes, false, kBwdThreads, steps, ud->sm_count, &pl->rows, &pl->k,
+                          &pl->smem);
+      pl->kernel = pl->why ? nullptr : pick(a, pl->k);
+    }
+    if (pl->why) pl->kernel = nullptr;
+    if (!pl->kernel) continue;
+    pl->kind = odd ? "dropout_bwd_odd" : "dropout_bwd";
     // the groups' sums of a vector step pass through the rings
-    if (pl->rows.groups > 1) pl->smem = std::max(pl->smem, kBwdThreads * 64);
+    if (odd || pl->rows.groups > 1) pl->smem = std::max(pl->smem, kBwdThreads * 64);
     int grid = 0;
     const int st = launch_rows(ud, pl->kernel, FusedBwdParams{}, pl->rows, pl->smem, nullptr, "", pl->k, &grid, true);
     if (st == RMSNORM_B200_OK) {
@@ -161,7 +170,7 @@ int run(const rmsnorm_b200_dropout_bwd_args* a, void* ws, size_t ws_bytes, cudaS
   p.db_part = a->dbias ? static_cast<float*>(ws) + (a->dweight ? pl.nparts * a->hidden : 0) : nullptr;
   expand_drop(a->drop, &p.drop);
   if (a->rows > 0) {
-    st = pl.kernel ? launch_rows(ud, pl.kernel, p, pl.rows, pl.smem, stream, "dropout_bwd", pl.k)
+    st = pl.kernel ? launch_rows(ud, pl.kernel, p, pl.rows, pl.smem, stream, pl.kind, pl.k)
                    : launch_generic(p, pl, ud, stream, pl.why);
     if (st) return st;
   } else {

@@ -158,7 +158,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fused_bwd_kernel(const FusedBw
       }
       float s = s2.x + s2.y;
       uint32_t unused = 0;
-      row_total<true, false>(pl, c, s, unused, kSiteBwdCluster);
+      // the first step's mask is drawn while the row's total comes together
+      uint32_t words[2][4];
+      row_total<true, false>(pl, c, s, unused, kSiteBwdCluster,
+                             [&] { draw8(p.drop, c.slice0 + c.gl * 8, row, offset, words); });
       const float t = -(rs * rs * rs * (s * inv_n));
 #pragma unroll
       for (int j = 0; j < K; ++j) {
@@ -183,7 +186,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fused_bwd_kernel(const FusedBw
           d[i] = mul2(d[i], splat2(p.drop.scale));
           zero[i] = make_float2(0.f, 0.f);
         }
-        select8(p.drop, c.slice0 + col, row, offset, d, zero, g);
+        if (j > 0) draw8(p.drop, c.slice0 + col, row, offset, words);
+        select8(p.drop, words, d, zero, g);
         Pair8<DY>::store(static_cast<unsigned char*>(p.dx) + (e0 + col) * kDy, g);
       }
       if constexpr (kTmem) __syncwarp();  // together again for the next row's tensor memory accesses

@@ -4,6 +4,7 @@
 #include "unit_state.cuh"
 
 #include "fused_fwd_kernels.cuh"
+#include "odd_kernels.cuh"
 #include "row_plan.h"
 
 namespace rmsb200 {
@@ -69,6 +70,11 @@ FwdKernel pick(int x, int res, int ro, int end, int k) {
   return nullptr;
 }
 
+template <bool kQuant>
+FwdKernel pick_odd(int k) {
+  return k == 1 ? odd_fwd_kernel<kQuant, 1> : k == 2 ? odd_fwd_kernel<kQuant, 2> : odd_fwd_kernel<kQuant, 4>;
+}
+
 int launch_generic(const FusedFwdParams& p, bool drop, UnitDevice* ud, cudaStream_t stream, const char* why) {
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(p.rows, int64_t{8} * ud->sm_count));
   if (drop)
@@ -98,31 +104,34 @@ int run(const FusedFwdParams& p, bool drop, cudaStream_t stream) {
   if (p.drop.step) ranges.add(p.drop.step, 8);
   st = ranges.send(stream);
   if (st) return st;
+  // Whole aligned vectors in a combination of types with a kernel of its own; else the odd
+  // rows' kernels; else (rows wider than a cluster holds) the generic one.
+  const int bytes[3] = {elem_bytes(p.x_dt), p.res ? elem_bytes(p.res_dt) : 0, 0};
+  RowPlan pl;
+  int k = 0, smem = 0;
   const void* ptrs[] = {p.x, p.res, p.out, p.ro};
-  const char* why = p.N % 8 ? "hidden % 8" : nullptr;
-  for (const void* ptr : ptrs)
-    if (!aligned_to(ptr, ptr == p.out && p.scales ? 8 : 16)) why = "unaligned pointer";
-  if (!why) {
-    const int bytes[3] = {elem_bytes(p.x_dt), p.res ? elem_bytes(p.res_dt) : 0, 0};
-    RowPlan pl;
-    int k = 0, smem = 0;
+  bool vectors = p.N % 8 == 0 && (!drop || p.out_dt == p.x_dt);
+  for (const void* ptr : ptrs) vectors = vectors && aligned_to(ptr, ptr == p.out && p.scales ? 8 : 16);
+  const char* why = nullptr;
+  if (vectors) {
     const bool few = p.rows <= ud->sm_count && p.N <= kFwdFewThreads * 8;
     why = plan_rows(p.rows, p.N, bytes, p.b != nullptr, few ? kFwdFewThreads : kFwdThreads, few ? 1 : kFwdSteps,
                     ud->sm_count, &pl, &k, &smem);
-    if (!why && (!drop || p.out_dt == p.x_dt)) {
+    if (!why) {
       const bool i8 = p.out_dt == RMSNORM_B200_I8;
       const int end = drop ? kDropped : p.group ? (i8 ? kI8Group : kE4M3Group) : (i8 ? kI8Row : kE4M3Row);
-      FwdKernel kernel = pick(p.x_dt, p.res ? p.res_dt : kNone, p.ro ? p.ro_dt : kNone, end, k);
-      if (kernel) {
+      if (FwdKernel kernel = pick(p.x_dt, p.res ? p.res_dt : kNone, p.ro ? p.ro_dt : kNone, end, k)) {
         st = launch_rows(ud, kernel, p, pl, smem, stream, drop ? "dropout_fwd" : "quant_fwd", k);
         if (st != RMSNORM_B200_ERR_UNSUPPORTED) return st;
-        why = "cluster not schedulable";
-      } else {
-        why = "dtype combination";
       }
-    } else if (!why) {
-      why = "dtype combination";
     }
+  }
+  why = plan_rows(p.rows, p.N, bytes, p.b != nullptr, kOddThreads, kOddSteps, ud->sm_count, &pl, &k, &smem, true);
+  if (!why) {
+    st = launch_rows(ud, drop ? pick_odd<false>(k) : pick_odd<true>(k), p, pl, smem, stream,
+                     drop ? "dropout_fwd_odd" : "quant_fwd_odd", k);
+    if (st != RMSNORM_B200_ERR_UNSUPPORTED) return st;
+    why = "cluster not schedulable";
   }
   return launch_generic(p, drop, ud, stream, why);
 }

@@ -79,7 +79,9 @@ __global__ void __launch_bounds__(K == 1 ? kFwdFewThreads : kFwdThreads, 1) fuse
             float2 kept[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) kept[i] = fma2(h[j][i], splat2(p.drop.scale), res[i]);
-            select8(p.drop, c.slice0 + col, row, offset, kept, res, h[j]);
+            uint32_t words[2][4];
+            draw8(p.drop, c.slice0 + col, row, offset, words);
+            select8(p.drop, words, kept, res, h[j]);
           } else if constexpr (kRes) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) h[j][i] = add2(h[j][i], res[i]);

@@ -80,14 +80,28 @@ bool vectorised(const rmsnorm_b200_rope_args* a, std::initializer_list<const rms
 }
 
 // U: heads a lane works on at a time.
-RopePlan plan(const rmsnorm_b200_rope_args* a, int u) {
-  RopePlan pl = {};
+struct RopeGrid {
+  RopePlan pl;
+  dim3 grid;
+  int threads;
+};
+
+RopeGrid plan(const rmsnorm_b200_rope_args* a, int u, int64_t most_ctas) {
+  RopeGrid g = {};
+  RopePlan& pl = g.pl;
   while ((8 << pl.lanes_shift) < a->head_dim) ++pl.lanes_shift;
-  const int heads = u * (32 >> pl.lanes_shift);  // of a job
+  const int heads = u * (32 >> pl.lanes_shift);  // of a warp
   pl.jobs[0] = (a->q_heads + heads - 1) / heads;
   pl.jobs[1] = (a->k_heads + heads - 1) / heads;
   pl.turned_lanes = a->rotary_dim / 8;
-  return pl;
+  const int jobs = pl.jobs[0] + pl.jobs[1];
+  pl.cta_jobs = std::min(jobs, kRopeWarps);
+  const int at_once = static_cast<int>(std::clamp<int64_t>(a->tokens, 1, kRopeWarps / pl.cta_jobs));
+  g.threads = at_once * pl.cta_jobs * 32;
+  const int64_t across = (jobs + pl.cta_jobs - 1) / pl.cta_jobs;
+  const int64_t along = std::clamp<int64_t>((a->tokens + at_once - 1) / at_once, 1, std::max<int64_t>(1, most_ctas / across));
+  g.grid = dim3(static_cast<unsigned>(along), static_cast<unsigned>(across));
+  return g;
 }
 
 struct RopeLaunch {  // for rmsnorm_b200_last_plan
@@ -128,18 +142,39 @@ int launch(Kernel kernel, dim3 grid, int threads, cudaStream_t stream, const Rop
   return launched(describe_rope, l);
 }
 
+#ifndef RMSB_ROPE_CTAS
+#define RMSB_ROPE_CTAS 2
+#endif
+constexpr int kFwdCtas = RMSB_ROPE_CTAS, kBwdCtas = RMSB_ROPE_CTAS;  // of an SM, at most
+
 using RopeKernel = void (*)(const RopeParams, const RopePlan);
 
-template <int U>
-RopeKernel pick_fwd(int dt) {
-  return dt == RMSNORM_B200_BF16 ? rope_fwd_kernel<__nv_bfloat16, U>
-         : dt == RMSNORM_B200_F16 ? rope_fwd_kernel<__half, U> : rope_fwd_kernel<float, U>;
+template <typename T, int U>
+RopeKernel pick_fwd(bool interleaved, bool norm) {
+  if (interleaved) return norm ? rope_fwd_kernel<T, U, true, true> : rope_fwd_kernel<T, U, true, false>;
+  return norm ? rope_fwd_kernel<T, U, false, true> : rope_fwd_kernel<T, U, false, false>;
 }
 
+template <int U>
+RopeKernel pick_fwd(const RopeParams& p) {
+  if (p.dt == RMSNORM_B200_BF16) return pick_fwd<__nv_bfloat16, U>(p.interleaved, p.norm);
+  return p.dt == RMSNORM_B200_F16 ? pick_fwd<__half, U>(p.interleaved, p.norm) : pick_fwd<float, U>(p.interleaved, p.norm);
+}
+
+template <typename T, int U, bool kPerHead>
+RopeKernel pick_bwd(bool interleaved, bool norm) {
+  if (interleaved)
+    return norm ? rope_bwd_kernel<T, U, true, true, kPerHead> : rope_bwd_kernel<T, U, true, false, kPerHead>;
+  return norm ? rope_bwd_kernel<T, U, false, true, kPerHead> : rope_bwd_kernel<T, U, false, false, kPerHead>;
+}
+
+constexpr int kBwdHeads16 = 4, kBwdHeads32 = 2;  // heads a lane in the backward, 16- and 32-bit types
+
 template <bool kPerHead>
-RopeKernel pick_bwd(int dt) {
-  return dt == RMSNORM_B200_BF16 ? rope_bwd_kernel<__nv_bfloat16, 4, kPerHead>
-         : dt == RMSNORM_B200_F16 ? rope_bwd_kernel<__half, 4, kPerHead> : rope_bwd_kernel<float, 2, kPerHead>;
+RopeKernel pick_bwd(const RopeParams& p) {
+  if (p.dt == RMSNORM_B200_BF16) return pick_bwd<__nv_bfloat16, kBwdHeads16, kPerHead>(p.interleaved, p.norm);
+  return p.dt == RMSNORM_B200_F16 ? pick_bwd<__half, kBwdHeads16, kPerHead>(p.interleaved, p.norm)
+                                  : pick_bwd<float, kBwdHeads32, kPerHead>(p.interleaved, p.norm);
 }
 
 int run_fwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_tensor* qo, const rmsnorm_b200_rope_tensor* ko,
@@ -166,13 +201,10 @@ int run_fwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_tensor* qo,
   if (ko) p.out[1] = tensor(*ko);
   if (vectorised(a, {&a->q, &a->k, qo, ko})) {
     // Four heads a lane where that leaves every SM eight warps to run; single heads below.
-    constexpr int kWarps = kRopeThreads / 32;
-    RopePlan pl = plan(a, 4);
-    const bool wide = a->tokens * (pl.jobs[0] + pl.jobs[1]) >= int64_t{kWarps} * ud->sm_count;
-    if (!wide) pl = plan(a, 1);
-    const int64_t ctas = (a->tokens * (pl.jobs[0] + pl.jobs[1]) + kWarps - 1) / kWarps;
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(ctas, int64_t{8} * ud->sm_count)));
-    return launch(wide ? pick_fwd<4>(a->dtype) : pick_fwd<1>(a->dtype), grid, kRopeThreads, stream, p, pl, "rope_fwd");
+    RopeGrid g = plan(a, 4, int64_t{kFwdCtas} * ud->sm_count);
+    const bool wide = a->tokens * (g.pl.jobs[0] + g.pl.jobs[1]) >= int64_t{8} * ud->sm_count;
+    if (!wide) g = plan(a, 1, int64_t{kFwdCtas} * ud->sm_count);
+    return launch(wide ? pick_fwd<4>(p) : pick_fwd<1>(p), g.grid, g.threads, stream, p, g.pl, "rope_fwd");
   }
   const int64_t work = a->tokens * (a->q_heads + a->k_heads);
   const int64_t warps = kGenericThreads / 32;
@@ -207,15 +239,11 @@ BwdPlan plan_bwd(const UnitDevice* ud, const rmsnorm_b200_rope_args* a, const rm
   pl.per_head = (a->q_weight && a->q_weight_heads > 1) || (a->k_weight && a->k_weight_heads > 1);
   pl.vec = vectorised(a, {&a->q, &a->k, &g->dq_out, &g->dk_out, &g->dq, &g->dk});
   if (pl.vec) {
-    pl.rope = plan(a, a->dtype == RMSNORM_B200_F32 ? 2 : 4);
-    const int jobs = pl.rope.jobs[0] + pl.rope.jobs[1];
-    pl.rope.cta_jobs = std::min(jobs, kRopeBwdWarps);
-    const int at_once = kRopeBwdWarps / pl.rope.cta_jobs;
-    pl.threads = at_once * pl.rope.cta_jobs * 32;
-    const int64_t across = (jobs + pl.rope.cta_jobs - 1) / pl.rope.cta_jobs;
-    const int64_t most = std::max<int64_t>(1, int64_t{2} * ud->sm_count / across);
-    const int64_t along = std::clamp<int64_t>((a->tokens + at_once - 1) / at_once, 1, most);
-    pl.grid = dim3(static_cast<unsigned>(along), static_cast<unsigned>(across));
+    const RopeGrid gr = plan(a, a->dtype == RMSNORM_B200_F32 ? kBwdHeads32 : kBwdHeads16, int64_t{kBwdCtas} * ud->sm_count);
+    pl.rope = gr.pl;
+    pl.threads = gr.threads;
+    pl.grid = gr.grid;
+    const int64_t along = gr.grid.x, across = gr.grid.y;
     pl.rows = pl.per_head ? along : along * across;
     pl.width = (pl.per_head ? heads : 2) * a->head_dim;
     return pl;
@@ -267,7 +295,7 @@ int run_bwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g, v
   p.part = need ? static_cast<float*>(ws) : nullptr;
   if (a->tokens > 0) {
     if (pl.vec) {
-      st = launch(pl.per_head ? pick_bwd<true>(a->dtype) : pick_bwd<false>(a->dtype), pl.grid, pl.threads, stream, p,
+      st = launch(pl.per_head ? pick_bwd<true>(p) : pick_bwd<false>(p), pl.grid, pl.threads, stream, p,
                   pl.rope, "rope_bwd");
     } else {
       const dim3 grid(static_cast<unsigned>(heads), static_cast<unsigned>(pl.chunks));

@@ -164,8 +164,6 @@ __global__ void __launch_bounds__(kGenericThreads) rope_bwd_generic_kernel(const
 // and a lane needs only four cosines and four sines, which serve every head it works on.
 // L = the smallest power of two with 8 L >= head_dim lanes hold a head; a warp holds 32 / L.
 // ---------------------------------------------------------------------------------------
-constexpr int kRopeThreads = 256;
-
 template <typename T>
 struct Chunk4 {
   uint2 v;
@@ -174,19 +172,14 @@ struct Chunk4 {
     const T* q = static_cast<const T*>(p) + e;
     v = RMSB_DBG_OK(q, 8, kDbgVecLoad) ? __ldcs(reinterpret_cast<const uint2*>(q)) : make_uint2(0u, 0u);
   }
-  __device__ __forceinline__ void get(float* f) const {
-    if constexpr (kB) {
-      unpack_bf16x2(v.x, f[0], f[1]);
-      unpack_bf16x2(v.y, f[2], f[3]);
-    } else {
-      unpack_f16x2(v.x, f[0], f[1]);
-      unpack_f16x2(v.y, f[2], f[3]);
-    }
+  __device__ __forceinline__ void get(float2* f) const {
+    f[0] = kB ? unpack_bf16x2_pair(v.x) : unpack_f16x2_pair(v.x);
+    f[1] = kB ? unpack_bf16x2_pair(v.y) : unpack_f16x2_pair(v.y);
   }
-  __device__ __forceinline__ static void store(void* p, int64_t e, const float* f) {
+  __device__ __forceinline__ static void store(void* p, int64_t e, const float2* f) {
     T* q = static_cast<T*>(p) + e;
-    const uint2 u = kB ? make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]))
-                       : make_uint2(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]));
+    const uint2 u = kB ? make_uint2(pack_bf16x2_pair(f[0]), pack_bf16x2_pair(f[1]))
+                       : make_uint2(pack_f16x2_pair(f[0]), pack_f16x2_pair(f[1]));
     if (RMSB_DBG_OK(q, 8, kDbgVecStore)) __stcs(reinterpret_cast<uint2*>(q), u);
   }
 };
@@ -197,20 +190,23 @@ struct Chunk4<float> {
     const float* q = static_cast<const float*>(p) + e;
     v = RMSB_DBG_OK(q, 16, kDbgVecLoad) ? __ldcs(reinterpret_cast<const float4*>(q)) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  __device__ __forceinline__ void get(float* f) const { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
-  __device__ __forceinline__ static void store(void* p, int64_t e, const float* f) {
+  __device__ __forceinline__ void get(float2* f) const {
+    f[0] = make_float2(v.x, v.y);
+    f[1] = make_float2(v.z, v.w);
+  }
+  __device__ __forceinline__ static void store(void* p, int64_t e, const float2* f) {
     float* q = static_cast<float*>(p) + e;
-    if (RMSB_DBG_OK(q, 16, kDbgVecStore)) __stcs(reinterpret_cast<float4*>(q), make_float4(f[0], f[1], f[2], f[3]));
+    if (RMSB_DBG_OK(q, 16, kDbgVecStore)) __stcs(reinterpret_cast<float4*>(q), make_float4(f[0].x, f[0].y, f[1].x, f[1].y));
   }
 };
 
-// Work of the vectorised kernels: a warp takes U * (32 / L) heads of one token, all of q or
-// all of k: jobs 0 .. jobs[0] - 1 of a token are of q, the others of k.
+// A warp takes U * (32 / L) heads of a token, all of q or all of k, and keeps them over all
+// the tokens it takes: the weight (and the backward's sums of its gradient) stay in registers.
 struct RopePlan {
   int32_t lanes_shift;  // log2(L)
-  int32_t jobs[2];      // of q and of k, per token
+  int32_t jobs[2];      // warps' shares of a token: of q first, then of k
   int32_t turned_lanes; // lanes of the turned part: rotary_dim / 8
-  int32_t cta_jobs;     // backward: jobs of a CTA, whose warps take warps / cta_jobs tokens at a time
+  int32_t cta_jobs;     // shares of a CTA, whose warps take warps / cta_jobs tokens at a time
 };
 
 struct RopeLane {
@@ -220,6 +216,7 @@ struct RopeLane {
   int a, b;       // first columns of its chunks
 };
 
+template <bool kInterleaved>
 __device__ __forceinline__ RopeLane rope_lane(const RopeParams& p, const RopePlan& pl) {
   RopeLane t;
   const int lane = threadIdx.x & 31;
@@ -227,8 +224,8 @@ __device__ __forceinline__ RopeLane rope_lane(const RopeParams& p, const RopePla
   t.sub = lane >> pl.lanes_shift;
   t.in = t.l * 8 < p.D;
   t.turned = t.l < pl.turned_lanes;
-  t.a = t.turned && !p.interleaved ? 4 * t.l : 8 * t.l;
-  t.b = t.turned && !p.interleaved ? t.a + p.rd / 2 : t.a + 4;
+  t.a = t.turned && !kInterleaved ? 4 * t.l : 8 * t.l;
+  t.b = t.turned && !kInterleaved ? t.a + p.rd / 2 : t.a + 4;
   return t;
 }
 
@@ -257,21 +254,22 @@ __device__ __forceinline__ void rope_lane_turn(const RopeParams& p, const RopeLa
   for (int i = 0; i < 4; ++i) rope_cos_sin(p, token, i0 + i, c[i], s[i]);
 }
 
-// y holds columns a .. a + 3, b .. b + 3. sign -1 turns back.
-__device__ __forceinline__ void rope_turn8(const RopeParams& p, const RopeLane& t, const float (&c)[4],
-                                           const float (&s)[4], float sign, float (&y)[8]) {
+// y holds columns a .. a + 3, b .. b + 3, in pairs of neighbours.
+template <bool kInterleaved>
+__device__ __forceinline__ void rope_turn8(const RopeLane& t, const float (&c)[4], const float (&s)[4],
+                                           float2 (&y)[4]) {
   if (!t.turned) return;
+  if constexpr (kInterleaved) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float sn = sign * s[i];
-    if (p.interleaved) {
-      const float u = y[2 * i], v = y[2 * i + 1];
-      y[2 * i] = u * c[i] - v * sn;
-      y[2 * i + 1] = v * c[i] + u * sn;
-    } else {
-      const float u = y[i], v = y[4 + i];
-      y[i] = u * c[i] - v * sn;
-      y[4 + i] = v * c[i] + u * sn;
+    for (int i = 0; i < 4; ++i)
+      y[i] = make_float2(y[i].x * c[i] - y[i].y * s[i], y[i].y * c[i] + y[i].x * s[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 u = y[i], v = y[2 + i];
+      const float2 cc = make_float2(c[2 * i], c[2 * i + 1]), ss = make_float2(s[2 * i], s[2 * i + 1]);
+      y[i] = fma2(v, make_float2(-ss.x, -ss.y), mul2(u, cc));
+      y[2 + i] = fma2(u, ss, mul2(v, cc));
     }
   }
 }
@@ -282,120 +280,155 @@ __device__ __forceinline__ float rope_head_sum(float v, int lanes_shift) {
 }
 
 __device__ __forceinline__ void rope_weight8(const RopeParams& p, int k, int64_t head, const RopeLane& t,
-                                             float (&w)[8]) {
+                                             float2 (&w)[4]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = 1.f;
+  for (int i = 0; i < 4; ++i) w[i] = make_float2(1.f, 1.f);
   if (!p.w[k] || !t.in) return;
   const int64_t e = p.w_per_head[k] ? head * p.D : 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    w[i] = load1_rt(p.w[k], p.w_dt, e + t.a + i);
-    w[4 + i] = load1_rt(p.w[k], p.w_dt, e + t.b + i);
+    const int64_t at = e + (i < 2 ? t.a + 2 * i : t.b + 2 * i - 4);
+    w[i] = make_float2(load1_rt(p.w[k], p.w_dt, at), load1_rt(p.w[k], p.w_dt, at + 1));
   }
 }
 
-template <typename T, int U>
-__global__ void __launch_bounds__(kRopeThreads) rope_fwd_kernel(const RopeParams p, const RopePlan pl) {
+// A warp's share of every token: its heads, and its first token and step.
+struct RopeJob {
+  bool works;
+  int k, job, head0;     // q or k; share of it; the lane's first head
+  int per;               // heads of the warp side by side: the lane's next head is head0 + per
+  int heads;
+  int64_t token, step;
+};
+
+__device__ __forceinline__ RopeJob rope_job(const RopeParams& p, const RopePlan& pl, const RopeLane& t, int u) {
+  RopeJob b;
+  const int warp = threadIdx.x >> 5;
+  const int at_once = (blockDim.x >> 5) / pl.cta_jobs;  // tokens
+  b.job = blockIdx.y * pl.cta_jobs + warp % pl.cta_jobs;
+  b.works = b.job < pl.jobs[0] + pl.jobs[1];
+  b.k = b.job >= pl.jobs[0];
+  if (b.k) b.job -= pl.jobs[0];
+  b.per = 32 >> pl.lanes_shift;
+  b.head0 = b.job * u * b.per + t.sub;
+  b.heads = b.k ? p.heads[1] : p.heads[0];
+  b.token = static_cast<int64_t>(blockIdx.x) * at_once + warp / pl.cta_jobs;
+  b.step = static_cast<int64_t>(gridDim.x) * at_once;
+  return b;
+}
+
+// The lane's chunks of a tensor: element offset of its first head in token 0, and strides.
+template <typename T>
+struct RopePlace {
+  T* p;
+  int64_t ts, us;
+  int da, db;
+  __device__ __forceinline__ RopePlace(const RopeTensor& x, const RopeLane& t, const RopeJob& b)
+      : p(static_cast<T*>(x.p) + b.head0 * x.hs), ts(x.ts), us(b.per * x.hs), da(t.a), db(t.b) {}
+  __device__ __forceinline__ void load(int64_t token, int u, Chunk4<T> (&c)[2]) const {
+    const int64_t e = token * ts + u * us;
+    c[0].load(p, e + da);
+    c[1].load(p, e + db);
+  }
+  __device__ __forceinline__ void store(int64_t token, int u, const float2 (&y)[4]) const {
+    const int64_t e = token * ts + u * us;
+    Chunk4<T>::store(p, e + da, y);
+    Chunk4<T>::store(p, e + db, y + 2);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void rope_get(const Chunk4<T> (&c)[2], float2 (&y)[4]) {
+  c[0].get(y);
+  c[1].get(y + 2);
+}
+
+#ifndef RMSB_ROPE_WARPS
+#define RMSB_ROPE_WARPS 16
+#endif
+constexpr int kRopeWarps = RMSB_ROPE_WARPS;  // of a CTA, at most
+
+template <typename T, int U, bool kInterleaved, bool kNorm>
+__global__ void __launch_bounds__(kRopeWarps * 32) rope_fwd_kernel(const RopeParams p, const RopePlan pl) {
   pdl_launch_dependents();
   pdl_wait();
-  const RopeLane t = rope_lane(p, pl);
-  const int per = 32 >> pl.lanes_shift;  // heads of a warp at a time
-  const int jobs = pl.jobs[0] + pl.jobs[1];
-  const int64_t work = p.tokens * jobs;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kRopeThreads / 32);
+  const RopeLane t = rope_lane<kInterleaved>(p, pl);
+  const RopeJob b = rope_job(p, pl, t, U);
+  if (!b.works) return;
+  const int k = b.k;
+  const RopePlace<T> in(k ? p.x[1] : p.x[0], t, b), out(k ? p.out[1] : p.out[0], t, b);
+  const bool per_head = p.w_per_head[k];
   const float inv_d = 1.f / static_cast<float>(p.D);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kRopeThreads / 32) + (threadIdx.x >> 5); i < work; i += step) {
-    const int64_t token = i / jobs;
-    int job = static_cast<int>(i - token * jobs);
-    const int k = job >= pl.jobs[0];
-    if (k) job -= pl.jobs[0];
-    const int head0 = job * U * per + t.sub;
+  float2 w[4];
+  if (!per_head) rope_weight8(p, k, 0, t, w);
+  for (int64_t token = b.token; token < p.tokens; token += b.step) {
     Chunk4<T> x[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int head = head0 + u * per;
-      if (t.in && head < p.heads[k]) {
-        const int64_t e = token * p.x[k].ts + head * p.x[k].hs;
-        x[u][0].load(p.x[k].p, e + t.a);
-        x[u][1].load(p.x[k].p, e + t.b);
-      } else {
+      if (t.in && b.head0 + u * b.per < b.heads)
+        in.load(token, u, x[u]);
+      else
         x[u][0].v = x[u][1].v = {};
-      }
     }
-    float c[4], s[4], w[8];
+    float c[4], s[4];
     rope_lane_turn(p, t, token, c, s);
-    if (!p.w_per_head[k]) rope_weight8(p, k, 0, t, w);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int head = head0 + u * per;
-      float y[8];
-      x[u][0].get(y);
-      x[u][1].get(y + 4);
-      if (p.norm) {
-        float ss = 0.f;
+      const int head = b.head0 + u * b.per;
+      float2 y[4];
+      rope_get(x[u], y);
+      if constexpr (kNorm) {
+        float2 ss = mul2(y[0], y[0]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
-        const float rs = rsqrtf(rope_head_sum(ss, pl.lanes_shift) * inv_d + p.eps);
+        for (int i = 1; i < 4; ++i) ss = fma2(y[i], y[i], ss);
+        const float rs = rsqrtf(rope_head_sum(ss.x + ss.y, pl.lanes_shift) * inv_d + p.eps);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] *= rs;
+        for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], splat2(rs));
       }
-      if (t.in && head < p.heads[k]) {
-        if (p.w_per_head[k]) rope_weight8(p, k, head, t, w);
+      if (t.in && head < b.heads) {
+        if (per_head) rope_weight8(p, k, head, t, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] *= w[e];
-        rope_turn8(p, t, c, s, 1.f, y);
-        const int64_t o = token * p.out[k].ts + head * p.out[k].hs;
-        Chunk4<T>::store(p.out[k].p, o + t.a, y);
-        Chunk4<T>::store(p.out[k].p, o + t.b, y + 4);
+        for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], w[i]);
+        rope_turn8<kInterleaved>(t, c, s, y);
+        out.store(token, u, y);
       }
     }
   }
 }
 
-constexpr int kRopeBwdWarps = 16;
-
-// A warp keeps its heads over all the tokens it takes, so the sums of dweight stay in its
-// registers: a set per head it works on (kPerHead), or one set. The CTA adds its warps' sums
-// in a fixed order and leaves one partial row: [q_heads + k_heads][head_dim] per blockIdx.x,
-// or [q, k][head_dim] per CTA.
-template <typename T, int U, bool kPerHead>
-__global__ void __launch_bounds__(kRopeBwdWarps * 32) rope_bwd_kernel(const RopeParams p, const RopePlan pl) {
+// The sums of dweight: a set per head the lane works on (kPerHead), or one set. The CTA adds
+// its warps' sums in a fixed order and leaves one partial row: [q_heads + k_heads][head_dim]
+// per blockIdx.x, or [q, k][head_dim] per CTA.
+template <typename T, int U, bool kInterleaved, bool kNorm, bool kPerHead>
+__global__ void __launch_bounds__(kRopeWarps * 32) rope_bwd_kernel(const RopeParams p, const RopePlan pl) {
   constexpr int kSets = kPerHead ? U : 1;
-  __shared__ float sums[kRopeBwdWarps][kRopeMaxDim];
+  __shared__ float sums[kRopeWarps][kRopeMaxDim];
   pdl_launch_dependents();
   pdl_wait();
-  const RopeLane t = rope_lane(p, pl);
-  const int per = 32 >> pl.lanes_shift;
+  const RopeLane t = rope_lane<kInterleaved>(p, pl);
+  const RopeJob b = rope_job(p, pl, t, U);
   const int warp = threadIdx.x >> 5;
-  const int at_once = (blockDim.x >> 5) / pl.cta_jobs;  // tokens
-  const int all = pl.jobs[0] + pl.jobs[1];
+  const int at_once = (blockDim.x >> 5) / pl.cta_jobs;
   const int first_job = blockIdx.y * pl.cta_jobs;
-  int job = first_job + warp % pl.cta_jobs;
-  const bool works = job < all;
-  const int k = job >= pl.jobs[0];
-  if (k) job -= pl.jobs[0];
-  const int head0 = job * U * per + t.sub;
+  const int all = pl.jobs[0] + pl.jobs[1];
+  const int k = b.k, per = b.per;
+  const RopePlace<T> in(k ? p.x[1] : p.x[0], t, b), grad(k ? p.dy[1] : p.dy[0], t, b),
+      out(k ? p.out[1] : p.out[0], t, b);
+  const bool per_head = kPerHead && p.w_per_head[k];
   const float inv_d = 1.f / static_cast<float>(p.D);
-  float acc[kSets][8], w[8];
+  float2 acc[kSets][4], w[4];
 #pragma unroll
   for (int i = 0; i < kSets; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[i][e] = 0.f;
-  if (!p.w_per_head[k]) rope_weight8(p, k, 0, t, w);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * at_once;
-  for (int64_t token = static_cast<int64_t>(blockIdx.x) * at_once + warp / pl.cta_jobs; works && token < p.tokens;
-       token += step) {
+    for (int e = 0; e < 4; ++e) acc[i][e] = make_float2(0.f, 0.f);
+  if (!per_head) rope_weight8(p, k, 0, t, w);
+  for (int64_t token = b.token; b.works && token < p.tokens; token += b.step) {
     Chunk4<T> x[U][2], dy[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int head = head0 + u * per;
-      if (t.in && head < p.heads[k]) {
-        const int64_t d = token * p.dy[k].ts + head * p.dy[k].hs;
-        dy[u][0].load(p.dy[k].p, d + t.a);
-        dy[u][1].load(p.dy[k].p, d + t.b);
-        const int64_t e = token * p.x[k].ts + head * p.x[k].hs;
-        x[u][0].load(p.x[k].p, e + t.a);
-        x[u][1].load(p.x[k].p, e + t.b);
+      if (t.in && b.head0 + u * per < b.heads) {
+        grad.load(token, u, dy[u]);
+        in.load(token, u, x[u]);
       } else {
         x[u][0].v = x[u][1].v = dy[u][0].v = dy[u][1].v = {};
       }
@@ -403,48 +436,53 @@ __global__ void __launch_bounds__(kRopeBwdWarps * 32) rope_bwd_kernel(const Rope
     float c[4], s[4];
     rope_lane_turn(p, t, token, c, s);
 #pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = -s[i];  // turned back
+#pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int head = head0 + u * per;
-      const bool in = t.in && head < p.heads[k];
-      float y[8], g[8];
-      x[u][0].get(y);
-      x[u][1].get(y + 4);
-      dy[u][0].get(g);
-      dy[u][1].get(g + 4);
-      rope_turn8(p, t, c, s, -1.f, g);
-      if (!in) {  // NaN cosines must not reach the sums of a lane without a head
+      const int head = b.head0 + u * per;
+      const bool has = t.in && head < b.heads;
+      float2 y[4], g[4];
+      rope_get(x[u], y);
+      rope_get(dy[u], g);
+      rope_turn8<kInterleaved>(t, c, s, g);
+      if (!has) {  // NaN cosines must not reach the sums of a lane without a head
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = 0.f;
+        for (int e = 0; e < 4; ++e) g[e] = make_float2(0.f, 0.f);
       }
-      if (p.w_per_head[k] && in) rope_weight8(p, k, head, t, w);
+      if (per_head && has) rope_weight8(p, k, head, t, w);
       float rs = 1.f, m = 0.f;
-      if (p.norm) {
-        float ss = 0.f, sg = 0.f;
+      float2 gw[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          ss = fmaf(y[e], y[e], ss);
-          sg = fmaf(y[e], g[e] * w[e], sg);
+      for (int e = 0; e < 4; ++e) gw[e] = mul2(g[e], w[e]);
+      if constexpr (kNorm) {
+        float2 ss = mul2(y[0], y[0]), sg = mul2(y[0], gw[0]);
+#pragma unroll
+        for (int e = 1; e < 4; ++e) {
+          ss = fma2(y[e], y[e], ss);
+          sg = fma2(y[e], gw[e], sg);
         }
-        ss = rope_head_sum(ss, pl.lanes_shift);
-        sg = rope_head_sum(sg, pl.lanes_shift);
-        rs = rsqrtf(ss * inv_d + p.eps);
-        m = sg * rs * inv_d;  // mean of xhat g w
+        rs = rsqrtf(rope_head_sum(ss.x + ss.y, pl.lanes_shift) * inv_d + p.eps);
+        m = rope_head_sum(sg.x + sg.y, pl.lanes_shift) * rs * inv_d;  // mean of xhat g w
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float xhat = y[e] * rs;
-        float& sum = acc[kPerHead ? u : 0][e];
-        sum = fmaf(g[e], xhat, sum);
-        y[e] = p.norm ? (g[e] * w[e] - xhat * m) * rs : g[e] * w[e];
+      for (int e = 0; e < 4; ++e) {
+        float2& sum = acc[kPerHead ? u : 0][e];
+        if constexpr (kNorm) {
+          const float2 xhat = mul2(y[e], splat2(rs));
+          sum = fma2(g[e], xhat, sum);
+          y[e] = mul2(fma2(xhat, splat2(-m), gw[e]), splat2(rs));
+        } else {
+          sum = fma2(g[e], y[e], sum);
+          y[e] = gw[e];
+        }
       }
-      if (in) {
-        const int64_t o = token * p.out[k].ts + head * p.out[k].hs;
-        Chunk4<T>::store(p.out[k].p, o + t.a, y);
-        Chunk4<T>::store(p.out[k].p, o + t.b, y + 4);
-      }
+      if (has) out.store(token, u, y);
     }
   }
   if (!p.part) return;
+  // a lane's column of its sums' element i
+  auto column = [&](int i) { return i < 4 ? t.a + i : t.b + i - 4; };
+  auto value = [](const float2(&v)[4], int i) { return i & 1 ? v[i >> 1].y : v[i >> 1].x; };
   if constexpr (kPerHead) {
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (p.heads[0] + p.heads[1]);
 #pragma unroll
@@ -452,18 +490,14 @@ __global__ void __launch_bounds__(kRopeBwdWarps * 32) rope_bwd_kernel(const Rope
       __syncthreads();
       // a warp's 32 / L heads side by side, head_dim columns each
       if (t.in) {
-        float* q = sums[warp] + t.sub * p.D;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          q[t.a + e] = acc[u][e];
-          q[t.b + e] = acc[u][4 + e];
-        }
+        for (int i = 0; i < 8; ++i) sums[warp][t.sub * p.D + column(i)] = value(acc[u], i);
       }
       __syncthreads();
-      if (works && warp < pl.cta_jobs) {
+      if (b.works && warp < pl.cta_jobs) {
         for (int i = threadIdx.x & 31; i < per * p.D; i += 32) {
-          const int head = job * U * per + u * per + i / p.D;
-          if (head >= p.heads[k]) continue;
+          const int head = b.job * U * per + u * per + i / p.D;
+          if (head >= b.heads) continue;
           float v = 0.f;
           for (int j = 0; j < at_once; ++j) v += sums[warp + j * pl.cta_jobs][i];
           st1(&p.part[(row + (k ? p.heads[0] : 0) + head) * p.D + i % p.D], v);
@@ -471,18 +505,16 @@ __global__ void __launch_bounds__(kRopeBwdWarps * 32) rope_bwd_kernel(const Rope
       }
     }
   } else {
-    float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[e] = acc[0][e];
-      for (int o = 16; o >= 1 << pl.lanes_shift; o >>= 1) v[e] += __shfl_xor_sync(0xffffffffu, v[e], o);
+    for (int e = 0; e < 4; ++e) {
+      for (int o = 16; o >= 1 << pl.lanes_shift; o >>= 1) {
+        acc[0][e].x += __shfl_xor_sync(0xffffffffu, acc[0][e].x, o);
+        acc[0][e].y += __shfl_xor_sync(0xffffffffu, acc[0][e].y, o);
+      }
     }
     if (t.in && t.sub == 0) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sums[warp][t.a + e] = v[e];
-        sums[warp][t.b + e] = v[4 + e];
-      }
+      for (int i = 0; i < 8; ++i) sums[warp][column(i)] = value(acc[0], i);
     }
     __syncthreads();
     float* row = p.part + (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * 2 * p.D;

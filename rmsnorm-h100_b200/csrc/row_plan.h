@@ -14,10 +14,11 @@ inline int pow2_ceil(int64_t v) {
   return p;
 }
 
-// Plans rows of N columns (a multiple of 8) whose tensors have elements of bytes[i] (0: absent).
+// Plans rows of N columns whose tensors have elements of bytes[i] (0: absent). odd: the kernels
+// of odd_kernels.cuh, otherwise N is a multiple of 8.
 // threads of a CTA, max_steps: vector steps a thread can hold. Returns why there is no plan, or null.
 inline const char* plan_rows(int64_t rows, int64_t N, const int (&bytes)[3], bool bias, int threads, int max_steps,
-                             int sms, RowPlan* pl, int* k, int* smem) {
+                             int sms, RowPlan* pl, int* k, int* smem, bool odd = false) {
   const int64_t cta_cols = static_cast<int64_t>(threads) * 8 * max_steps;
   if (N > cta_cols * kMaxRowCtas) return "rows wider than a cluster holds";
   pl->C = N > cta_cols ? pow2_ceil((N + cta_cols - 1) / cta_cols) : 1;
@@ -31,7 +32,6 @@ inline const char* plan_rows(int64_t rows, int64_t N, const int (&bytes)[3], boo
   // hold it, so that a CTA works on several rows at once and their totals overlap.
   const int steps = rows <= sms ? 1 : max_steps;
   pl->G = std::clamp(pow2_ceil((vecs + steps - 1) / steps), 32, threads);
-  if (pl->G > 32 && threads / pl->G > 15) pl->G *= 2;  // a named barrier per group: 15 beside barrier 0
   *k = pow2_ceil((vecs + pl->G - 1) / pl->G);
   pl->groups = pl->C > 1 ? 1 : threads / pl->G;
   const int elem = bytes[0] + bytes[1] + bytes[2];
@@ -49,11 +49,13 @@ inline const char* plan_rows(int64_t rows, int64_t N, const int (&bytes)[3], boo
   uint32_t off = 0;
   for (int i = 0; i < 3; ++i) {
     pl->off[i] = off;
-    off += static_cast<uint32_t>(unit_cols) * bytes[i];
+    // odd rows: up to 15 bytes before the first element, and up to the end of its last granule
+    if (bytes[i]) off += odd ? (unit_cols * bytes[i] + 45) & ~15 : unit_cols * bytes[i];
   }
   pl->unit_bytes = (off + 127u) & ~127u;
   pl->bias = bias;
   pl->tiles = (rows + pl->R - 1) / pl->R;
+  if (odd) pl->slice = (pl->slice + 7) & ~7;  // the affine copies keep the barriers' alignment
   const int affine = pl->slice * 4 * (bias ? 2 : 1);
   const int fixed = affine + static_cast<int>(sizeof(RowBars)) + 16;
   const int unit = pl->groups * static_cast<int>(pl->unit_bytes);

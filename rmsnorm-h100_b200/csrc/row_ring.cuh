@@ -40,6 +40,7 @@ struct RowPlan {
 struct RowBars {
   uint64_t full[kMaxUnits];
   uint64_t xbar[2];
+  uint64_t gbar[2][kRowWarps];  // [.][group]: a row's total within the group
   int done[kMaxUnits];
   float xpart[2][kMaxRowCtas][2];
   float red[2][kRowWarps][2];
@@ -95,6 +96,10 @@ __device__ __forceinline__ RowCtx row_begin(const RowPlan& pl, int64_t N) {
     }
     mbar_init(&c.bars->xbar[0], 1);
     mbar_init(&c.bars->xbar[1], 1);
+    for (int g = 0; g < pl.groups; ++g) {
+      mbar_init(&c.bars->gbar[0][g], c.nwarps);
+      mbar_init(&c.bars->gbar[1][g], c.nwarps);
+    }
     fence_mbar_init();
   }
   __syncthreads();
@@ -105,11 +110,30 @@ __device__ __forceinline__ RowCtx row_begin(const RowPlan& pl, int64_t N) {
 // weight (ones where absent) and bias of the slice, in fp32. Ends with a CTA barrier.
 __device__ __forceinline__ void load_affine(const RowPlan& pl, const RowCtx& c, const void* w, int w_dt, const void* b,
                                             int b_dt) {
-  for (int i = threadIdx.x; i < pl.slice; i += blockDim.x) {
-    const bool in = i < c.ncols;
-    const int at = (i & 4 ? pl.slice / 2 : 0) + (i >> 3) * 4 + (i & 3);
-    c.w[at] = in ? (w ? load1_rt(w, w_dt, c.slice0 + i) : 1.f) : 0.f;
-    if (pl.bias) c.b[at] = in ? load1_rt(b, b_dt, c.slice0 + i) : 0.f;
+  const bool vec = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && (reinterpret_cast<uintptr_t>(b) & 15) == 0;
+  for (int v = threadIdx.x; v * 8 < c.ncols; v += blockDim.x) {
+    float f[2][8];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const void* a = k == 0 ? w : b;
+      const int dt = k == 0 ? w_dt : b_dt;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[k][i] = 1.f;
+      if (!a) continue;
+      if (vec) {
+        load8_rt(a, dt, c.slice0 + v * 8, f[k], true);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[k][i] = load1_rt(a, dt, c.slice0 + v * 8 + i);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (k == 1 && !pl.bias) continue;
+      float4* dst = reinterpret_cast<float4*>(k == 0 ? c.w : c.b) + v;
+      dst[0] = make_float4(f[k][0], f[k][1], f[k][2], f[k][3]);
+      dst[pl.slice / 8] = make_float4(f[k][4], f[k][5], f[k][6], f[k][7]);
+    }
   }
   __syncthreads();
 }
@@ -169,26 +193,36 @@ __device__ __forceinline__ bool release_unit(const RowCtx& c, int slot) {
 
 // A row's sum and largest magnitude (bits) over the group's threads and the cluster's CTAs.
 // Every thread gets the same bits: the warps' values are added in one shuffle tree in warp
-// order, the CTAs' in rank order.
+// order, the CTAs' in rank order. `meanwhile` runs between a warp's contribution and its wait
+// for the others': work that does not need the total.
+// A warp writes slot k again two totals later, after it has taken the total in between; every
+// warp contributed to that one after it had taken slot k.
 // Across the cluster, `xbar[k]` completes when the C CTAs' 8-byte contributions have landed
-// (they may land before it is armed). Slot k is written again two exchanges later, by a peer
-// that has this CTA's contribution to the exchange in between; warp 0 sends that after the
-// barrier in which every warp has arrived with slot k read.
-template <bool kSum, bool kMax>
-__device__ __forceinline__ void row_total(const RowPlan& pl, RowCtx& c, float& sum, uint32_t& most, int site) {
+// (they may land before it is armed). A peer writes slot k again two totals later, when it has
+// this CTA's contribution to the one in between; warp 0 sends that after every warp of this
+// CTA has contributed to it, with slot k read.
+template <bool kSum, bool kMax, typename F>
+__device__ __forceinline__ void row_total(const RowPlan& pl, RowCtx& c, float& sum, uint32_t& most, int site,
+                                          F&& meanwhile) {
   if (kSum) sum = warp_sum(sum);
   if (kMax) most = __reduce_max_sync(0xffffffffu, most);
-  const uint32_t k = c.reds & 1u;
+  const uint32_t k = c.reds & 1u, parity = (c.reds >> 1) & 1u;
   if (pl.G > 32) {
     float(*red)[2] = c.bars->red[k];
+    uint64_t* bar = &c.bars->gbar[k][c.gid];
     if (c.lane == 0) {
       if (kSum) red[c.warp][0] = sum;
       if (kMax) red[c.warp][1] = __uint_as_float(most);
+      mbar_arrive(bar);
     }
-    named_barrier(1 + c.gid, pl.G);
+    meanwhile();
+    mbar_wait(bar, parity, site);
+    __syncwarp();
     const int w = c.gid * c.nwarps + c.lane;
     if (kSum) sum = warp_sum(c.lane < c.nwarps ? red[w][0] : 0.f);
     if (kMax) most = __reduce_max_sync(0xffffffffu, c.lane < c.nwarps ? __float_as_uint(red[w][1]) : 0u);
+  } else {
+    meanwhile();
   }
   if (pl.C > 1) {
     float(*part)[2] = c.bars->xpart[k];
@@ -201,11 +235,17 @@ __device__ __forceinline__ void row_total(const RowPlan& pl, RowCtx& c, float& s
         st_async_peer(map_peer(smem_u32(&part[c.rank][1]), c.lane), __uint_as_float(most), to_bar);
       }
     }
-    mbar_wait<true>(bar, (c.reds >> 1) & 1u, site);
+    mbar_wait<true>(bar, parity, site);
+    __syncwarp();
     if (kSum) sum = warp_sum(c.lane < pl.C ? part[c.lane][0] : 0.f);
     if (kMax) most = __reduce_max_sync(0xffffffffu, c.lane < pl.C ? __float_as_uint(part[c.lane][1]) : 0u);
   }
   ++c.reds;
+}
+
+template <bool kSum, bool kMax>
+__device__ __forceinline__ void row_total(const RowPlan& pl, RowCtx& c, float& sum, uint32_t& most, int site) {
+  row_total<kSum, kMax>(pl, c, sum, most, site, [] {});
 }
 
 // The end of a kernel: after a wait that ran out, the group's copies in flight land first; a
@@ -217,18 +257,23 @@ __device__ __forceinline__ void row_end(const RowPlan& pl, const RowCtx& c) {
   if (pl.C > 1) cluster_sync_all();
 }
 
-// Columns col .. col + 7 (col a multiple of 8): kept values of `a`, `b` elsewhere.
-__device__ __forceinline__ void select8(const DropParams& d, int64_t col, int64_t row, uint64_t offset,
-                                        const float2 (&a)[4], const float2 (&b)[4], float2 (&v)[4]) {
+// The mask's words of columns col .. col + 7 (col a multiple of 8).
+__device__ __forceinline__ void draw8(const DropParams& d, int64_t col, int64_t row, uint64_t offset,
+                                      uint32_t (&w)[2][4]) {
   const uint32_t quad = static_cast<uint32_t>(col >> 2), mrow = static_cast<uint32_t>(d.row0 + row);
+  philox(d, quad, mrow, offset, w[0]);
+  philox(d, quad + 1, mrow, offset, w[1]);
+}
+
+// Kept values of `a`, `b` elsewhere.
+__device__ __forceinline__ void select8(const DropParams& d, const uint32_t (&w)[2][4], const float2 (&a)[4],
+                                        const float2 (&b)[4], float2 (&v)[4]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    uint32_t w[4];
-    philox(d, quad + i, mrow, offset, w);
-    v[2 * i].x = w[0] >= d.least ? a[2 * i].x : b[2 * i].x;
-    v[2 * i].y = w[1] >= d.least ? a[2 * i].y : b[2 * i].y;
-    v[2 * i + 1].x = w[2] >= d.least ? a[2 * i + 1].x : b[2 * i + 1].x;
-    v[2 * i + 1].y = w[3] >= d.least ? a[2 * i + 1].y : b[2 * i + 1].y;
+    v[2 * i].x = w[i][0] >= d.least ? a[2 * i].x : b[2 * i].x;
+    v[2 * i].y = w[i][1] >= d.least ? a[2 * i].y : b[2 * i].y;
+    v[2 * i + 1].x = w[i][2] >= d.least ? a[2 * i + 1].x : b[2 * i + 1].x;
+    v[2 * i + 1].y = w[i][3] >= d.least ? a[2 * i + 1].y : b[2 * i + 1].y;
   }
 }
 
