@@ -21,35 +21,42 @@ struct Plan {
   const char* why = nullptr;  // why the generic path is taken
 };
 
+// g: threads of a row group where the kernel has them built in, else 0.
 template <typename H, typename DY, typename DRO, typename DRES>
-BwdKernel pick_steps(int k) {
-  if (k == 1) return fused_bwd_kernel<H, DY, DRO, DRES, 1>;
-  if (k == 2) return fused_bwd_kernel<H, DY, DRO, DRES, 2>;
+BwdKernel pick_steps(int k, int g) {
   // four steps hold a row of 16-bit values only
-  if constexpr (sizeof(H) == 2 && sizeof(DY) == 2) return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps>;
-  return nullptr;
+  if constexpr (sizeof(H) == 2 && sizeof(DY) == 2) {
+    switch (g) {
+      case 32: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 32>;
+      case 64: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 64>;
+      case 128: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 128>;
+      case 256: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 256>;
+      case 512: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 512>;
+    }
+  }
+  return k == 1 ? fused_bwd_kernel<H, DY, DRO, DRES, 1, 0> : fused_bwd_kernel<H, DY, DRO, DRES, 2, 0>;
 }
 
 template <typename H, typename DY>
-BwdKernel pick_residual(bool dro, bool dres, int k) {
-  if (dro) return dres ? pick_steps<H, DY, H, H>(k) : pick_steps<H, DY, H, NoT>(k);
-  return dres ? pick_steps<H, DY, NoT, H>(k) : pick_steps<H, DY, NoT, NoT>(k);
+BwdKernel pick_residual(bool dro, bool dres, int k, int g) {
+  if (dro) return dres ? pick_steps<H, DY, H, H>(k, g) : pick_steps<H, DY, H, NoT>(k, g);
+  return dres ? pick_steps<H, DY, NoT, H>(k, g) : pick_steps<H, DY, NoT, NoT>(k, g);
 }
 
 // The saved input in dout's type or in fp32; dresidual_out and dresidual have its type, dx has
 // dout's.
-BwdKernel pick(const rmsnorm_b200_dropout_bwd_args* a, int k) {
+BwdKernel pick(const rmsnorm_b200_dropout_bwd_args* a, int k, int g) {
   constexpr int H = RMSNORM_B200_F16, B = RMSNORM_B200_BF16, F = RMSNORM_B200_F32;
   using h16 = __half;
   using b16 = __nv_bfloat16;
   const int h = a->h_dtype, dy = a->dout_dtype;
   const bool dro = a->dresidual_out, dres = a->dresidual;
   if (a->dx_dtype != dy || (dro && a->dresidual_out_dtype != h) || (dres && a->dresidual_dtype != h)) return nullptr;
-  if (h == B && dy == B) return pick_residual<b16, b16>(dro, dres, k);
-  if (h == H && dy == H) return pick_residual<h16, h16>(dro, dres, k);
-  if (h == F && dy == F) return pick_residual<float, float>(dro, dres, k);
-  if (h == F && dy == B) return pick_residual<float, b16>(dro, dres, k);
-  if (h == F && dy == H) return pick_residual<float, h16>(dro, dres, k);
+  if (h == B && dy == B) return pick_residual<b16, b16>(dro, dres, k, g);
+  if (h == H && dy == H) return pick_residual<h16, h16>(dro, dres, k, g);
+  if (h == F && dy == F) return pick_residual<float, float>(dro, dres, k, g);
+  if (h == F && dy == B) return pick_residual<float, b16>(dro, dres, k, g);
+  if (h == F && dy == H) return pick_residual<float, h16>(dro, dres, k, g);
   return nullptr;
 }
 
@@ -81,11 +88,15 @@ int make_plan(UnitDevice* ud, const rmsnorm_b200_dropout_bwd_args* a, Plan* pl) 
                           &pl->smem, true);
       pl->kernel = pl->k == 1 ? odd_bwd_kernel<1> : odd_bwd_kernel<2>;
     } else {
-      const int64_t in_registers = kBwdThreads * 8 * kBwdRegSteps;
-      const int steps = a->h_dtype == RMSNORM_B200_F32 || a->hidden <= in_registers ? kBwdRegSteps : kBwdTmemSteps;
-      pl->why = plan_rows(a->rows, a->hidden, bytes, false, kBwdThreads, steps, ud->sm_count, &pl->rows, &pl->k,
-                          &pl->smem);
-      pl->kernel = pl->why ? nullptr : pick(a, pl->k);
+      // 16-bit rows that fill more than two steps of a warp: four steps a thread, sums in tensor
+      // memory. The others: sums in registers.
+      int g = 0;
+      if (a->h_dtype != RMSNORM_B200_F32 && a->dout_dtype == a->h_dtype && a->hidden > 32 * 8 * kBwdRegSteps)
+        g = std::min(pow2_ceil((a->hidden + 8 * kBwdTmemSteps - 1) / (8 * kBwdTmemSteps)), kBwdThreads);
+      pl->why = plan_rows(a->rows, a->hidden, bytes, false, kBwdThreads, g ? kBwdTmemSteps : kBwdRegSteps, ud->sm_count,
+                          &pl->rows, &pl->k, &pl->smem, false, g);
+      if (g) pl->k = kBwdTmemSteps;
+      pl->kernel = pl->why ? nullptr : pick(a, pl->k, g);
     }
     if (pl->why) pl->kernel = nullptr;
     if (!pl->kernel) continue;

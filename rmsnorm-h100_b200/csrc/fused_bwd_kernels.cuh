@@ -39,19 +39,32 @@ struct Raw8 {
   }
 };
 
+// A vector's contribution to its columns' sums: dweight, then dbias. g becomes dy rs.
+__device__ __forceinline__ void add_sums(float2 (&sum)[8], const float2 (&h)[4], float2 (&g)[4], float rs) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sum[4 + i] = add2(g[i], sum[4 + i]);
+    g[i] = mul2(g[i], splat2(rs));
+    sum[i] = fma2(h[i], g[i], sum[i]);
+  }
+}
+
 // H: type of h (and of dresidual), DY: of dout (and of dx), DRO: of dresidual_out, DRES: of
 // dresidual (NoT: absent).
 //   dh = rs dy w - h rs^3 mean(h dy w) (+ dresidual_out)
-// dweight and dbias are summed over a thread's rows in registers, 16 a vector step; with four
-// steps (rows of up to 16384 columns) in tensor memory, which this kernel has no other use
-// for: 16 columns of the thread's lane a step, read and written once a row. (Four steps in
-// registers leave no room for the row itself.)
-template <typename H, typename DY, typename DRO, typename DRES, int K>
+// What a warp does once a row (waits, releases, the total) costs as much as a vector step, so
+// four steps a thread pay, for 16-bit rows at least. dweight and dbias are summed over a
+// thread's rows: 16 registers a step, which with four steps leave no room for the row itself.
+// They are kept in tensor memory then, which this kernel has no other use for: 16 columns of
+// the thread's lane a step, read and written once a row. Those kernels have the row group's
+// size kG built in (0: chosen at run time).
+template <typename H, typename DY, typename DRO, typename DRES, int K, int kG>
 __global__ void __launch_bounds__(kBwdThreads, 1) fused_bwd_kernel(const FusedBwdParams p, const RowPlan pl) {
   constexpr bool kDro = Present<DRO>::value, kDres = Present<DRES>::value, kTmem = K > kBwdRegSteps;
   constexpr int kStreams = kDro ? 3 : 2;
   constexpr int kH = Vec8<H>::kBytes / 8, kDy = Vec8<DY>::kBytes / 8;
   RowCtx c = row_begin(pl, p.N);
+  const int G = kTmem ? kG : pl.G, KC = kTmem ? bwd_unit_steps(kG) : pl.KC, R = kTmem ? 1 : pl.R;
   pdl_launch_dependents();
   if constexpr (kTmem) {
     if (c.warp == 0) tmem_alloc_warp(&c.bars->tmem, kTmemCols);
@@ -94,58 +107,43 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fused_bwd_kernel(const FusedBw
   int slot = 0;
   uint32_t phase = 0;
   int64_t unit = 0;
+  float rs_next = c.units > 0 ? ld1(&p.rstd[c.first * R]) : 0.f;  // a row ahead of its use
   for (int64_t tile = c.first; tile < pl.tiles; tile += c.step) {
-    const int64_t row0 = tile * pl.R;
-    const int nrows = static_cast<int>(min(static_cast<int64_t>(pl.R), p.rows - row0));
+    const int64_t row0 = tile * R;
+    const int nrows = kTmem ? 1 : static_cast<int>(min(static_cast<int64_t>(R), p.rows - row0));
     for (int r = 0; r < nrows; ++r) {
       const int64_t row = row0 + r;
       const int64_t e0 = row * p.N + c.slice0;
-      const float rs = ld1(&p.rstd[row]);
+      const float rs = rs_next;
+      const int64_t next = r + 1 < nrows ? row + 1 : (tile + c.step) * R;
+      if (next < p.rows) rs_next = ld1(&p.rstd[next]);
       Raw8<H> h[K];
       Raw8<DY> dy[K];
       Raw8<std::conditional_t<kDro, DRO, __half>> dro[kDro ? K : 1];
       float2 s2 = make_float2(0.f, 0.f);
-      if constexpr (kTmem) tmem_wait_st();  // of the row before
 #pragma unroll
       for (int j = 0; j < K; ++j) {
-        const int first_step = j & ~(pl.KC - 1);
-        const int col = (j * pl.G + c.gl) * 8;
-        float2(&sum)[8] = sums[kTmem ? 0 : j];
-        if constexpr (kTmem) tmem_ld16(sums_at + j * 16, sum);
+        const int first_step = j & ~(KC - 1);
+        const int col = j * (G * 8) + c.gl * 8;
         if (r == 0 && j == first_step) mbar_wait(&c.full[slot], phase, kSiteBwdFull);
-        float2 hg[4], g[4];
         if (col < c.ncols) {
           const unsigned char* base = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;
-          const int at = r * static_cast<int>(p.N) + col - first_step * pl.G * 8;
+          const int at = (kTmem ? 0 : r * static_cast<int>(p.N)) + c.gl * 8 + (j - first_step) * (G * 8);
           h[j].load(base + at * kH);
           dy[j].load(base + pl.off[1] + at * kDy);
           if constexpr (kDro) dro[j].load(base + pl.off[2] + at * (Vec8<DRO>::kBytes / 8));
-          float2 w[4];
-          h[j].get(hg);
+          float2 hv[4], g[4], w[4];
+          h[j].get(hv);
           dy[j].get(g);
           affine8(pl, c.w, col, w);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            hg[i] = mul2(hg[i], g[i]);
-            s2 = fma2(hg[i], w[i], s2);
-          }
+          for (int i = 0; i < 4; ++i) s2 = fma2(mul2(hv[i], g[i]), w[i], s2);
+          if constexpr (!kTmem) add_sums(sums[j], hv, g, rs);
         } else {
           h[j].zero();
           dy[j].zero();
-#pragma unroll
-          for (int i = 0; i < 4; ++i) hg[i] = g[i] = make_float2(0.f, 0.f);
         }
-        if constexpr (kTmem) {
-          __syncwarp();
-          tmem_wait_ld();
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sum[i] = fma2(hg[i], splat2(rs), sum[i]);
-          sum[4 + i] = add2(g[i], sum[4 + i]);
-        }
-        if constexpr (kTmem) tmem_st16(sums_at + j * 16, sum);
-        if (r == nrows - 1 && ((j + 1) & (pl.KC - 1)) == 0) {
+        if (r == nrows - 1 && ((j + 1) & (KC - 1)) == 0) {
           if (release_unit(c, slot) && unit + pl.S < c.units)
             issue_unit(pl, c, unit + pl.S, slot, p.rows, p.N, src, bytes, policy);
           __syncwarp();
@@ -163,16 +161,33 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fused_bwd_kernel(const FusedBw
       row_total<true, false>(pl, c, s, unused, kSiteBwdCluster,
                              [&] { draw8(p.drop, c.slice0 + c.gl * 8, row, offset, words); });
       const float t = -(rs * rs * rs * (s * inv_n));
+      if constexpr (kTmem) tmem_wait_st();  // of the row before
 #pragma unroll
       for (int j = 0; j < K; ++j) {
-        const int col = (j * pl.G + c.gl) * 8;
-        if (col >= c.ncols) continue;
+        const int col = j * (G * 8) + c.gl * 8;
+        // tensor memory is slow to answer: asked before the mask is drawn, read after it
+        if constexpr (kTmem) {
+          __syncwarp();
+          tmem_ld16(sums_at + j * 16, sums[0]);
+        } else if (col >= c.ncols) {
+          continue;
+        }
+        if (j > 0) draw8(p.drop, c.slice0 + col, row, offset, words);
         float2 d[4], g[4], w[4];
         h[j].get(d);
         dy[j].get(g);
+        if constexpr (kTmem) {
+          tmem_wait_ld();
+          add_sums(sums[0], d, g, rs);
+          tmem_st16(sums_at + j * 16, sums[0]);
+          if (col >= c.ncols) continue;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) g[i] = mul2(g[i], splat2(rs));
+        }
         affine8(pl, c.w, col, w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = fma2(mul2(g[i], w[i]), splat2(rs), mul2(d[i], splat2(t)));
+        for (int i = 0; i < 4; ++i) d[i] = fma2(g[i], w[i], mul2(d[i], splat2(t)));
         if constexpr (kDro) {
           dro[j].get(g);
 #pragma unroll
@@ -186,7 +201,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fused_bwd_kernel(const FusedBw
           d[i] = mul2(d[i], splat2(p.drop.scale));
           zero[i] = make_float2(0.f, 0.f);
         }
-        if (j > 0) draw8(p.drop, c.slice0 + col, row, offset, words);
         select8(p.drop, words, d, zero, g);
         Pair8<DY>::store(static_cast<unsigned char*>(p.dx) + (e0 + col) * kDy, g);
       }

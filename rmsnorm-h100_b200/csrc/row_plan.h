@@ -15,10 +15,11 @@ inline int pow2_ceil(int64_t v) {
 }
 
 // Plans rows of N columns whose tensors have elements of bytes[i] (0: absent). odd: the kernels
-// of odd_kernels.cuh, otherwise N is a multiple of 8.
-// threads of a CTA, max_steps: vector steps a thread can hold. Returns why there is no plan, or null.
+// of odd_kernels.cuh, otherwise N is a multiple of 8. threads of a CTA, max_steps: vector steps
+// a thread can hold, built_in: the row group of a kernel made for one (four steps, units of
+// bwd_unit_steps, a row each), 0: chosen here. Returns why there is no plan, or null.
 inline const char* plan_rows(int64_t rows, int64_t N, const int (&bytes)[3], bool bias, int threads, int max_steps,
-                             int sms, RowPlan* pl, int* k, int* smem, bool odd = false) {
+                             int sms, RowPlan* pl, int* k, int* smem, bool odd = false, int built_in = 0) {
   const int64_t cta_cols = static_cast<int64_t>(threads) * 8 * max_steps;
   if (N > cta_cols * kMaxRowCtas) return "rows wider than a cluster holds";
   pl->C = N > cta_cols ? pow2_ceil((N + cta_cols - 1) / cta_cols) : 1;
@@ -31,17 +32,18 @@ inline const char* plan_rows(int64_t rows, int64_t N, const int (&bytes)[3], boo
   // Few rows: as many threads to a row as it has vectors, for the latency. Otherwise as few as
   // hold it, so that a CTA works on several rows at once and their totals overlap.
   const int steps = rows <= sms ? 1 : max_steps;
-  pl->G = std::clamp(pow2_ceil((vecs + steps - 1) / steps), 32, threads);
-  *k = pow2_ceil((vecs + pl->G - 1) / pl->G);
+  pl->G = built_in ? built_in : std::clamp(pow2_ceil((vecs + steps - 1) / steps), 32, threads);
+  *k = built_in ? max_steps : pow2_ceil((vecs + pl->G - 1) / pl->G);
   pl->groups = pl->C > 1 ? 1 : threads / pl->G;
   const int elem = bytes[0] + bytes[1] + bytes[2];
   pl->KC = *k;
   while (pl->KC > 1 && pl->KC * pl->G * 8 * elem > 32768) pl->KC >>= 1;
+  if (built_in) pl->KC = bwd_unit_steps(built_in);
   pl->unit_shift = 0;
   while ((pl->KC << pl->unit_shift) < *k) ++pl->unit_shift;
   // Short rows go several to a unit: a copy of about 4 KB at least, but no fewer tiles than groups.
   pl->R = 1;
-  if (pl->C == 1 && pl->KC == *k) {
+  if (pl->C == 1 && pl->KC == *k && !built_in) {
     const int64_t fair = rows / (static_cast<int64_t>(sms) * pl->groups);
     pl->R = static_cast<int>(std::clamp<int64_t>(std::min<int64_t>(4096 / (N * elem), fair), 1, 8));
   }

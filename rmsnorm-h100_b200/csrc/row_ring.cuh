@@ -36,6 +36,10 @@ struct RowPlan {
   int64_t tiles;        // units of R rows
 };
 
+// Steps of a ring unit in the kernels with a built-in row group of g threads and four steps:
+// units of 24 KB at most.
+__host__ __device__ constexpr int bwd_unit_steps(int g) { return g <= 128 ? 4 : g == 256 ? 2 : 1; }
+
 // Shared memory after the rings and the affine copies.
 struct RowBars {
   uint64_t full[kMaxUnits];
@@ -197,7 +201,7 @@ __device__ __forceinline__ bool release_unit(const RowCtx& c, int slot) {
 // for the others': work that does not need the total.
 // A warp writes slot k again two totals later, after it has taken the total in between; every
 // warp contributed to that one after it had taken slot k.
-// Across the cluster, `xbar[k]` completes when the C CTAs' 8-byte contributions have landed
+// Across the cluster (one group a CTA), `xbar[k]` completes when the C CTAs' 8-byte contributions have landed
 // (they may land before it is armed). A peer writes slot k again two totals later, when it has
 // this CTA's contribution to the one in between; warp 0 sends that after every warp of this
 // CTA has contributed to it, with slot k read.
