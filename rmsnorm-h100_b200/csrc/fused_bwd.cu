@@ -89,9 +89,10 @@ int make_plan(UnitDevice* ud, const rmsnorm_b200_dropout_bwd_args* a, Plan* pl) 
       pl->kernel = pl->k == 1 ? odd_bwd_kernel<1> : odd_bwd_kernel<2>;
     } else {
       // 16-bit rows that fill more than two steps of a warp: four steps a thread, sums in tensor
-      // memory. The others: sums in registers.
+      // memory. The others, and few rows (a CTA each, as many threads as it has): registers.
       int g = 0;
-      if (a->h_dtype != RMSNORM_B200_F32 && a->dout_dtype == a->h_dtype && a->hidden > 32 * 8 * kBwdRegSteps)
+      const bool few = a->rows <= ud->sm_count && a->hidden <= kBwdThreads * 8 * kBwdRegSteps;
+      if (!few && a->h_dtype != RMSNORM_B200_F32 && a->dout_dtype == a->h_dtype && a->hidden > 32 * 8 * kBwdRegSteps)
         g = std::min(pow2_ceil((a->hidden + 8 * kBwdTmemSteps - 1) / (8 * kBwdTmemSteps)), kBwdThreads);
       pl->why = plan_rows(a->rows, a->hidden, bytes, false, kBwdThreads, g ? kBwdTmemSteps : kBwdRegSteps, ud->sm_count,
                           &pl->rows, &pl->k, &pl->smem, false, g);

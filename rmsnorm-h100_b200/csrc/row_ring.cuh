@@ -36,9 +36,11 @@ struct RowPlan {
   int64_t tiles;        // units of R rows
 };
 
-// Steps of a ring unit in the kernels with a built-in row group of g threads and four steps:
-// units of 24 KB at most.
-__host__ __device__ constexpr int bwd_unit_steps(int g) { return g <= 128 ? 4 : g == 256 ? 2 : 1; }
+// Steps of a ring unit in the kernels with a built-in row group of g threads and four steps.
+// Every unit costs each warp a wait and a release: at 1.3e8 elements, 16384 columns (g = 512)
+// take 256 us in units of two steps (48 KB), 298 us of one; 8192 columns (g = 256) 237 us in
+// units of four steps, 251 us of two.
+__host__ __device__ constexpr int bwd_unit_steps(int g) { return g <= 256 ? 4 : 2; }
 
 // Shared memory after the rings and the affine copies.
 struct RowBars {
@@ -183,7 +185,8 @@ __device__ __forceinline__ void issue_unit(const RowPlan& pl, const RowCtx& c, i
 }
 
 // Every lane of a warp, after its last read of the slot. True on lane 0 of the group's last
-// warp: it refills the slot.
+// warp: it refills the slot. (Refilling when the row's total is complete, which needs no count,
+// starts the copies later: 7 % slower with four warps a row or fewer.)
 __device__ __forceinline__ bool release_unit(const RowCtx& c, int slot) {
   __syncwarp();
   if (c.lane != 0) return false;
