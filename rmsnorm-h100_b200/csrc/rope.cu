@@ -70,23 +70,27 @@ RopeParams params(const rmsnorm_b200_rope_args* a) {
   return p;
 }
 
-// Whether the vectorised kernels take these tensors; nothing but whole chunks of 4 elements.
+// Whether the vectorised kernels take these tensors: nothing but whole 16-byte granules.
 bool vectorised(const rmsnorm_b200_rope_args* a, std::initializer_list<const rmsnorm_b200_rope_tensor*> tensors) {
   if (a->head_dim % 8 || a->rotary_dim % 8 || !aligned_to(a->table, 16)) return false;
-  const uintptr_t chunk = 4 * elem_bytes(a->dtype);
+  const int granule = 16 / elem_bytes(a->dtype);
   for (const auto* t : tensors)
-    if (t && (!aligned_to(t->data, chunk) || t->token_stride % 4 || t->head_stride % 4)) return false;
+    if (t && (!aligned_to(t->data, 16) || t->token_stride % granule || t->head_stride % granule)) return false;
   return true;
 }
 
-// U: heads a lane works on at a time.
+constexpr int kRopeSlots = 8;         // ring slots of a warp, at most
+constexpr int kRopeSmem = 208 * 1024;  // beside the backward's 16 KB of static shared memory
+
+// u: heads a lane works on at a time.
 struct RopeGrid {
   RopePlan pl;
   dim3 grid;
-  int threads;
+  int threads, smem;
 };
 
-RopeGrid plan(const rmsnorm_b200_rope_args* a, int u, int64_t most_ctas) {
+// tensors: that stream through a warp's ring (0: no ring).
+RopeGrid plan(const rmsnorm_b200_rope_args* a, int u, int tensors, int sms) {
   RopeGrid g = {};
   RopePlan& pl = g.pl;
   while ((8 << pl.lanes_shift) < a->head_dim) ++pl.lanes_shift;
@@ -97,10 +101,20 @@ RopeGrid plan(const rmsnorm_b200_rope_args* a, int u, int64_t most_ctas) {
   const int jobs = pl.jobs[0] + pl.jobs[1];
   pl.cta_jobs = std::min(jobs, kRopeWarps);
   const int at_once = static_cast<int>(std::clamp<int64_t>(a->tokens, 1, kRopeWarps / pl.cta_jobs));
-  g.threads = at_once * pl.cta_jobs * 32;
+  const int warps = at_once * pl.cta_jobs;
+  g.threads = warps * 32;
   const int64_t across = (jobs + pl.cta_jobs - 1) / pl.cta_jobs;
-  const int64_t along = std::clamp<int64_t>((a->tokens + at_once - 1) / at_once, 1, std::max<int64_t>(1, most_ctas / across));
+  // one CTA an SM where its rings take the shared memory
+  const int64_t most = std::max<int64_t>(1, (tensors ? 1 : 2) * static_cast<int64_t>(sms) / across);
+  const int64_t along = std::clamp<int64_t>((a->tokens + at_once - 1) / at_once, 1, most);
   g.grid = dim3(static_cast<unsigned>(along), static_cast<unsigned>(across));
+  if (tensors) {
+    pl.slot_bytes = static_cast<uint32_t>(heads * a->head_dim * elem_bytes(a->dtype));
+    const int slot = warps * tensors * static_cast<int>(pl.slot_bytes) + warps * 8;
+    const int64_t tokens = (a->tokens + along * at_once - 1) / (along * at_once);  // of a warp
+    pl.S = static_cast<int>(std::clamp<int64_t>(tokens, 1, std::min(kRopeSlots, kRopeSmem / slot)));
+    g.smem = pl.S * slot;
+  }
   return g;
 }
 
@@ -114,22 +128,32 @@ struct RopeLaunch {  // for rmsnorm_b200_last_plan
 std::string describe_rope(const void* data) {
   const RopeLaunch& l = *static_cast<const RopeLaunch*>(data);
   char buf[128];
-  std::snprintf(buf, sizeof(buf), "%s grid=%ux%u threads=%d lanes=%d jobs=%d+%d", l.kind, l.x, l.y, l.threads,
-                1 << l.pl.lanes_shift, l.pl.jobs[0], l.pl.jobs[1]);
+  std::snprintf(buf, sizeof(buf), "%s grid=%ux%u threads=%d lanes=%d jobs=%d+%d S=%d", l.kind, l.x, l.y, l.threads,
+                1 << l.pl.lanes_shift, l.pl.jobs[0], l.pl.jobs[1], l.pl.S);
   return buf;
 }
 
 // Launches with programmatic dependent launch: the kernels wait for the one before them
 // before their first global access.
 template <typename Kernel>
-int launch(Kernel kernel, dim3 grid, int threads, cudaStream_t stream, const RopeParams& p, const RopePlan& pl,
+int launch(UnitDevice* ud, Kernel kernel, const RopeGrid& g, cudaStream_t stream, const RopeParams& p,
            const char* kind) {
+  const RopePlan& pl = g.pl;
+  const dim3 grid = g.grid;
+  const int threads = g.threads;
+  {
+    std::lock_guard<std::mutex> lock(ud->mu);
+    if (ud->attrs_done.insert(reinterpret_cast<const void*>(kernel)).second &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRopeSmem) != cudaSuccess)
+      return RMSNORM_B200_ERR_CUDA;
+  }
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = g.smem;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -142,17 +166,14 @@ int launch(Kernel kernel, dim3 grid, int threads, cudaStream_t stream, const Rop
   return launched(describe_rope, l);
 }
 
-#ifndef RMSB_ROPE_CTAS
-#define RMSB_ROPE_CTAS 2
-#endif
-constexpr int kFwdCtas = RMSB_ROPE_CTAS, kBwdCtas = RMSB_ROPE_CTAS;  // of an SM, at most
-
 using RopeKernel = void (*)(const RopeParams, const RopePlan);
 
+// One head a lane without a ring, or several with one.
 template <typename T, int U>
 RopeKernel pick_fwd(bool interleaved, bool norm) {
-  if (interleaved) return norm ? rope_fwd_kernel<T, U, true, true> : rope_fwd_kernel<T, U, true, false>;
-  return norm ? rope_fwd_kernel<T, U, false, true> : rope_fwd_kernel<T, U, false, false>;
+  constexpr bool kRing = U > 1;
+  if (interleaved) return norm ? rope_fwd_kernel<T, U, true, true, kRing> : rope_fwd_kernel<T, U, true, false, kRing>;
+  return norm ? rope_fwd_kernel<T, U, false, true, kRing> : rope_fwd_kernel<T, U, false, false, kRing>;
 }
 
 template <int U>
@@ -163,18 +184,21 @@ RopeKernel pick_fwd(const RopeParams& p) {
 
 template <typename T, int U, bool kPerHead>
 RopeKernel pick_bwd(bool interleaved, bool norm) {
+  constexpr int kBatch = 2;
   if (interleaved)
-    return norm ? rope_bwd_kernel<T, U, true, true, kPerHead> : rope_bwd_kernel<T, U, true, false, kPerHead>;
-  return norm ? rope_bwd_kernel<T, U, false, true, kPerHead> : rope_bwd_kernel<T, U, false, false, kPerHead>;
+    return norm ? rope_bwd_kernel<T, U, kBatch, true, true, kPerHead> : rope_bwd_kernel<T, U, kBatch, true, false, kPerHead>;
+  return norm ? rope_bwd_kernel<T, U, kBatch, false, true, kPerHead> : rope_bwd_kernel<T, U, kBatch, false, false, kPerHead>;
 }
 
-constexpr int kBwdHeads16 = 4, kBwdHeads32 = 2;  // heads a lane in the backward, 16- and 32-bit types
+// Heads a lane in the backward: two with sums for each of them.
+constexpr int bwd_heads(bool per_head) { return per_head ? 2 : 4; }
 
 template <bool kPerHead>
 RopeKernel pick_bwd(const RopeParams& p) {
-  if (p.dt == RMSNORM_B200_BF16) return pick_bwd<__nv_bfloat16, kBwdHeads16, kPerHead>(p.interleaved, p.norm);
-  return p.dt == RMSNORM_B200_F16 ? pick_bwd<__half, kBwdHeads16, kPerHead>(p.interleaved, p.norm)
-                                  : pick_bwd<float, kBwdHeads32, kPerHead>(p.interleaved, p.norm);
+  constexpr int kHeads = bwd_heads(kPerHead);
+  if (p.dt == RMSNORM_B200_BF16) return pick_bwd<__nv_bfloat16, kHeads, kPerHead>(p.interleaved, p.norm);
+  return p.dt == RMSNORM_B200_F16 ? pick_bwd<__half, kHeads, kPerHead>(p.interleaved, p.norm)
+                                  : pick_bwd<float, kHeads, kPerHead>(p.interleaved, p.norm);
 }
 
 int run_fwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_tensor* qo, const rmsnorm_b200_rope_tensor* ko,
@@ -201,10 +225,10 @@ int run_fwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_tensor* qo,
   if (ko) p.out[1] = tensor(*ko);
   if (vectorised(a, {&a->q, &a->k, qo, ko})) {
     // Four heads a lane where that leaves every SM eight warps to run; single heads below.
-    RopeGrid g = plan(a, 4, int64_t{kFwdCtas} * ud->sm_count);
+    RopeGrid g = plan(a, 4, 1, ud->sm_count);
     const bool wide = a->tokens * (g.pl.jobs[0] + g.pl.jobs[1]) >= int64_t{8} * ud->sm_count;
-    if (!wide) g = plan(a, 1, int64_t{kFwdCtas} * ud->sm_count);
-    return launch(wide ? pick_fwd<4>(p) : pick_fwd<1>(p), g.grid, g.threads, stream, p, g.pl, "rope_fwd");
+    if (!wide) g = plan(a, 1, 0, ud->sm_count);
+    return launch(ud, wide ? pick_fwd<4>(p) : pick_fwd<1>(p), g, stream, p, "rope_fwd");
   }
   const int64_t work = a->tokens * (a->q_heads + a->k_heads);
   const int64_t warps = kGenericThreads / 32;
@@ -217,9 +241,7 @@ struct BwdPlan {
   int64_t chunk = 1, chunks = 1;  // scalar kernel
   bool vec = false;
   bool per_head = false;          // partial rows of every head
-  int threads = 0;
-  dim3 grid;
-  RopePlan rope;
+  RopeGrid rope;
   int64_t rows = 0, width = 0;    // partial rows of dweight
 };
 
@@ -239,11 +261,8 @@ BwdPlan plan_bwd(const UnitDevice* ud, const rmsnorm_b200_rope_args* a, const rm
   pl.per_head = (a->q_weight && a->q_weight_heads > 1) || (a->k_weight && a->k_weight_heads > 1);
   pl.vec = vectorised(a, {&a->q, &a->k, &g->dq_out, &g->dk_out, &g->dq, &g->dk});
   if (pl.vec) {
-    const RopeGrid gr = plan(a, a->dtype == RMSNORM_B200_F32 ? kBwdHeads32 : kBwdHeads16, int64_t{kBwdCtas} * ud->sm_count);
-    pl.rope = gr.pl;
-    pl.threads = gr.threads;
-    pl.grid = gr.grid;
-    const int64_t along = gr.grid.x, across = gr.grid.y;
+    pl.rope = plan(a, bwd_heads(pl.per_head), 2, ud->sm_count);
+    const int64_t along = pl.rope.grid.x, across = pl.rope.grid.y;
     pl.rows = pl.per_head ? along : along * across;
     pl.width = (pl.per_head ? heads : 2) * a->head_dim;
     return pl;
@@ -295,8 +314,7 @@ int run_bwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g, v
   p.part = need ? static_cast<float*>(ws) : nullptr;
   if (a->tokens > 0) {
     if (pl.vec) {
-      st = launch(pl.per_head ? pick_bwd<true>(p) : pick_bwd<false>(p), pl.grid, pl.threads, stream, p,
-                  pl.rope, "rope_bwd");
+      st = launch(ud, pl.per_head ? pick_bwd<true>(p) : pick_bwd<false>(p), pl.rope, stream, p, "rope_bwd");
     } else {
       const dim3 grid(static_cast<unsigned>(heads), static_cast<unsigned>(pl.chunks));
       rope_bwd_generic_kernel<<<grid, kGenericThreads, 0, stream>>>(p, pl.chunk);

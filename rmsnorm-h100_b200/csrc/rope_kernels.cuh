@@ -33,15 +33,19 @@ struct RopeParams {
   float eps;
 };
 
-// Row of the table for pair i of a token, or -1 where the position lies outside it.
-__device__ __forceinline__ int64_t rope_row(const RopeParams& p, int64_t token, int pair) {
-  const int axis = static_cast<int>(p.axis_of[pair >> 5] >> (2 * (pair & 31))) & 3;
-  const int64_t at = axis * p.pos_axis + token;
+// Row of the table for the position at index `at`, or -1 where it lies outside the table.
+__device__ __forceinline__ int64_t rope_row_at(const RopeParams& p, int64_t at) {
   const int64_t t = p.pos64 ? ld1(static_cast<const int64_t*>(p.pos) + at)
                             : static_cast<int64_t>(ld1(static_cast<const int32_t*>(p.pos) + at));
   if (t >= 0 && t < p.table_rows) return t;
   record_error(RMSNORM_B200_ERR_INVALID_ARGUMENT, kSiteRopePosition);
   return -1;
+}
+
+// The same for a pair of a token.
+__device__ __forceinline__ int64_t rope_row(const RopeParams& p, int64_t token, int pair) {
+  const int axis = static_cast<int>(p.axis_of[pair >> 5] >> (2 * (pair & 31))) & 3;
+  return rope_row_at(p, axis * p.pos_axis + token);
 }
 
 __device__ __forceinline__ void rope_cos_sin(const RopeParams& p, int64_t token, int pair, float& c, float& s) {
@@ -155,7 +159,7 @@ __global__ void __launch_bounds__(kGenericThreads) rope_bwd_generic_kernel(const
 
 // ---------------------------------------------------------------------------------------
 // Vectorised kernels: head_dim and rotary_dim multiples of 8, strides and addresses of whole
-// 4-element chunks.
+// 16-byte granules.
 //
 // A lane owns two 4-element chunks of a head, chosen so that both columns of a pair are its
 // own: a lane of the turned part has pairs 4l .. 4l + 3, that is columns 4l .. and
@@ -163,6 +167,12 @@ __global__ void __launch_bounds__(kGenericThreads) rope_bwd_generic_kernel(const
 // lane of the rest has eight neighbouring columns. So no value crosses lanes for the turn,
 // and a lane needs only four cosines and four sines, which serve every head it works on.
 // L = the smallest power of two with 8 L >= head_dim lanes hold a head; a warp holds 32 / L.
+//
+// A warp streams its heads of token after token through a ring in shared memory of its own
+// (one bulk copy per tensor and token, or one per head where a token's heads are not
+// neighbours), so it waits for nobody but its copies; what a token costs beyond its data
+// (positions, table, addresses) is spread over the U heads of a lane and fetched ahead: the
+// position two tokens, cosines and sines one.
 // ---------------------------------------------------------------------------------------
 template <typename T>
 struct Chunk4 {
@@ -170,7 +180,7 @@ struct Chunk4 {
   static constexpr bool kB = std::is_same_v<T, __nv_bfloat16>;
   __device__ __forceinline__ void load(const void* p, int64_t e) {
     const T* q = static_cast<const T*>(p) + e;
-    v = RMSB_DBG_OK(q, 8, kDbgVecLoad) ? __ldcs(reinterpret_cast<const uint2*>(q)) : make_uint2(0u, 0u);
+    v = RMSB_DBG_OK(q, 8, kDbgVecLoad) ? *reinterpret_cast<const uint2*>(q) : make_uint2(0u, 0u);
   }
   __device__ __forceinline__ void get(float2* f) const {
     f[0] = kB ? unpack_bf16x2_pair(v.x) : unpack_f16x2_pair(v.x);
@@ -188,7 +198,7 @@ struct Chunk4<float> {
   float4 v;
   __device__ __forceinline__ void load(const void* p, int64_t e) {
     const float* q = static_cast<const float*>(p) + e;
-    v = RMSB_DBG_OK(q, 16, kDbgVecLoad) ? __ldcs(reinterpret_cast<const float4*>(q)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    v = RMSB_DBG_OK(q, 16, kDbgVecLoad) ? *reinterpret_cast<const float4*>(q) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
   __device__ __forceinline__ void get(float2* f) const {
     f[0] = make_float2(v.x, v.y);
@@ -203,6 +213,8 @@ struct Chunk4<float> {
 // A warp takes U * (32 / L) heads of a token, all of q or all of k, and keeps them over all
 // the tokens it takes: the weight (and the backward's sums of its gradient) stay in registers.
 struct RopePlan {
+  int32_t S;            // ring slots of a warp
+  uint32_t slot_bytes;  // of one tensor in a slot
   int32_t lanes_shift;  // log2(L)
   int32_t jobs[2];      // warps' shares of a token: of q first, then of k
   int32_t turned_lanes; // lanes of the turned part: rotary_dim / 8
@@ -229,18 +241,40 @@ __device__ __forceinline__ RopeLane rope_lane(const RopeParams& p, const RopePla
   return t;
 }
 
-// The lane's four cosines and sines for a token.
-__device__ __forceinline__ void rope_lane_turn(const RopeParams& p, const RopeLane& t, int64_t token, float (&c)[4],
-                                               float (&s)[4]) {
-  if (!t.turned) return;
-  const int i0 = 4 * t.l;
-  const uint32_t axis = static_cast<uint32_t>(p.axis_of[i0 >> 5] >> (2 * (i0 & 31))) & 0xffu;  // of four pairs
-  if (axis == (axis & 3u) * 0x55u) {  // one axis for all four
-    const int64_t r = rope_row(p, token, i0);
-    if (r >= 0) {
-      const float* row = p.table + r * p.rd + i0;
-      const float4 cv = RMSB_DBG_OK(row, 16, kDbgVecLoad) ? __ldg(reinterpret_cast<const float4*>(row)) : float4{};
-      const float* srow = row + p.rd / 2;
+// The lane's four cosines and sines, a token ahead of their use, and the table row they come
+// from a token before that. Where the four pairs have several axes, their rows are looked up
+// with the cosines.
+struct RopeTurn {
+  float c[4], s[4];
+  int64_t row;    // of the token after the one whose cosines are held; -1: outside the table
+  int64_t first;  // the lane's axis in the positions
+  bool one_axis;
+  __device__ __forceinline__ RopeTurn(const RopeParams& p, const RopeLane& t, int64_t token, int64_t step) : row(-1) {
+    const int i0 = 4 * t.l;
+    const uint32_t axes = t.turned ? static_cast<uint32_t>(p.axis_of[i0 >> 5] >> (2 * (i0 & 31))) & 0xffu : 0u;
+    one_axis = axes == (axes & 3u) * 0x55u;
+    first = (axes & 3u) * p.pos_axis;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = s[i] = 0.f;
+    look_up(p, t, token);
+    advance(p, t, token, token + step);
+  }
+  __device__ __forceinline__ void look_up(const RopeParams& p, const RopeLane& t, int64_t token) {
+    if (t.turned && one_axis && token < p.tokens) row = rope_row_at(p, first + token);
+  }
+  // Loads the cosines of `token` (whose row is held) and looks up the row of `after`.
+  __device__ __forceinline__ void advance(const RopeParams& p, const RopeLane& t, int64_t token, int64_t after) {
+    if (!t.turned || token >= p.tokens) return;
+    const int i0 = 4 * t.l;
+    if (!one_axis) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rope_cos_sin(p, token, i0 + i, c[i], s[i]);
+      return;
+    }
+    if (row >= 0) {
+      const float* crow = p.table + row * p.rd + i0;
+      const float* srow = crow + p.rd / 2;
+      const float4 cv = RMSB_DBG_OK(crow, 16, kDbgVecLoad) ? __ldg(reinterpret_cast<const float4*>(crow)) : float4{};
       const float4 sv = RMSB_DBG_OK(srow, 16, kDbgVecLoad) ? __ldg(reinterpret_cast<const float4*>(srow)) : float4{};
       c[0] = cv.x; c[1] = cv.y; c[2] = cv.z; c[3] = cv.w;
       s[0] = sv.x; s[1] = sv.y; s[2] = sv.z; s[3] = sv.w;
@@ -248,35 +282,52 @@ __device__ __forceinline__ void rope_lane_turn(const RopeParams& p, const RopeLa
 #pragma unroll
       for (int i = 0; i < 4; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);
     }
-    return;
+    look_up(p, t, after);
   }
+};
+
+// A token's cosines and sines as the turn uses them, the sines with both signs (the paired
+// instructions negate no operand). sign -1 turns back.
+struct RopeAngles {
+  float2 c[2], s[2], n[2];
+  __device__ __forceinline__ RopeAngles(const RopeTurn& t, bool back) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) rope_cos_sin(p, token, i0 + i, c[i], s[i]);
-}
+    for (int i = 0; i < 2; ++i) {
+      c[i] = make_float2(t.c[2 * i], t.c[2 * i + 1]);
+      const float2 plus = make_float2(t.s[2 * i], t.s[2 * i + 1]), minus = make_float2(-plus.x, -plus.y);
+      s[i] = back ? minus : plus;
+      n[i] = back ? plus : minus;
+    }
+  }
+};
 
 // y holds columns a .. a + 3, b .. b + 3, in pairs of neighbours.
 template <bool kInterleaved>
-__device__ __forceinline__ void rope_turn8(const RopeLane& t, const float (&c)[4], const float (&s)[4],
-                                           float2 (&y)[4]) {
+__device__ __forceinline__ void rope_turn8(const RopeLane& t, const RopeAngles& r, float2 (&y)[4]) {
   if (!t.turned) return;
   if constexpr (kInterleaved) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      y[i] = make_float2(y[i].x * c[i] - y[i].y * s[i], y[i].y * c[i] + y[i].x * s[i]);
+    for (int i = 0; i < 4; ++i) {
+      const float c = i & 1 ? r.c[i >> 1].y : r.c[i >> 1].x, s = i & 1 ? r.s[i >> 1].y : r.s[i >> 1].x;
+      y[i] = make_float2(y[i].x * c - y[i].y * s, y[i].y * c + y[i].x * s);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float2 u = y[i], v = y[2 + i];
-      const float2 cc = make_float2(c[2 * i], c[2 * i + 1]), ss = make_float2(s[2 * i], s[2 * i + 1]);
-      y[i] = fma2(v, make_float2(-ss.x, -ss.y), mul2(u, cc));
-      y[2 + i] = fma2(u, ss, mul2(v, cc));
+      y[i] = fma2(v, r.n[i], mul2(u, r.c[i]));
+      y[2 + i] = fma2(u, r.s[i], mul2(v, r.c[i]));
     }
   }
 }
 
-__device__ __forceinline__ float rope_head_sum(float v, int lanes_shift) {
-  for (int o = 1 << lanes_shift >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// Sums over the lanes of a head, of N values at once: their shuffles overlap.
+template <int N>
+__device__ __forceinline__ void rope_head_sums(float (&v)[N], int lanes_shift) {
+  for (int o = 1 << lanes_shift >> 1; o > 0; o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  }
 }
 
 __device__ __forceinline__ void rope_weight8(const RopeParams& p, int k, int64_t head, const RopeLane& t,
@@ -317,24 +368,112 @@ __device__ __forceinline__ RopeJob rope_job(const RopeParams& p, const RopePlan&
   return b;
 }
 
-// The lane's chunks of a tensor: element offset of its first head in token 0, and strides.
+// Where the lane's heads lie in a tensor in global memory: its first head of the current token,
+// moved on from token to token and from head to head.
 template <typename T>
 struct RopePlace {
   T* p;
-  int64_t ts, us;
+  int64_t token_step, head_step;
   int da, db;
   __device__ __forceinline__ RopePlace(const RopeTensor& x, const RopeLane& t, const RopeJob& b)
-      : p(static_cast<T*>(x.p) + b.head0 * x.hs), ts(x.ts), us(b.per * x.hs), da(t.a), db(t.b) {}
-  __device__ __forceinline__ void load(int64_t token, int u, Chunk4<T> (&c)[2]) const {
-    const int64_t e = token * ts + u * us;
-    c[0].load(p, e + da);
-    c[1].load(p, e + db);
+      : p(static_cast<T*>(x.p) + b.token * x.ts + b.head0 * x.hs), token_step(b.step * x.ts), head_step(b.per * x.hs),
+        da(t.a), db(t.b) {}
+  __device__ __forceinline__ void load(const T* head, Chunk4<T> (&c)[2]) const {
+    c[0].load(head, da);
+    c[1].load(head, db);
   }
-  __device__ __forceinline__ void store(int64_t token, int u, const float2 (&y)[4]) const {
-    const int64_t e = token * ts + u * us;
-    Chunk4<T>::store(p, e + da, y);
-    Chunk4<T>::store(p, e + db, y + 2);
+  __device__ __forceinline__ void store(T* head, const float2 (&y)[4]) const {
+    Chunk4<T>::store(head, da, y);
+    Chunk4<T>::store(head, db, y + 2);
   }
+};
+
+// A warp's ring: its heads of kTensors tensors for S tokens. Every lane of the warp calls.
+template <typename T, int U, int kTensors>
+struct RopeRing {
+  unsigned char* slots;
+  uint64_t* full;
+  const T* src[kTensors];  // the warp's first head of token `next`
+  int64_t token_step[kTensors], hs[kTensors];
+  int heads;               // of the warp
+  int slot;
+  uint32_t phase;
+  int64_t next;            // token to be copied next
+  __device__ __forceinline__ RopeRing(const RopePlan& pl, const RopeJob& b, const RopeTensor (&x)[kTensors]) {
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    slots = rmsb_dyn_smem + static_cast<size_t>(warp) * pl.S * kTensors * pl.slot_bytes;
+    full = reinterpret_cast<uint64_t*>(rmsb_dyn_smem + static_cast<size_t>(warps) * pl.S * kTensors * pl.slot_bytes) +
+           warp * pl.S;
+    const int first = b.job * U * b.per;
+    heads = min(U * b.per, b.heads - first);
+    for (int i = 0; i < kTensors; ++i) {
+      src[i] = static_cast<const T*>(x[i].p) + b.token * x[i].ts + first * x[i].hs;
+      token_step[i] = b.step * x[i].ts;
+      hs[i] = x[i].hs;
+    }
+    slot = 0;
+    phase = 0;
+    next = b.token;
+    if ((threadIdx.x & 31) == 0) {
+      for (int s = 0; s < pl.S; ++s) mbar_init(&full[s], 1);
+      fence_mbar_init();
+    }
+    __syncwarp();
+  }
+  // Copies token `next` into slot s.
+  __device__ __forceinline__ void issue(const RopeParams& p, const RopeJob& b, const RopePlan& pl, int s,
+                                        uint64_t policy) {
+    if (next < p.tokens) {
+      const int lane = threadIdx.x & 31;
+      const uint32_t head_bytes = p.D * sizeof(T);
+      if (lane == 0) mbar_arrive_expect_tx(&full[s], kTensors * heads * head_bytes);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kTensors; ++i) {
+        unsigned char* dst = slots + static_cast<size_t>(s * kTensors + i) * pl.slot_bytes;
+        if (hs[i] == p.D) {
+          if (lane == 0) bulk_load(dst, src[i], heads * head_bytes, &full[s], policy);
+        } else if (lane < heads) {
+          bulk_load(dst + lane * head_bytes, src[i] + lane * hs[i], head_bytes, &full[s], policy);
+        }
+        src[i] += token_step[i];
+      }
+    }
+    next += b.step;
+  }
+  __device__ __forceinline__ void start(const RopeParams& p, const RopeJob& b, const RopePlan& pl, uint64_t policy) {
+    for (int s = 0; s < pl.S; ++s) issue(p, b, pl, s, policy);
+  }
+  __device__ __forceinline__ void wait(int site) {
+    mbar_wait(&full[slot], phase, site);
+    __syncwarp();
+  }
+  // The lane's first head of the current token.
+  __device__ __forceinline__ const T* held(const RopePlan& pl, const RopeParams& p, const RopeLane& t,
+                                           int tensor) const {
+    return reinterpret_cast<const T*>(slots + (slot * kTensors + tensor) * pl.slot_bytes) + t.sub * p.D;
+  }
+  // After the last load of a token: its slot takes the token S further on.
+  __device__ __forceinline__ void advance(const RopeParams& p, const RopeJob& b, const RopePlan& pl, uint64_t policy) {
+    __syncwarp();
+    fence_proxy_async_smem();
+    issue(p, b, pl, slot, policy);
+    if (++slot == pl.S) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+  // After a wait that ran out: the copies in flight land before the warp leaves.
+  __device__ __forceinline__ void drain(const RopeParams& p, const RopeJob& b, const RopePlan& pl) {
+    if (!abort_requested()) return;
+    const int64_t n = b.token < p.tokens ? (p.tokens - 1 - b.token) / b.step + 1 : 0;
+    for (int s = 0; s < pl.S && s < n; ++s)
+      mbar_wait(&full[s], static_cast<uint32_t>((n - 1 - s) / pl.S) & 1u, kSiteDrain, false);
+  }
+};
+
+struct RopeNoRing {
+  __device__ __forceinline__ RopeNoRing(const RopePlan&, const RopeJob&, const RopeTensor (&)[1]) {}
 };
 
 template <typename T>
@@ -343,12 +482,10 @@ __device__ __forceinline__ void rope_get(const Chunk4<T> (&c)[2], float2 (&y)[4]
   c[1].get(y + 2);
 }
 
-#ifndef RMSB_ROPE_WARPS
-#define RMSB_ROPE_WARPS 16
-#endif
-constexpr int kRopeWarps = RMSB_ROPE_WARPS;  // of a CTA, at most
+constexpr int kRopeWarps = 16;  // of a CTA, at most
 
-template <typename T, int U, bool kInterleaved, bool kNorm>
+// kRing false: few tokens, whose heads a lane loads itself.
+template <typename T, int U, bool kInterleaved, bool kNorm, bool kRing>
 __global__ void __launch_bounds__(kRopeWarps * 32) rope_fwd_kernel(const RopeParams p, const RopePlan pl) {
   pdl_launch_dependents();
   pdl_wait();
@@ -356,52 +493,83 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_fwd_kernel(const RopePar
   const RopeJob b = rope_job(p, pl, t, U);
   if (!b.works) return;
   const int k = b.k;
-  const RopePlace<T> in(k ? p.x[1] : p.x[0], t, b), out(k ? p.out[1] : p.out[0], t, b);
+  const RopeTensor tensors[1] = {k ? p.x[1] : p.x[0]};
+  [[maybe_unused]] RopePlace<T> in(tensors[0], t, b);
+  RopePlace<T> out(k ? p.out[1] : p.out[0], t, b);
+  const uint64_t policy = l2_policy_evict_first();
+  std::conditional_t<kRing, RopeRing<T, U, 1>, RopeNoRing> ring(pl, b, tensors);
+  if constexpr (kRing) ring.start(p, b, pl, policy);
   const bool per_head = p.w_per_head[k];
   const float inv_d = 1.f / static_cast<float>(p.D);
+  const int mine = t.in ? (b.heads - b.head0 + b.per - 1) / b.per : 0;  // the lane has heads u < mine
   float2 w[4];
+  RopeTurn turn(p, t, b.token, b.step);
   if (!per_head) rope_weight8(p, k, 0, t, w);
   for (int64_t token = b.token; token < p.tokens; token += b.step) {
+    const T* head = in.p;
+    int64_t head_step = in.head_step;
+    if constexpr (kRing) {
+      ring.wait(kSiteFwdFull);
+      head = ring.held(pl, p, t, 0);
+      head_step = b.per * p.D;
+    }
     Chunk4<T> x[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (t.in && b.head0 + u * b.per < b.heads)
-        in.load(token, u, x[u]);
+      if (u < mine)
+        in.load(head + u * head_step, x[u]);
       else
         x[u][0].v = x[u][1].v = {};
     }
-    float c[4], s[4];
-    rope_lane_turn(p, t, token, c, s);
+    if constexpr (kRing) ring.advance(p, b, pl, policy);
+    in.p += in.token_step;
+    const RopeAngles angles(turn, false);
+    turn.advance(p, t, token + b.step, token + 2 * b.step);
+    float rs[U];
+    if constexpr (kNorm) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int head = b.head0 + u * b.per;
-      float2 y[4];
-      rope_get(x[u], y);
-      if constexpr (kNorm) {
+      for (int u = 0; u < U; ++u) {
+        float2 y[4];
+        rope_get(x[u], y);
         float2 ss = mul2(y[0], y[0]);
 #pragma unroll
         for (int i = 1; i < 4; ++i) ss = fma2(y[i], y[i], ss);
-        const float rs = rsqrtf(rope_head_sum(ss.x + ss.y, pl.lanes_shift) * inv_d + p.eps);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], splat2(rs));
+        rs[u] = ss.x + ss.y;
       }
-      if (t.in && head < b.heads) {
-        if (per_head) rope_weight8(p, k, head, t, w);
+      rope_head_sums(rs, pl.lanes_shift);
+#pragma unroll
+      for (int u = 0; u < U; ++u) rs[u] = rsqrtf(rs[u] * inv_d + p.eps);
+    }
+    T* to = out.p;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u < mine) {
+        float2 y[4];
+        rope_get(x[u], y);
+        if constexpr (kNorm) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], splat2(rs[u]));
+        }
+        if (per_head) rope_weight8(p, k, b.head0 + u * b.per, t, w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], w[i]);
-        rope_turn8<kInterleaved>(t, c, s, y);
-        out.store(token, u, y);
+        rope_turn8<kInterleaved>(t, angles, y);
+        out.store(to, y);
       }
+      to += out.head_step;
     }
+    out.p += out.token_step;
   }
+  if constexpr (kRing) ring.drain(p, b, pl);
 }
 
 // The sums of dweight: a set per head the lane works on (kPerHead), or one set. The CTA adds
 // its warps' sums in a fixed order and leaves one partial row: [q_heads + k_heads][head_dim]
-// per blockIdx.x, or [q, k][head_dim] per CTA.
-template <typename T, int U, bool kInterleaved, bool kNorm, bool kPerHead>
+// per blockIdx.x, or [q, k][head_dim] per CTA. A lane works on kBatch of its U heads at a time.
+template <typename T, int U, int kBatch, bool kInterleaved, bool kNorm, bool kPerHead>
 __global__ void __launch_bounds__(kRopeWarps * 32) rope_bwd_kernel(const RopeParams p, const RopePlan pl) {
   constexpr int kSets = kPerHead ? U : 1;
+  static_assert(!kPerHead || U == kBatch, "sums of every head have registers of their own");
   __shared__ float sums[kRopeWarps][kRopeMaxDim];
   pdl_launch_dependents();
   pdl_wait();
@@ -412,73 +580,99 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_bwd_kernel(const RopePar
   const int first_job = blockIdx.y * pl.cta_jobs;
   const int all = pl.jobs[0] + pl.jobs[1];
   const int k = b.k, per = b.per;
-  const RopePlace<T> in(k ? p.x[1] : p.x[0], t, b), grad(k ? p.dy[1] : p.dy[0], t, b),
-      out(k ? p.out[1] : p.out[0], t, b);
+  RopePlace<T> out(k ? p.out[1] : p.out[0], t, b);
+  const RopeTensor tensors[2] = {k ? p.x[1] : p.x[0], k ? p.dy[1] : p.dy[0]};
+  const uint64_t policy = l2_policy_evict_first();
+  RopeRing<T, U, 2> ring(pl, b, tensors);
+  if (b.works) ring.start(p, b, pl, policy);
   const bool per_head = kPerHead && p.w_per_head[k];
   const float inv_d = 1.f / static_cast<float>(p.D);
+  const int mine = t.in ? (b.heads - b.head0 + per - 1) / per : 0;  // the lane has heads u < mine
   float2 acc[kSets][4], w[4];
 #pragma unroll
   for (int i = 0; i < kSets; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[i][e] = make_float2(0.f, 0.f);
   if (!per_head) rope_weight8(p, k, 0, t, w);
+  RopeTurn turn(p, t, b.works ? b.token : p.tokens, b.step);
   for (int64_t token = b.token; b.works && token < p.tokens; token += b.step) {
-    Chunk4<T> x[U][2], dy[U][2];
+    ring.wait(kSiteBwdFull);
+    const T* head_x = ring.held(pl, p, t, 0);
+    const T* head_dy = ring.held(pl, p, t, 1);
+    const RopeAngles angles(turn, true);
+    turn.advance(p, t, token + b.step, token + 2 * b.step);
+    T* to = out.p;
+#pragma unroll 1
+    for (int u0 = 0; u0 < U; u0 += kBatch) {
+      Chunk4<T> x[kBatch][2], dy[kBatch][2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (t.in && b.head0 + u * per < b.heads) {
-        grad.load(token, u, dy[u]);
-        in.load(token, u, x[u]);
-      } else {
-        x[u][0].v = x[u][1].v = dy[u][0].v = dy[u][1].v = {};
-      }
-    }
-    float c[4], s[4];
-    rope_lane_turn(p, t, token, c, s);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = -s[i];  // turned back
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int head = b.head0 + u * per;
-      const bool has = t.in && head < b.heads;
-      float2 y[4], g[4];
-      rope_get(x[u], y);
-      rope_get(dy[u], g);
-      rope_turn8<kInterleaved>(t, c, s, g);
-      if (!has) {  // NaN cosines must not reach the sums of a lane without a head
-#pragma unroll
-        for (int e = 0; e < 4; ++e) g[e] = make_float2(0.f, 0.f);
-      }
-      if (per_head && has) rope_weight8(p, k, head, t, w);
-      float rs = 1.f, m = 0.f;
-      float2 gw[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) gw[e] = mul2(g[e], w[e]);
-      if constexpr (kNorm) {
-        float2 ss = mul2(y[0], y[0]), sg = mul2(y[0], gw[0]);
-#pragma unroll
-        for (int e = 1; e < 4; ++e) {
-          ss = fma2(y[e], y[e], ss);
-          sg = fma2(y[e], gw[e], sg);
-        }
-        rs = rsqrtf(rope_head_sum(ss.x + ss.y, pl.lanes_shift) * inv_d + p.eps);
-        m = rope_head_sum(sg.x + sg.y, pl.lanes_shift) * rs * inv_d;  // mean of xhat g w
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float2& sum = acc[kPerHead ? u : 0][e];
-        if constexpr (kNorm) {
-          const float2 xhat = mul2(y[e], splat2(rs));
-          sum = fma2(g[e], xhat, sum);
-          y[e] = mul2(fma2(xhat, splat2(-m), gw[e]), splat2(rs));
+      for (int i = 0; i < kBatch; ++i) {
+        if (u0 + i < mine) {
+          out.load(head_x + i * per * p.D, x[i]);
+          out.load(head_dy + i * per * p.D, dy[i]);
         } else {
-          sum = fma2(g[e], y[e], sum);
-          y[e] = gw[e];
+          x[i][0].v = x[i][1].v = dy[i][0].v = dy[i][1].v = {};
         }
       }
-      if (has) out.store(token, u, y);
+      head_x += kBatch * per * p.D;
+      head_dy += kBatch * per * p.D;
+      if (u0 + kBatch == U) ring.advance(p, b, pl, policy);
+      // g = dout turned back; the sums of x^2 and x g w of all heads of the batch together
+      float2 g[kBatch][4];
+      float totals[2 * kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        rope_get(dy[i], g[i]);
+        rope_turn8<kInterleaved>(t, angles, g[i]);
+        if (u0 + i >= mine) {  // NaN cosines must not reach the sums of a lane without a head
+#pragma unroll
+          for (int e = 0; e < 4; ++e) g[i][e] = make_float2(0.f, 0.f);
+        }
+        if constexpr (kNorm) {
+          if (per_head && u0 + i < mine) rope_weight8(p, k, b.head0 + (u0 + i) * per, t, w);
+          float2 y[4];
+          rope_get(x[i], y);
+          float2 ss = mul2(y[0], y[0]), sg = mul2(y[0], mul2(g[i][0], w[0]));
+#pragma unroll
+          for (int e = 1; e < 4; ++e) {
+            ss = fma2(y[e], y[e], ss);
+            sg = fma2(y[e], mul2(g[i][e], w[e]), sg);
+          }
+          totals[2 * i] = ss.x + ss.y;
+          totals[2 * i + 1] = sg.x + sg.y;
+        }
+      }
+      if constexpr (kNorm) rope_head_sums(totals, pl.lanes_shift);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (per_head && u0 + i < mine) rope_weight8(p, k, b.head0 + (u0 + i) * per, t, w);
+        float2 y[4];
+        rope_get(x[i], y);
+        float rs = 1.f, m = 0.f;
+        if constexpr (kNorm) {
+          rs = rsqrtf(totals[2 * i] * inv_d + p.eps);
+          m = -totals[2 * i + 1] * rs * inv_d;  // -mean of xhat g w
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float2& sum = acc[kPerHead ? i : 0][e];
+          const float2 gw = mul2(g[i][e], w[e]);
+          if constexpr (kNorm) {
+            const float2 xhat = mul2(y[e], splat2(rs));
+            sum = fma2(g[i][e], xhat, sum);
+            y[e] = mul2(fma2(xhat, splat2(m), gw), splat2(rs));
+          } else {
+            sum = fma2(g[i][e], y[e], sum);
+            y[e] = gw;
+          }
+        }
+        if (u0 + i < mine) out.store(to, y);
+        to += out.head_step;
+      }
     }
+    out.p += out.token_step;
   }
+  if (b.works) ring.drain(p, b, pl);
   if (!p.part) return;
   // a lane's column of its sums' element i
   auto column = [&](int i) { return i < 4 ? t.a + i : t.b + i - 4; };
