@@ -72,7 +72,7 @@ RopeParams params(const rmsnorm_b200_rope_args* a) {
 
 // Whether the vectorised kernels take these tensors: nothing but whole 16-byte granules.
 bool vectorised(const rmsnorm_b200_rope_args* a, std::initializer_list<const rmsnorm_b200_rope_tensor*> tensors) {
-  if (a->head_dim % 8 || a->rotary_dim % 8 || !aligned_to(a->table, 16)) return false;
+  if (a->head_dim % 8 || a->rotary_dim % 8 || !aligned_to(a->table, 16) || a->table_rows > INT32_MAX) return false;
   const int granule = 16 / elem_bytes(a->dtype);
   for (const auto* t : tensors)
     if (t && (!aligned_to(t->data, 16) || t->token_stride % granule || t->head_stride % granule)) return false;
@@ -184,7 +184,7 @@ RopeKernel pick_fwd(const RopeParams& p) {
 
 template <typename T, int U, bool kPerHead>
 RopeKernel pick_bwd(bool interleaved, bool norm) {
-  constexpr int kBatch = 2;
+  constexpr int kBatch = kPerHead ? 2 : 1;
   if (interleaved)
     return norm ? rope_bwd_kernel<T, U, kBatch, true, true, kPerHead> : rope_bwd_kernel<T, U, kBatch, true, false, kPerHead>;
   return norm ? rope_bwd_kernel<T, U, kBatch, false, true, kPerHead> : rope_bwd_kernel<T, U, kBatch, false, false, kPerHead>;
