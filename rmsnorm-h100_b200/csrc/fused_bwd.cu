@@ -60,6 +60,25 @@ BwdKernel pick(const rmsnorm_b200_dropout_bwd_args* a, int k, int g) {
   return nullptr;
 }
 
+template <typename H, typename DY>
+BwdKernel pick_odd(int k) {
+  return k == 1 ? odd_bwd_kernel<H, DY, 1> : odd_bwd_kernel<H, DY, 2>;
+}
+
+BwdKernel pick_odd(const rmsnorm_b200_dropout_bwd_args* a, int k) {
+  constexpr int H = RMSNORM_B200_F16, B = RMSNORM_B200_BF16, F = RMSNORM_B200_F32;
+  const int h = a->h_dtype, dy = a->dout_dtype;
+  if (a->dx_dtype != dy || (a->dresidual_out && a->dresidual_out_dtype != h) ||
+      (a->dresidual && a->dresidual_dtype != h))
+    return pick_odd<Any, Any>(k);
+  if (h == B && dy == B) return pick_odd<__nv_bfloat16, __nv_bfloat16>(k);
+  if (h == H && dy == H) return pick_odd<__half, __half>(k);
+  if (h == F && dy == F) return pick_odd<float, float>(k);
+  if (h == F && dy == B) return pick_odd<float, __nv_bfloat16>(k);
+  if (h == F && dy == H) return pick_odd<float, __half>(k);
+  return pick_odd<Any, Any>(k);
+}
+
 int check(const rmsnorm_b200_dropout_bwd_args* a) {
   if (!a || a->rows < 0 || a->hidden < 1) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
   if (!valid_dt(a->h_dtype) || !valid_dt(a->dout_dtype) || !valid_dt(a->dx_dtype))
@@ -86,7 +105,7 @@ int make_plan(UnitDevice* ud, const rmsnorm_b200_dropout_bwd_args* a, Plan* pl) 
     if (odd) {
       pl->why = plan_rows(a->rows, a->hidden, bytes, false, kOddThreads, kOddBwdSteps, ud->sm_count, &pl->rows, &pl->k,
                           &pl->smem, true);
-      pl->kernel = pl->k == 1 ? odd_bwd_kernel<1> : odd_bwd_kernel<2>;
+      pl->kernel = pick_odd(a, pl->k);
     } else {
       // 16-bit rows that fill more than two steps of a warp: four steps a thread, sums in tensor
       // memory. The others, and few rows (a CTA each, as many threads as it has): registers.

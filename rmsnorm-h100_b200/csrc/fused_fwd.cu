@@ -70,9 +70,22 @@ FwdKernel pick(int x, int res, int ro, int end, int k) {
   return nullptr;
 }
 
-template <bool kQuant>
-FwdKernel pick_odd(int k) {
-  return k == 1 ? odd_fwd_kernel<kQuant, 1> : k == 2 ? odd_fwd_kernel<kQuant, 2> : odd_fwd_kernel<kQuant, 4>;
+template <typename X, typename RO>
+FwdKernel pick_odd(bool drop, int k) {
+  if (drop) return k == 1 ? odd_fwd_kernel<X, RO, false, 1> : k == 2 ? odd_fwd_kernel<X, RO, false, 2> : odd_fwd_kernel<X, RO, false, 4>;
+  return k == 1 ? odd_fwd_kernel<X, RO, true, 1> : k == 2 ? odd_fwd_kernel<X, RO, true, 2> : odd_fwd_kernel<X, RO, true, 4>;
+}
+
+FwdKernel pick_odd(const FusedFwdParams& p, bool drop, int k) {
+  constexpr int H = RMSNORM_B200_F16, B = RMSNORM_B200_BF16, F = RMSNORM_B200_F32;
+  const int x = p.x_dt, ro = p.ro ? p.ro_dt : x;
+  if ((p.res && p.res_dt != x) || (drop && p.out_dt != x)) return pick_odd<Any, Any>(drop, k);
+  if (x == B && ro == B) return pick_odd<__nv_bfloat16, __nv_bfloat16>(drop, k);
+  if (x == H && ro == H) return pick_odd<__half, __half>(drop, k);
+  if (x == F && ro == F) return pick_odd<float, float>(drop, k);
+  if (x == B && ro == F) return pick_odd<__nv_bfloat16, float>(drop, k);
+  if (x == H && ro == F) return pick_odd<__half, float>(drop, k);
+  return pick_odd<Any, Any>(drop, k);
 }
 
 int launch_generic(const FusedFwdParams& p, bool drop, UnitDevice* ud, cudaStream_t stream, const char* why) {
@@ -128,7 +141,7 @@ int run(const FusedFwdParams& p, bool drop, cudaStream_t stream) {
   }
   why = plan_rows(p.rows, p.N, bytes, p.b != nullptr, kOddThreads, kOddSteps, ud->sm_count, &pl, &k, &smem, true);
   if (!why) {
-    st = launch_rows(ud, drop ? pick_odd<false>(k) : pick_odd<true>(k), p, pl, smem, stream,
+    st = launch_rows(ud, pick_odd(p, drop, k), p, pl, smem, stream,
                      drop ? "dropout_fwd_odd" : "quant_fwd_odd", k);
     if (st != RMSNORM_B200_ERR_UNSUPPORTED) return st;
     why = "cluster not schedulable";

@@ -7,8 +7,12 @@
 // granule that would leave the tensor at its very beginning or end is not copied; the
 // issuing thread moves those elements itself. A lane then owns every 32nd column of its
 // warp's 256 (not 8 in a row), so that scalar accesses to shared and global memory are
-// consecutive across the warp at any alignment. Types are chosen at run time, once a vector.
+// consecutive across the warp at any alignment. Types are fixed at compile time where x, the
+// residual and the output share one and residual_out has it or fp32; other combinations (Any)
+// choose at run time, once a vector.
 #pragma once
+
+#include <type_traits>
 
 #include "fused_generic.cuh"
 #include "row_ring.cuh"
@@ -41,39 +45,50 @@ __device__ __forceinline__ int64_t odd_unit(const RowPlan& pl, const RowCtx& c, 
   return row0 * N + c.slice0 + col0;
 }
 
+// The granules of `bytes` of elements at `begin` that lie within the tensor [base, limit): those
+// outside are shrunk away, and their elements moved one by one to `dst` (the slot's address of
+// the first granule). Only a tensor's first and last rows come here.
+__device__ __noinline__ void odd_edges(uintptr_t base, uintptr_t limit, uintptr_t begin, uintptr_t end, int size,
+                                       unsigned char* dst, uintptr_t* lo, uintptr_t* hi) {
+  if (*lo < base) *lo += 16;
+  if (*hi > limit) *hi -= 16;
+  for (uintptr_t a = begin; a < end; a += size) {
+    if (a >= *lo && a < *hi) {
+      a = *hi - size;
+      continue;
+    }
+    const void* from = reinterpret_cast<const void*>(a);
+    if (!RMSB_DBG_OK(from, size, kDbgScalarLoad)) continue;
+    unsigned char* to = dst + (begin & 15) + (a - begin);
+    if (size == 4)
+      *reinterpret_cast<uint32_t*>(to) = *static_cast<const uint32_t*>(from);
+    else
+      *reinterpret_cast<uint16_t*>(to) = *static_cast<const uint16_t*>(from);
+  }
+}
+
 template <int kStreams>
 __device__ __forceinline__ void odd_issue(const RowPlan& pl, const RowCtx& c, int64_t u, int slot, int64_t rows,
                                           int64_t N, const OddStream (&src)[kStreams], uint64_t policy) {
   int64_t elems;
   const int64_t e = odd_unit(pl, c, u, rows, N, &elems);
   uint64_t* bar = &c.full[slot];
+  unsigned char* slot_at = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;
   uintptr_t lo[kStreams], hi[kStreams];
+  uint32_t off[kStreams];  // in the slot, of the first copied granule
   uint32_t total = 0;
 #pragma unroll
   for (int i = 0; i < kStreams; ++i) {
     lo[i] = hi[i] = 0;
     if (!src[i].p || elems == 0) continue;
-    const uintptr_t base = reinterpret_cast<uintptr_t>(src[i].p), limit = base + rows * N * src[i].bytes;
+    const uintptr_t base = reinterpret_cast<uintptr_t>(src[i].p);
     const uintptr_t begin = base + e * src[i].bytes, end = begin + elems * src[i].bytes;
-    unsigned char* dst = c.ring + static_cast<size_t>(slot) * pl.unit_bytes + pl.off[i];
-    lo[i] = begin & ~static_cast<uintptr_t>(15);
+    const uintptr_t first = begin & ~static_cast<uintptr_t>(15), limit = base + rows * N * src[i].bytes;
+    lo[i] = first;
     hi[i] = (end + 15) & ~static_cast<uintptr_t>(15);
-    if (lo[i] < base) lo[i] += 16;
-    if (hi[i] > limit) hi[i] -= 16;
-    // elements outside the copied granules
-    for (uintptr_t a = begin; a < end; a += src[i].bytes) {
-      if (a >= lo[i] && a < hi[i]) {
-        a = hi[i] - src[i].bytes;
-        continue;
-      }
-      const void* from = reinterpret_cast<const void*>(a);
-      if (!RMSB_DBG_OK(from, src[i].bytes, kDbgScalarLoad)) continue;
-      unsigned char* to = dst + odd_lead(reinterpret_cast<const void*>(begin)) + (a - begin);
-      if (src[i].bytes == 4)
-        *reinterpret_cast<uint32_t*>(to) = *static_cast<const uint32_t*>(from);
-      else
-        *reinterpret_cast<uint16_t*>(to) = *static_cast<const uint16_t*>(from);
-    }
+    if (lo[i] < base || hi[i] > limit)
+      odd_edges(base, limit, begin, end, src[i].bytes, slot_at + pl.off[i], &lo[i], &hi[i]);
+    off[i] = pl.off[i] + static_cast<uint32_t>(lo[i] - first);
     if (hi[i] > lo[i]) total += static_cast<uint32_t>(hi[i] - lo[i]);
   }
   if (total == 0) {
@@ -82,13 +97,10 @@ __device__ __forceinline__ void odd_issue(const RowPlan& pl, const RowCtx& c, in
   }
   mbar_arrive_expect_tx(bar, total);
 #pragma unroll
-  for (int i = 0; i < kStreams; ++i) {
-    if (hi[i] <= lo[i]) continue;
-    const uintptr_t begin = reinterpret_cast<uintptr_t>(src[i].p) + e * src[i].bytes;
-    unsigned char* dst = c.ring + static_cast<size_t>(slot) * pl.unit_bytes + pl.off[i];
-    bulk_load(dst + (lo[i] - (begin & ~static_cast<uintptr_t>(15))), reinterpret_cast<const void*>(lo[i]),
-              static_cast<uint32_t>(hi[i] - lo[i]), bar, policy);
-  }
+  for (int i = 0; i < kStreams; ++i)
+    if (hi[i] > lo[i])
+      bulk_load(slot_at + off[i], reinterpret_cast<const void*>(lo[i]), static_cast<uint32_t>(hi[i] - lo[i]), bar,
+                policy);
 }
 
 // Columns of a lane: col0 + 32 e + lane, e < 8. The first out of range ends them. `full` and
@@ -117,13 +129,18 @@ __device__ __forceinline__ void odd_load(const unsigned char* p, const OddCols& 
   for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(raw[e]);
 }
 
+struct Any {};  // a type chosen at run time
+
+template <typename T>
 __device__ __forceinline__ void odd_read(const unsigned char* p, int dt, const OddCols& o, float (&v)[8]) {
-  if (dt == RMSNORM_B200_F32) {
-    if (o.full) odd_load<float, true>(p, o, v); else odd_load<float, false>(p, o, v);
+  if constexpr (!std::is_same_v<T, Any>) {
+    if (o.full) odd_load<T, true>(p, o, v); else odd_load<T, false>(p, o, v);
+  } else if (dt == RMSNORM_B200_F32) {
+    odd_read<float>(p, dt, o, v);
   } else if (dt == RMSNORM_B200_BF16) {
-    if (o.full) odd_load<__nv_bfloat16, true>(p, o, v); else odd_load<__nv_bfloat16, false>(p, o, v);
+    odd_read<__nv_bfloat16>(p, dt, o, v);
   } else {
-    if (o.full) odd_load<__half, true>(p, o, v); else odd_load<__half, false>(p, o, v);
+    odd_read<__half>(p, dt, o, v);
   }
 }
 
@@ -135,13 +152,16 @@ __device__ __forceinline__ void odd_store(void* base, int64_t at, const OddCols&
     if (kFull || e < o.n) st1(p + e * 32, static_cast<T>(v[e]));
 }
 
+template <typename T>
 __device__ __forceinline__ void odd_write(void* base, int dt, int64_t at, const OddCols& o, const float (&v)[8]) {
-  if (dt == RMSNORM_B200_F32) {
-    if (o.full) odd_store<float, true>(base, at, o, v); else odd_store<float, false>(base, at, o, v);
+  if constexpr (!std::is_same_v<T, Any>) {
+    if (o.full) odd_store<T, true>(base, at, o, v); else odd_store<T, false>(base, at, o, v);
+  } else if (dt == RMSNORM_B200_F32) {
+    odd_write<float>(base, dt, at, o, v);
   } else if (dt == RMSNORM_B200_BF16) {
-    if (o.full) odd_store<__nv_bfloat16, true>(base, at, o, v); else odd_store<__nv_bfloat16, false>(base, at, o, v);
+    odd_write<__nv_bfloat16>(base, dt, at, o, v);
   } else {
-    if (o.full) odd_store<__half, true>(base, at, o, v); else odd_store<__half, false>(base, at, o, v);
+    odd_write<__half>(base, dt, at, o, v);
   }
 }
 
@@ -195,7 +215,8 @@ __device__ __forceinline__ uint32_t odd_keep(const DropParams& d, int64_t block_
   return keep;
 }
 
-template <bool kQuant, int K>
+// X: type of x, the residual and a floating output; RO: of residual_out.
+template <typename X, typename RO, bool kQuant, int K>
 __global__ void __launch_bounds__(kOddThreads, 1) odd_fwd_kernel(const FusedFwdParams p, const RowPlan pl) {
   RowCtx c = row_begin(pl, p.N);
   pdl_launch_dependents();
@@ -233,11 +254,11 @@ __global__ void __launch_bounds__(kOddThreads, 1) odd_fwd_kernel(const FusedFwdP
         const unsigned char* base = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;
         const int64_t first = row0 * p.N + c.slice0 + first_step * pl.G * 8;  // element of the unit
         const int at = r * static_cast<int>(p.N) + o.col - first_step * pl.G * 8;
-        odd_read(base + odd_lead(static_cast<const unsigned char*>(p.x) + first * src[0].bytes) + at * src[0].bytes,
+        odd_read<X>(base + odd_lead(static_cast<const unsigned char*>(p.x) + first * src[0].bytes) + at * src[0].bytes,
                  p.x_dt, o, h[j]);
         float res[8];
         if (p.res)
-          odd_read(base + pl.off[1] + odd_lead(static_cast<const unsigned char*>(p.res) + first * src[1].bytes) +
+          odd_read<X>(base + pl.off[1] + odd_lead(static_cast<const unsigned char*>(p.res) + first * src[1].bytes) +
                        at * src[1].bytes,
                    p.res_dt, o, res);
         if constexpr (!kQuant) {
@@ -254,7 +275,7 @@ __global__ void __launch_bounds__(kOddThreads, 1) odd_fwd_kernel(const FusedFwdP
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(h[j][e], h[j][e], ss);
-        if (p.ro) odd_write(p.ro, p.ro_dt, e0 + o.col, o, h[j]);
+        if (p.ro) odd_write<RO>(p.ro, p.ro_dt, e0 + o.col, o, h[j]);
         }
         if (r == nrows - 1 && ((j + 1) & (pl.KC - 1)) == 0) {
           if (release_unit(c, slot) && unit + pl.S < c.units)
@@ -287,7 +308,7 @@ __global__ void __launch_bounds__(kOddThreads, 1) odd_fwd_kernel(const FusedFwdP
           for (int e = 0; e < 8; ++e)
             if (e >= o.n) h[j][e] = 0.f;  // rs may be NaN
         }
-        if constexpr (!kQuant) odd_write(p.out, p.out_dt, e0 + o.col, o, h[j]);
+        if constexpr (!kQuant) odd_write<X>(p.out, p.out_dt, e0 + o.col, o, h[j]);
       }
       if constexpr (kQuant) {
         float inv_row = 0.f;
@@ -321,12 +342,17 @@ __global__ void __launch_bounds__(kOddThreads, 1) odd_fwd_kernel(const FusedFwdP
             if (p.group >= 256)
 #pragma unroll
               for (int e = 0; e < 8; ++e) m[e] = max(m[0], m[4]);
+            float* scale = p.scales + row * p.scale_row + ((c.slice0 + o.col - c.lane) >> p.group_shift) * p.scale_group;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
+              if (e > 0 && (e * 32 & (p.group - 1)) != 0) {  // the scale of the step before
+                inv[e] = inv[e - 1];
+                continue;
+              }
               const float s = scale_of(__uint_as_float(m[e]), inv_q);
               inv[e] = inverse(s);
-              if (c.lane == 0 && e < o.n && (e * 32 & (p.group - 1)) == 0)  // blocks begin at whole groups
-                st1(&p.scales[row * p.scale_row + ((c.slice0 + o.col + e * 32) >> p.group_shift) * p.scale_group], s);
+              if (c.lane == 0 && e < o.n) st1(scale, s);
+              scale += p.scale_group;
             }
           } else {
 #pragma unroll
@@ -356,7 +382,8 @@ __global__ void __launch_bounds__(kOddThreads, 1) odd_fwd_kernel(const FusedFwdP
   row_end(pl, c);
 }
 
-template <int K>
+// H: type of h, dresidual_out and dresidual; DY: of dout and dx.
+template <typename H, typename DY, int K>
 __global__ void __launch_bounds__(kOddThreads, 1) odd_bwd_kernel(const FusedBwdParams p, const RowPlan pl) {
   RowCtx c = row_begin(pl, p.N);
   pdl_launch_dependents();
@@ -401,9 +428,9 @@ __global__ void __launch_bounds__(kOddThreads, 1) odd_bwd_kernel(const FusedBwdP
           return base + pl.off[i] + odd_lead(static_cast<const unsigned char*>(src[i].p) + first * src[i].bytes) +
                  at * src[i].bytes;
         };
-        odd_read(slot_of(0), p.h_dt, o, h[j]);
-        odd_read(slot_of(1), p.dy_dt, o, g[j]);
-        if (p.dro) odd_read(slot_of(2), p.dro_dt, o, d[j]);
+        odd_read<H>(slot_of(0), p.h_dt, o, h[j]);
+        odd_read<DY>(slot_of(1), p.dy_dt, o, g[j]);
+        if (p.dro) odd_read<H>(slot_of(2), p.dro_dt, o, d[j]);
         float w[8];
         odd_affine8(c.w, o, w);
 #pragma unroll
@@ -437,12 +464,12 @@ __global__ void __launch_bounds__(kOddThreads, 1) odd_bwd_kernel(const FusedBwdP
           const float v = fmaf(g[j][e], rs, h[j][e] * t);
           d[j][e] = p.dro ? v + d[j][e] : v;
         }
-        if (p.dres) odd_write(p.dres, p.dres_dt, e0 + o.col, o, d[j]);
+        if (p.dres) odd_write<H>(p.dres, p.dres_dt, e0 + o.col, o, d[j]);
         __syncwarp();
         const uint32_t keep = odd_keep(p.drop, c.slice0 + o.col - c.lane, row, offset, c.lane);
 #pragma unroll
         for (int e = 0; e < 8; ++e) d[j][e] = keep >> e & 1u ? d[j][e] * p.drop.scale : 0.f;
-        odd_write(p.dx, p.dx_dt, e0 + o.col, o, d[j]);
+        odd_write<DY>(p.dx, p.dx_dt, e0 + o.col, o, d[j]);
       }
     }
   }
