@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fused_bwd_kernel(const FusedBw
       uint32_t words[2][4];
       row_total<true, false>(pl, c, s, unused, kSiteBwdCluster,
                              [&] { draw8(p.drop, c.slice0 + c.gl * 8, row, offset, words); });
-      const float t = -(rs * rs * rs * (s * inv_n));
+      const float t = -(s * inv_n * rs * rs * rs);  // rs^3 by itself may overflow
       if constexpr (kTmem) tmem_wait_st();  // of the row before
 #pragma unroll
       for (int j = 0; j < K; ++j) {

@@ -107,7 +107,7 @@ int run(const FusedFwdParams& p, bool drop, cudaStream_t stream) {
   if (p.res) ranges.add(p.res, n * elem_bytes(p.res_dt));
   if (p.w) ranges.add(p.w, p.N * elem_bytes(p.w_dt));
   if (p.b) ranges.add(p.b, p.N * elem_bytes(p.b_dt));
-  ranges.add(p.out, n * (p.scales ? 1 : elem_bytes(p.out_dt)));
+  ranges.add_out(p.out, n * (p.scales ? 1 : elem_bytes(p.out_dt)));
   if (p.ro) ranges.add(p.ro, n * elem_bytes(p.ro_dt));
   if (p.rstd) ranges.add(p.rstd, p.rows * 4);
   if (p.scales) {

@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kOddThreads, 1) odd_bwd_kernel(const FusedBwdP
       }
       uint32_t unused = 0;
       row_total<true, false>(pl, c, s, unused, kSiteBwdCluster);
-      const float t = -(rs * rs * rs * (s * inv_n));
+      const float t = -(s * inv_n * rs * rs * rs);  // rs^3 by itself may overflow
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         const OddCols o = odd_cols(pl, c, j);

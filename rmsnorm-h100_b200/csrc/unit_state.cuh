@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cstdio>
+#include <cstdlib>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -73,6 +74,12 @@ struct Ranges {
     r.hi[r.n] = r.lo[r.n] + bytes;
     ++r.n;
   }
+  // Self test of the checker: RMSNORM_B200_DEBUG_CLIP_OUT=k registers an output k bytes short.
+  void add_out(const void* p, size_t bytes) {
+    const char* v = std::getenv("RMSNORM_B200_DEBUG_CLIP_OUT");
+    const size_t clip = v ? static_cast<size_t>(std::atoi(v)) : 0;
+    add(p, clip < bytes ? bytes - clip : bytes);
+  }
   int send(cudaStream_t stream) {
     dbg_ranges_kernel<<<1, 32, 0, stream>>>(r);
     return cudaGetLastError() == cudaSuccess ? RMSNORM_B200_OK : RMSNORM_B200_ERR_CUDA;
@@ -81,6 +88,7 @@ struct Ranges {
 #else
 struct Ranges {
   void add(const void*, size_t) {}
+  void add_out(const void*, size_t) {}
   int send(cudaStream_t) { return RMSNORM_B200_OK; }
 };
 #endif

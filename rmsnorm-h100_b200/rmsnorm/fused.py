@@ -138,7 +138,7 @@ def rmsnorm_quant_fwd(
     column by column (the strides of a transposed tensor), as block-scaled products take
     them. residual_out as in `rmsnorm_fwd`."""
     if _is_compiling():
-        return _outside_graph(rmsnorm_quant_fwd)(
+        return _quant_untraced(
             x, weight, bias, residual, quant_dtype, group_size, residual_dtype, eps, scales_column_major)
     shape, n, device, xc, wc, bc, rc = _row_codes(x, weight, bias, residual)
     roc = 0 if residual_dtype is None else _dtype_code("residual_dtype", residual_dtype)
@@ -185,12 +185,6 @@ def rmsnorm_quant_fwd(
     name = "rmsnorm_b200_quant_fwd"
     _lib.enqueue(_lib.packed_entry(name, _BYTES, _STREAM), name, device.index, args)
     return q, scales, x if residual_out is None else residual_out
-
-
-@functools.lru_cache(maxsize=None)
-def _outside_graph(fn):
-    """`fn` as torch.compile calls it: untraced."""
-    return torch.compiler.disable(fn)
 
 
 # ---------------------------------------------------------------------------------------
@@ -253,7 +247,7 @@ def dropout_add_rmsnorm_fwd(
     CUDA graph can draw new masks. `row_offset` is the row of the whole tensor's mask that x
     begins with, for tensors whose rows are spread over ranks."""
     if _is_compiling():
-        return _outside_graph(dropout_add_rmsnorm_fwd)(
+        return _drop_fwd_untraced(
             x, weight, bias, residual, p, rng, out_dtype, residual_dtype, eps, store_rstd, rng_step, row_offset)
     shape, n, device, xc, wc, bc, rc = _row_codes(x, weight, bias, residual)
     if out_dtype is None:
@@ -308,7 +302,7 @@ def dropout_add_rmsnorm_bwd(
     (None unless has_residual) in dresidual_dtype (default: residual_out's); dweight and dbias
     follow the affine tensors (dbias without a bias tensor: weight's dtype, else dout's)."""
     if _is_compiling():
-        return _outside_graph(dropout_add_rmsnorm_bwd)(
+        return _drop_bwd_untraced(
             residual_out, weight, dout, rstd, dresidual_out, p, rng, has_bias, has_residual, bias, dx_dtype,
             dresidual_dtype, rng_step, row_offset)
     h = residual_out
@@ -408,7 +402,7 @@ def dropout_add_rmsnorm(
 ):
     """`dropout_add_rmsnorm_fwd` with autograd: out, or (out, residual_out) when prenorm."""
     if _is_compiling():
-        return _outside_graph(dropout_add_rmsnorm)(
+        return _drop_untraced(
             x, weight, bias, residual, p, rng, out_dtype, residual_dtype, eps, prenorm, rng_step, row_offset)
     return DropoutAddRMSNormFunction.apply(
         x, weight, bias, residual, p, tuple(rng), out_dtype, residual_dtype, eps, prenorm, rng_step, row_offset)
@@ -576,7 +570,7 @@ def qk_norm_rope_fwd(
     `rope_table`'s. A position outside the table gives NaN columns, and on CUDA an
     invalid-argument entry in the device status word."""
     if _is_compiling():
-        return _outside_graph(qk_norm_rope_fwd)(
+        return _rope_fwd_untraced(
             q, k, positions, table, q_weight, k_weight, axes, interleaved, norm, eps, inplace)
     checked = _check_rope(q, k, positions, table, q_weight, k_weight, axes)
     if not q.is_cuda:
@@ -633,7 +627,7 @@ def qk_norm_rope_bwd(
     """(dq, dk, dq_weight, dk_weight) from the forward's inputs and the gradients of its
     outputs; the weights' gradients (None without a weight) are summed in a fixed order."""
     if _is_compiling():
-        return _outside_graph(qk_norm_rope_bwd)(
+        return _rope_bwd_untraced(
             q, k, positions, table, dq_out, dk_out, q_weight, k_weight, axes, interleaved, norm, eps)
     checked = _check_rope(q, k, positions, table, q_weight, k_weight, axes)
     for name, g, t in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
@@ -705,7 +699,17 @@ def qk_norm_rope(
 ) -> Tuple[Tensor, Optional[Tensor]]:
     """`qk_norm_rope_fwd` with autograd (for q, k and the weights)."""
     if _is_compiling():
-        return _outside_graph(qk_norm_rope)(
+        return _rope_untraced(
             q, k, positions, table, q_weight, k_weight, axes, interleaved, norm, eps)
     return QKNormRopeFunction.apply(
         q, k, positions, table, q_weight, k_weight, None if axes is None else tuple(axes), interleaved, norm, eps)
+
+
+# The same functions as torch.compile calls them: untraced, a graph break each.
+_quant_untraced = torch.compiler.disable(rmsnorm_quant_fwd)
+_drop_fwd_untraced = torch.compiler.disable(dropout_add_rmsnorm_fwd)
+_drop_bwd_untraced = torch.compiler.disable(dropout_add_rmsnorm_bwd)
+_drop_untraced = torch.compiler.disable(dropout_add_rmsnorm)
+_rope_fwd_untraced = torch.compiler.disable(qk_norm_rope_fwd)
+_rope_bwd_untraced = torch.compiler.disable(qk_norm_rope_bwd)
+_rope_untraced = torch.compiler.disable(qk_norm_rope)

@@ -244,6 +244,27 @@ def test_rope_helpers_and_positions_outside_the_table():
     assert none is None and out[0].isfinite().all() and out[1, 0, :4].isnan().all() and out[1, 0, 4:].isfinite().all()
 
 
+def test_under_torch_compile():
+    """The operators break the graph and compute what they compute in eager mode."""
+    torch._dynamo.reset()
+    x, r, w = torch.randn(4, 64), torch.randn(4, 64), torch.ones(64)
+    q, pos, table = torch.randn(4, 2, 16), torch.arange(4), fused.rope_table(8, 16)
+
+    def f(x, q):
+        h, res = fused.dropout_add_rmsnorm(x * 2, w, residual=r, p=0.25, rng=(1, 2), prenorm=True)
+        a, _ = fused.qk_norm_rope(q + 1, None, pos, table)
+        v, s, _ = fused.rmsnorm_quant_fwd(h, w)
+        return (h + res) * 3, a - 1, v.float() * s[:, None]
+
+    x1, x2 = (x.clone().requires_grad_(True) for _ in range(2))
+    want, got = f(x1, q), torch.compile(f, backend="eager")(x2, q)
+    for s, t in zip(want, got):
+        assert torch.equal(s, t)
+    want[0].sum().backward()
+    got[0].sum().backward()
+    assert torch.equal(x1.grad, x2.grad)
+
+
 # ------------------------------------------------------------------ refusals
 def test_quant_refusals():
     x = torch.randn(2, 64)

@@ -280,6 +280,17 @@ def test_dropout_rows_of_a_whole_tensor():
     assert torch.equal(torch.cat(parts), whole)
 
 
+@pytest.mark.parametrize("n", [512, 1003])
+def test_dropout_bwd_of_zero_rows_with_a_tiny_eps(n):
+    """rstd = eps^-1/2 = 1e16 and its cube does not fit fp32; dx = dout w rstd does."""
+    h, dout = torch.zeros(40, n, device=DEV), rand(40, n, seed=1)
+    w, _ = affine(n)
+    rstd = torch.full((40,), 1e16, device=DEV)
+    dx, dw, _, _ = fused.dropout_add_rmsnorm_bwd(h, w, dout, rstd)
+    ref.check(dx, dout.double() * w.double() * 1e16, 0.0, "dx")
+    assert (dw == 0).all()
+
+
 def test_dropout_autograd_and_empty():
     x, r = (rand(6, 4, 128, dtype=BF16, seed=s).requires_grad_(True) for s in (1, 2))
     w, b = (t.requires_grad_(True) for t in affine(128))
