@@ -359,6 +359,7 @@ int rmsnorm_b200_dropout_rmsnorm_bwd(const rmsnorm_b200_dropout_bwd_args* args, 
  * columns NaN and records RMSNORM_B200_ERR_INVALID_ARGUMENT (site 10) in the device status
  * word. Only the last dimension of a tensor has to be contiguous. */
 #define RMSNORM_B200_ROPE_MAX_HEAD_DIM 256
+#define RMSNORM_B200_ROPE_MAX_HEADS 65536
 typedef struct rmsnorm_b200_rope_tensor {
   void* data;                 /* [tokens, heads, head_dim] */
   int64_t token_stride;       /* in elements */
@@ -376,8 +377,8 @@ typedef struct rmsnorm_b200_rope_args {
   rmsnorm_b200_rope_tensor q; /* inputs; k_heads may be 0 */
   rmsnorm_b200_rope_tensor k;
   uint64_t axis_of_pair[4];   /* two bits per pair: pair i in word i / 32 at bit 2 * (i % 32) */
-  int32_t q_heads;
-  int32_t k_heads;
+  int32_t q_heads;            /* 1 .. RMSNORM_B200_ROPE_MAX_HEADS */
+  int32_t k_heads;            /* 0 .. RMSNORM_B200_ROPE_MAX_HEADS */
   int32_t head_dim;           /* 1 .. RMSNORM_B200_ROPE_MAX_HEAD_DIM */
   int32_t rotary_dim;         /* even, 0 .. head_dim */
   int32_t axes;               /* 1 .. 4 */

@@ -727,4 +727,19 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// Threads of the scalar kernels.
+constexpr int kGenericThreads = 256;
+
+// Block-wide sum, summed in warp order so every thread gets the same bits.
+__device__ __forceinline__ float block_sum_fixed(float v, float* red) {
+  v = warp_sum(v);
+  const int nw = blockDim.x >> 5;
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float t = 0.f;
+  for (int j = 0; j < nw; ++j) t += red[j];
+  __syncthreads();
+  return t;
+}
+
 }  // namespace rmsb200

@@ -2,6 +2,7 @@
 #define RMSB_UNIT fused_bwd
 #include "unit_state.cuh"
 
+#include "column_sums.cuh"
 #include "fused_bwd_kernels.cuh"
 #include "odd_kernels.cuh"
 #include "row_plan.h"
@@ -232,13 +233,7 @@ int run(const rmsnorm_b200_dropout_bwd_args* a, void* ws, size_t ws_bytes, cudaS
   return launched("");
 }
 
-}  // namespace
-}  // namespace rmsb200
-
-using namespace rmsb200;
-
-extern "C" int rmsnorm_b200_dropout_rmsnorm_bwd_workspace_size(const rmsnorm_b200_dropout_bwd_args* a,
-                                                               size_t* bytes) {
+int workspace_size(const rmsnorm_b200_dropout_bwd_args* a, size_t* bytes) {
   if (!bytes) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
   *bytes = 0;
   int st = check(a);
@@ -253,7 +248,17 @@ extern "C" int rmsnorm_b200_dropout_rmsnorm_bwd_workspace_size(const rmsnorm_b20
   return RMSNORM_B200_OK;
 }
 
+}  // namespace
+}  // namespace rmsb200
+
+using namespace rmsb200;
+
+extern "C" int rmsnorm_b200_dropout_rmsnorm_bwd_workspace_size(const rmsnorm_b200_dropout_bwd_args* a,
+                                                               size_t* bytes) {
+  return entry([&] { return workspace_size(a, bytes); });
+}
+
 extern "C" int rmsnorm_b200_dropout_rmsnorm_bwd(const rmsnorm_b200_dropout_bwd_args* a, void* workspace,
                                                 size_t workspace_bytes, void* stream) {
-  return run(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  return entry([&] { return run(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)); });
 }

@@ -149,12 +149,7 @@ int run(const FusedFwdParams& p, bool drop, cudaStream_t stream) {
   return launch_generic(p, drop, ud, stream, why);
 }
 
-}  // namespace
-}  // namespace rmsb200
-
-using namespace rmsb200;
-
-extern "C" int rmsnorm_b200_quant_fwd(const rmsnorm_b200_quant_args* a, void* stream) {
+int quant_fwd(const rmsnorm_b200_quant_args* a, void* stream) {
   if (!a || a->rows < 0 || a->hidden < 1) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
   if (!valid_dt(a->x_dtype) || (a->q_dtype != RMSNORM_B200_E4M3 && a->q_dtype != RMSNORM_B200_I8))
     return RMSNORM_B200_ERR_INVALID_ARGUMENT;
@@ -181,7 +176,7 @@ extern "C" int rmsnorm_b200_quant_fwd(const rmsnorm_b200_quant_args* a, void* st
   return run(p, false, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int rmsnorm_b200_dropout_rmsnorm_fwd(const rmsnorm_b200_dropout_fwd_args* a, void* stream) {
+int dropout_fwd(const rmsnorm_b200_dropout_fwd_args* a, void* stream) {
   if (!a || a->rows < 0 || a->hidden < 1) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
   if (!valid_dt(a->x_dtype) || !valid_dt(a->out_dtype)) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
   if ((a->residual && !valid_dt(a->residual_dtype)) || (a->residual_out && !valid_dt(a->residual_out_dtype)) ||
@@ -202,4 +197,17 @@ extern "C" int rmsnorm_b200_dropout_rmsnorm_fwd(const rmsnorm_b200_dropout_fwd_a
   p.eps = a->eps;
   expand_drop(a->drop, &p.drop);
   return run(p, true, static_cast<cudaStream_t>(stream));
+}
+
+}  // namespace
+}  // namespace rmsb200
+
+using namespace rmsb200;
+
+extern "C" int rmsnorm_b200_quant_fwd(const rmsnorm_b200_quant_args* a, void* stream) {
+  return entry([&] { return quant_fwd(a, stream); });
+}
+
+extern "C" int rmsnorm_b200_dropout_rmsnorm_fwd(const rmsnorm_b200_dropout_fwd_args* a, void* stream) {
+  return entry([&] { return dropout_fwd(a, stream); });
 }

@@ -1,11 +1,9 @@
-// fused_generic.cuh -- the fused row operators for every shape, type and alignment: one CTA
-// per row, scalar accesses with types chosen at run time, the row read again from cache for
-// each pass. The path of rows wider than a cluster holds and of type combinations outside
-// the specialised set.
+// fused_generic.cuh -- parameters of the fused row operators, and their forward for rows wider
+// than a cluster holds: one CTA per row, scalar accesses with types chosen at run time, the row
+// read again from cache for each pass.
 #pragma once
 
 #include "fused_common.cuh"
-#include "generic_kernels.cuh"
 
 namespace rmsb200 {
 
@@ -99,31 +97,6 @@ __global__ void __launch_bounds__(kGenericThreads) fused_fwd_generic_kernel(cons
       const float s = scale_of(__uint_as_float(most), inv_q);
       if (threadIdx.x == 0) st1(&p.scales[r * p.scale_row], s);
       for (int64_t n = threadIdx.x; n < N; n += blockDim.x) store1_q(p.out, p.out_dt, r * N + n, y(n) * inverse(s));
-    }
-  }
-}
-
-// dx and dresidual; dweight and dbias are column sums of their own (bwd_generic_partials_kernel).
-__global__ void __launch_bounds__(kGenericThreads) fused_bwd_generic_kernel(const FusedBwdParams p) {
-  __shared__ float red[32];
-  pdl_wait();
-  const uint64_t offset = drop_offset(p.drop);
-  const int64_t N = p.N;
-  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    const float rs = ld1(&p.rstd[r]);
-    auto wdy = [&](int64_t n) {
-      const float w = p.w ? load1_rt(p.w, p.w_dt, n) : 1.f;
-      return load1_rt(p.dy, p.dy_dt, r * N + n) * w;
-    };
-    float c = 0.f;
-    for (int64_t n = threadIdx.x; n < N; n += blockDim.x) c = fmaf(load1_rt(p.h, p.h_dt, r * N + n) * rs, wdy(n), c);
-    c = block_sum_fixed(c, red) / static_cast<float>(N);
-    for (int64_t n = threadIdx.x; n < N; n += blockDim.x) {
-      const int64_t e = r * N + n;
-      float d = (wdy(n) - load1_rt(p.h, p.h_dt, e) * rs * c) * rs;
-      if (p.dro) d += load1_rt(p.dro, p.dro_dt, e);
-      if (p.dres) store1_rt(p.dres, p.dres_dt, e, d);
-      store1_rt(p.dx, p.dx_dt, e, keep1(p.drop, n, r, offset) ? d * p.drop.scale : 0.f);
     }
   }
 }

@@ -251,31 +251,31 @@ __global__ void __launch_bounds__(kOddThreads, 1) odd_fwd_kernel(const FusedFwdP
 #pragma unroll
           for (int e = 0; e < 8; ++e) h[j][e] = 0.f;
         } else {
-        const unsigned char* base = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;
-        const int64_t first = row0 * p.N + c.slice0 + first_step * pl.G * 8;  // element of the unit
-        const int at = r * static_cast<int>(p.N) + o.col - first_step * pl.G * 8;
-        odd_read<X>(base + odd_lead(static_cast<const unsigned char*>(p.x) + first * src[0].bytes) + at * src[0].bytes,
-                 p.x_dt, o, h[j]);
-        float res[8];
-        if (p.res)
-          odd_read<X>(base + pl.off[1] + odd_lead(static_cast<const unsigned char*>(p.res) + first * src[1].bytes) +
-                       at * src[1].bytes,
-                   p.res_dt, o, res);
-        if constexpr (!kQuant) {
-          __syncwarp();
-          const uint32_t keep = odd_keep(p.drop, c.slice0 + o.col - c.lane, row, offset, c.lane);
+          const unsigned char* base = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;
+          const int64_t first = row0 * p.N + c.slice0 + first_step * pl.G * 8;  // element of the unit
+          const int at = r * static_cast<int>(p.N) + o.col - first_step * pl.G * 8;
+          odd_read<X>(base + odd_lead(static_cast<const unsigned char*>(p.x) + first * src[0].bytes) + at * src[0].bytes,
+                   p.x_dt, o, h[j]);
+          float res[8];
+          if (p.res)
+            odd_read<X>(base + pl.off[1] + odd_lead(static_cast<const unsigned char*>(p.res) + first * src[1].bytes) +
+                         at * src[1].bytes,
+                     p.res_dt, o, res);
+          if constexpr (!kQuant) {
+            __syncwarp();
+            const uint32_t keep = odd_keep(p.drop, c.slice0 + o.col - c.lane, row, offset, c.lane);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float v = p.res ? res[e] : 0.f;
-            h[j][e] = keep >> e & 1u ? fmaf(h[j][e], p.drop.scale, v) : v;
+            for (int e = 0; e < 8; ++e) {
+              const float v = p.res ? res[e] : 0.f;
+              h[j][e] = keep >> e & 1u ? fmaf(h[j][e], p.drop.scale, v) : v;
+            }
+          } else if (p.res) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[j][e] += res[e];
           }
-        } else if (p.res) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) h[j][e] += res[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(h[j][e], h[j][e], ss);
-        if (p.ro) odd_write<RO>(p.ro, p.ro_dt, e0 + o.col, o, h[j]);
+          for (int e = 0; e < 8; ++e) ss = fmaf(h[j][e], h[j][e], ss);
+          if (p.ro) odd_write<RO>(p.ro, p.ro_dt, e0 + o.col, o, h[j]);
         }
         if (r == nrows - 1 && ((j + 1) & (pl.KC - 1)) == 0) {
           if (release_unit(c, slot) && unit + pl.S < c.units)
@@ -421,26 +421,26 @@ __global__ void __launch_bounds__(kOddThreads, 1) odd_bwd_kernel(const FusedBwdP
         if (r == 0 && j == first_step) mbar_wait(&c.full[slot], phase, kSiteBwdFull);
         const OddCols o = odd_cols(pl, c, j);
         if (o.any) {
-        const unsigned char* base = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;
-        const int64_t first = row0 * p.N + c.slice0 + first_step * pl.G * 8;
-        const int at = r * static_cast<int>(p.N) + o.col - first_step * pl.G * 8;
-        auto slot_of = [&](int i) {
-          return base + pl.off[i] + odd_lead(static_cast<const unsigned char*>(src[i].p) + first * src[i].bytes) +
-                 at * src[i].bytes;
-        };
-        odd_read<H>(slot_of(0), p.h_dt, o, h[j]);
-        odd_read<DY>(slot_of(1), p.dy_dt, o, g[j]);
-        if (p.dro) odd_read<H>(slot_of(2), p.dro_dt, o, d[j]);
-        float w[8];
-        odd_affine8(c.w, o, w);
+          const unsigned char* base = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;
+          const int64_t first = row0 * p.N + c.slice0 + first_step * pl.G * 8;
+          const int at = r * static_cast<int>(p.N) + o.col - first_step * pl.G * 8;
+          auto slot_of = [&](int i) {
+            return base + pl.off[i] + odd_lead(static_cast<const unsigned char*>(src[i].p) + first * src[i].bytes) +
+                   at * src[i].bytes;
+          };
+          odd_read<H>(slot_of(0), p.h_dt, o, h[j]);
+          odd_read<DY>(slot_of(1), p.dy_dt, o, g[j]);
+          if (p.dro) odd_read<H>(slot_of(2), p.dro_dt, o, d[j]);
+          float w[8];
+          odd_affine8(c.w, o, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float hg = h[j][e] * g[j][e];
-          s = fmaf(hg, w[e], s);
-          dw[j][e] = fmaf(hg, rs, dw[j][e]);
-          db[j][e] += g[j][e];
-          g[j][e] *= w[e];
-        }
+          for (int e = 0; e < 8; ++e) {
+            const float hg = h[j][e] * g[j][e];
+            s = fmaf(hg, w[e], s);
+            dw[j][e] = fmaf(hg, rs, dw[j][e]);
+            db[j][e] += g[j][e];
+            g[j][e] *= w[e];
+          }
         }
         if (r == nrows - 1 && ((j + 1) & (pl.KC - 1)) == 0) {
           if (release_unit(c, slot) && unit + pl.S < c.units)

@@ -24,8 +24,7 @@
 // kARThreads) fits a B200 at once, so those CTAs are resident together.
 #pragma once
 
-#include "device_common.cuh"
-#include "generic_kernels.cuh"
+#include "column_sums.cuh"
 
 namespace rmsb200 {
 

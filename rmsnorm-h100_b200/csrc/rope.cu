@@ -4,6 +4,7 @@
 
 #include <cstring>
 
+#include "column_sums.cuh"
 #include "rope_kernels.cuh"
 
 namespace rmsb200 {
@@ -15,6 +16,8 @@ bool valid_tensor(const rmsnorm_b200_rope_tensor& t, int64_t tokens, int heads) 
 
 int check(const rmsnorm_b200_rope_args* a) {
   if (!a || a->tokens < 0 || a->q_heads < 1 || a->k_heads < 0) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if (a->q_heads > RMSNORM_B200_ROPE_MAX_HEADS || a->k_heads > RMSNORM_B200_ROPE_MAX_HEADS)
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
   if (a->head_dim < 1 || a->head_dim > kRopeMaxDim || a->rotary_dim < 0 || a->rotary_dim > a->head_dim ||
       (a->rotary_dim & 1))
     return RMSNORM_B200_ERR_INVALID_ARGUMENT;
@@ -350,18 +353,7 @@ int run_bwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g, v
   return launched("");
 }
 
-}  // namespace
-}  // namespace rmsb200
-
-using namespace rmsb200;
-
-extern "C" int rmsnorm_b200_rope_fwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_tensor* q_out,
-                                     const rmsnorm_b200_rope_tensor* k_out, void* stream) {
-  return run_fwd(a, q_out, k_out, static_cast<cudaStream_t>(stream));
-}
-
-extern "C" int rmsnorm_b200_rope_bwd_workspace_size(const rmsnorm_b200_rope_args* a,
-                                                    const rmsnorm_b200_rope_grads* g, size_t* bytes) {
+int workspace_size(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g, size_t* bytes) {
   if (!bytes) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
   *bytes = 0;
   int st = check_bwd(a, g);
@@ -373,7 +365,22 @@ extern "C" int rmsnorm_b200_rope_bwd_workspace_size(const rmsnorm_b200_rope_args
   return RMSNORM_B200_OK;
 }
 
+}  // namespace
+}  // namespace rmsb200
+
+using namespace rmsb200;
+
+extern "C" int rmsnorm_b200_rope_fwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_tensor* q_out,
+                                     const rmsnorm_b200_rope_tensor* k_out, void* stream) {
+  return entry([&] { return run_fwd(a, q_out, k_out, static_cast<cudaStream_t>(stream)); });
+}
+
+extern "C" int rmsnorm_b200_rope_bwd_workspace_size(const rmsnorm_b200_rope_args* a,
+                                                    const rmsnorm_b200_rope_grads* g, size_t* bytes) {
+  return entry([&] { return workspace_size(a, g, bytes); });
+}
+
 extern "C" int rmsnorm_b200_rope_bwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_grads* g,
                                      void* workspace, size_t workspace_bytes, void* stream) {
-  return run_bwd(a, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  return entry([&] { return run_bwd(a, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)); });
 }

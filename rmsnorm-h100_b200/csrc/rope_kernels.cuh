@@ -4,7 +4,6 @@
 #include <type_traits>
 
 #include "device_common.cuh"
-#include "generic_kernels.cuh"
 
 namespace rmsb200 {
 

@@ -25,7 +25,7 @@
 #include <unordered_set>
 #include <vector>
 
-#include "generic_kernels.cuh"
+#include "device_common.cuh"
 #include "translation_units.h"
 
 namespace rmsb200 {
@@ -142,6 +142,17 @@ int launched(rmsb_units::PlanText make, const Plan& plan) {
   rmsb_units::count_launches(1);
   rmsb_units::set_last_plan(make, &plan, sizeof(plan));
   return RMSNORM_B200_OK;
+}
+
+// The body of a C entry: no exception leaves the library (what can throw here is the host's
+// memory running out).
+template <typename Body>
+int entry(Body&& body) noexcept {
+  try {
+    return body();
+  } catch (...) {
+    return RMSNORM_B200_ERR_CUDA;
+  }
 }
 
 }  // namespace

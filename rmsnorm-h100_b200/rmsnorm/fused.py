@@ -48,6 +48,7 @@ __all__ = [
 ]
 
 _CODE = _lib._DTYPE_CODES
+_MAX_HEADS = 65536
 _GROUP_SIZES = (None, 32, 64, 128, 256)
 _is_compiling = torch.compiler.is_compiling
 
@@ -480,8 +481,8 @@ def _check_rope(q, k, positions, table, q_weight, k_weight, axes):
     device = q.device
     if not 1 <= d <= 256:
         raise ValueError(f"head_dim must be 1 to 256, got {d}")
-    if shape[-2] < 1:
-        raise ValueError("q must have at least one head")
+    if not 1 <= shape[-2] <= _MAX_HEADS:
+        raise ValueError(f"q must have at least one head and at most {_MAX_HEADS}, got {shape[-2]}")
     tokens = shape[:-2]
     k_heads = 0
     if k is not None:
@@ -493,6 +494,8 @@ def _check_rope(q, k, positions, table, q_weight, k_weight, axes):
         if k.device != device:
             raise ValueError("k must be on the same device as q")
         k_heads = kshape[-2]
+        if k_heads > _MAX_HEADS:
+            raise ValueError(f"k must have at most {_MAX_HEADS} heads, got {k_heads}")
     elif k_weight is not None:
         raise ValueError("k_weight needs k")
     tshape = table.shape
