@@ -6,6 +6,7 @@
 #include "fused_bwd_kernels.cuh"
 #include "odd_kernels.cuh"
 #include "row_plan.h"
+#include "shift_bwd_kernel.cuh"
 
 namespace rmsb200 {
 namespace {
@@ -93,39 +94,65 @@ int check(const rmsnorm_b200_dropout_bwd_args* a) {
   return RMSNORM_B200_OK;
 }
 
+BwdKernel pick_shift(const rmsnorm_b200_dropout_bwd_args* a) {
+  constexpr int H = RMSNORM_B200_F16, B = RMSNORM_B200_BF16, F = RMSNORM_B200_F32;
+  const int h = a->h_dtype, dy = a->dout_dtype;
+  if (a->dx_dtype != dy || (a->dresidual_out && a->dresidual_out_dtype != h) ||
+      (a->dresidual && a->dresidual_dtype != h))
+    return nullptr;
+  if (h == B && dy == B) return shift_bwd_kernel<__nv_bfloat16, __nv_bfloat16>;
+  if (h == H && dy == H) return shift_bwd_kernel<__half, __half>;
+  if (h == F && dy == F) return shift_bwd_kernel<float, float>;
+  if (h == F && dy == B) return shift_bwd_kernel<float, __nv_bfloat16>;
+  if (h == F && dy == H) return shift_bwd_kernel<float, __half>;
+  return nullptr;
+}
+
 int make_plan(UnitDevice* ud, const rmsnorm_b200_dropout_bwd_args* a, Plan* pl) {
-  // Whole aligned vectors in a combination of types with a kernel of its own; else the odd
-  // rows' kernels; else (rows wider than a cluster holds) the generic ones.
+  // Aligned tensors in a combination of types with a kernel of its own: whole vectors where rows
+  // consist of them, shifted ones where they do not; else the odd rows' kernels; else (rows
+  // wider than a cluster holds) the generic ones.
   const int bytes[3] = {elem_bytes(a->h_dtype), elem_bytes(a->dout_dtype),
                         a->dresidual_out ? elem_bytes(a->dresidual_out_dtype) : 0};
   const void* ptrs[] = {a->h, a->dout, a->dresidual_out, a->dx, a->dresidual};
-  bool vectors = a->hidden % 8 == 0;
-  for (const void* ptr : ptrs) vectors = vectors && aligned_to(ptr, 16);
+  bool aligned = true;
+  for (const void* ptr : ptrs) aligned = aligned && aligned_to(ptr, 16);
   for (const bool odd : {false, true}) {
-    if (!odd && !vectors) continue;
+    if (!odd && !aligned) continue;
+    const bool shifted = !odd && a->hidden % 8 != 0;
+    RowWants want;
     if (odd) {
+      want.odd = true;
       pl->why = plan_rows(a->rows, a->hidden, bytes, false, kOddThreads, kOddBwdSteps, ud->sm_count, &pl->rows, &pl->k,
-                          &pl->smem, true);
+                          &pl->smem, want);
       pl->kernel = pick_odd(a, pl->k);
+    } else if (shifted) {
+      // four steps a thread where two whole rows fit the ring; wider ones are split
+      const int elem = bytes[0] + bytes[1] + bytes[2];
+      const int steps = 2 * shifted_columns(a->hidden) * elem <= kRingBytes || elem <= 6 ? kShiftBwdSteps : kShiftBwdSteps / 2;
+      want.shifted = want.whole = true;
+      pl->why = plan_rows(a->rows, shifted_columns(a->hidden), bytes, false, kShiftThreads, steps, ud->sm_count,
+                          &pl->rows, &pl->k, &pl->smem, want);
+      pl->kernel = pick_shift(a);
     } else {
       // 16-bit rows that fill more than two steps of a warp: four steps a thread, sums in tensor
       // memory. The others, and few rows (a CTA each, as many threads as it has): registers.
-      int g = 0;
       const bool few = a->rows <= ud->sm_count && a->hidden <= kBwdThreads * 8 * kBwdRegSteps;
       if (!few && a->h_dtype != RMSNORM_B200_F32 && a->dout_dtype == a->h_dtype && a->hidden > 32 * 8 * kBwdRegSteps)
-        g = std::min(pow2_ceil((a->hidden + 8 * kBwdTmemSteps - 1) / (8 * kBwdTmemSteps)), kBwdThreads);
-      pl->why = plan_rows(a->rows, a->hidden, bytes, false, kBwdThreads, g ? kBwdTmemSteps : kBwdRegSteps, ud->sm_count,
-                          &pl->rows, &pl->k, &pl->smem, false, g);
-      if (g) pl->k = kBwdTmemSteps;
-      pl->kernel = pl->why ? nullptr : pick(a, pl->k, g);
+        want.built_in = std::min(pow2_ceil((a->hidden + 8 * kBwdTmemSteps - 1) / (8 * kBwdTmemSteps)), kBwdThreads);
+      pl->why = plan_rows(a->rows, a->hidden, bytes, false, kBwdThreads, want.built_in ? kBwdTmemSteps : kBwdRegSteps,
+                          ud->sm_count, &pl->rows, &pl->k, &pl->smem, want);
+      if (want.built_in) pl->k = kBwdTmemSteps;
+      pl->kernel = pl->why ? nullptr : pick(a, pl->k, want.built_in);
     }
     if (pl->why) pl->kernel = nullptr;
     if (!pl->kernel) continue;
-    pl->kind = odd ? "dropout_bwd_odd" : "dropout_bwd";
+    pl->kind = odd ? "dropout_bwd_odd" : shifted ? "dropout_bwd_sh" : "dropout_bwd";
     // the groups' sums of a vector step pass through the rings
-    if (odd || pl->rows.groups > 1) pl->smem = std::max(pl->smem, kBwdThreads * 64);
+    if (odd || shifted || pl->rows.groups > 1) pl->smem = std::max(pl->smem, kBwdThreads * 64);
     int grid = 0;
-    const int st = launch_rows(ud, pl->kernel, FusedBwdParams{}, pl->rows, pl->smem, nullptr, "", pl->k, &grid, true);
+    const int st = (shifted ? launch_shifted<BwdKernel, FusedBwdParams> : launch_rows<BwdKernel, FusedBwdParams>)(
+        ud, pl->kernel, FusedBwdParams{}, pl->rows, pl->smem, nullptr, "", pl->k, &grid, true);
     if (st == RMSNORM_B200_OK) {
       pl->nparts = a->dweight || a->dbias ? grid / pl->rows.C : 0;
       return st;

@@ -6,6 +6,7 @@
 #include "fused_fwd_kernels.cuh"
 #include "odd_kernels.cuh"
 #include "row_plan.h"
+#include "shift_fwd_kernel.cuh"
 
 namespace rmsb200 {
 namespace {
@@ -88,6 +89,26 @@ FwdKernel pick_odd(const FusedFwdParams& p, bool drop, int k) {
   return pick_odd<Any, Any>(drop, k);
 }
 
+template <typename X, typename E>
+FwdKernel pick_shift(int k) {
+  return k == 1 ? shift_fwd_kernel<X, E, 1> : shift_fwd_kernel<X, E, kShiftFwdSteps>;
+}
+
+template <typename X>
+FwdKernel pick_shift(int end, int k) {
+  switch (end) {
+    case kDropped: return pick_shift<X, Dropped>(k);
+    case kE4M3Row: return pick_shift<X, Scaled<E4M3, true>>(k);
+    case kI8Row: return pick_shift<X, Scaled<I8, true>>(k);
+    default: return nullptr;
+  }
+}
+
+FwdKernel pick_shift(int x, int end, int k) {
+  if (x == RMSNORM_B200_F32) return pick_shift<float>(end, k);
+  return x == RMSNORM_B200_BF16 ? pick_shift<__nv_bfloat16>(end, k) : pick_shift<__half>(end, k);
+}
+
 int launch_generic(const FusedFwdParams& p, bool drop, UnitDevice* ud, cudaStream_t stream, const char* why) {
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(p.rows, int64_t{8} * ud->sm_count));
   if (drop)
@@ -117,29 +138,43 @@ int run(const FusedFwdParams& p, bool drop, cudaStream_t stream) {
   if (p.drop.step) ranges.add(p.drop.step, 8);
   st = ranges.send(stream);
   if (st) return st;
-  // Whole aligned vectors in a combination of types with a kernel of its own; else the odd
+  // Aligned tensors in a combination of types with a kernel of its own: whole vectors where rows
+  // consist of them, shifted ones where they do not (and a scale is a row's); else the odd
   // rows' kernels; else (rows wider than a cluster holds) the generic one.
   const int bytes[3] = {elem_bytes(p.x_dt), p.res ? elem_bytes(p.res_dt) : 0, 0};
   RowPlan pl;
   int k = 0, smem = 0;
   const void* ptrs[] = {p.x, p.res, p.out, p.ro};
-  bool vectors = p.N % 8 == 0 && (!drop || p.out_dt == p.x_dt);
-  for (const void* ptr : ptrs) vectors = vectors && aligned_to(ptr, ptr == p.out && p.scales ? 8 : 16);
+  bool aligned = !drop || p.out_dt == p.x_dt;
+  for (const void* ptr : ptrs) aligned = aligned && aligned_to(ptr, ptr == p.out && p.scales ? 8 : 16);
+  const bool i8 = p.out_dt == RMSNORM_B200_I8;
+  const int end = drop ? kDropped : p.group ? (i8 ? kI8Group : kE4M3Group) : (i8 ? kI8Row : kE4M3Row);
   const char* why = nullptr;
-  if (vectors) {
+  if (aligned && p.N % 8 == 0) {
     const bool few = p.rows <= ud->sm_count && p.N <= kFwdFewThreads * 8;
     why = plan_rows(p.rows, p.N, bytes, p.b != nullptr, few ? kFwdFewThreads : kFwdThreads, few ? 1 : kFwdSteps,
                     ud->sm_count, &pl, &k, &smem);
     if (!why) {
-      const bool i8 = p.out_dt == RMSNORM_B200_I8;
-      const int end = drop ? kDropped : p.group ? (i8 ? kI8Group : kE4M3Group) : (i8 ? kI8Row : kE4M3Row);
       if (FwdKernel kernel = pick(p.x_dt, p.res ? p.res_dt : kNone, p.ro ? p.ro_dt : kNone, end, k)) {
         st = launch_rows(ud, kernel, p, pl, smem, stream, drop ? "dropout_fwd" : "quant_fwd", k);
         if (st != RMSNORM_B200_ERR_UNSUPPORTED) return st;
       }
     }
+  } else if (aligned && (!p.res || p.res_dt == p.x_dt || p.res_dt == RMSNORM_B200_F32) &&
+             (!p.ro || p.ro_dt == p.x_dt || p.ro_dt == RMSNORM_B200_F32)) {
+    RowWants want;
+    want.shifted = true;
+    why = plan_rows(p.rows, shifted_columns(p.N), bytes, p.b != nullptr, kShiftThreads, kShiftFwdSteps, ud->sm_count,
+                    &pl, &k, &smem, want);
+    FwdKernel kernel = why ? nullptr : pick_shift(p.x_dt, end, k);
+    if (kernel) {
+      st = launch_shifted(ud, kernel, p, pl, smem, stream, drop ? "dropout_fwd_sh" : "quant_fwd_sh", k);
+      if (st != RMSNORM_B200_ERR_UNSUPPORTED) return st;
+    }
   }
-  why = plan_rows(p.rows, p.N, bytes, p.b != nullptr, kOddThreads, kOddSteps, ud->sm_count, &pl, &k, &smem, true);
+  RowWants want;
+  want.odd = true;
+  why = plan_rows(p.rows, p.N, bytes, p.b != nullptr, kOddThreads, kOddSteps, ud->sm_count, &pl, &k, &smem, want);
   if (!why) {
     st = launch_rows(ud, pick_odd(p, drop, k), p, pl, smem, stream,
                      drop ? "dropout_fwd_odd" : "quant_fwd_odd", k);

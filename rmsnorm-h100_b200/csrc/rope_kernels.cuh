@@ -586,6 +586,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_bwd_kernel(const RopePar
   const bool per_head = kPerHead && p.w_per_head[k];
   const float inv_d = 1.f / static_cast<float>(p.D);
   const int mine = t.in ? (b.heads - b.head0 + per - 1) / per : 0;  // the lane has heads u < mine
+  const int used = min(U, (b.heads - b.job * U * per + per - 1) / per);  // u < used: some lane of the warp has the head
   float2 acc[kSets][4], w[4];
 #pragma unroll
   for (int i = 0; i < kSets; ++i)
@@ -601,7 +602,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_bwd_kernel(const RopePar
     turn.advance(p, t, token + b.step, token + 2 * b.step);
     T* to = out.p;
 #pragma unroll 1
-    for (int u0 = 0; u0 < U; u0 += kBatch) {
+    for (int u0 = 0; u0 < used; u0 += kBatch) {
       Chunk4<T> x[kBatch][2], dy[kBatch][2];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
@@ -614,7 +615,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_bwd_kernel(const RopePar
       }
       head_x += kBatch * per * p.D;
       head_dy += kBatch * per * p.D;
-      if (u0 + kBatch == U) ring.advance(p, b, pl);
+      if (u0 + kBatch >= used) ring.advance(p, b, pl);
       // g = dout turned back; the sums of x^2 and x g w of all heads of the batch together
       float2 g[kBatch][4];
       float totals[2 * kBatch];

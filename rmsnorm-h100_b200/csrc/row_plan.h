@@ -14,12 +14,28 @@ inline int pow2_ceil(int64_t v) {
   return p;
 }
 
-// Plans rows of N columns whose tensors have elements of bytes[i] (0: absent). odd: the kernels
-// of odd_kernels.cuh, otherwise N is a multiple of 8. threads of a CTA, max_steps: vector steps
-// a thread can hold, built_in: the row group of a kernel made for one (four steps, units of
-// bwd_unit_steps, a row each), 0: chosen here. Returns why there is no plan, or null.
+constexpr int kRingBytes = 200 * 1024;  // of shared memory, for two whole rows of every group
+
+// What a kernel asks of its plan.
+struct RowWants {
+  bool odd = false;      // the kernels of odd_kernels.cuh; otherwise N is a multiple of 8
+  int built_in = 0;      // row group of a kernel made for one: four steps, units of bwd_unit_steps, a row each
+  bool shifted = false;  // units of one row; one step or max_steps
+  bool whole = false;    // a row's slice is one unit; two of them a group
+};
+
+// Columns of a row of N on shifted vectors (shift_rows.cuh), whatever its lead.
+inline int64_t shifted_columns(int64_t N) {
+  const int64_t most = N % 2 ? 7 : N % 4 ? 6 : N % 8 ? 4 : 0;
+  return (N + most + 7) / 8 * 8;
+}
+
+// Plans rows of N columns whose tensors have elements of bytes[i] (0: absent); threads of a CTA,
+// max_steps: vector steps a thread can hold. Returns why there is no plan, or null.
 inline const char* plan_rows(int64_t rows, int64_t N, const int (&bytes)[3], bool bias, int threads, int max_steps,
-                             int sms, RowPlan* pl, int* k, int* smem, bool odd = false, int built_in = 0) {
+                             int sms, RowPlan* pl, int* k, int* smem, const RowWants& want = {}) {
+  const bool odd = want.odd;
+  const int built_in = want.built_in;
   const int64_t cta_cols = static_cast<int64_t>(threads) * 8 * max_steps;
   if (N > cta_cols * kMaxRowCtas) return "rows wider than a cluster holds";
   pl->C = N > cta_cols ? pow2_ceil((N + cta_cols - 1) / cta_cols) : 1;
@@ -32,20 +48,34 @@ inline const char* plan_rows(int64_t rows, int64_t N, const int (&bytes)[3], boo
   // Few rows: as many threads to a row as it has vectors, for the latency. Otherwise as few as
   // hold it, so that a CTA works on several rows at once and their totals overlap.
   const int steps = rows <= sms ? 1 : max_steps;
-  pl->G = built_in ? built_in : std::clamp(pow2_ceil((vecs + steps - 1) / steps), 32, threads);
-  *k = built_in ? max_steps : pow2_ceil((vecs + pl->G - 1) / pl->G);
-  pl->groups = pl->C > 1 ? 1 : threads / pl->G;
+  const int per_row = (vecs + steps - 1) / steps;
   const int elem = bytes[0] + bytes[1] + bytes[2];
+  if (built_in) {
+    pl->G = built_in;
+    pl->groups = pl->C > 1 ? 1 : threads / pl->G;
+  } else if (odd || rows <= sms) {
+    pl->G = std::clamp(pow2_ceil(per_row), 32, threads);
+    pl->groups = pl->C > 1 ? 1 : threads / pl->G;
+  } else {
+    // as many groups as their rows' vectors allow, of any number of warps, the steps shared out
+    // evenly: 2368 columns in five groups of 96 threads 247 us, in four of 128 301 us (5.7e4 rows, bf16)
+    pl->groups = pl->C > 1 ? 1 : threads / std::clamp((per_row + 31) / 32 * 32, 32, threads);
+    while (want.whole && pl->groups > 1 && 2 * pl->groups * vecs * 8 * elem > kRingBytes) --pl->groups;
+    const int most = threads / pl->groups / 32 * 32, used = (vecs + most - 1) / most;
+    pl->G = ((vecs + used - 1) / used + 31) / 32 * 32;
+  }
+  *k = built_in ? max_steps : pow2_ceil((vecs + pl->G - 1) / pl->G);
+  if (want.shifted && *k > 1) *k = max_steps;
   // Units of up to 32 KB: larger ones leave too few in flight (32768 x 16384 bf16 + residual,
   // fp32 residual_out, 8 bits: 748 us in five units of 32 KB, 842 us in two of 64 KB).
   pl->KC = *k;
-  while (pl->KC > 1 && pl->KC * pl->G * 8 * elem > 32768) pl->KC >>= 1;
+  while (!want.whole && pl->KC > 1 && pl->KC * pl->G * 8 * elem > 32768) pl->KC >>= 1;
   if (built_in) pl->KC = bwd_unit_steps(built_in);
   pl->unit_shift = 0;
   while ((pl->KC << pl->unit_shift) < *k) ++pl->unit_shift;
   // Short rows go several to a unit: a copy of about 4 KB at least, but no fewer tiles than groups.
   pl->R = 1;
-  if (pl->C == 1 && pl->KC == *k && !built_in) {
+  if (pl->C == 1 && pl->KC == *k && !built_in && !want.shifted) {
     const int64_t fair = rows / (static_cast<int64_t>(sms) * pl->groups);
     pl->R = static_cast<int>(std::clamp<int64_t>(std::min<int64_t>(4096 / (N * elem), fair), 1, 8));
   }
@@ -158,6 +188,17 @@ int launch_rows(UnitDevice* ud, Kernel kernel, const Params& p, const RowPlan& p
   RowLaunch l = {pl, {}, static_cast<int>(grid), k, smem};
   std::strncpy(l.kind, kind, sizeof(l.kind) - 1);
   return launched(describe_rows, l);
+}
+
+// The same for kernels on shifted vectors, whose every class of rows needs a cluster.
+template <typename Kernel, typename Params>
+int launch_shifted(UnitDevice* ud, Kernel kernel, const Params& p, const RowPlan& pl, int smem, cudaStream_t stream,
+                   const char* kind, int k, int* grid_out = nullptr, bool dry_run = false) {
+  int clusters = 0;
+  const int st = resident_clusters(ud, kernel, pl, smem, &clusters);
+  if (st) return st;
+  if (clusters < 8) return RMSNORM_B200_ERR_UNSUPPORTED;
+  return launch_rows(ud, kernel, p, pl, smem, stream, kind, k, grid_out, dry_run);
 }
 
 }  // namespace
