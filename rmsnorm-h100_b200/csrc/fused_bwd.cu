@@ -31,12 +31,24 @@ BwdKernel pick_steps(int k, int g) {
     switch (g) {
       case 32: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 32>;
       case 64: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 64>;
+      case 96: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 96>;
       case 128: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 128>;
+      case 160: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 160>;
+      case 192: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 192>;
       case 256: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 256>;
+      case 320: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 320>;
+      case 384: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 384>;
       case 512: return fused_bwd_kernel<H, DY, DRO, DRES, kBwdTmemSteps, 512>;
     }
   }
   return k == 1 ? fused_bwd_kernel<H, DY, DRO, DRES, 1, 0> : fused_bwd_kernel<H, DY, DRO, DRES, 2, 0>;
+}
+
+// The smallest of them that holds a row's `threads`, or the largest.
+int built_in_group(int64_t threads) {
+  for (const int g : {32, 64, 96, 128, 160, 192, 256, 320, 384})
+    if (threads <= g) return g;
+  return kBwdThreads;
 }
 
 template <typename H, typename DY>
@@ -119,31 +131,40 @@ int make_plan(UnitDevice* ud, const rmsnorm_b200_dropout_bwd_args* a, Plan* pl) 
   for (const void* ptr : ptrs) aligned = aligned && aligned_to(ptr, 16);
   for (const bool odd : {false, true}) {
     if (!odd && !aligned) continue;
-    const bool shifted = !odd && a->hidden % 8 != 0;
+    bool shifted = !odd && a->hidden % 8 != 0;
     RowWants want;
     if (odd) {
       want.odd = true;
       pl->why = plan_rows(a->rows, a->hidden, bytes, false, kOddThreads, kOddBwdSteps, ud->sm_count, &pl->rows, &pl->k,
                           &pl->smem, want);
       pl->kernel = pick_odd(a, pl->k);
-    } else if (shifted) {
-      // four steps a thread where two whole rows fit the ring; wider ones are split
-      const int elem = bytes[0] + bytes[1] + bytes[2];
-      const int steps = 2 * shifted_columns(a->hidden) * elem <= kRingBytes || elem <= 6 ? kShiftBwdSteps : kShiftBwdSteps / 2;
-      want.shifted = want.whole = true;
-      pl->why = plan_rows(a->rows, shifted_columns(a->hidden), bytes, false, kShiftThreads, steps, ud->sm_count,
-                          &pl->rows, &pl->k, &pl->smem, want);
-      pl->kernel = pick_shift(a);
-    } else {
+    } else if (!shifted) {
       // 16-bit rows that fill more than two steps of a warp: four steps a thread, sums in tensor
-      // memory. The others, and few rows (a CTA each, as many threads as it has): registers.
+      // memory, by groups of the size that fits (32263 x 4160: three of 160 threads 279 us, two of
+      // 256 365 us). The others, and few rows (a CTA each, as many threads as it has): registers.
       const bool few = a->rows <= ud->sm_count && a->hidden <= kBwdThreads * 8 * kBwdRegSteps;
       if (!few && a->h_dtype != RMSNORM_B200_F32 && a->dout_dtype == a->h_dtype && a->hidden > 32 * 8 * kBwdRegSteps)
-        want.built_in = std::min(pow2_ceil((a->hidden + 8 * kBwdTmemSteps - 1) / (8 * kBwdTmemSteps)), kBwdThreads);
+        want.built_in = built_in_group((a->hidden + 8 * kBwdTmemSteps - 1) / (8 * kBwdTmemSteps));
       pl->why = plan_rows(a->rows, a->hidden, bytes, false, kBwdThreads, want.built_in ? kBwdTmemSteps : kBwdRegSteps,
                           ud->sm_count, &pl->rows, &pl->k, &pl->smem, want);
       if (want.built_in) pl->k = kBwdTmemSteps;
       pl->kernel = pl->why ? nullptr : pick(a, pl->k, want.built_in);
+      // A CTA's single row of which two steps in registers leave a third of the threads idle goes to
+      // the shifted kernel, which holds four steps: 32263 x 4160, fp32 h, bf16 dout 406 against 564 us.
+      if (!pl->why && !few && !want.built_in && pl->k == kBwdRegSteps && pl->rows.groups == 1 &&
+          pl->rows.slice * 3 < kBwdThreads * kBwdRegSteps * 8 * 2)
+        shifted = true;
+    }
+    if (shifted) {
+      // four steps a thread where two whole rows fit the ring, or 16-bit rows one at least; wider
+      // ones are split
+      const int elem = bytes[0] + bytes[1] + bytes[2];
+      const bool two_fit = 2 * shifted_columns(a->hidden) * elem <= kRingBytes;
+      const int steps = two_fit || elem <= 6 ? kShiftBwdSteps : kShiftBwdSteps / 2;
+      want.shifted = want.whole = true;
+      pl->why = plan_rows(a->rows, shifted_columns(a->hidden), bytes, false, kShiftThreads, steps, ud->sm_count,
+                          &pl->rows, &pl->k, &pl->smem, want);
+      pl->kernel = pick_shift(a);
     }
     if (pl->why) pl->kernel = nullptr;
     if (!pl->kernel) continue;

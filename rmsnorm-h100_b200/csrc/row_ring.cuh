@@ -1,7 +1,7 @@
 // row_ring.cuh -- the skeleton of the fused row kernels: persistent row groups that stream
 // their rows through shared-memory rings, row totals within a group and across a cluster.
 //
-//   * A CTA of 512 or 1024 threads holds `groups` row groups of G threads. A group owns a ring
+//   * A CTA of up to 1024 threads holds `groups` row groups of G threads. A group owns a ring
 //     of S units of its own and drifts freely: nothing but the total of a row ties its warps
 //     together, and nothing ties the groups of a CTA.
 //   * A unit is R whole rows, or KC of a row's K vector steps where a row would fill the

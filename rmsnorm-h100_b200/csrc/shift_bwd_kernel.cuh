@@ -9,8 +9,10 @@ namespace rmsb200 {
 
 constexpr int kShiftBwdSteps = 4;  // vector steps a thread, at most: their masks are the bytes of a word
 
-// The backward, with the sums of dweight and dbias in tensor memory and the row read from its
-// slot a second time: neither takes registers, so the number of steps is free.
+//   dh = rs dy w - h rs^3 mean(h dy w) (+ dresidual_out)
+// The sums of dweight and dbias lie in tensor memory and the row is read from its slot a second
+// time: neither takes registers, so the number of steps is free (the aligned kernel, which keeps
+// the row in registers, has the slot reloaded sooner: 227 against 299 us at 32768 x 4096 bf16).
 // H: type of h, dresidual_out and dresidual; DY: of dout and dx.
 template <typename H, typename DY>
 __global__ void __launch_bounds__(kShiftThreads, 1) shift_bwd_kernel(const FusedBwdParams p, const RowPlan pl) {

@@ -8,7 +8,10 @@
 // rows of one class modulo 8 (4, 2 where N divides by 2, 4) share their lead: a cluster works
 // on one class, so that a thread keeps its columns from row to row and the affine parameters
 // lie in shared memory at the row's offset. With 148 clusters a class has 18 or 19 of them,
-// which costs 3 %.
+// which costs 3 %. Measured at 1.3e8 elements (x, residual and outputs bf16, dropout), against
+// the scalar accesses of odd_kernels.cuh: 4097 columns forward 354 / 592 us, backward 421 / 1372,
+// 8-bit rows 238 / 531; 1001 columns 302 / 401, 389 / 787, 215 / 361. Bound by the instructions
+// of the generator, as the aligned kernels, plus a ninth of the draws and their shuffles.
 #pragma once
 
 #include <type_traits>
