@@ -99,7 +99,9 @@ FwdKernel pick_shift(int end, int k) {
   switch (end) {
     case kDropped: return pick_shift<X, Dropped>(k);
     case kE4M3Row: return pick_shift<X, Scaled<E4M3, true>>(k);
+    case kE4M3Group: return pick_shift<X, Scaled<E4M3, false>>(k);
     case kI8Row: return pick_shift<X, Scaled<I8, true>>(k);
+    case kI8Group: return pick_shift<X, Scaled<I8, false>>(k);
     default: return nullptr;
   }
 }
@@ -139,8 +141,8 @@ int run(const FusedFwdParams& p, bool drop, cudaStream_t stream) {
   st = ranges.send(stream);
   if (st) return st;
   // Aligned tensors in a combination of types with a kernel of its own: whole vectors where rows
-  // consist of them, shifted ones where they do not (and a scale is a row's); else the odd
-  // rows' kernels; else (rows wider than a cluster holds) the generic one.
+  // consist of them, shifted ones where they do not; else the odd rows' kernels; else (rows wider
+  // than a cluster holds) the generic one.
   const int bytes[3] = {elem_bytes(p.x_dt), p.res ? elem_bytes(p.res_dt) : 0, 0};
   RowPlan pl;
   int k = 0, smem = 0;
@@ -164,10 +166,11 @@ int run(const FusedFwdParams& p, bool drop, cudaStream_t stream) {
              (!p.ro || p.ro_dt == p.x_dt || p.ro_dt == RMSNORM_B200_F32)) {
     RowWants want;
     want.shifted = true;
+    want.scale = p.group;
     why = plan_rows(p.rows, shifted_columns(p.N), bytes, p.b != nullptr, kShiftThreads, kShiftFwdSteps, ud->sm_count,
                     &pl, &k, &smem, want);
-    FwdKernel kernel = why ? nullptr : pick_shift(p.x_dt, end, k);
-    if (kernel) {
+    if (!why && !(p.group && pl.C > 1)) {  // a scale's columns may lie in two CTAs' slices
+      FwdKernel kernel = pick_shift(p.x_dt, end, k);
       st = launch_shifted(ud, kernel, p, pl, smem, stream, drop ? "dropout_fwd_sh" : "quant_fwd_sh", k);
       if (st != RMSNORM_B200_ERR_UNSUPPORTED) return st;
     }

@@ -24,10 +24,19 @@ struct Scaled {  // 8-bit values Q; one scale per row, or one per group of colum
   using Type = Q;
 };
 
+//   h = x + residual, or keep x / (1 - p) + residual;  y = h rsqrt(mean(h^2) + eps) w + b
+//   8 bits: scale = max(largest |y| of the row or group / Q, 2^-126), q = round(y / scale)
 // X, RT, ROT: types of x, of the residual and of residual_out (NoT: absent).
-// Per element 5 (8-bit) to 12 (dropout) bytes cross HBM, which bounds the kernel.
+// A row is read once and stays in registers from its sum of squares to its output, so HBM sees
+// 4 (8-bit output, no residual) to 12 bytes an element and nothing else. Measured with copies at
+// 6.5 TB/s: 8 bits, one scale a row, bf16 + fp32 residual 32768 x 16384 725 to 795 us (738 us of
+// bytes; the slower runs are under the power cap); scales of 128 columns, bf16 8192 x 4096 43 us
+// (36 us of bytes, the rest the kernel's start and end); dropout, bf16 in, fp32 residual out,
+// 32768 x 4096 216 us (205). Dropout between bf16 tensors is bound by the generator instead: 80
+// instructions for 8 columns, 227 us for 164 us of bytes (72315 x 1856).
 template <typename X, typename RT, typename ROT, typename End, int K>
-__global__ void __launch_bounds__(K == 1 ? kFwdFewThreads : kFwdThreads, 1) fused_fwd_kernel(const FusedFwdParams p, const RowPlan pl) {
+__global__ void __launch_bounds__(K == 1 ? kFwdFewThreads : kFwdThreads, 1)
+    fused_fwd_kernel(const FusedFwdParams p, const RowPlan pl) {
   constexpr bool kRes = Present<RT>::value, kRo = Present<ROT>::value;
   constexpr bool kQuant = End::kQuant, kRowScale = End::kRowScale;
   constexpr int kStreams = kRes ? 2 : 1;

@@ -1,6 +1,7 @@
 // odd_kernels.cuh -- the fused row operators where the aligned and the shifted vector kernels
 // (shift_rows.cuh) do not apply: tensors that begin off a 16-byte boundary, combinations of types
-// without a kernel of their own, scales of column groups at a width that 8 does not divide.
+// without a kernel of their own, scales of column groups in rows of an odd width that take a
+// cluster.
 //
 // The rows stream through the same rings: a bulk copy brings the aligned 16-byte granules
 // that cover a unit, and the threads read the unit from its offset in the first of them. A

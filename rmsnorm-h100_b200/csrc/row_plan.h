@@ -21,6 +21,7 @@ struct RowWants {
   bool odd = false;      // the kernels of odd_kernels.cuh; otherwise N is a multiple of 8
   int built_in = 0;      // row group of a kernel made for one: four steps, units of bwd_unit_steps, a row each
   bool shifted = false;  // units of one row; one step or max_steps
+  int scale = 0;         // columns of a scale whose largest value passes through shared memory
   bool whole = false;    // a row's slice is one unit; two of them a group
 };
 
@@ -91,7 +92,8 @@ inline const char* plan_rows(int64_t rows, int64_t N, const int (&bytes)[3], boo
   pl->tiles = (rows + pl->R - 1) / pl->R;
   if (odd) pl->slice = (pl->slice + 7) & ~7;  // the affine copies keep the barriers' alignment
   const int affine = pl->slice * 4 * (bias ? 2 : 1);
-  const int fixed = affine + static_cast<int>(sizeof(RowBars)) + 16;
+  pl->scale_slots = want.scale ? pl->slice / want.scale + 1 : 0;
+  const int fixed = affine + static_cast<int>(sizeof(RowBars)) + 8 * pl->scale_slots * pl->groups + 16;
   const int unit = pl->groups * static_cast<int>(pl->unit_bytes);
   const int64_t per_group = (pl->tiles * pl->C + static_cast<int64_t>(sms) * pl->groups - 1) /
                             (static_cast<int64_t>(sms) * pl->groups);

@@ -33,6 +33,7 @@ struct RowPlan {
   uint32_t unit_bytes;
   uint32_t off[3];      // byte offset of tensor i in a unit
   int32_t bias;         // a bias follows the weight in shared memory
+  int32_t scale_slots;  // words a group has twice after the barriers, for the scales of odd rows
   int64_t tiles;        // units of R rows
 };
 

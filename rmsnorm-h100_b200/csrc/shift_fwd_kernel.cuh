@@ -9,10 +9,15 @@ namespace rmsb200 {
 constexpr int kShiftFwdSteps = 4;  // vector steps a thread, or one
 
 // X: type of x and of a floating output; residual and residual_out have it too, or fp32, or are
-// absent. 8-bit outputs have a scale a row.
+// absent.
+// A scale's columns begin `lead` elements into a vector, so the largest values of the groups are
+// put together in shared memory: a group's lanes are neighbours, their first lane adds the
+// maximum of its own elements and, of the elements before them, to the group before.
+// Maxima do not depend on their order. Two sets take turns; a row's is cleared after the
+// total of the row after it, which every warp reaches when it has read the scales.
 template <typename X, typename End, int K>
 __global__ void __launch_bounds__(kShiftThreads, 1) shift_fwd_kernel(const FusedFwdParams p, const RowPlan pl) {
-  constexpr bool kQuant = End::kQuant;
+  constexpr bool kQuant = End::kQuant, kGroups = kQuant && !End::kRowScale;
   constexpr int kX = sizeof(X);
   RowCtx c = row_begin(pl, p.N);
   const RowShift sh = shift_begin(pl, c, p.rows, p.N);
@@ -25,6 +30,10 @@ __global__ void __launch_bounds__(kShiftThreads, 1) shift_fwd_kernel(const Fused
   const uint64_t policy = l2_policy_evict_first();
   if (c.gl == 0)
     for (int u = 0; u < pl.S && u < c.units; ++u) shift_issue(pl, c, sh, u, u, p.rows, p.N, src, bytes, policy);
+  uint32_t* largest = reinterpret_cast<uint32_t*>(c.bars + 1) + c.gid * 2 * pl.scale_slots;  // of this row; then of the row before
+  uint32_t* cleared = largest + pl.scale_slots;
+  if constexpr (kGroups)
+    for (int i = c.gl; i < 2 * pl.scale_slots; i += pl.G) largest[i] = 0;
   shift_affine(pl, c, sh, p.w, p.w_dt, p.b, p.b_dt);
   const uint64_t offset = kQuant ? 0ull : drop_offset(p.drop);
   const float inv_n = 1.f / static_cast<float>(p.N);
@@ -109,25 +118,70 @@ __global__ void __launch_bounds__(kShiftThreads, 1) shift_fwd_kernel(const Fused
       }
       if constexpr (kQuant) {
         if (!edge.whole()) edge.mask(h[j]);  // rs may be NaN
-        most = largest8(most, h[j]);
+        if constexpr (!kGroups) most = largest8(most, h[j]);
       } else {
         shift_store<X>(p.out, e0 + col, edge, h[j]);
       }
     }
     if constexpr (kQuant) {
       using Q = typename End::Type;
-      bits = magnitude(most);
+      float inv_row = 0.f;
       float unused = 0.f;
-      row_total<false, true>(pl, c, unused, bits, kSiteFwdCluster);
-      const float s = scale_of(__uint_as_float(bits), Q::kInvQ), inv = inverse(s);
-      if (c.gl == 0 && c.rank == 0) st1(&p.scales[row * p.scale_row], s);
+      bits = magnitude(most);
+      if constexpr (kGroups) {
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+          const int col = (j * pl.G + c.gl) * 8;
+          const bool first = (col & (p.group - 1)) == 0;
+          const int own = first ? sh.lead : 0;  // elements from there on are this group's
+          uint32_t here = 0, before = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t m = magnitude(i & 1 ? h[j][i >> 1].y : h[j][i >> 1].x);
+            if (i >= own)
+              here = max(here, m);
+            else
+              before = max(before, m);
+          }
+          for (int o = p.group >> 4; o > 0; o >>= 1) here = max(here, __shfl_xor_sync(0xffffffffu, here, o));
+          if (first && col < c.ncols) {
+            atomicMax(&largest[col >> p.group_shift], here);
+            if (own > 0 && col > 0) atomicMax(&largest[(col >> p.group_shift) - 1], before);
+          }
+        }
+        __syncwarp();
+        row_total<false, true>(pl, c, unused, bits, kSiteFwdCluster);
+        __syncwarp();
+        for (int i = c.gl; i < pl.scale_slots; i += pl.G) cleared[i] = 0;
+      } else {
+        row_total<false, true>(pl, c, unused, bits, kSiteFwdCluster);
+        const float s = scale_of(__uint_as_float(bits), Q::kInvQ);
+        inv_row = inverse(s);
+        if (c.gl == 0 && c.rank == 0) st1(&p.scales[row * p.scale_row], s);
+      }
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         const int col = (j * pl.G + c.gl) * 8;
         if (col >= c.ncols) continue;
         const ShiftEdge edge(sh, c.slice0 + col);
+        if constexpr (kGroups) {
+          const int g = col >> p.group_shift;
+          const bool first = (col & (p.group - 1)) == 0;
+          const float s = scale_of(__uint_as_float(largest[g]), Q::kInvQ);
+          const float inv = inverse(s);
+          const float inv_before =
+              first && g > 0 ? inverse(scale_of(__uint_as_float(largest[g - 1]), Q::kInvQ)) : inv;
+          if (first && col < p.N) st1(&p.scales[row * p.scale_row + g * p.scale_group], s);
+          const int own = first ? sh.lead : 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[j][i] = mul2(h[j][i], splat2(inv));
+          for (int i = 0; i < 4; ++i) {
+            h[j][i].x *= 2 * i >= own ? inv : inv_before;
+            h[j][i].y *= 2 * i + 1 >= own ? inv : inv_before;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) h[j][i] = mul2(h[j][i], splat2(inv_row));
+        }
         const uint32_t q[2] = {Q::pack4(h[j][0], h[j][1]), Q::pack4(h[j][2], h[j][3])};
         uint8_t* dst = static_cast<uint8_t*>(p.out) + e0 + col;
         if (edge.whole()) {
@@ -138,6 +192,9 @@ __global__ void __launch_bounds__(kShiftThreads, 1) shift_fwd_kernel(const Fused
             if (i >= edge.lo && i < edge.hi) st1(dst + i, static_cast<uint8_t>(q[i >> 2] >> (8 * (i & 3))));
         }
       }
+      uint32_t* last = largest;
+      largest = cleared;
+      cleared = last;
     }
   }
   row_end(pl, c);
