@@ -33,6 +33,12 @@ def cases():
         yield f"dropout fwd {n}", lambda n=n, r=rows: t.drop_case(r, n, BF16, BF16, F32, None, True, True)
         yield f"dropout bwd {n}", lambda n=n, r=rows: t.bwd_case(r, n, BF16, BF16, BF16, True, True)
         yield f"dropout bwd f32 {n}", lambda n=n, r=rows: t.bwd_case(r, n, F32, BF16, F32, True, False)
+    for n in (3, 9, 252, 1003, 1006, 4099, 16387):  # vectors shared by neighbouring rows
+        for r in (1, 5, 301):
+            yield f"odd quant {n} {r}", lambda n=n, r=r: t.quant_case(r, n, BF16, BF16, None, True, True, E4M3, 32)
+            yield f"odd quant row {n} {r}", lambda n=n, r=r: t.quant_case(r, n, F32, None, None, True, False, I8, None)
+            yield f"odd dropout fwd {n} {r}", lambda n=n, r=r: t.drop_case(r, n, F16, F16, F32, None, True, True)
+            yield f"odd dropout bwd {n} {r}", lambda n=n, r=r: t.bwd_case(r, n, F32, BF16, F32, True, True)
     for rows in (1, 147, 149):
         yield f"quant rows {rows}", lambda r=rows: t.quant_case(r, 4096, F32, F32, None, True, False, E4M3, None)
         yield f"dropout rows {rows}", lambda r=rows: t.bwd_case(r, 4096, F16, F16, None, True, True)

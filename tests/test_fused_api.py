@@ -324,6 +324,15 @@ def test_dropout_refusals():
         fused.dropout_add_rmsnorm_bwd(x, None, x, rstd, dx_dtype=torch.int8)
 
 
+def test_rope_refuses_more_heads_than_the_kernels_count():
+    q, table, pos = torch.zeros(1, 65537, 2), torch.ones(1, 2), torch.zeros(1, dtype=torch.int64)
+    with pytest.raises(ValueError, match="65536"):
+        fused.qk_norm_rope_fwd(q, None, pos, table)
+    with pytest.raises(ValueError, match="65536"):
+        fused.qk_norm_rope_fwd(q[:, :1], q, pos, table)
+    fused.qk_norm_rope_fwd(q[:, 1:], q[:, :1], pos, table)
+
+
 def test_rope_refusals():
     q, k, pos, table, qw, kw, axes = _rope_inputs(4, 2, 1, 8, 8, (2, 2))
     ok = dict(q=q, k=k, positions=pos, table=table, q_weight=qw, k_weight=kw, axes=axes)

@@ -480,6 +480,53 @@ def test_rope_special_rows_autograd_and_empty():
     assert (dw == 0).all()
 
 
+# ------------------------------------------------------------------ widths that 8 does not divide
+# every remainder modulo 8, fewer rows than remainders, rows that end and begin inside a vector,
+# one and several vector steps, groups of one and more warps, a cluster
+ODD_WIDTHS = [2, 3, 5, 9, 250, 252, 1002, 1003, 1006, 1007, 2050, 4099, 5124, 8191, 12289, 16387, 33001]
+
+
+@pytest.mark.parametrize("n", ODD_WIDTHS)
+@pytest.mark.parametrize("rows", [1, 7, 301])
+def test_odd_widths(n, rows):
+    quant_case(rows, n, BF16, BF16, None, True, True, E4M3, None)
+    quant_case(rows, n, F16, F16, F32, True, False, I8, 32)
+    quant_case(rows, n, F32, None, None, True, True, E4M3, 256)
+    drop_case(rows, n, BF16, BF16, None, None, True, True)
+    drop_case(rows, n, F32, F32, None, None, True, False, row_offset=5)
+    bwd_case(rows, n, BF16, BF16, BF16, True, True)
+    bwd_case(rows, n, F32, BF16, F32, True, True)
+
+
+@pytest.mark.parametrize("n", [9, 1003, 4100])
+def test_odd_widths_keep_rows_apart(n):
+    """A row's NaN and infinities stay in it, although it shares vectors with its neighbours."""
+    x, dout, w = rand(61, n, dtype=BF16), rand(61, n, dtype=BF16, seed=1), rand(n, seed=2)
+    bad = torch.arange(61, device=DEV) % 3 == 1
+    dirty = torch.where(bad[:, None], torch.where(rand(61, n, seed=3) > 0, float("nan"), float("inf")).to(BF16), x)
+    for group in (None, 32):
+        a, b = (fused.rmsnorm_quant_fwd(t, w, group_size=group) for t in (x, dirty))
+        assert torch.equal(a[0].view(torch.uint8)[~bad], b[0].view(torch.uint8)[~bad])
+        assert torch.equal(a[1][~bad], b[1][~bad]) and not b[1][bad].isfinite().all()
+    rng = (5, 6)
+    a, b = (fused.dropout_add_rmsnorm_fwd(t, w, residual=dout, p=0.2, rng=rng, store_rstd=True) for t in (x, dirty))
+    for s, t in zip(a, b):
+        assert torch.equal(s[~bad], t[~bad])
+    rstd = a[2]
+    a, b = (fused.dropout_add_rmsnorm_bwd(t, w, dout, rstd, None, 0.2, rng, False, True) for t in (x, dirty))
+    assert torch.equal(a[0][~bad], b[0][~bad]) and torch.equal(a[3][~bad], b[3][~bad])
+
+
+@pytest.mark.parametrize("n", [520, 2368, 4160, 5120, 9216, 10240])
+def test_widths_between_powers_of_two(n):
+    """Row groups of every number of warps."""
+    quant_case(601, n, BF16, BF16, None, True, True, E4M3, 64)
+    drop_case(601, n, F16, F16, None, None, True, True)
+    bwd_case(601, n, F16, F16, F16, True, True)
+    bwd_case(601, n, F32, F32, F32, True, True)
+    bwd_case(601, n, F32, BF16, None, True, False)
+
+
 # ------------------------------------------------------------------ refusals that need a device
 def test_refusals_on_device():
     x = rand(2, 64)
