@@ -523,28 +523,41 @@ def _check_rope(q, k, positions, table, q_weight, k_weight, axes):
     return axes, words, naxes, device, code, kwc if q_weight is None else qwc, qwh, kwh
 
 
-def _flat(t: Tensor) -> Tensor:
-    """[tokens, heads, head_dim] with a contiguous last dimension; a view wherever the strides
-    allow one (q and k as slices of a packed projection)."""
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        t = t.contiguous()
-    return t if t.dim() == 3 else t.reshape(-1, t.shape[-2], t.shape[-1])
+_NOWHERE = (0, 0, 0)
 
 
-def _place(t: Optional[Tensor]) -> Tuple[int, int, int]:
-    """Address, token stride and head stride of a _flat tensor."""
+def _place(t: Optional[Tensor]) -> Tuple[Optional[Tensor], Tuple[int, int, int]]:
+    """t as [tokens, heads, head_dim] with a contiguous last dimension, a view wherever the
+    strides allow one (q and k as slices of a packed projection); its address, token stride
+    and head stride."""
     if t is None:
-        return 0, 0, 0
-    return t.data_ptr(), t.stride(0), t.stride(1)
+        return None, _NOWHERE
+    stride = t.stride()
+    if stride[-1] != 1 and t.shape[-1] > 1:
+        t = t.contiguous()
+        stride = t.stride()
+    if len(stride) != 3:
+        t = t.reshape(-1, t.shape[-2], t.shape[-1])
+        stride = t.stride()
+    return t, (t.data_ptr(), stride[0], stride[1])
 
 
-def _rope_args(q, k, positions, table, q_weight, k_weight, checked, interleaved, norm, eps) -> bytes:
+def _new_like(t: Optional[Tensor]) -> Tuple[Optional[Tensor], Tuple[int, int, int]]:
+    """A contiguous tensor of t's shape, and its place as _place gives it."""
+    if t is None:
+        return None, _NOWHERE
+    new = torch.empty_like(t, memory_format=torch.contiguous_format)
+    d = t.shape[-1]
+    return new, (new.data_ptr(), t.shape[-2] * d, d)
+
+
+def _rope_args(q, q_place, k, k_place, positions, table, q_weight, k_weight, checked, interleaved, norm, eps) -> bytes:
     _, words, naxes, _, code, wc, qwh, kwh = checked
     tokens, heads, d = q.shape
     return _ROPE.pack(
         tokens, table.shape[0], positions.data_ptr(), tokens, table.data_ptr(),
-        0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), *_place(q),
-        *_place(k), *words, heads, 0 if k is None else k.shape[1], d, table.shape[1], naxes, bool(interleaved),
+        0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), *q_place,
+        *k_place, *words, heads, 0 if k is None else k.shape[1], d, table.shape[1], naxes, bool(interleaved),
         bool(norm), positions.dtype == torch.int64, code, wc, qwh, kwh, eps, 0)
 
 
@@ -586,30 +599,24 @@ def qk_norm_rope_fwd(
                     t.copy_(o)
             return q, k
         return tuple(outs)
-    qf = _flat(q)
-    kf = None if k is None else _flat(k)
-    q_out, k_out = q, k
+    qf, q_place = _place(q)
+    kf, k_place = _place(k)
     if inplace:
-        for t, f in ((q, qf), (k, kf)):
-            if t is not None and f.data_ptr() != t.data_ptr():
+        for t, place in ((q, q_place), (k, k_place)):
+            if t is not None and place[0] != t.data_ptr():
                 raise ValueError("inplace needs q and k whose leading dimensions collapse to one stride")
-        qo, ko = qf, kf
+        q_out, k_out, qo_place, ko_place = q, k, q_place, k_place
     else:
-        q_out = qo = torch.empty_like(q, memory_format=torch.contiguous_format)
-        ko = None
-        if k is not None:
-            k_out = ko = torch.empty_like(k, memory_format=torch.contiguous_format)
-        if q.dim() != 3:
-            qo = qo.view(qf.shape)
-            ko = None if ko is None else ko.view(kf.shape)
+        q_out, qo_place = _new_like(q)
+        k_out, ko_place = _new_like(k)
     positions = positions.contiguous()
     table = table.contiguous()
     q_weight = _contig(q_weight)
     k_weight = _contig(k_weight)
-    args = _rope_args(qf, kf, positions, table, q_weight, k_weight, checked, interleaved, norm, eps)
+    args = _rope_args(qf, q_place, kf, k_place, positions, table, q_weight, k_weight, checked, interleaved, norm, eps)
     name = "rmsnorm_b200_rope_fwd"
     _lib.enqueue(_lib.packed_entry(name, _BYTES, _BYTES, _BYTES, _STREAM), name, checked[3].index, args,
-                 _ROPE_TENSOR.pack(*_place(qo)), _ROPE_TENSOR.pack(*_place(ko)))
+                 _ROPE_TENSOR.pack(*qo_place), _ROPE_TENSOR.pack(*ko_place))
     return q_out, k_out
 
 
@@ -646,23 +653,22 @@ def qk_norm_rope_bwd(
             dk, dkw = _host.qk_norm_rope_bwd(k, k_weight, dk_out, cos, sin, interleaved, norm, eps)
         return dq, dk, dqw, dkw
     device = checked[3]
-    qf = _flat(q)
-    kf = None if k is None else _flat(k)
-    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
-    dk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+    qf, q_place = _place(q)
+    kf, k_place = _place(k)
+    dqo, dqo_place = _place(dq_out)  # named, so that copies live until the launch
+    dko, dko_place = _place(dk_out)
+    dq, dq_place = _new_like(q)
+    dk, dk_place = _new_like(k)
     q_weight = _contig(q_weight)
     k_weight = _contig(k_weight)
     dqw = None if q_weight is None else torch.empty_like(q_weight)
     dkw = None if k_weight is None else torch.empty_like(k_weight)
     positions = positions.contiguous()
     table = table.contiguous()
-    dqo = _flat(dq_out)
-    dko = None if k is None else _flat(dk_out)
-    args = _rope_args(qf, kf, positions, table, q_weight, k_weight, checked, interleaved, norm, eps)
+    args = _rope_args(qf, q_place, kf, k_place, positions, table, q_weight, k_weight, checked, interleaved, norm, eps)
     grads = _ROPE_GRADS.pack(
-        *_place(dqo), *_place(dko), dq.data_ptr(), dq.stride(-2) * q.shape[-2], dq.stride(-2),
-        *((0, 0, 0) if k is None else (dk.data_ptr(), dk.stride(-2) * k.shape[-2], dk.stride(-2))),
-        0 if dqw is None else dqw.data_ptr(), 0 if dkw is None else dkw.data_ptr())
+        *dqo_place, *dko_place, *dq_place, *dk_place, 0 if dqw is None else dqw.data_ptr(),
+        0 if dkw is None else dkw.data_ptr())
     nbytes = 0
     if dqw is not None or dkw is not None:
         name = "rmsnorm_b200_rope_bwd_workspace_size"
