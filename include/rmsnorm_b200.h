@@ -356,8 +356,9 @@ int rmsnorm_b200_dropout_rmsnorm_bwd(const rmsnorm_b200_dropout_bwd_args* args, 
  * interleaved; with position t = positions[axis(i)][token], c = table[t][i] and
  * s = table[t][rotary_dim / 2 + i] it becomes (y_a c - y_b s, y_b c + y_a s). Columns from
  * rotary_dim on are not turned. A position outside the table makes the token's turned
- * columns NaN and records RMSNORM_B200_ERR_INVALID_ARGUMENT (site 10) in the device status
- * word. Only the last dimension of a tensor has to be contiguous. */
+ * columns NaN and records RMSNORM_B200_ERR_INVALID_ARGUMENT (site 10) for
+ * rmsnorm_b200_device_status; nothing else changes, in this call or later ones. Only the last
+ * dimension of a tensor has to be contiguous. */
 #define RMSNORM_B200_ROPE_MAX_HEAD_DIM 256
 #define RMSNORM_B200_ROPE_MAX_HEADS 65536
 typedef struct rmsnorm_b200_rope_tensor {
@@ -417,9 +418,11 @@ int rmsnorm_b200_rope_bwd(const rmsnorm_b200_rope_args* args, const rmsnorm_b200
 /* Static, human-readable message for a status code. */
 const char* rmsnorm_b200_strerror(int status);
 
-/* Reads (and optionally clears) the current device's status word, in stream order:
+/* Reads (and optionally clears) the current device's status words, in stream order:
  * 0 when no kernel has reported a problem, RMSNORM_B200_ERR_DEVICE_TIMEOUT when a bounded
- * device-side wait ran out. Synchronises `stream`. */
+ * device-side wait ran out (every wait gives up from then on, until the word is cleared), else
+ * RMSNORM_B200_ERR_INVALID_ARGUMENT when a call met a value among its data that it answered
+ * with NaN. Synchronises `stream`. */
 int rmsnorm_b200_device_status(void* stream, int32_t* status, int32_t* where, int32_t clear);
 
 /* Upper bound of every device-side wait on the current device (default 2 s; at least 1 ms,

@@ -15,12 +15,17 @@
 namespace rmsb200 {
 
 // ---------------------------------------------------------------------------------------
-// Device status word (one per device: file-scope __device__ variables live in each
-// device's copy of the module). 0 = OK; otherwise the first error recorded. The library
-// is a single translation unit, so the variables are defined here.
+// Device status words (one set per device and translation unit: file-scope __device__
+// variables live in each device's copy of the module, and translation_units.h tells how the
+// units' are put together). 0 = OK; otherwise the first error recorded.
+// g_status holds a wait that ran out: from then on every wait gives up (abort_requested).
+// g_data_status holds a value among a call's data that the kernels answer with NaN; no wait
+// looks at it, so it changes nothing but the answer of rmsnorm_b200_device_status.
 // ---------------------------------------------------------------------------------------
 __device__ int g_status = 0;
 __device__ int g_status_where = 0;
+__device__ int g_data_status = 0;
+__device__ int g_data_status_where = 0;
 __device__ unsigned long long g_wait_timeout_ns = 2000000000ull;
 
 // Where a bounded wait gave up (reported through rmsnorm_b200_device_status).
@@ -39,6 +44,12 @@ enum WaitSite : int {
 __device__ __forceinline__ void record_error(int code, int where) {
   if (atomicCAS(&g_status, 0, code) == 0) {
     atomicExch(&g_status_where, where);
+  }
+}
+
+__device__ __forceinline__ void record_data_error(int code, int where) {
+  if (atomicCAS(&g_data_status, 0, code) == 0) {
+    atomicExch(&g_data_status_where, where);
   }
 }
 

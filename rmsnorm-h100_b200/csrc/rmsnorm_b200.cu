@@ -1453,13 +1453,18 @@ extern "C" int rmsnorm_b200_device_status(void* stream, int32_t* status, int32_t
         cudaMemcpyToSymbolAsync(g_status_where, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s) != cudaSuccess)
       return RMSNORM_B200_ERR_CUDA;
   }
-  int unit_st[kUnits] = {}, unit_wh[kUnits] = {};
+  rmsb_units::UnitStatus units[kUnits];
   for (int i = 0; i < kUnits; ++i)
-    if (const int err = kUnitHooks[i]->status(s, &unit_st[i], &unit_wh[i], clear != 0)) return err;
+    if (const int err = kUnitHooks[i]->status(s, &units[i], clear != 0)) return err;
   if (cudaStreamSynchronize(s) != cudaSuccess) return RMSNORM_B200_ERR_CUDA;
+  // a wait that ran out before values among the data: it leaves more in doubt
   for (int i = 0; i < kUnits && st == 0; ++i) {
-    st = unit_st[i];
-    wh = unit_wh[i];
+    st = units[i].status;
+    wh = units[i].where;
+  }
+  for (int i = 0; i < kUnits && st == 0; ++i) {
+    st = units[i].data_status;
+    wh = units[i].data_where;
   }
   if (status) *status = st;
   if (where) *where = wh;

@@ -37,7 +37,7 @@ __device__ __forceinline__ int64_t rope_row_at(const RopeParams& p, int64_t at) 
   const int64_t t = p.pos64 ? ld1(static_cast<const int64_t*>(p.pos) + at)
                             : static_cast<int64_t>(ld1(static_cast<const int32_t*>(p.pos) + at));
   if (t >= 0 && t < p.table_rows) return t;
-  record_error(RMSNORM_B200_ERR_INVALID_ARGUMENT, kSiteRopePosition);
+  record_data_error(RMSNORM_B200_ERR_INVALID_ARGUMENT, kSiteRopePosition);
   return -1;
 }
 

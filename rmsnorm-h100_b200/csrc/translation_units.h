@@ -14,9 +14,15 @@
 
 namespace rmsb_units {
 
+// A unit's status words: a wait that ran out, and a value among a call's data.
+struct UnitStatus {
+  int status = 0, where = 0;
+  int data_status = 0, data_where = 0;
+};
+
 struct UnitHooks {
-  // Enqueues the read (and clear) of the unit's status word; the caller synchronises.
-  int (*status)(cudaStream_t stream, int* status, int* where, bool clear);
+  // Enqueues the read (and clear) of the unit's status words; the caller synchronises.
+  int (*status)(cudaStream_t stream, UnitStatus* words, bool clear);
   int (*set_wait_timeout)(unsigned long long ns);
   // The four words of the unit's bounds-check report (bounds-checked build only).
   int (*report)(unsigned long long (&words)[4], bool clear);

@@ -93,14 +93,21 @@ struct Ranges {
 };
 #endif
 
-int unit_status(cudaStream_t s, int* status, int* where, bool clear) {
-  if (cudaMemcpyFromSymbolAsync(status, g_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-      cudaMemcpyFromSymbolAsync(where, g_status_where, sizeof(int), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess)
+int unit_status(cudaStream_t s, rmsb_units::UnitStatus* words, bool clear) {
+  if (cudaMemcpyFromSymbolAsync(&words->status, g_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+      cudaMemcpyFromSymbolAsync(&words->where, g_status_where, sizeof(int), 0, cudaMemcpyDeviceToHost, s) !=
+          cudaSuccess ||
+      cudaMemcpyFromSymbolAsync(&words->data_status, g_data_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s) !=
+          cudaSuccess ||
+      cudaMemcpyFromSymbolAsync(&words->data_where, g_data_status_where, sizeof(int), 0, cudaMemcpyDeviceToHost, s) !=
+          cudaSuccess)
     return RMSNORM_B200_ERR_CUDA;
   if (clear) {
     static const int zero = 0;
     if (cudaMemcpyToSymbolAsync(g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
-        cudaMemcpyToSymbolAsync(g_status_where, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s) != cudaSuccess)
+        cudaMemcpyToSymbolAsync(g_status_where, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
+        cudaMemcpyToSymbolAsync(g_data_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
+        cudaMemcpyToSymbolAsync(g_data_status_where, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s) != cudaSuccess)
       return RMSNORM_B200_ERR_CUDA;
   }
   return RMSNORM_B200_OK;

@@ -603,7 +603,7 @@ def bwd_noalloc(a: BwdArgs, device: torch.device) -> int:
 
 
 def device_status(device: torch.device, clear: bool = False) -> tuple:
-    """(status, site) of the device status word, read in stream order."""
+    """(status, site) of the device status words, read in stream order."""
     lib = load_library()
     st = ctypes.c_int32(0)
     wh = ctypes.c_int32(0)

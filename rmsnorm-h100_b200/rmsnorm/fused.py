@@ -583,8 +583,8 @@ def qk_norm_rope_fwd(
     positions (int32 or int64) has the leading shape of q, or (axes, ...) of it; `axes` names
     the axis of each of the rotary_dim / 2 pairs (`rope_axes`; default: axis 0). Pair i is the
     columns (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when `interleaved`. `table` is
-    `rope_table`'s. A position outside the table gives NaN columns, and on CUDA an
-    invalid-argument entry in the device status word."""
+    `rope_table`'s. A position outside the table makes its token's turned columns NaN, and on
+    CUDA the device status tells of an invalid argument; nothing else changes."""
     if _is_compiling():
         return _rope_fwd_untraced(
             q, k, positions, table, q_weight, k_weight, axes, interleaved, norm, eps, inplace)
