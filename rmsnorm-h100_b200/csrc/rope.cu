@@ -85,19 +85,24 @@ bool vectorised(const rmsnorm_b200_rope_args* a, std::initializer_list<const rms
 constexpr int kRopeSlots = 8;         // ring slots of a warp, at most
 constexpr int kRopeSmem = 208 * 1024;  // beside the backward's 16 KB of static shared memory
 
-// u: heads a lane works on at a time.
+// Whether a tensor's heads are not neighbours.
+bool heads_apart(const rmsnorm_b200_rope_tensor& t, int heads, int head_dim) {
+  return heads > 1 && t.head_stride != head_dim;
+}
+
 struct RopeGrid {
   RopePlan pl;
   dim3 grid;
   int threads, smem;
 };
 
-// tensors: that stream through a warp's ring (0: no ring).
-RopeGrid plan(const rmsnorm_b200_rope_args* a, int u, int tensors, int sms) {
+// u: heads a lane works on. tensors: that stream through a warp's ring (0: no ring); apart: some
+// of them head by head, which a warp's 32 lanes copy one each.
+RopeGrid plan(const rmsnorm_b200_rope_args* a, int u, int tensors, bool apart, int sms) {
   RopeGrid g = {};
   RopePlan& pl = g.pl;
   while ((8 << pl.lanes_shift) < a->head_dim) ++pl.lanes_shift;
-  const int heads = u * (32 >> pl.lanes_shift);  // of a warp
+  const int heads = pl.warp_heads = std::min(u * (32 >> pl.lanes_shift), apart ? 32 : INT32_MAX);
   pl.jobs[0] = (a->q_heads + heads - 1) / heads;
   pl.jobs[1] = (a->k_heads + heads - 1) / heads;
   pl.turned_lanes = a->rotary_dim / 8;
@@ -228,9 +233,10 @@ int run_fwd(const rmsnorm_b200_rope_args* a, const rmsnorm_b200_rope_tensor* qo,
   if (ko) p.out[1] = tensor(*ko);
   if (vectorised(a, {&a->q, &a->k, qo, ko})) {
     // Four heads a lane where that leaves every SM eight warps to run; single heads below.
-    RopeGrid g = plan(a, 4, 1, ud->sm_count);
+    const bool apart = heads_apart(a->q, a->q_heads, a->head_dim) || heads_apart(a->k, a->k_heads, a->head_dim);
+    RopeGrid g = plan(a, 4, 1, apart, ud->sm_count);
     const bool wide = a->tokens * (g.pl.jobs[0] + g.pl.jobs[1]) >= int64_t{8} * ud->sm_count;
-    if (!wide) g = plan(a, 1, 0, ud->sm_count);
+    if (!wide) g = plan(a, 1, 0, false, ud->sm_count);
     return launch(ud, wide ? pick_fwd<4>(p) : pick_fwd<1>(p), g, stream, p, "rope_fwd");
   }
   const int64_t work = a->tokens * (a->q_heads + a->k_heads);
@@ -264,7 +270,10 @@ BwdPlan plan_bwd(const UnitDevice* ud, const rmsnorm_b200_rope_args* a, const rm
   pl.per_head = (a->q_weight && a->q_weight_heads > 1) || (a->k_weight && a->k_weight_heads > 1);
   pl.vec = vectorised(a, {&a->q, &a->k, &g->dq_out, &g->dk_out, &g->dq, &g->dk});
   if (pl.vec) {
-    pl.rope = plan(a, bwd_heads(pl.per_head), 2, ud->sm_count);
+    bool apart = false;
+    for (const auto* t : {&a->q, &g->dq_out}) apart = apart || heads_apart(*t, a->q_heads, a->head_dim);
+    for (const auto* t : {&a->k, &g->dk_out}) apart = apart || heads_apart(*t, a->k_heads, a->head_dim);
+    pl.rope = plan(a, bwd_heads(pl.per_head), 2, apart, ud->sm_count);
     const int64_t along = pl.rope.grid.x, across = pl.rope.grid.y;
     pl.rows = pl.per_head ? along : along * across;
     pl.width = (pl.per_head ? heads : 2) * a->head_dim;

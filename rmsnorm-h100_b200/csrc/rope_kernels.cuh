@@ -211,10 +211,12 @@ struct Chunk4<float> {
 
 // A warp takes U * (32 / L) heads of a token, all of q or all of k, and keeps them over all
 // the tokens it takes: the weight (and the backward's sums of its gradient) stay in registers.
+// Where its heads are copied one by one, a lane each, it takes 32 at most.
 struct RopePlan {
   int32_t S;            // ring slots of a warp
   uint32_t slot_bytes;  // of one tensor in a slot
   int32_t lanes_shift;  // log2(L)
+  int32_t warp_heads;   // of a warp's share: a multiple of 32 / L
   int32_t jobs[2];      // warps' shares of a token: of q first, then of k
   int32_t turned_lanes; // lanes of the turned part: rotary_dim / 8
   int32_t cta_jobs;     // shares of a CTA, whose warps take warps / cta_jobs tokens at a time
@@ -346,12 +348,13 @@ __device__ __forceinline__ void rope_weight8(const RopeParams& p, int k, int64_t
 struct RopeJob {
   bool works;
   int k, job, head0;     // q or k; share of it; the lane's first head
+  int first;             // the warp's first head
   int per;               // heads of the warp side by side: the lane's next head is head0 + per
   int heads;
   int64_t token, step;
 };
 
-__device__ __forceinline__ RopeJob rope_job(const RopeParams& p, const RopePlan& pl, const RopeLane& t, int u) {
+__device__ __forceinline__ RopeJob rope_job(const RopeParams& p, const RopePlan& pl, const RopeLane& t) {
   RopeJob b;
   const int warp = threadIdx.x >> 5;
   const int at_once = (blockDim.x >> 5) / pl.cta_jobs;  // tokens
@@ -360,7 +363,8 @@ __device__ __forceinline__ RopeJob rope_job(const RopeParams& p, const RopePlan&
   b.k = b.job >= pl.jobs[0];
   if (b.k) b.job -= pl.jobs[0];
   b.per = 32 >> pl.lanes_shift;
-  b.head0 = b.job * u * b.per + t.sub;
+  b.first = b.job * pl.warp_heads;
+  b.head0 = b.first + t.sub;
   b.heads = b.k ? p.heads[1] : p.heads[0];
   b.token = static_cast<int64_t>(blockIdx.x) * at_once + warp / pl.cta_jobs;
   b.step = static_cast<int64_t>(gridDim.x) * at_once;
@@ -418,12 +422,12 @@ struct RopeRing {
   }
   __device__ __forceinline__ const T* first_head(const RopeParams& p, const RopeJob& b, int i, int64_t token) const {
     const RopeTensor& x = tensor(p, b, i);
-    return static_cast<const T*>(x.p) + token * x.ts + static_cast<int64_t>(b.job * U * b.per) * x.hs;
+    return static_cast<const T*>(x.p) + token * x.ts + static_cast<int64_t>(b.first) * x.hs;
   }
   // Copies token `next` into slot s.
   __device__ __forceinline__ void issue(const RopeParams& p, const RopeJob& b, const RopePlan& pl, int s) {
     const int lane = threadIdx.x & 31;
-    const int heads = min(U * b.per, b.heads - b.job * U * b.per);
+    const int heads = min(pl.warp_heads, b.heads - b.first);
     if (next < p.tokens) {
       const uint64_t policy = l2_policy_evict_first();
       const uint32_t head_bytes = p.D * sizeof(T);
@@ -435,7 +439,7 @@ struct RopeRing {
         unsigned char* dst = rmsb_dyn_smem + slots + (s * kTensors + i) * pl.slot_bytes;
         const T* from = kTensors == 1 ? src : first_head(p, b, i, next);
         const bool together = x.hs == p.D;
-        if (lane < (together ? 1 : heads))
+        if (lane < (together ? 1 : heads))  // heads apart: 32 at most
           bulk_load(dst + lane * head_bytes, from + lane * x.hs, together ? heads * head_bytes : head_bytes, bar(s),
                     policy);
         if (kTensors == 1) src += b.step * x.ts;
@@ -497,7 +501,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_fwd_kernel(const RopePar
   pdl_launch_dependents();
   pdl_wait();
   const RopeLane t = rope_lane<kInterleaved>(p, pl);
-  const RopeJob b = rope_job(p, pl, t, U);
+  const RopeJob b = rope_job(p, pl, t);
   if (!b.works) return;
   const int k = b.k;
   [[maybe_unused]] RopePlace<T> in(k ? p.x[1] : p.x[0], t, b);
@@ -506,7 +510,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_fwd_kernel(const RopePar
   if constexpr (kRing) ring.start(p, b, pl);
   const bool per_head = p.w_per_head[k];
   const float inv_d = 1.f / static_cast<float>(p.D);
-  const int mine = t.in ? (b.heads - b.head0 + b.per - 1) / b.per : 0;  // the lane has heads u < mine
+  const int mine = t.in ? (min(b.heads, b.first + pl.warp_heads) - b.head0 + b.per - 1) / b.per : 0;  // the lane has heads u < mine
   float2 w[4];
   RopeTurn turn(p, t, b.token, b.step);
   if (!per_head) rope_weight8(p, k, 0, t, w);
@@ -582,7 +586,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_bwd_kernel(const RopePar
   pdl_launch_dependents();
   pdl_wait();
   const RopeLane t = rope_lane<kInterleaved>(p, pl);
-  const RopeJob b = rope_job(p, pl, t, U);
+  const RopeJob b = rope_job(p, pl, t);
   const int warp = threadIdx.x >> 5;
   const int at_once = (blockDim.x >> 5) / pl.cta_jobs;
   const int first_job = blockIdx.y * pl.cta_jobs;
@@ -593,8 +597,9 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_bwd_kernel(const RopePar
   if (b.works) ring.start(p, b, pl);
   const bool per_head = kPerHead && p.w_per_head[k];
   const float inv_d = 1.f / static_cast<float>(p.D);
-  const int mine = t.in ? (b.heads - b.head0 + per - 1) / per : 0;  // the lane has heads u < mine
-  const int used = min(U, (b.heads - b.job * U * per + per - 1) / per);  // u < used: some lane of the warp has the head
+  const int end = min(b.heads, b.first + pl.warp_heads);           // of the warp's heads
+  const int mine = t.in ? (end - b.head0 + per - 1) / per : 0;     // the lane has heads u < mine
+  const int used = (end - b.first + per - 1) / per;                // u < used: some lane of the warp has the head
   float2 acc[kSets][4], w[4];
 #pragma unroll
   for (int i = 0; i < kSets; ++i)
@@ -697,8 +702,8 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_bwd_kernel(const RopePar
       __syncthreads();
       if (b.works && warp < pl.cta_jobs) {
         for (int i = threadIdx.x & 31; i < per * p.D; i += 32) {
-          const int head = b.job * U * per + u * per + i / p.D;
-          if (head >= b.heads) continue;
+          const int head = b.first + u * per + i / p.D;
+          if (head >= end) continue;
           float v = 0.f;
           for (int j = 0; j < at_once; ++j) v += sums[warp + j * pl.cta_jobs][i];
           st1(&p.part[(row + (k ? p.heads[0] : 0) + head) * p.D + i % p.D], v);

@@ -1,14 +1,22 @@
 # SPDX-License-Identifier: MIT
 """The rotary kernels that stream a warp's heads through a ring, where their data or layout is
-out of the ordinary: positions outside the table beside ordinary ones."""
+out of the ordinary: positions outside the table beside ordinary ones, heads that are not
+neighbours."""
 
 from __future__ import annotations
+
+import json
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
 
+import fused_ref as ref
 from rmsnorm import _lib, fused
-from test_gpu_fused import BF16, DEV, F32, rand
+from test_gpu_fused import BF16, DEV, F16, F32, rand
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
 
@@ -77,3 +85,89 @@ def test_a_wait_that_ran_out_is_told_before_a_position():
     assert _lib.device_status(DEV) == (1, 10)
     _lib.selftest_wait_timeout(DEV, 5_000_000)
     assert _lib.device_status(DEV, clear=True) == (_lib.ERR_DEVICE_TIMEOUT, 8)
+
+
+# ------------------------------------------------------------------ heads that are not neighbours
+def apart(tokens, heads, d, gap, dtype, seed):
+    """[tokens, heads, d] with a head stride of `gap` head sizes; 0: [heads, tokens, d] transposed."""
+    if gap == 0:
+        return rand(heads, tokens, d, dtype=dtype, seed=seed).transpose(0, 1)
+    return rand(tokens, heads, gap * d, dtype=dtype, seed=seed)[..., :d]
+
+
+def apart_case(tokens, hq, hk, d, gap, dtype=BF16, weights="shared", interleaved=False, grad_gap=None, ring=True):
+    grad_gap = gap if grad_gap is None else grad_gap
+    q, k = apart(tokens, hq, d, gap, dtype, 1), apart(tokens, hk, d, gap, dtype, 2)
+    dq, dk = apart(tokens, hq, d, grad_gap, dtype, 3), apart(tokens, hk, d, grad_gap, dtype, 4)
+    table = fused.rope_table(3000, d, device=DEV)
+    pos = torch.randint(0, 3000, (1, tokens), device=DEV, generator=torch.Generator(device=DEV).manual_seed(5))
+    axes = (0,) * (d // 2)
+    cos, sin = ref.cos_sin(pos, table, axes)
+    shape = (lambda h: (h, d)) if weights == "heads" else (lambda h: (d,))
+    qw, kw = 1 + 0.1 * rand(*shape(hq), seed=6), 1 + 0.1 * rand(*shape(hk), seed=7)
+    qo, ko = fused.qk_norm_rope_fwd(q, k, pos, table, qw, kw, axes, interleaved)
+    assert on_the_ring() == ring
+    gx, gy, gw, gu = fused.qk_norm_rope_bwd(q, k, pos, table, dq, dk, qw, kw, axes, interleaved)
+    assert on_the_ring()
+    for name, x, w, out, dout, dx, dw in (("q", q, qw, qo, dq, gx, gw), ("k", k, kw, ko, dk, gy, gu)):
+        want, size = ref.rope(x, w, cos, sin, interleaved, True)
+        ref.check(out, want, size, name)
+        want, size, each, each_size = ref.rope_backward(x, w, dout, cos, sin, interleaved, True)
+        ref.check(dx, want, size, "d" + name)
+        over = tuple(range(each.dim() - w.dim()))
+        ref.check(dw, each.sum(over), each_size.sum(over), f"d{name}_weight")
+
+
+# a lane copies a head: more heads than a warp has lanes, at head sizes of which a warp could hold
+# 128, 64, 32, 16 and 8 (half of that with a weight a head)
+@pytest.mark.parametrize("d,hq,hk", [(8, 130, 33), (8, 200, 64), (16, 64, 33), (16, 65, 1), (32, 40, 33), (64, 33, 2),
+                                     (128, 33, 8), (24, 64, 40), (48, 35, 4)])
+@pytest.mark.parametrize("gap", [0, 2, 3])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_heads_apart(d, hq, hk, gap, dtype):
+    apart_case(1500, hq, hk, d, gap, dtype)
+
+
+@pytest.mark.parametrize("d,hq,hk", [(8, 130, 33), (16, 64, 33), (16, 65, 1), (32, 40, 33), (128, 33, 8)])
+@pytest.mark.parametrize("gap", [0, 3])
+def test_heads_apart_with_a_weight_a_head(d, hq, hk, gap):
+    apart_case(1200, hq, hk, d, gap, F16, "heads", interleaved=True)
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 50])
+@pytest.mark.parametrize("d", [8, 16])
+def test_few_tokens_with_heads_apart(tokens, d):
+    """The forward without a ring, the backward with one."""
+    apart_case(tokens, 130, 33, d, 2, ring=False)
+    apart_case(tokens, 64, 40, d, 3, F16, "heads", ring=False)
+
+
+def test_inputs_and_gradients_laid_out_differently():
+    apart_case(1300, 64, 33, 16, 1, grad_gap=3)
+    apart_case(1300, 64, 33, 16, 3, grad_gap=1)
+    apart_case(1300, 130, 33, 8, 2, F32, grad_gap=0)
+
+
+def test_heads_apart_on_the_bounds_checked_build():
+    """The same on librmsnorm_b200_debug.so, in a process of its own: no access out of range."""
+    here = Path(__file__).resolve().parent
+    lib = here.parent / "rmsnorm-h100_b200" / "rmsnorm" / "lib" / "librmsnorm_b200_debug.so"
+    assert lib.exists(), "librmsnorm_b200_debug.so is missing: run __graft_entry__.build()"
+    code = """
+import json, sys
+sys.path[:0] = [%r, %r, %r]
+import torch
+import test_gpu_rope_ring as t
+from rmsnorm import _lib
+for c in ((1200, 130, 33, 8, 2), (1200, 64, 33, 16, 3), (1200, 33, 8, 128, 2), (3, 64, 33, 16, 0)):
+    t.apart_case(*c, ring=c[0] > 3)
+    t.apart_case(*c, t.F16, "heads", ring=c[0] > 3)
+torch.cuda.synchronize()
+print(json.dumps({"build": _lib.debug_bounds_build(), "report": _lib.debug_report(t.DEV), "status": _lib.device_status(t.DEV)}))
+""" % (str(here), str(here.parent), str(here.parent / "rmsnorm-h100_b200"))
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, RMSNORM_B200_LIBRARY=str(lib)), capture_output=True,
+                       text=True, timeout=600)
+    lines = [ln for ln in r.stdout.splitlines() if ln.startswith("{")]
+    assert lines, f"no summary (exit {r.returncode}):\n{r.stdout[-2000:]}\n{r.stderr[-2000:]}"
+    summary = json.loads(lines[-1])
+    assert summary["build"] and summary["report"]["violations"] == 0 and summary["status"] == [0, 0], summary
