@@ -605,6 +605,9 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_bwd_kernel(const RopePar
   for (int i = 0; i < kSets; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[i][e] = make_float2(0.f, 0.f);
+  // ones beside the head: 0 w of such a lane is part of the head's sums
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = make_float2(1.f, 1.f);
   if (!per_head) rope_weight8(p, k, 0, t, w);
   RopeTurn turn(p, t, b.works ? b.token : p.tokens, b.step);
   for (int64_t token = b.token; b.works && token < p.tokens; token += b.step) {

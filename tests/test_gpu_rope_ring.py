@@ -1,7 +1,7 @@
 # SPDX-License-Identifier: MIT
 """The rotary kernels that stream a warp's heads through a ring, where their data or layout is
 out of the ordinary: positions outside the table beside ordinary ones, heads that are not
-neighbours."""
+neighbours, head sizes with lanes to spare."""
 
 from __future__ import annotations
 
@@ -146,6 +146,16 @@ def test_inputs_and_gradients_laid_out_differently():
     apart_case(1300, 64, 33, 16, 1, grad_gap=3)
     apart_case(1300, 64, 33, 16, 3, grad_gap=1)
     apart_case(1300, 130, 33, 8, 2, F32, grad_gap=0)
+
+
+# ------------------------------------------------------------------ head sizes with lanes to spare
+@pytest.mark.parametrize("d", [24, 40, 48, 72, 80, 96, 112, 136, 160, 192, 248])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_a_weight_a_head_with_lanes_to_spare(d, dtype, interleaved):
+    """Lanes beside the head's columns have no weight of their own and must not reach its sums."""
+    apart_case(1200, 7, 3, d, 1, dtype, "heads", interleaved)
+    apart_case(1200, 33, 8, d, 1, dtype, "heads", interleaved)
 
 
 def test_heads_apart_on_the_bounds_checked_build():
