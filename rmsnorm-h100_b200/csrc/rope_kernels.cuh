@@ -660,28 +660,30 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_bwd_kernel(const RopePar
       if constexpr (kNorm) rope_head_sums(totals, pl.lanes_shift);
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        if (per_head && u0 + i < mine) rope_weight8(p, k, b.head0 + (u0 + i) * per, t, w);
-        float2 y[4];
-        rope_get(x[i], y);
-        float rs = 1.f, m = 0.f;
-        if constexpr (kNorm) {
-          rs = rsqrtf(totals[2 * i] * inv_d + p.eps);
-          m = -totals[2 * i + 1] * rs * inv_d;  // -mean of xhat g w
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float2& sum = acc[kPerHead ? i : 0][e];
-          const float2 gw = mul2(g[i][e], w[e]);
+        if (u0 + i < mine) {  // also for the sums: with eps 0 the rstd of no head is infinite
+          if (per_head) rope_weight8(p, k, b.head0 + (u0 + i) * per, t, w);
+          float2 y[4];
+          rope_get(x[i], y);
+          float rs = 1.f, m = 0.f;
           if constexpr (kNorm) {
-            const float2 xhat = mul2(y[e], splat2(rs));
-            sum = fma2(g[i][e], xhat, sum);
-            y[e] = mul2(fma2(xhat, splat2(m), gw), splat2(rs));
-          } else {
-            sum = fma2(g[i][e], y[e], sum);
-            y[e] = gw;
+            rs = rsqrtf(totals[2 * i] * inv_d + p.eps);
+            m = -totals[2 * i + 1] * rs * inv_d;  // -mean of xhat g w
           }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float2& sum = acc[kPerHead ? i : 0][e];
+            const float2 gw = mul2(g[i][e], w[e]);
+            if constexpr (kNorm) {
+              const float2 xhat = mul2(y[e], splat2(rs));
+              sum = fma2(g[i][e], xhat, sum);
+              y[e] = mul2(fma2(xhat, splat2(m), gw), splat2(rs));
+            } else {
+              sum = fma2(g[i][e], y[e], sum);
+              y[e] = gw;
+            }
+          }
+          out.store(to, y);
         }
-        if (u0 + i < mine) out.store(to, y);
         to += out.head_step;
       }
     }

@@ -1,7 +1,7 @@
 # SPDX-License-Identifier: MIT
 """The rotary kernels that stream a warp's heads through a ring, where their data or layout is
 out of the ordinary: positions outside the table beside ordinary ones, heads that are not
-neighbours, head sizes with lanes to spare."""
+neighbours, head sizes with lanes to spare, eps 0 with heads that do not fill a warp."""
 
 from __future__ import annotations
 
@@ -156,6 +156,31 @@ def test_a_weight_a_head_with_lanes_to_spare(d, dtype, interleaved):
     """Lanes beside the head's columns have no weight of their own and must not reach its sums."""
     apart_case(1200, 7, 3, d, 1, dtype, "heads", interleaved)
     apart_case(1200, 33, 8, d, 1, dtype, "heads", interleaved)
+
+
+# ------------------------------------------------------------------ eps 0
+@pytest.mark.parametrize("d,hq,hk", [(8, 5, 1), (16, 33, 2), (64, 5, 3), (80, 7, 1), (128, 5, 1), (128, 9, 2), (256, 3, 5)])
+@pytest.mark.parametrize("weights", ["shared", "heads"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_eps_zero_where_heads_do_not_fill_a_warp(d, hq, hk, weights, dtype):
+    """Lanes without a head, whose rstd would be infinite, leave nothing in the weights' gradients."""
+    tokens = 1200
+    q, k = rand(tokens, hq, d, dtype=dtype, seed=1), rand(tokens, hk, d, dtype=dtype, seed=2)
+    dq, dk = rand(tokens, hq, d, dtype=dtype, seed=3), rand(tokens, hk, d, dtype=dtype, seed=4)
+    shape = (lambda h: (h, d)) if weights == "heads" else (lambda h: (d,))
+    qw, kw = 1 + 0.1 * rand(*shape(hq), seed=5), 1 + 0.1 * rand(*shape(hk), seed=6)
+    table, pos = fused.rope_table(tokens, d, device=DEV), torch.arange(tokens, device=DEV)
+    cos, sin = ref.cos_sin(pos[None], table, (0,) * (d // 2))
+    outs = fused.qk_norm_rope_fwd(q, k, pos, table, qw, kw, eps=0.0)
+    gx, gy, gw, gu = fused.qk_norm_rope_bwd(q, k, pos, table, dq, dk, qw, kw, eps=0.0)
+    assert on_the_ring()
+    for name, x, w, out, dout, dx, dw in (("q", q, qw, outs[0], dq, gx, gw), ("k", k, kw, outs[1], dk, gy, gu)):
+        want, size = ref.rope(x, w, cos, sin, False, True, 0.0)
+        ref.check(out, want, size, name)
+        want, size, each, each_size = ref.rope_backward(x, w, dout, cos, sin, False, True, 0.0)
+        ref.check(dx, want, size, "d" + name)
+        over = tuple(range(each.dim() - w.dim()))
+        ref.check(dw, each.sum(over), each_size.sum(over), f"d{name}_weight")
 
 
 def test_heads_apart_on_the_bounds_checked_build():
