@@ -578,7 +578,8 @@ def qk_norm_rope_fwd(
     may be None) normalised over head_dim (unless norm is False), multiplied by its weight
     ((head_dim,) or (heads, head_dim)), and its first rotary_dim columns turned by the
     token's positions. q and k may be strided views, such as slices of a packed projection;
-    `inplace` writes into them, otherwise the outputs are new and contiguous.
+    `inplace` writes into them, otherwise the outputs are new and contiguous. On CUDA `inplace`
+    is outside autograd: it refuses q and k that require gradients while those are recorded.
 
     positions (int32 or int64) has the leading shape of q, or (axes, ...) of it; `axes` names
     the axis of each of the rotary_dim / 2 pairs (`rope_axes`; default: axis 0). Pair i is the
@@ -603,8 +604,13 @@ def qk_norm_rope_fwd(
     kf, k_place = _place(k)
     if inplace:
         for t, place in ((q, q_place), (k, k_place)):
-            if t is not None and place[0] != t.data_ptr():
+            if t is None:
+                continue
+            if place[0] != t.data_ptr():
                 raise ValueError("inplace needs q and k whose leading dimensions collapse to one stride")
+            if t.requires_grad and torch.is_grad_enabled():
+                raise ValueError("inplace on CUDA is outside autograd: q and k must not require gradients "
+                                 "(qk_norm_rope has them; torch.no_grad() leaves them out)")
         q_out, k_out, qo_place, ko_place = q, k, q_place, k_place
     else:
         q_out, qo_place = _new_like(q)
@@ -617,6 +623,8 @@ def qk_norm_rope_fwd(
     name = "rmsnorm_b200_rope_fwd"
     _lib.enqueue(_lib.packed_entry(name, _BYTES, _BYTES, _BYTES, _STREAM), name, checked[3].index, args,
                  _ROPE_TENSOR.pack(*qo_place), _ROPE_TENSOR.pack(*ko_place))
+    if inplace:  # as torch's own in-place operations: what autograd saved of q and k is no longer valid
+        torch.autograd.graph.increment_version(q if k is None else (q, k))
     return q_out, k_out
 
 
