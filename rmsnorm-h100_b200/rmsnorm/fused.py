@@ -542,6 +542,12 @@ def _place(t: Optional[Tensor]) -> Tuple[Optional[Tensor], Tuple[int, int, int]]
     return t, (t.data_ptr(), stride[0], stride[1])
 
 
+def _repeats(t: Tensor) -> bool:
+    """Whether t is an expanded view: a dimension that stays at one place."""
+    stride = t.stride()
+    return 0 in stride and any(s == 0 and n > 1 for s, n in zip(stride, t.shape))
+
+
 def _new_like(t: Optional[Tensor]) -> Tuple[Optional[Tensor], Tuple[int, int, int]]:
     """A contiguous tensor of t's shape, and its place as _place gives it."""
     if t is None:
@@ -590,6 +596,8 @@ def qk_norm_rope_fwd(
         return _rope_fwd_untraced(
             q, k, positions, table, q_weight, k_weight, axes, interleaved, norm, eps, inplace)
     checked = _check_rope(q, k, positions, table, q_weight, k_weight, axes)
+    if inplace and (_repeats(q) or k is not None and _repeats(k)):
+        raise ValueError("inplace needs q and k whose elements have places of their own, not expanded views")
     if not q.is_cuda:
         cos, sin = _host.rope_cos_sin(positions.reshape(checked[2], *q.shape[:-2]), table, checked[0])
         outs = [t if t is None else _host.qk_norm_rope_fwd(t, w, cos, sin, interleaved, norm, eps)

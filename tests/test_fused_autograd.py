@@ -1,5 +1,5 @@
 # SPDX-License-Identifier: MIT
-"""The fused operators and autograd beyond plain gradients: writing in place."""
+"""The fused operators beyond plain calls: writing in place, as autograd sees it."""
 
 from __future__ import annotations
 
@@ -75,3 +75,21 @@ def test_inplace_with_weights_that_train_and_in_inference_mode(device):
         a = packed.clone()
         fused.qk_norm_rope_fwd(a[:, :2], a[:, 2:4], pos, table, w, w, inplace=True)
         assert torch.equal(a[:, :2], want[0]) and torch.equal(a[:, 2:4], want[1])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", ["q", "k"])
+@pytest.mark.parametrize("dim", [0, 1, 2])
+def test_inplace_refuses_expanded_views(device, which, dim):
+    """Elements that share a place would be turned more than once."""
+    packed, pos, table = rope_inputs(device)
+    q, k = packed[:, :2].clone(), packed[:, 2:4].clone()
+    one = (q if which == "q" else k).narrow(dim, 0, 1).clone()
+    wide = one.expand(6, 2, 16)
+    a, b = (wide, k) if which == "q" else (q, wide)
+    held = one.clone()
+    with pytest.raises(ValueError, match="expanded"):
+        fused.qk_norm_rope_fwd(a, b, pos, table, inplace=True)
+    assert torch.equal(one, held)
+    fused.qk_norm_rope_fwd(a, b, pos, table)  # as inputs they are fine
+    fused.qk_norm_rope_fwd(q[:1].expand(1, 2, 16), k[:1].expand(1, 2, 16), pos[:1], table, inplace=True)
