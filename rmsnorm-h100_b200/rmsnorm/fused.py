@@ -24,6 +24,7 @@ from torch import Tensor
 
 from . import _host_fused as _host
 from . import _lib
+from ._autograd import first_order
 from .rmsnorm import (
     _check_optional_dtype,
     _check_same_device,
@@ -384,7 +385,8 @@ class DropoutAddRMSNormFunction(torch.autograd.Function):
         dx, dw, db, dresidual = dropout_add_rmsnorm_bwd(
             h, weight, dout, rstd, dresidual_out, ctx.p, ctx.rng, bias is not None, ctx.residual_dtype is not None,
             bias, ctx.x_dtype, ctx.residual_dtype, step, ctx.row_offset)
-        return dx, dw, db, dresidual, *([None] * 8)
+        # on the host too: what the forward saved of its sum and rstd has no graph
+        return *first_order("dropout_add_rmsnorm", (dx, dw, db, dresidual)), *([None] * 8)
 
 
 def dropout_add_rmsnorm(
@@ -401,7 +403,8 @@ def dropout_add_rmsnorm(
     rng_step: Optional[Tensor] = None,
     row_offset: int = 0,
 ):
-    """`dropout_add_rmsnorm_fwd` with autograd: out, or (out, residual_out) when prenorm."""
+    """`dropout_add_rmsnorm_fwd` with autograd: out, or (out, residual_out) when prenorm. Its
+    gradients cannot be differentiated again: that is an error."""
     if _is_compiling():
         return _drop_untraced(
             x, weight, bias, residual, p, rng, out_dtype, residual_dtype, eps, prenorm, rng_step, row_offset)
@@ -707,6 +710,8 @@ class QKNormRopeFunction(torch.autograd.Function):
     def backward(ctx, dq_out, dk_out):
         q, k, positions, table, q_weight, k_weight = ctx.saved_tensors
         dq, dk, dqw, dkw = qk_norm_rope_bwd(q, k, positions, table, dq_out, dk_out, q_weight, k_weight, *ctx.rest)
+        if q.is_cuda:  # the host's are plain PyTorch
+            dq, dk, dqw, dkw = first_order("qk_norm_rope", (dq, dk, dqw, dkw))
         return dq, dk, None, None, dqw, dkw, None, None, None, None
 
 
@@ -722,7 +727,8 @@ def qk_norm_rope(
     norm: bool = True,
     eps: float = 1e-6,
 ) -> Tuple[Tensor, Optional[Tensor]]:
-    """`qk_norm_rope_fwd` with autograd (for q, k and the weights)."""
+    """`qk_norm_rope_fwd` with autograd (for q, k and the weights). On CUDA its gradients cannot
+    be differentiated again: that is an error."""
     if _is_compiling():
         return _rope_untraced(
             q, k, positions, table, q_weight, k_weight, axes, interleaved, norm, eps)
