@@ -21,6 +21,7 @@ from torch import Tensor
 
 from . import _host
 from . import _lib
+from ._autograd import first_order
 
 _SUPPORTED_DTYPES = {torch.float16, torch.bfloat16, torch.float32}
 _SUPPORTED_DTYPE_NAMES = "float32, float16 or bfloat16"
@@ -359,7 +360,7 @@ class RMSNormFunction(torch.autograd.Function):
             dx = dx.to(ctx.x_dtype)
         if dresidual is not None and ctx.residual_dtype is not None and dresidual.dtype != ctx.residual_dtype:
             dresidual = dresidual.to(ctx.residual_dtype)
-        return dx, dw, db, dresidual, *([None] * 4)
+        return *first_order("rmsnorm", (dx, dw, db, dresidual)), *([None] * 4)
 
 
 def rmsnorm(
