@@ -540,7 +540,7 @@ def _place(t: Optional[Tensor]) -> Tuple[Optional[Tensor], Tuple[int, int, int]]
         t = t.contiguous()
         stride = t.stride()
     if len(stride) != 3:
-        t = t.reshape(-1, t.shape[-2], t.shape[-1])
+        t = t.reshape(t.shape[:-2].numel(), t.shape[-2], t.shape[-1])  # no -1: k may have no heads
         stride = t.stride()
     return t, (t.data_ptr(), stride[0], stride[1])
 

@@ -1,0 +1,34 @@
+# SPDX-License-Identifier: MIT
+"""Calls of the fused operators at the edges of what they accept, on the host and on CUDA."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from rmsnorm import fused
+
+GPU = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
+DEVICES = [pytest.param("cpu"), pytest.param("cuda", marks=GPU)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lead", [(), (5,), (2, 3), (2, 1, 3), (0, 3), (2, 0)])
+@pytest.mark.parametrize("d", [16, 6])  # the vectorised kernels, the scalar ones
+def test_k_without_heads(device, lead, d):
+    """As k = None, with an empty k_out and dk; a weight of k's has a gradient of zeros."""
+    torch.manual_seed(0)
+    q, dq = torch.randn(*lead, 2, d, device=device), torch.randn(*lead, 2, d, device=device)
+    k, w = q[..., :0, :], torch.ones(d, device=device)
+    pos, table = torch.zeros(lead, dtype=torch.int64, device=device), fused.rope_table(4, d, device=device)
+    want, _ = fused.qk_norm_rope_fwd(q, None, pos, table, w)
+    got, none = fused.qk_norm_rope_fwd(q, k, pos, table, w, w)
+    assert torch.equal(got, want) and none.shape == k.shape
+    want = fused.qk_norm_rope_bwd(q, None, pos, table, dq, None, w)
+    got = fused.qk_norm_rope_bwd(q, k, pos, table, dq, k, w, w)
+    assert torch.equal(got[0], want[0]) and got[1].shape == k.shape and torch.equal(got[2], want[2])
+    assert torch.equal(got[3], torch.zeros_like(w))
+    if device == "cpu" or len(lead) < 2:  # on CUDA a view of several leading dimensions has to collapse
+        a = q.clone()
+        fused.qk_norm_rope_fwd(a, a[..., :0, :], pos, table, w, inplace=True)
+        assert torch.equal(a, fused.qk_norm_rope_fwd(q, None, pos, table, w)[0])
