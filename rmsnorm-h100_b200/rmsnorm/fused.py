@@ -51,7 +51,8 @@ __all__ = [
 _CODE = _lib._DTYPE_CODES
 _MAX_HEADS = 65536
 _GROUP_SIZES = (None, 32, 64, 128, 256)
-_is_compiling = torch.compiler.is_compiling
+# Dynamo alone breaks its graph at the untraced functions; a non-strict export runs their code.
+_is_compiling = torch.compiler.is_dynamo_compiling
 
 # The C argument structs as packed bytes, field by field as _lib declares them (null pointers
 # are 0). A decoding step calls these operators with microseconds of work, so the checks and

@@ -32,3 +32,30 @@ def test_k_without_heads(device, lead, d):
         a = q.clone()
         fused.qk_norm_rope_fwd(a, a[..., :0, :], pos, table, w, inplace=True)
         assert torch.equal(a, fused.qk_norm_rope_fwd(q, None, pos, table, w)[0])
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_under_non_strict_export_on_the_host(which):
+    """Non-strict export runs the Python code: the host's operators are exported as the PyTorch
+    operations they consist of."""
+    torch.manual_seed(0)
+    w, pos, table = torch.rand(16) + 0.5, torch.arange(6), fused.rope_table(6, 16)
+
+    class Quant(torch.nn.Module):
+        def forward(self, x):
+            q, s, h = fused.rmsnorm_quant_fwd(x, w, residual=x * 2)
+            return q.float(), s, h
+
+    class Drop(torch.nn.Module):
+        def forward(self, x):
+            return fused.dropout_add_rmsnorm_fwd(x, w, p=0.25, rng=(1, 2), store_rstd=True)
+
+    class Rope(torch.nn.Module):
+        def forward(self, x):
+            return fused.qk_norm_rope_fwd(x[:, :2], x[:, 2:], pos, table, w, w)
+
+    module = (Quant, Drop, Rope)[which]()
+    x = torch.randn(6, 3, 16)
+    program = torch.export.export(module, (x,), strict=False)
+    for s, t in zip(program.module()(x + 1), module(x + 1)):
+        assert torch.equal(s, t)
