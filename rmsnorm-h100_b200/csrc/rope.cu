@@ -151,9 +151,14 @@ int launch(UnitDevice* ud, Kernel kernel, const RopeGrid& g, cudaStream_t stream
   const int threads = g.threads;
   {
     std::lock_guard<std::mutex> lock(ud->mu);
-    if (ud->attrs_done.insert(reinterpret_cast<const void*>(kernel)).second &&
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRopeSmem) != cudaSuccess)
-      return RMSNORM_B200_ERR_CUDA;
+    const void* fn = reinterpret_cast<const void*>(kernel);
+    if (!ud->attrs_done.count(fn)) {  // noted once it is done: a call that fails is made again
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRopeSmem) != cudaSuccess) {
+        cudaGetLastError();
+        return RMSNORM_B200_ERR_CUDA;
+      }
+      ud->attrs_done.insert(fn);
+    }
   }
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
