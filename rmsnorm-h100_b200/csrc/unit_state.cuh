@@ -32,7 +32,6 @@ namespace rmsb200 {
 namespace {
 
 constexpr int kSmemOptIn = 232448;  // largest dynamic shared memory of a CTA (227 KB)
-constexpr int kSmemPerSm = 233472;  // shared memory of an SM (228 KB)
 
 int elem_bytes(int dt) { return dt == RMSNORM_B200_F32 ? 4 : 2; }
 bool valid_dt(int dt) { return dt == RMSNORM_B200_F16 || dt == RMSNORM_B200_BF16 || dt == RMSNORM_B200_F32; }
