@@ -259,6 +259,16 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int wh
   return mbar_wait_slow<kClusterScope>(bar, parity, where, honor_abort);
 }
 
+// A wait that all lanes of a warp make. They come together first: a lane that spins can keep
+// lanes of its own warp that are elsewhere from running at all, and one of these may still have
+// to issue the copy, or make the arrival, that the wait is for. (Seen in a ring of one slot: the
+// lanes beside lane 0 spun to the wait's limit of 2 s while lane 0 was about to issue the copy.)
+template <bool kClusterScope = false>
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int where) {
+  __syncwarp();
+  return mbar_wait<kClusterScope>(bar, parity, where);
+}
+
 // ---------------------------------------------------------------------------------------
 // TMA bulk copy (global -> this CTA's shared memory), completion counted in bytes on an
 // mbarrier. Source and destination 16-byte aligned, size a multiple of 16. No multicast.
@@ -354,9 +364,10 @@ __device__ __forceinline__ uint32_t cluster_count_x() {
   return r;
 }
 
-// All threads of all CTAs of the cluster. Used once, at kernel start, so that every
-// CTA's mbarriers are initialised before any peer signals them.
+// All threads of all CTAs of the cluster: at kernel start, so that every CTA's mbarriers are
+// initialised before any peer signals them, and at its end. The aligned forms take whole warps.
 __device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();
   asm volatile(
       "barrier.cluster.arrive.release.aligned;\n\t"
       "barrier.cluster.wait.acquire.aligned;" ::

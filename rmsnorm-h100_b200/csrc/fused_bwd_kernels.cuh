@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fused_bwd_kernel(const FusedBw
       for (int j = 0; j < K; ++j) {
         const int first_step = j & ~(KC - 1);
         const int col = j * (G * 8) + c.gl * 8;
-        if (r == 0 && j == first_step) mbar_wait(&c.full[slot], phase, kSiteBwdFull);
+        if (r == 0 && j == first_step) mbar_wait_warp(&c.full[slot], phase, kSiteBwdFull);
         if (col < c.ncols) {
           const unsigned char* base = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;
           const int at = (kTmem ? 0 : r * static_cast<int>(p.N)) + c.gl * 8 + (j - first_step) * (G * 8);
@@ -211,6 +211,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fused_bwd_kernel(const FusedBw
     }
   }
   row_end(pl, c);
+  __syncwarp();
   // One partial row of dweight and of dbias per cluster. Several groups add theirs in group
   // order through the rings, whose every copy has landed and been read.
   if constexpr (kTmem) tmem_wait_st();

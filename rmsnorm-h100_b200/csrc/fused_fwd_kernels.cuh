@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(K == 1 ? kFwdFewThreads : kFwdThreads, 1)
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         const int first_step = j & ~(pl.KC - 1);  // of this unit
-        if (r == 0 && j == first_step) mbar_wait(&c.full[slot], phase, kSiteFwdFull);
+        if (r == 0 && j == first_step) mbar_wait_warp(&c.full[slot], phase, kSiteFwdFull);
         const int col = (j * pl.G + c.gl) * 8;
         if (col < c.ncols) {
           const unsigned char* base = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;

@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kOddThreads, 1) odd_fwd_kernel(const FusedFwdP
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         const int first_step = j & ~(pl.KC - 1);
-        if (r == 0 && j == first_step) mbar_wait(&c.full[slot], phase, kSiteFwdFull);
+        if (r == 0 && j == first_step) mbar_wait_warp(&c.full[slot], phase, kSiteFwdFull);
         const OddCols o = odd_cols(pl, c, j);
         if (!o.any) {
 #pragma unroll
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kOddThreads, 1) odd_bwd_kernel(const FusedBwdP
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         const int first_step = j & ~(pl.KC - 1);
-        if (r == 0 && j == first_step) mbar_wait(&c.full[slot], phase, kSiteBwdFull);
+        if (r == 0 && j == first_step) mbar_wait_warp(&c.full[slot], phase, kSiteBwdFull);
         const OddCols o = odd_cols(pl, c, j);
         if (o.any) {
           const unsigned char* base = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;

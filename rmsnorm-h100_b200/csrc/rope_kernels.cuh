@@ -451,7 +451,7 @@ struct RopeRing {
     for (int s = 0; s < pl.S; ++s) issue(p, b, pl, s);
   }
   __device__ __forceinline__ void wait(int site) {
-    mbar_wait(bar(slot), phase, site);
+    mbar_wait_warp(bar(slot), phase, site);
     __syncwarp();
   }
   // The lane's first head of the current token.
@@ -471,6 +471,7 @@ struct RopeRing {
   }
   // After a wait that ran out: the copies in flight land before the warp leaves.
   __device__ __forceinline__ void drain(const RopeParams& p, const RopeJob& b, const RopePlan& pl) {
+    __syncwarp();
     if (!abort_requested()) return;
     const int64_t n = b.token < p.tokens ? (p.tokens - 1 - b.token) / b.step + 1 : 0;
     for (int s = 0; s < pl.S && s < n; ++s)

@@ -224,7 +224,7 @@ __device__ __forceinline__ void row_total(const RowPlan& pl, RowCtx& c, float& s
       mbar_arrive(bar);
     }
     meanwhile();
-    mbar_wait(bar, parity, site);
+    mbar_wait_warp(bar, parity, site);
     __syncwarp();
     const int w = c.gid * c.nwarps + c.lane;
     if (kSum) sum = warp_sum(c.lane < c.nwarps ? red[w][0] : 0.f);
@@ -243,7 +243,7 @@ __device__ __forceinline__ void row_total(const RowPlan& pl, RowCtx& c, float& s
         st_async_peer(map_peer(smem_u32(&part[c.rank][1]), c.lane), __uint_as_float(most), to_bar);
       }
     }
-    mbar_wait<true>(bar, parity, site);
+    mbar_wait_warp<true>(bar, parity, site);
     __syncwarp();
     if (kSum) sum = warp_sum(c.lane < pl.C ? part[c.lane][0] : 0.f);
     if (kMax) most = __reduce_max_sync(0xffffffffu, c.lane < pl.C ? __float_as_uint(part[c.lane][1]) : 0u);

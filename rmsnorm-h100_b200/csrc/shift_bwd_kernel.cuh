@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kShiftThreads, 1) shift_bwd_kernel(const Fused
     const float rs = rs_next;
     if (row + c.step < p.rows) rs_next = ld1(&p.rstd[row + c.step]);
     const unsigned char* base = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;
-    mbar_wait(&c.full[slot], phase, kSiteBwdFull);
+    mbar_wait_warp(&c.full[slot], phase, kSiteBwdFull);
     float2 s2 = make_float2(0.f, 0.f);
     for (int j = 0; j < steps; ++j) {
       const int col = j * width + c.gl * 8;

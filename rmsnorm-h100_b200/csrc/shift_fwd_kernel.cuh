@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kShiftThreads, 1) shift_fwd_kernel(const Fused
 #pragma unroll
     for (int j = 0; j < K; ++j) {
       const int first_step = j & ~(pl.KC - 1);
-      if (j == first_step) mbar_wait(&c.full[slot], phase, kSiteFwdFull);
+      if (j == first_step) mbar_wait_warp(&c.full[slot], phase, kSiteFwdFull);
       const int col = (j * pl.G + c.gl) * 8;
       if (col < c.ncols) {
         const unsigned char* base = c.ring + static_cast<size_t>(slot) * pl.unit_bytes;

@@ -183,8 +183,9 @@ def test_eps_zero_where_heads_do_not_fill_a_warp(d, hq, hk, weights, dtype):
         ref.check(dw, each.sum(over), each_size.sum(over), f"d{name}_weight")
 
 
-def test_heads_apart_on_the_bounds_checked_build():
-    """The same on librmsnorm_b200_debug.so, in a process of its own: no access out of range."""
+def on_the_bounds_checked_build(calls):
+    """Runs lines of code that use this module as `t` on librmsnorm_b200_debug.so, in a process of
+    its own: no access out of range, no wait that ran out."""
     here = Path(__file__).resolve().parent
     lib = here.parent / "rmsnorm-h100_b200" / "rmsnorm" / "lib" / "librmsnorm_b200_debug.so"
     assert lib.exists(), "librmsnorm_b200_debug.so is missing: run __graft_entry__.build()"
@@ -194,15 +195,32 @@ sys.path[:0] = [%r, %r, %r]
 import torch
 import test_gpu_rope_ring as t
 from rmsnorm import _lib
-for c in ((1200, 130, 33, 8, 2), (1200, 64, 33, 16, 3), (1200, 33, 8, 128, 2), (3, 64, 33, 16, 0)):
-    t.apart_case(*c, ring=c[0] > 3)
-    t.apart_case(*c, t.F16, "heads", ring=c[0] > 3)
+%s
 torch.cuda.synchronize()
 print(json.dumps({"build": _lib.debug_bounds_build(), "report": _lib.debug_report(t.DEV), "status": _lib.device_status(t.DEV)}))
-""" % (str(here), str(here.parent), str(here.parent / "rmsnorm-h100_b200"))
+""" % (str(here), str(here.parent), str(here.parent / "rmsnorm-h100_b200"), calls)
     r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, RMSNORM_B200_LIBRARY=str(lib)), capture_output=True,
                        text=True, timeout=600)
     lines = [ln for ln in r.stdout.splitlines() if ln.startswith("{")]
     assert lines, f"no summary (exit {r.returncode}):\n{r.stdout[-2000:]}\n{r.stderr[-2000:]}"
     summary = json.loads(lines[-1])
     assert summary["build"] and summary["report"]["violations"] == 0 and summary["status"] == [0, 0], summary
+
+
+def test_heads_apart_on_the_bounds_checked_build():
+    on_the_bounds_checked_build("""
+for c in ((1200, 130, 33, 8, 2), (1200, 64, 33, 16, 3), (1200, 33, 8, 128, 2), (3, 64, 33, 16, 0)):
+    t.apart_case(*c, ring=c[0] > 3)
+    t.apart_case(*c, t.F16, "heads", ring=c[0] > 3)
+""")
+
+
+def test_a_ring_of_one_slot_on_the_bounds_checked_build():
+    """fp32 gradients of heads that leave lanes idle: the lanes without a head reach the next wait
+    first, while lane 0 may still have to issue the copy that it is for."""
+    on_the_bounds_checked_build("""
+for c in ((9215, 5, 5, 8), (2759, 1, 1, 8), (5479, 7, 2, 64), (4227, 3, 1, 64), (6696, 8, 20, 32), (3001, 5, 1, 128)):
+    t.apart_case(*c, 1, t.F32)
+    assert t._lib.last_plan().endswith("S=1")
+    t.apart_case(*c, 1, t.F32, "heads")
+""")
