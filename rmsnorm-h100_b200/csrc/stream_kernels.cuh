@@ -155,7 +155,7 @@ __device__ __forceinline__ void group_post(float v, const SmemLayout& L, int gid
 
 __device__ __forceinline__ float group_take(const StreamPlan& pl, const SmemLayout& L, int gid, int lane, int j,
                                             uint32_t use) {
-  mbar_wait(&L.gbar[gid * kGroupRed + j], use & 1u, kSiteFwdCluster);
+  mbar_wait_warp(&L.gbar[gid * kGroupRed + j], use & 1u, kSiteFwdCluster);
   const int nw = pl.G >> 5;
   return warp_sum(lane < nw ? L.gpart[j * 16 + gid * nw + lane] : 0.f);
 }
@@ -273,7 +273,7 @@ __device__ __forceinline__ float cluster_recv(const StreamPlan& pl, const SmemLa
   const uint32_t slot = seq & (kXSlots - 1);
   if (pl.xmode == kXGlobal) {
     if (kBcast && pl.xbcast && warp != 0) {
-      mbar_wait(&L.xbar[slot], (seq / kXSlots) & 1u, site);
+      mbar_wait_warp(&L.xbar[slot], (seq / kXSlots) & 1u, site);
       return L.xpart[slot * kMaxCluster];
     }
     const uint32_t want = xrec_tag(pl, seq);
@@ -298,7 +298,7 @@ __device__ __forceinline__ float cluster_recv(const StreamPlan& pl, const SmemLa
     }
     return tot;
   }
-  mbar_wait<true>(&L.xbar[slot], (seq / kXSlots) & 1u, site);
+  mbar_wait_warp<true>(&L.xbar[slot], (seq / kXSlots) & 1u, site);
   const float* xp = L.xpart + slot * kMaxCluster;
   return warp_sum(lane < pl.P ? xp[lane] : 0.f);
 }
@@ -325,11 +325,11 @@ __device__ __forceinline__ void cluster_recv2(const StreamPlan& pl, const SmemLa
     const uint32_t slot_a = seq_a & (kXSlots - 1);
     const uint32_t slot_b = (seq_a + 1) & (kXSlots - 1);
     if (pl.xbcast && warp != 0) {
-      mbar_wait(&L.xbar[slot_a], (seq_a / kXSlots) & 1u, site);
+      mbar_wait_warp(&L.xbar[slot_a], (seq_a / kXSlots) & 1u, site);
       ta = L.xpart[slot_a * kMaxCluster];
       tb = 0.f;
       if (hb) {
-        mbar_wait(&L.xbar[slot_b], ((seq_a + 1) / kXSlots) & 1u, site);
+        mbar_wait_warp(&L.xbar[slot_b], ((seq_a + 1) / kXSlots) & 1u, site);
         tb = L.xpart[slot_b * kMaxCluster];
       }
       return;
@@ -757,7 +757,7 @@ __global__ void __launch_bounds__(kBlock, kMinBlocks) fwd_stream_kernel(const Fw
       const int rstep = pl.rps * kRpt;
       for (int64_t q = 0; q < n_local; ++q) {
         const int64_t tile = cid + q * ncl;
-        mbar_wait(&L.full[s], ph, kSiteFwdFull);
+        mbar_wait_warp(&L.full[s], ph, kSiteFwdFull);
         const X* xs0 = stage_x(s);
         const RTe* rs0 = stage_r(s);
         const int64_t row0 = tile * pl.R;
@@ -836,7 +836,7 @@ __global__ void __launch_bounds__(kBlock, kMinBlocks) fwd_stream_kernel(const Fw
       const X* xs_q = nullptr;
       const uint32_t slot = static_cast<uint32_t>(q) & 3u;
       if (q < n_local) {
-        mbar_wait(&L.full[s], ph, kSiteFwdFull);
+        mbar_wait_warp(&L.full[s], ph, kSiteFwdFull);
         const int64_t row0 = (cid + q * ncl) * pl.R;
         act_q = in_group && row0 + gid < pl.nrows;
         row_q = row0 + gid;
@@ -876,7 +876,7 @@ __global__ void __launch_bounds__(kBlock, kMinBlocks) fwd_stream_kernel(const Fw
       }
       if (q >= 1) {
         const uint32_t ps = (slot + 3u) & 3u;
-        mbar_wait(&L.gbar[gid * kGroupRed + ps], static_cast<uint32_t>((q - 1) >> 2) & 1u, kSiteFwdCluster);
+        mbar_wait_warp(&L.gbar[gid * kGroupRed + ps], static_cast<uint32_t>((q - 1) >> 2) & 1u, kSiteFwdCluster);
         float m = L.gpart[ps * 16 + gid * nw + (lane & (nw - 1))];
         float M2 = L.xpart[ps * 16 + gid * nw + (lane & (nw - 1))];
         lanes_stats(m, M2, n_warp, nw);  // every lane combines the group's nw warps
@@ -918,7 +918,7 @@ __global__ void __launch_bounds__(kBlock, kMinBlocks) fwd_stream_kernel(const Fw
       const X* xs_q = nullptr;
       const uint32_t par = static_cast<uint32_t>(q) & 1u;
       if (q < n_local) {
-        mbar_wait(&L.full[s], ph, kSiteFwdFull);
+        mbar_wait_warp(&L.full[s], ph, kSiteFwdFull);
         const int64_t row0 = (cid + q * ncl) * pl.R;
         act_q = in_group && row0 + gid < pl.nrows;
         row_q = row0 + gid;
@@ -979,7 +979,7 @@ __global__ void __launch_bounds__(kBlock, kMinBlocks) fwd_stream_kernel(const Fw
       const RTe* rs_q = nullptr;
       const uint32_t slot = static_cast<uint32_t>(q) & 3u;
       if (q < n_local) {
-        mbar_wait(&L.full[s], ph, kSiteFwdFull);
+        mbar_wait_warp(&L.full[s], ph, kSiteFwdFull);
         const int64_t row0 = (cid + q * ncl) * pl.R;
         act_q = in_group && row0 + gid < pl.nrows;
         row_q = row0 + gid;
@@ -1022,7 +1022,7 @@ __global__ void __launch_bounds__(kBlock, kMinBlocks) fwd_stream_kernel(const Fw
     uint32_t seq = 0;
     for (int64_t q = 0; q < n_local; ++q) {
       const int64_t tile = cid + q * ncl;
-      mbar_wait(&L.full[s], ph, kSiteFwdFull);
+      mbar_wait_warp(&L.full[s], ph, kSiteFwdFull);
       const X* xs0 = stage_x(s);
       const RTe* rs0 = stage_r(s);
       const int64_t row0 = tile * pl.R;
@@ -1125,11 +1125,11 @@ __global__ void __launch_bounds__(kBlock, kMinBlocks) fwd_stream_kernel(const Fw
         const int64_t ra = 2 * j;
         const bool hb = ra + 1 < n_local;
         float pa[kVecs], pb[kVecs];
-        mbar_wait(&L.full[s1], ph1, kSiteFwdFull);
+        mbar_wait_warp(&L.full[s1], ph1, kSiteFwdFull);
         pass1(stage_x(s1), stage_r(s1), pa);
         if (++s1 == S) { s1 = 0; ph1 ^= 1u; }
         if (hb) {
-          mbar_wait(&L.full[s1], ph1, kSiteFwdFull);
+          mbar_wait_warp(&L.full[s1], ph1, kSiteFwdFull);
           pass1(stage_x(s1), stage_r(s1), pb);
           if (++s1 == S) { s1 = 0; ph1 ^= 1u; }
         } else {
@@ -1177,13 +1177,13 @@ __global__ void __launch_bounds__(kBlock, kMinBlocks) fwd_stream_kernel(const Fw
       if (i < n_local) {
         float part[kVecs];
         if (K == 1) {
-          mbar_wait(&L.full[s1], ph1, kSiteFwdFull);
+          mbar_wait_warp(&L.full[s1], ph1, kSiteFwdFull);
           pass1(stage_x(s1), stage_r(s1), part);
         } else {
           for (int j = 0; j < K; ++j) {
             uint32_t ph;
             const int s = chunk_slot(s1, ph1, j, S, &ph);
-            mbar_wait(&L.full[s], ph, kSiteFwdFull);
+            mbar_wait_warp(&L.full[s], ph, kSiteFwdFull);
           }
           pass1c(s1, part);
         }
@@ -1571,7 +1571,7 @@ __global__ void __launch_bounds__(kBlock, kMinBlocks) bwd_stream_kernel(const Bw
       const int rstep = pl.rps * (kVecs / kCols);
       for (int64_t q = 0; q < n_local; ++q) {
         const int64_t tile = cid + q * ncl;
-        mbar_wait(&L.full[s], ph, kSiteBwdFull);
+        mbar_wait_warp(&L.full[s], ph, kSiteBwdFull);
         const int64_t row0 = tile * pl.R;
         const int rows = static_cast<int>(min(static_cast<int64_t>(pl.R), pl.nrows - row0));
         const RowPtrs rp = row_ptrs(s, 0);
@@ -1628,7 +1628,7 @@ __global__ void __launch_bounds__(kBlock, kMinBlocks) bwd_stream_kernel(const Bw
       float rstd_q = 0.f;
       const uint32_t slot = static_cast<uint32_t>(q) & 3u;
       if (q < n_local) {
-        mbar_wait(&L.full[s], ph, kSiteBwdFull);
+        mbar_wait_warp(&L.full[s], ph, kSiteBwdFull);
         const int64_t row0 = (cid + q * ncl) * pl.R;
         act_q = in_group && row0 + gid < pl.nrows;
         row_q = row0 + gid;
@@ -1668,7 +1668,7 @@ __global__ void __launch_bounds__(kBlock, kMinBlocks) bwd_stream_kernel(const Bw
     uint32_t seq = 0;
     for (int64_t q = 0; q < n_local; ++q) {
       const int64_t tile = cid + q * ncl;
-      mbar_wait(&L.full[s], ph, kSiteBwdFull);
+      mbar_wait_warp(&L.full[s], ph, kSiteBwdFull);
       const int64_t row0 = tile * pl.R;
       const int rows = static_cast<int>(min(static_cast<int64_t>(pl.R), pl.nrows - row0));
       for (int sw = 0; sw < pl.R; sw += pl.rps) {
@@ -1707,14 +1707,14 @@ __global__ void __launch_bounds__(kBlock, kMinBlocks) bwd_stream_kernel(const Bw
       if (i < n_local) {
         float part[kVecs];
         if (K == 1) {
-          mbar_wait(&L.full[s1], ph1, kSiteBwdFull);
+          mbar_wait_warp(&L.full[s1], ph1, kSiteBwdFull);
           float rstd_k[kVecs];
           pass1(row_ptrs(s1, 0), part, rstd_k);
         } else {
           for (int j = 0; j < K; ++j) {
             uint32_t ph;
             const int s = chunk_slot(s1, ph1, j, S, &ph);
-            mbar_wait(&L.full[s], ph, kSiteBwdFull);
+            mbar_wait_warp(&L.full[s], ph, kSiteBwdFull);
           }
           pass1c(s1, row_ptrs(s1, 0).rstd[0], part);
         }
