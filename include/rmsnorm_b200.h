@@ -251,9 +251,11 @@ int rmsnorm_b200_layernorm_fwd(const rmsnorm_b200_ln_fwd_args* args, void* strea
  * all in fp32; then for the whole row (group = 0) or each group of `group` consecutive
  * columns (the last one may be shorter)
  *   scale = max(max |y| / Q, 2^-126), Q = 448 (E4M3) or 127 (I8)
- *   q     = y / scale rounded to nearest, ties to even, never beyond +-Q.
- * A NaN in a group makes its scale NaN; an infinity makes it infinite. residual_out
- * receives h. */
+ *   q     = y * (1 / scale) rounded to nearest, ties to even, never beyond +-Q; the reciprocal
+ *           is good to one place of fp32, so a y / scale within one part in 2^22 of the
+ *           midpoint of two values may take either.
+ * A NaN among a group's y makes its scale NaN (an infinite h does: its row's rsqrt is 0), an
+ * infinite y infinite, and the group's finite values 0. residual_out receives h. */
 typedef struct rmsnorm_b200_quant_args {
   int64_t rows;               /* >= 0 */
   int64_t hidden;             /* >= 1 */

@@ -136,8 +136,10 @@ def rmsnorm_quant_fwd(
     (shape x.shape[:-1]) or, with `group_size` 32, 64, 128 or 256, one per group of that
     many columns (shape x.shape[:-1] + (groups,), the last group possibly shorter).
 
-    A scale is max |y| / 448 (e4m3) or / 127 (int8), at least 2^-126; q is rounded to nearest
-    even. NaN in a group makes its scale NaN. `scales_column_major` lays grouped scales out
+    A scale is max |y| / 448 (e4m3) or / 127 (int8), at least 2^-126; q is y / scale rounded to
+    nearest even (on CUDA y times the reciprocal of the scale: within one part in 2^22 of the
+    midpoint of two values either is possible). A NaN among a group's y makes its scale NaN, an
+    infinite y infinite. `scales_column_major` lays grouped scales out
     column by column (the strides of a transposed tensor), as block-scaled products take
     them. residual_out as in `rmsnorm_fwd`."""
     if _is_compiling():

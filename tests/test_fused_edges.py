@@ -59,3 +59,34 @@ def test_under_non_strict_export_on_the_host(which):
     program = torch.export.export(module, (x,), strict=False)
     for s, t in zip(program.module()(x + 1), module(x + 1)):
         assert torch.equal(s, t)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("quant_dtype", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("n", [256, 257, 300])
+def test_infinite_values_in_eight_bits(device, quant_dtype, n):
+    """An infinite y makes its scale infinite and its finite neighbours 0; itself it is infinity /
+    infinity, NaN in e4m3 and 0 in int8. An infinite h makes its own y NaN and the rest of its row 0."""
+    torch.manual_seed(0)
+    x, w = torch.randn(9, n, device=device), torch.ones(n, device=device)
+    w[70] = float("inf")
+    for group in (None, 64):
+        q, s, _ = fused.rmsnorm_quant_fwd(x, w, quant_dtype=quant_dtype, group_size=group)
+        plain, t, _ = fused.rmsnorm_quant_fwd(x, quant_dtype=quant_dtype, group_size=group)
+        here = slice(None) if group is None else slice(64, 128)
+        at = s if group is None else s[:, 1]
+        assert (at == float("inf")).all()
+        q = q.float()
+        assert (q[:, 70].isnan() if quant_dtype != torch.int8 else q[:, 70] == 0).all()
+        q[:, 70] = 0
+        assert (q[:, here] == 0).all()
+        if group:
+            assert torch.equal(s[:, [0, 2, 3]], t[:, [0, 2, 3]]) and torch.equal(q[:, 128:], plain.float()[:, 128:])
+        y = x.clone()
+        y[4, 70] = float("-inf")
+        q, s, _ = fused.rmsnorm_quant_fwd(y, quant_dtype=quant_dtype, group_size=group)
+        assert torch.equal(s[[0, 8]], t[[0, 8]])
+        at = s[4] if group is None else s[4, 1]
+        assert at.isnan()
+        if group:
+            assert (s[4, [0, 2, 3]] == 2.0**-126).all() and (q[4, 128:].float() == 0).all()
