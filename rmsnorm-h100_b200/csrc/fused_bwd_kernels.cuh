@@ -58,8 +58,9 @@ __device__ __forceinline__ void add_sums(float2 (&sum)[8], const float2 (&h)[4],
 // They are kept in tensor memory then, which this kernel has no other use for: 16 columns of
 // the thread's lane a step, read and written once a row. Those kernels have the row group's
 // size kG built in (0: chosen at run time).
-// Measured: bf16 throughout, 32768 x 16384 990 us (820 us of bytes at a copy's rate; bound by
-// instructions, a third of them the generator's); 1.3e8 elements at 1024, 4096 and 8192 columns
+// Measured: bf16 throughout, 32768 x 16384 990 to 1000 us (820 us of bytes at a copy's rate; bound
+// by instructions, 304 for eight columns, 80 of them the generator's and 16 the choice by its
+// words, issued at half the SM's rate by 16 warps); 1.3e8 elements at 1024, 4096 and 8192 columns
 // 217, 227 and 236 us (205 us of bytes); fp32 h, 4096 columns 359 us (328 us).
 template <typename H, typename DY, typename DRO, typename DRES, int K, int kG>
 __global__ void __launch_bounds__(kBwdThreads, 1) fused_bwd_kernel(const FusedBwdParams p, const RowPlan pl) {

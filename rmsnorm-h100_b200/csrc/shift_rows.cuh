@@ -10,9 +10,11 @@
 // lie in shared memory at the row's offset. With 148 clusters a class has 18 or 19 of them,
 // which costs 3 %. Measured at 1.3e8 elements (x, residual and outputs bf16, dropout), against
 // the scalar accesses of odd_kernels.cuh: 4097 columns forward 354 / 592 us, backward 421 / 1372,
-// 8 bits with a scale a row 238 / 531, a scale per 128 columns 392 / 531; 1001 columns 302 / 401,
-// 389 / 787, 215 / 361, 342 / 361. Bound by the instructions
-// of the generator, as the aligned kernels, plus a ninth of the draws and their shuffles.
+// 8 bits with a scale a row 240 / 531, a scale per 128 columns 396 / 531; 1001 columns 304 / 401,
+// 389 / 787, 218 / 361, 344 / 361. Bound by instructions at 15 warps: for eight columns 389
+// (dropout forward), 489 (backward), 458 (a scale per 128 columns), where the aligned kernels take
+// 253, 304 and 200. The edges, a ninth more draws and the shuffles of their bits, and in the
+// 8-bit forward a second total a row and the scales' way through shared memory make the rest.
 #pragma once
 
 #include <type_traits>
