@@ -9,7 +9,8 @@
 
 They follow the conventions of `rmsnorm.rmsnorm`: arguments are checked before anything
 runs, CUDA tensors go to the native library on the current stream of their device, tensors
-on the host are computed in plain PyTorch. Under `torch.compile` they run as graph breaks.
+on the host are computed in plain PyTorch. Under `torch.compile` they run as graph breaks (so
+`fullgraph=True` refuses them, unlike `rmsnorm`).
 """
 
 from __future__ import annotations
