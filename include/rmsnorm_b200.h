@@ -417,6 +417,139 @@ int rmsnorm_b200_rope_bwd_workspace_size(const rmsnorm_b200_rope_args* args, con
 int rmsnorm_b200_rope_bwd(const rmsnorm_b200_rope_args* args, const rmsnorm_b200_rope_grads* grads, void* workspace,
                           size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * 8-bit products. E4M3 values with fp32 scales for groups of 128 columns of a row, or for
+ * blocks of 128 x 128: an operand of R rows and C columns holds q[r][c] * scale[r / b][c / 128],
+ * b = 1 or 128. The last groups and blocks of a row or column may be shorter.
+ * ------------------------------------------------------------------------------------ */
+#define RMSNORM_B200_BLOCK 128
+
+/* Quantises x, and from the same read x transposed:
+ *   scale = the smallest power of two that brings the group's (or block's) largest magnitude
+ *           to 448 or below, at least 2^-126
+ *   q     = x / scale rounded to nearest, ties to even (x / scale is exact)
+ * A NaN in a group makes its scale NaN, an infinite value infinite (and the group's finite
+ * values 0). column_sums receives the sums of x's columns, added in fp32 in a fixed order. */
+typedef struct rmsnorm_b200_block_quant_args {
+  int64_t rows;               /* >= 0 */
+  int64_t cols;               /* >= 1 */
+  const void* x;              /* [rows, cols] */
+  int64_t x_row_stride;       /* strides in elements */
+  void* q;                    /* nullable, [rows, cols], one byte each */
+  int64_t q_row_stride;
+  float* scales;              /* scale of (row or block of rows i, group g) at i * scale_row_stride + g * scale_group_stride */
+  int64_t scale_row_stride;
+  int64_t scale_group_stride;
+  void* q_t;                  /* nullable, [cols, rows] */
+  int64_t q_t_row_stride;
+  float* scales_t;            /* [cols or blocks of columns][groups of rows], contiguous */
+  void* column_sums;          /* nullable, [cols] */
+  int32_t x_dtype;
+  int32_t block_rows;         /* 1 or 128, for x and for x transposed */
+  int32_t column_sums_dtype;
+  int32_t reserved0;
+} rmsnorm_b200_block_quant_args;
+
+/* Bytes of device workspace (16-byte aligned; 0 without column_sums). */
+int rmsnorm_b200_block_quant_workspace_size(const rmsnorm_b200_block_quant_args* args, size_t* bytes);
+int rmsnorm_b200_block_quant(const rmsnorm_b200_block_quant_args* args, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* out[m][n] = sum over groups g of a_scale[m][g] * b_scale[n or n / 128][g] *
+ *             (sum over the columns k of g of a[m][k] * b[n][k])  (+ bias[n])
+ * The sums are held in fp32, the result rounded once. */
+typedef struct rmsnorm_b200_block_mm_args {
+  int64_t m, n, k;            /* m >= 0, n and k >= 1, below 2^31 */
+  const void* a;              /* [m, k] E4M3 */
+  int64_t a_row_stride;       /* strides in elements */
+  const void* b;              /* [n, k] E4M3 */
+  int64_t b_row_stride;
+  const float* a_scales;      /* of (row, group) */
+  int64_t a_scale_row_stride;
+  int64_t a_scale_group_stride;
+  const float* b_scales;      /* of (row or block of rows, group) */
+  int64_t b_scale_row_stride;
+  int64_t b_scale_group_stride;
+  const void* bias;           /* nullable, [n] */
+  void* out;                  /* [m, n] */
+  int32_t b_block_rows;       /* 1 or 128 */
+  int32_t bias_dtype;
+  int32_t out_dtype;
+  int32_t reserved0;
+} rmsnorm_b200_block_mm_args;
+
+/* Bytes of device workspace (16-byte aligned): copies of operands whose address or row stride
+ * is not a multiple of 16; 0 where both are. */
+int rmsnorm_b200_block_mm_workspace_size(const rmsnorm_b200_block_mm_args* args, size_t* bytes);
+int rmsnorm_b200_block_mm(const rmsnorm_b200_block_mm_args* args, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * A cache of keys and values in 8 bits, in pages of page_size slots, with an fp32 scale for
+ * every head of a slot: value = q * scale. Strides are in elements; only a head's values have
+ * to be contiguous.
+ * ------------------------------------------------------------------------------------ */
+typedef struct rmsnorm_b200_cache_tensor {
+  void* data;                 /* [pages, page_size, heads, head_dim] */
+  int64_t page_stride;
+  int64_t slot_stride;
+  int64_t head_stride;
+  float* scales;              /* [pages, page_size, heads] */
+  int64_t scale_page_stride;
+  int64_t scale_slot_stride;
+  int64_t scale_head_stride;
+} rmsnorm_b200_cache_tensor;
+
+typedef struct rmsnorm_b200_cache_args {
+  int64_t pages;
+  rmsnorm_b200_cache_tensor k;
+  rmsnorm_b200_cache_tensor v;
+  int32_t page_size;          /* >= 1 */
+  int32_t heads;              /* 1 .. RMSNORM_B200_ROPE_MAX_HEADS */
+  int32_t head_dim;           /* 1 .. RMSNORM_B200_ROPE_MAX_HEAD_DIM */
+  int32_t cache_dtype;        /* RMSNORM_B200_E4M3 or RMSNORM_B200_I8 */
+} rmsnorm_b200_cache_args;
+
+/* Writes token t's heads into slot slots[t] = page * page_size + place in the page:
+ *   scale = max(max |x| / Q, 2^-126), Q = 448 (E4M3) or 127 (I8); q = x / scale rounded to
+ *   nearest, ties to even. NaN and infinities as in rmsnorm_b200_quant_fwd.
+ * A negative slot leaves its token out. A slot beyond the cache leaves it out too and records
+ * RMSNORM_B200_ERR_INVALID_ARGUMENT (site 11) for rmsnorm_b200_device_status. Slots named more
+ * than once hold bytes of any of their tokens. */
+typedef struct rmsnorm_b200_cache_write_args {
+  int64_t tokens;             /* >= 0 */
+  rmsnorm_b200_rope_tensor k; /* [tokens, heads, head_dim] */
+  rmsnorm_b200_rope_tensor v;
+  const void* slots;          /* [tokens], int32 or int64 */
+  int32_t slots_64bit;
+  int32_t dtype;              /* of k and v */
+} rmsnorm_b200_cache_write_args;
+
+int rmsnorm_b200_cache_write(const rmsnorm_b200_cache_args* cache, const rmsnorm_b200_cache_write_args* args,
+                             void* stream);
+
+/* Reads `tokens` rows of packed sequences: row t belongs to the last sequence s with
+ * starts[s] <= t < starts[s + 1], is its token p = t - starts[s], and lies in page
+ * page_table[s][p / page_size] at place p % page_size. k and v = q * scale, rounded once. Rows
+ * from starts[sequences] on are left as they are, or zeros with zero_rest. A row before
+ * starts[0], beyond the page table's width or in a page that the cache does not have is NaN and
+ * records RMSNORM_B200_ERR_INVALID_ARGUMENT (site 12) for rmsnorm_b200_device_status. */
+typedef struct rmsnorm_b200_cache_read_args {
+  int64_t tokens;             /* >= 0 */
+  int64_t sequences;          /* >= 0, below 2^31 */
+  int64_t table_width;        /* pages of a sequence in the table */
+  int64_t table_stride;
+  const int32_t* page_table;  /* [sequences, table_width] */
+  const int32_t* starts;      /* [sequences + 1], ascending */
+  void* k;                    /* [tokens, heads, head_dim], contiguous */
+  void* v;
+  int32_t dtype;              /* of k and v */
+  int32_t zero_rest;
+} rmsnorm_b200_cache_read_args;
+
+int rmsnorm_b200_cache_read(const rmsnorm_b200_cache_args* cache, const rmsnorm_b200_cache_read_args* args,
+                            void* stream);
+
 /* Static, human-readable message for a status code. */
 const char* rmsnorm_b200_strerror(int status);
 

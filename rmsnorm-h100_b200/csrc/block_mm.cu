@@ -1,0 +1,267 @@
+// block_mm.cu -- rmsnorm_b200_block_mm: argument checks, choice of the kernel and launch.
+#define RMSB_UNIT block_mm
+#include "unit_state.cuh"
+
+#include "block_mm_kernels.cuh"
+
+namespace rmsb200 {
+namespace {
+
+using FewKernel = void (*)(const CUtensorMap, const CUtensorMap, const BlockMmParams, const FewPlan);
+using WideKernel = void (*)(const CUtensorMap, const CUtensorMap, const BlockMmParams, const WidePlan);
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+
+// The driver's function that makes tensor maps (the library does not link the driver).
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    cudaGetLastError();
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// Boxes of `box_rows` rows and kTileK bytes of a byte matrix.
+int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64_t row_stride, int box_rows) {
+  const EncodeTiled encode = encode_tiled();
+  if (!encode) return RMSNORM_B200_ERR_CUDA;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_stride)};
+  const cuuint32_t box[2] = {kTileK, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t each[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, each,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? RMSNORM_B200_OK
+             : RMSNORM_B200_ERR_CUDA;
+}
+
+// TMA reads operands at addresses and row strides that are multiples of 16.
+bool tma_ready(const void* base, int64_t rows, int64_t row_stride) {
+  return aligned_to(base, 16) && (row_stride % 16 == 0 || rows == 1);
+}
+
+struct Plan {
+  int64_t pitch = 0;  // row stride of the copies
+  size_t copy_a = 0, copy_b = 0;
+};
+
+int check(const rmsnorm_b200_block_mm_args* a) {
+  constexpr int64_t kMost = int64_t{1} << 31;
+  if (!a || a->m < 0 || a->n < 1 || a->k < 1 || a->m >= kMost || a->n >= kMost || a->k >= kMost)
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if ((a->b_block_rows != 1 && a->b_block_rows != kBlock) || !valid_dt(a->out_dtype) ||
+      (a->bias && !valid_dt(a->bias_dtype)))
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if (a->m == 0) return RMSNORM_B200_OK;
+  if (!a->a || !a->b || !a->a_scales || !a->b_scales || !a->out) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if (a->a_row_stride < 0 || a->b_row_stride < 0 || a->a_scale_row_stride < 0 || a->a_scale_group_stride < 0 ||
+      a->b_scale_row_stride < 0 || a->b_scale_group_stride < 0)
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  if ((a->m > 1 && a->a_row_stride < a->k) || (a->n > 1 && a->b_row_stride < a->k))
+    return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  return RMSNORM_B200_OK;
+}
+
+Plan make_plan(const rmsnorm_b200_block_mm_args* a) {
+  Plan pl;
+  pl.pitch = (a->k + 15) / 16 * 16;
+  if (!tma_ready(a->a, a->m, a->a_row_stride)) pl.copy_a = static_cast<size_t>(a->m) * pl.pitch;
+  if (!tma_ready(a->b, a->n, a->b_row_stride)) pl.copy_b = static_cast<size_t>(a->n) * pl.pitch;
+  return pl;
+}
+
+struct MmLaunch {
+  const char* kind;
+  unsigned grid;
+  int tile, splits, stages;
+};
+
+std::string describe(const void* data) {
+  const MmLaunch& l = *static_cast<const MmLaunch*>(data);
+  char buf[128];
+  std::snprintf(buf, sizeof(buf), "%s grid=%u tile=%d splits=%d stages=%d", l.kind, l.grid, l.tile, l.splits, l.stages);
+  return buf;
+}
+
+template <typename Kernel, typename KernelPlan>
+int launch(UnitDevice* ud, Kernel kernel, const CUtensorMap& ma, const CUtensorMap& mb, const BlockMmParams& p,
+           const KernelPlan& kp, int threads, int smem, int cluster, cudaStream_t stream, const MmLaunch& l) {
+  {
+    const void* fn = reinterpret_cast<const void*>(kernel);
+    std::lock_guard<std::mutex> lock(ud->mu);
+    if (!ud->attrs_done.count(fn)) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemOptIn) != cudaSuccess)
+        return RMSNORM_B200_ERR_CUDA;
+      ud->attrs_done.insert(fn);
+    }
+  }
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(l.grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, ma, mb, p, kp) != cudaSuccess) {
+    cudaGetLastError();
+    return RMSNORM_B200_ERR_CUDA;
+  }
+  return launched(describe, l);
+}
+
+int repack(const void* src, int64_t row_stride, int64_t rows, int64_t k, void* dst, int64_t pitch, cudaStream_t stream) {
+  const int64_t pieces = pitch / 16, total = rows * pieces;
+  if (total > (int64_t{1} << 31) * 255) return RMSNORM_B200_ERR_UNSUPPORTED;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((total + 255) / 256));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, repack_kernel, static_cast<const unsigned char*>(src), row_stride, rows,
+                         static_cast<int32_t>(k), static_cast<unsigned char*>(dst), static_cast<int32_t>(pieces)) !=
+      cudaSuccess) {
+    cudaGetLastError();
+    return RMSNORM_B200_ERR_CUDA;
+  }
+  return launched("");
+}
+
+template <int T>
+int launch_few(UnitDevice* ud, const void* a, int64_t a_row, const CUtensorMap& map_b, const rmsnorm_b200_block_mm_args* args,
+               const BlockMmParams& p, cudaStream_t stream) {
+  CUtensorMap map_a;
+  const int st = make_map(&map_a, a, args->m, args->k, a_row, T);
+  if (st) return st;
+  FewPlan pl = {};
+  pl.tiles_n = static_cast<int>((args->n + kBlock - 1) / kBlock);
+  const int64_t tiles = (args->m + T - 1) / T * pl.tiles_n;
+  const int fit = T >= 128 ? 1 : 2;  // CTAs an SM
+  pl.splits = static_cast<int>(std::clamp<int64_t>(fit * ud->sm_count / tiles, 1, std::min(8, p.groups)));
+  const int each = (p.groups + pl.splits - 1) / pl.splits;
+  const int fixed = 1024 + static_cast<int>(sizeof(FewBars)) + 2 * T * 4;
+  const int room = (fit == 2 ? kSmemOptIn / 2 - 1024 : kSmemOptIn) - fixed;
+  pl.stages = std::min({kFewMaxStages, each, room / Few<T>::kStageBytes});
+  pl.ring_bytes = std::max(pl.stages * Few<T>::kStageBytes, pl.splits > 1 ? T * kBlock * 4 : 0);
+  const int smem = pl.ring_bytes + fixed;
+  if (tiles * pl.splits >= int64_t{1} << 31) return RMSNORM_B200_ERR_UNSUPPORTED;
+  const MmLaunch l = {"block_mm_few", static_cast<unsigned>(tiles * pl.splits), T, pl.splits, pl.stages};
+  return launch<FewKernel>(ud, block_mm_few_kernel<T>, map_a, map_b, p, pl, kFewThreads, smem, pl.splits, stream, l);
+}
+
+template <bool kPair>
+int launch_wide(UnitDevice* ud, const CUtensorMap& map_a, const CUtensorMap& map_b, const rmsnorm_b200_block_mm_args* a,
+                const BlockMmParams& p, cudaStream_t stream) {
+  using W = Wide<kPair>;
+  WidePlan pl = {};
+  pl.tiles_m = static_cast<int>((a->m + W::kRows - 1) / W::kRows);
+  pl.tiles_n = static_cast<int>((a->n + kWideN - 1) / kWideN);
+  pl.band = kPair ? 8 : 16;
+  const int64_t tiles = static_cast<int64_t>(pl.tiles_m) * pl.tiles_n;
+  const int per = kPair ? 2 : 1;
+  const int64_t units = std::min<int64_t>(tiles, ud->sm_count / per);
+  const int smem = 1024 + W::kStages * W::kStageBytes + static_cast<int>(sizeof(WideBars)) + 2 * kWideN * 4;
+  const MmLaunch l = {kPair ? "block_mm_pair" : "block_mm_wide", static_cast<unsigned>(units * per), kWideN, 1, W::kStages};
+  return launch<WideKernel>(ud, p.b_rows ? block_mm_wide_kernel<kPair, true> : block_mm_wide_kernel<kPair, false>, map_a,
+                            map_b, p, pl, kWideThreads, smem, per, stream, l);
+}
+
+int run(const rmsnorm_b200_block_mm_args* a, void* ws, size_t ws_bytes, cudaStream_t stream) {
+  int st = check(a);
+  if (st) return st;
+  if (a->m == 0) {
+    rmsb_units::set_last_plan("block_mm empty");
+    return RMSNORM_B200_OK;
+  }
+  UnitDevice* ud = nullptr;
+  st = unit_device(&ud);
+  if (st) return st;
+  const Plan pl = make_plan(a);
+  const size_t need = pl.copy_a + pl.copy_b;
+  if (need > ws_bytes || (need > 0 && (!ws || !aligned_to(ws, 16)))) return RMSNORM_B200_ERR_WORKSPACE;
+  const int64_t groups = (a->k + kBlock - 1) / kBlock;
+  Ranges ranges;
+  ranges.add(a->a, (a->m - 1) * a->a_row_stride + a->k);
+  ranges.add(a->b, (a->n - 1) * a->b_row_stride + a->k);
+  ranges.add(a->a_scales, ((a->m - 1) * a->a_scale_row_stride + (groups - 1) * a->a_scale_group_stride + 1) * 4);
+  const int64_t b_rows = (a->n + a->b_block_rows - 1) / a->b_block_rows;
+  ranges.add(a->b_scales, ((b_rows - 1) * a->b_scale_row_stride + (groups - 1) * a->b_scale_group_stride + 1) * 4);
+  if (a->bias) ranges.add(a->bias, a->n * elem_bytes(a->bias_dtype));
+  ranges.add_out(a->out, static_cast<size_t>(a->m) * a->n * elem_bytes(a->out_dtype));
+  ranges.add(ws, need);
+  st = ranges.send(stream);
+  if (st) return st;
+
+  const void *qa = a->a, *qb = a->b;
+  int64_t a_row = a->m == 1 ? pl.pitch : a->a_row_stride, b_row = a->n == 1 ? pl.pitch : a->b_row_stride;
+  if (pl.copy_a) {
+    st = repack(a->a, a->a_row_stride, a->m, a->k, ws, pl.pitch, stream);
+    if (st) return st;
+    qa = ws;
+    a_row = pl.pitch;
+  }
+  if (pl.copy_b) {
+    void* to = static_cast<unsigned char*>(ws) + pl.copy_a;
+    st = repack(a->b, a->b_row_stride, a->n, a->k, to, pl.pitch, stream);
+    if (st) return st;
+    qb = to;
+    b_row = pl.pitch;
+  }
+  BlockMmParams p = {};
+  p.m = a->m; p.n = static_cast<int32_t>(a->n); p.groups = static_cast<int32_t>(groups);
+  p.sa = a->a_scales; p.sa_row = a->a_scale_row_stride; p.sa_group = a->a_scale_group_stride;
+  p.sb = a->b_scales; p.sb_row = a->b_scale_row_stride; p.sb_group = a->b_scale_group_stride;
+  p.bias = a->bias; p.bias_dt = a->bias_dtype;
+  p.out = a->out; p.out_dt = a->out_dtype;
+  p.b_rows = a->b_block_rows == 1;
+  p.vec_out = aligned_to(a->out, 16) && a->n * elem_bytes(a->out_dtype) % 16 == 0;
+  CUtensorMap map_a, map_b;
+  st = make_map(&map_b, qb, a->n, a->k, b_row, kBlock);
+  if (st) return st;
+  if (a->m <= 16) return launch_few<16>(ud, qa, a_row, map_b, a, p, stream);
+  if (a->m <= 32) return launch_few<32>(ud, qa, a_row, map_b, a, p, stream);
+  if (a->m <= 64) return launch_few<64>(ud, qa, a_row, map_b, a, p, stream);
+  if (a->m <= 128) return launch_few<128>(ud, qa, a_row, map_b, a, p, stream);
+  st = make_map(&map_a, qa, a->m, a->k, a_row, kBlock);
+  if (st) return st;
+  return launch_wide<false>(ud, map_a, map_b, a, p, stream);
+}
+
+int workspace_size(const rmsnorm_b200_block_mm_args* a, size_t* bytes) {
+  if (!bytes) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
+  *bytes = 0;
+  const int st = check(a);
+  if (st || a->m == 0) return st;
+  const Plan pl = make_plan(a);
+  *bytes = pl.copy_a + pl.copy_b;
+  return RMSNORM_B200_OK;
+}
+
+}  // namespace
+}  // namespace rmsb200
+
+using namespace rmsb200;
+
+extern "C" int rmsnorm_b200_block_mm_workspace_size(const rmsnorm_b200_block_mm_args* a, size_t* bytes) {
+  return entry([&] { return workspace_size(a, bytes); });
+}
+
+extern "C" int rmsnorm_b200_block_mm(const rmsnorm_b200_block_mm_args* a, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
+  return entry([&] { return run(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)); });
+}

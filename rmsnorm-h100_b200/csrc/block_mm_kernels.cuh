@@ -1,0 +1,536 @@
+// block_mm_kernels.cuh -- products of e4m3 matrices whose values have an fp32 scale per group of
+// 128 columns (block_mm.cu chooses among them).
+//
+//   out[m][n] = sum_g a_scale[m][g] b_scale[n][g] sum_{k in g} a[m][k] b[n][k]  (+ bias[n])
+//
+// The tensor cores sum one group of 128 columns at a time into tensor memory; a scale holds for a
+// group, so the sum over the groups is made outside of them, in registers and in fp32, while the
+// next group is on its way: two fp32 instructions' width per element and group.
+#pragma once
+
+#include "block_scale.cuh"
+#include "tensor_core.cuh"
+
+namespace rmsb200 {
+
+constexpr int kSiteMmFull = 12, kSiteMmEmpty = 13, kSiteMmSum = 14, kSiteMmSumEmpty = 15;
+
+struct BlockMmParams {
+  int64_t m;
+  int32_t n, groups;
+  const float* sa;
+  int64_t sa_row, sa_group;
+  const float* sb;
+  int64_t sb_row, sb_group;
+  const void* bias;
+  void* out;
+  int32_t bias_dt, out_dt;
+  bool b_rows;      // b's scales are per row
+  bool vec_out;     // 8-element vectors of out
+};
+
+__device__ __forceinline__ const float* sb_of(const BlockMmParams& p, int64_t n) {
+  return p.sb + (p.b_rows ? n : n / kBlock) * p.sb_row;
+}
+
+// ---------------------------------------------------------------------------------------
+// Many rows: 128 x 256 of the result a CTA.
+// ---------------------------------------------------------------------------------------
+constexpr int kWideN = 256;        // columns of a tile
+constexpr int kWideThreads = 384;  // warps 0 - 7 sum, 8 copies, 9 multiplies
+constexpr int kWideSums = 2;       // accumulators in tensor memory, 256 columns each
+constexpr int kTileBytes = kBlock * kTileK;  // 128 rows of an operand
+
+template <bool kPair>
+struct Wide {
+  static constexpr int kStages = kPair ? 6 : 4;
+  static constexpr int kStageBytes = kTileBytes * (kPair ? 2 : 3);
+  static constexpr int kRows = kPair ? 256 : 128;  // rows of a tile
+};
+
+struct WideBars {
+  uint64_t full[6], empty[6], sum[kWideSums], sum_empty[kWideSums], done;
+  uint32_t tmem;
+};
+
+struct WidePlan {
+  int32_t tiles_m, tiles_n, band;  // tiles go down `band` rows of tiles before the next column
+};
+
+__device__ __forceinline__ void wide_tile(const WidePlan& pl, int64_t i, int* tm, int* tn) {
+  const int64_t per = static_cast<int64_t>(pl.band) * pl.tiles_n;
+  const int b = static_cast<int>(i / per);
+  const int64_t at = i - b * per;
+  const int high = min(pl.band, pl.tiles_m - b * pl.band);
+  *tn = static_cast<int>(at / high);
+  *tm = b * pl.band + static_cast<int>(at - static_cast<int64_t>(*tn) * high);
+}
+
+// acc += sums * scale, or acc += sums * (column scales) * scale.
+template <bool kRowScales>
+__device__ __forceinline__ void add_scaled(float2* acc, const float2 (&v)[16], float s, const float* col) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    if constexpr (kRowScales) {
+      const float4 c = *reinterpret_cast<const float4*>(col + 2 * i);
+      acc[i] = fma2(mul2(v[i], make_float2(c.x, c.y)), splat2(s), acc[i]);
+      acc[i + 1] = fma2(mul2(v[i + 1], make_float2(c.z, c.w)), splat2(s), acc[i + 1]);
+    } else {
+      acc[i] = fma2(v[i], splat2(s), acc[i]);
+      acc[i + 1] = fma2(v[i + 1], splat2(s), acc[i + 1]);
+    }
+  }
+}
+
+template <bool kPair, bool kRowScales>
+__global__ void __launch_bounds__(kWideThreads, 1)
+    block_mm_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                         const BlockMmParams p, const WidePlan pl) {
+  using W = Wide<kPair>;
+  unsigned char* smem = rmsb_dyn_smem + ((1024u - (smem_u32(rmsb_dyn_smem) & 1023u)) & 1023u);
+  WideBars* bars = reinterpret_cast<WideBars*>(smem + W::kStages * W::kStageBytes);
+  float* col_scales = reinterpret_cast<float*>(bars + 1);  // [2][kWideN]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = kPair ? cluster_ctarank() : 0;
+  const int64_t unit = kPair ? blockIdx.x >> 1 : blockIdx.x, units = kPair ? gridDim.x >> 1 : gridDim.x;
+  const int64_t tiles = static_cast<int64_t>(pl.tiles_m) * pl.tiles_n;
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < W::kStages; ++i) {
+      mbar_init(&bars->full[i], 1);
+      mbar_init(&bars->empty[i], 1);
+    }
+    for (int i = 0; i < kWideSums; ++i) {
+      mbar_init(&bars->sum[i], 1);
+      mbar_init(&bars->sum_empty[i], kPair ? 16 : 8);
+    }
+    mbar_init(&bars->done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    if constexpr (kPair) tmem_alloc_pair(&bars->tmem, kWideSums * kWideN);
+    else tmem_alloc_warp(&bars->tmem, kWideSums * kWideN);
+  }
+  if (threadIdx.x == 256) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_b);
+  }
+  tmem_fence_before_sync();
+  __syncthreads();
+  if constexpr (kPair) cluster_sync_all();
+  tmem_fence_after_sync();
+  const uint32_t tmem = bars->tmem;
+  pdl_wait();
+
+  if (warp >= 8) {
+    regs_down<40>();
+    if (warp == 8) {  // copies
+      int s = 0;
+      uint32_t pass = 0;
+      bool ok = true;
+      for (int64_t t = unit; ok && t < tiles; t += units) {
+        int tm, tn;
+        wide_tile(pl, t, &tm, &tn);
+        const int ya = tm * W::kRows + static_cast<int>(rank) * kBlock, yb = tn * kWideN + static_cast<int>(rank) * kBlock;
+        for (int g = 0; g < p.groups; ++g) {
+          ok = mbar_wait_warp<kPair>(&bars->empty[s], pass ^ 1u, kSiteMmEmpty);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) {
+            unsigned char* at = smem + s * W::kStageBytes;
+            if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], W::kStageBytes * (kPair ? 2 : 1));
+            tile_load<kPair>(at, &map_a, g * kTileK, ya, &bars->full[s]);
+            tile_load<kPair>(at + kTileBytes, &map_b, g * kTileK, yb, &bars->full[s]);
+            if constexpr (!kPair)
+              tile_load<kPair>(at + 2 * kTileBytes, &map_b, g * kTileK, yb + kBlock, &bars->full[s]);
+          }
+          __syncwarp();
+          if (++s == W::kStages) {
+            s = 0;
+            pass ^= 1u;
+          }
+        }
+      }
+      // Nobody leaves while copies may land in its memory or arrivals at its barriers.
+      if (lane == 0 && rank == 0 && abort_requested())
+        for (int i = 0; i < W::kStages; ++i) mbar_wait(&bars->full[i], i < s ? pass : pass ^ 1u, kSiteDrain, false);
+      for (int i = 0; i < W::kStages; ++i)
+        mbar_wait_warp<kPair>(&bars->empty[i], i < s ? pass : pass ^ 1u, kSiteMmEmpty);
+    } else if (warp == 9 && rank == 0) {  // products
+      constexpr uint32_t idesc = product_desc(W::kRows, kWideN);
+      int s = 0;
+      uint32_t pass = 0, u = 0;
+      bool ok = true;
+      for (int64_t t = unit; ok && t < tiles; t += units)
+        for (int g = 0; g < p.groups; ++g, ++u) {
+          const uint32_t d = u & 1u;
+          ok = mbar_wait_warp<kPair>(&bars->sum_empty[d], ((u >> 1) & 1u) ^ 1u, kSiteMmSumEmpty);
+          ok = mbar_wait_warp<kPair>(&bars->full[s], pass, kSiteMmFull) && ok;
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tmem_fence_after_sync();
+          if (lane == 0) {
+            const uint32_t at = smem_u32(smem + s * W::kStageBytes);
+            const uint64_t a = operand_desc(at), b = operand_desc(at + kTileBytes);
+#pragma unroll
+            for (int k = 0; k < kTileK / 32; ++k) mma_e4m3<kPair>(tmem + d * kWideN, a + 2 * k, b + 2 * k, idesc, k > 0);
+            mma_commit<kPair>(&bars->empty[s]);
+            mma_commit<kPair>(&bars->sum[d]);
+          }
+          __syncwarp();
+          if (++s == W::kStages) {
+            s = 0;
+            pass ^= 1u;
+          }
+        }
+      if (abort_requested()) {
+        if (lane == 0) {
+          mma_commit<kPair>(&bars->done);
+          mbar_wait(&bars->done, 0, kSiteDrain, false);
+        }
+        __syncwarp();
+      }
+      for (int i = 0; i < kWideSums; ++i, ++u)
+        mbar_wait_warp<kPair>(&bars->sum_empty[u & 1u], ((u >> 1) & 1u) ^ 1u, kSiteMmSumEmpty);
+    }
+  } else {  // sums: warp w has rows 32 (w % 4) .. + 31, the half w / 4 of the columns
+    regs_up<232>();
+    const int half = warp >> 2;
+    const uint32_t from = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * (kWideN / 2);
+    uint32_t u = 0;
+    for (int64_t t = unit; t < tiles; t += units) {
+      int tm, tn;
+      wide_tile(pl, t, &tm, &tn);
+      const int64_t row = static_cast<int64_t>(tm) * W::kRows + rank * kBlock + (warp & 3) * 32 + lane;
+      const int64_t col0 = static_cast<int64_t>(tn) * kWideN + half * (kWideN / 2);
+      const bool live = row < p.m;
+      // scales two groups ahead; b's per row: thread i of the 256 brings column i's, else every
+      // thread its half's
+      const int64_t own = kRowScales ? static_cast<int64_t>(tn) * kWideN + threadIdx.x : col0;
+      const bool own_live = own < p.n;
+      const float* sa = p.sa + row * p.sa_row;
+      const float* sb = sb_of(p, own);
+      auto next_a = [&](int g) {
+        const float v = live && g < p.groups ? ld1(sa) : 0.f;
+        sa += p.sa_group;
+        return v;
+      };
+      auto next_b = [&](int g) {
+        const float v = own_live && g < p.groups ? ld1(sb) : 0.f;
+        sb += p.sb_group;
+        return v;
+      };
+      float a0 = next_a(0), a1 = next_a(1), b0 = next_b(0), b1 = next_b(1);
+      float2 acc[kWideN / 4];
+#pragma unroll
+      for (int i = 0; i < kWideN / 4; ++i) acc[i] = make_float2(0.f, 0.f);
+      for (int g = 0; g < p.groups; ++g, ++u) {
+        const uint32_t d = u & 1u;
+        float s = a0;
+        const float* cols = col_scales + d * kWideN;
+        if constexpr (kRowScales) {
+          col_scales[d * kWideN + threadIdx.x] = b0;
+          __syncwarp();
+          named_barrier(1, 256);
+          cols += half * (kWideN / 2);
+        } else {
+          s *= b0;
+        }
+        a0 = a1;
+        b0 = b1;
+        a1 = next_a(g + 2);
+        b1 = next_b(g + 2);
+        mbar_spin_warp<kPair>(&bars->sum[d], (u >> 1) & 1u, kSiteMmSum);
+        __syncwarp();
+        tmem_fence_after_sync();
+        const uint32_t at = from + d * kWideN;
+        float2 v0[16], v1[16];
+        tmem_ld(at, v0);
+        tmem_landed(v0);
+        tmem_ld(at + 32, v1);
+        add_scaled<kRowScales>(acc, v0, s, cols);
+        tmem_landed(v1);
+        tmem_ld(at + 64, v0);
+        add_scaled<kRowScales>(acc + 16, v1, s, cols + 32);
+        tmem_landed(v0);
+        tmem_ld(at + 96, v1);
+        add_scaled<kRowScales>(acc + 32, v0, s, cols + 64);
+        tmem_landed(v1);
+        tmem_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (kPair) mbar_arrive_peer(&bars->sum_empty[d], 0);
+          else mbar_arrive(&bars->sum_empty[d]);
+        }
+        add_scaled<kRowScales>(acc + 48, v1, s, cols + 96);
+      }
+      if (!live) continue;
+#pragma unroll
+      for (int i = 0; i < kWideN / 2; i += 8) {
+        const int64_t col = col0 + i;
+        if (col >= p.n) break;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          v[k] = k & 1 ? acc[(i + k) / 2].y : acc[(i + k) / 2].x;
+          if (p.bias && col + k < p.n) v[k] += load1_rt(p.bias, p.bias_dt, col + k);
+        }
+        const int64_t e = row * p.n + col;
+        if (p.vec_out && col + 8 <= p.n) {
+          store8_rt(p.out, p.out_dt, e, v);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (col + k < p.n) store1_rt(p.out, p.out_dt, e + k, v[k]);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tmem_fence_before_sync();
+  __syncthreads();
+  if constexpr (kPair) cluster_sync_all();
+  tmem_fence_after_sync();
+  if (warp == 9) {
+    if constexpr (kPair) tmem_dealloc_pair(tmem, kWideSums * kWideN);
+    else tmem_dealloc_warp(tmem, kWideSums * kWideN);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Few rows: the rows of b take the tensor cores' 128 rows and the T rows of a their columns, so
+// that b streams through once. The groups of k are split over the CTAs of a cluster, each of
+// which then adds up some rows of the result.
+// ---------------------------------------------------------------------------------------
+constexpr int kFewThreads = 192;  // warps 0 - 3 sum, 4 copies, 5 multiplies
+constexpr int kFewMaxStages = 16;
+
+template <int T>
+struct Few {
+  static constexpr int kSums = T >= 128 ? 2 : 4;
+  static constexpr int kTmem = kSums * T;  // columns: a power of two, at least 32
+  static constexpr int kStageBytes = kTileBytes + T * kTileK;
+};
+
+struct FewBars {
+  uint64_t full[kFewMaxStages], empty[kFewMaxStages], sum[4], sum_empty[4], done;
+  uint32_t tmem;
+};
+
+struct FewPlan {
+  int32_t tiles_n, splits, stages;
+  int32_t ring_bytes;  // of the stages, and room for the sums that take their place
+};
+
+template <int T>
+__global__ void __launch_bounds__(kFewThreads, T >= 128 ? 1 : 2)
+    block_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                        const BlockMmParams p, const FewPlan pl) {
+  using F = Few<T>;
+  constexpr int kChunk = T < 32 ? 16 : 32;
+  unsigned char* smem = rmsb_dyn_smem + ((1024u - (smem_u32(rmsb_dyn_smem) & 1023u)) & 1023u);
+  FewBars* bars = reinterpret_cast<FewBars*>(smem + pl.ring_bytes);
+  float* row_scales = reinterpret_cast<float*>(bars + 1);  // [2][T]: of the rows of a
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(blockIdx.x % pl.splits);
+  const int64_t tile = blockIdx.x / pl.splits;
+  const int tn = static_cast<int>(tile % pl.tiles_n);
+  const int64_t t0 = tile / pl.tiles_n * T;  // first row of a
+  const int g0 = static_cast<int>(static_cast<int64_t>(p.groups) * rank / pl.splits);
+  const int g1 = static_cast<int>(static_cast<int64_t>(p.groups) * (rank + 1) / pl.splits);
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < pl.stages; ++i) {
+      mbar_init(&bars->full[i], 1);
+      mbar_init(&bars->empty[i], 1);
+    }
+    for (int i = 0; i < F::kSums; ++i) {
+      mbar_init(&bars->sum[i], 1);
+      mbar_init(&bars->sum_empty[i], 4);
+    }
+    mbar_init(&bars->done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 5) tmem_alloc_warp(&bars->tmem, F::kTmem);
+  if (threadIdx.x == 128) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_b);
+  }
+  tmem_fence_before_sync();
+  __syncthreads();
+  tmem_fence_after_sync();
+  const uint32_t tmem = bars->tmem;
+  pdl_wait();
+
+  float2 acc[T / 2];
+  const int64_t n = static_cast<int64_t>(tn) * kBlock + threadIdx.x;  // warps 0 - 3: this thread's row of b
+  if (warp == 4) {
+    int u = 0;
+    bool ok = true;
+    for (int g = g0; ok && g < g1; ++g, ++u) {
+      const int s = u % pl.stages;
+      if (u >= pl.stages)
+        ok = __all_sync(0xffffffffu, mbar_wait_warp(&bars->empty[s], static_cast<uint32_t>(u / pl.stages - 1) & 1u,
+                                                    kSiteMmEmpty));
+      if (!ok) break;
+      if (lane == 0) {
+        unsigned char* at = smem + s * F::kStageBytes;
+        mbar_arrive_expect_tx(&bars->full[s], F::kStageBytes);
+        tile_load<false>(at, &map_b, g * kTileK, tn * kBlock, &bars->full[s]);
+        tile_load<false>(at + kTileBytes, &map_a, g * kTileK, static_cast<int>(t0), &bars->full[s]);
+      }
+      __syncwarp();
+    }
+    if (lane == 0 && abort_requested())
+      for (int j = max(0, u - pl.stages); j < u; ++j)
+        mbar_wait(&bars->full[j % pl.stages], static_cast<uint32_t>(j / pl.stages) & 1u, kSiteDrain, false);
+    for (int j = max(0, u - pl.stages); j < u; ++j)
+      mbar_wait_warp(&bars->empty[j % pl.stages], static_cast<uint32_t>(j / pl.stages) & 1u, kSiteMmEmpty);
+  } else if (warp == 5) {
+    constexpr uint32_t idesc = product_desc(kBlock, T);
+    int u = 0;
+    bool ok = true;
+    for (int g = g0; ok && g < g1; ++g, ++u) {
+      const int s = u % pl.stages, d = u % F::kSums;
+      if (u >= F::kSums)
+        ok = mbar_wait_warp(&bars->sum_empty[d], static_cast<uint32_t>(u / F::kSums - 1) & 1u, kSiteMmSumEmpty);
+      ok = mbar_wait_warp(&bars->full[s], static_cast<uint32_t>(u / pl.stages) & 1u, kSiteMmFull) && ok;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tmem_fence_after_sync();
+      if (lane == 0) {
+        const uint32_t at = smem_u32(smem + s * F::kStageBytes);
+        const uint64_t a = operand_desc(at), b = operand_desc(at + kTileBytes);
+#pragma unroll
+        for (int k = 0; k < kTileK / 32; ++k) mma_e4m3<false>(tmem + d * T, a + 2 * k, b + 2 * k, idesc, k > 0);
+        mma_commit<false>(&bars->empty[s]);
+        mma_commit<false>(&bars->sum[d]);
+      }
+      __syncwarp();
+    }
+    if (abort_requested()) {
+      if (lane == 0) {
+        mma_commit<false>(&bars->done);
+        mbar_wait(&bars->done, 0, kSiteDrain, false);
+      }
+      __syncwarp();
+    }
+  } else {
+    const uint32_t from = tmem + (static_cast<uint32_t>(warp) << 21);
+    const int64_t t = t0 + threadIdx.x;
+    const bool b_live = n < p.n, a_live = threadIdx.x < T && t < p.m;
+    const float* sa = p.sa + t * p.sa_row;
+    const float* sb = sb_of(p, n);
+    auto load_a = [&](int g) { return a_live && g < g1 ? ld1(sa + g * p.sa_group) : 0.f; };
+    auto load_b = [&](int g) { return b_live && g < g1 ? ld1(sb + g * p.sb_group) : 0.f; };
+    float a0 = load_a(g0), a1 = load_a(g0 + 1), b0 = load_b(g0), b1 = load_b(g0 + 1);
+#pragma unroll
+    for (int i = 0; i < T / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+    int u = 0;
+    for (int g = g0; g < g1; ++g, ++u) {
+      const int d = u % F::kSums;
+      const float s = b0;
+      float* rows = row_scales + (u & 1) * T;
+      if (threadIdx.x < T) rows[threadIdx.x] = a0;
+      a0 = a1;
+      b0 = b1;
+      a1 = load_a(g + 2);
+      b1 = load_b(g + 2);
+      __syncwarp();
+      named_barrier(1, 128);
+      mbar_wait_warp(&bars->sum[d], static_cast<uint32_t>(u / F::kSums) & 1u, kSiteMmSum);
+      __syncwarp();
+      tmem_fence_after_sync();
+#pragma unroll
+      for (int c = 0; c < T; c += kChunk) {
+        float2 v[kChunk / 2];
+        tmem_ld(from + d * T + c, v);
+        tmem_landed(v);
+        if (c + kChunk == T) {
+          tmem_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->sum_empty[d]);
+        }
+#pragma unroll
+        for (int i = 0; i < kChunk / 2; i += 2) {
+          const float4 r = *reinterpret_cast<const float4*>(rows + c + 2 * i);
+          acc[c / 2 + i] = fma2(mul2(v[i], make_float2(r.x, r.y)), splat2(s), acc[c / 2 + i]);
+          acc[c / 2 + i + 1] = fma2(mul2(v[i + 1], make_float2(r.z, r.w)), splat2(s), acc[c / 2 + i + 1]);
+        }
+      }
+    }
+    const float bias = p.bias && b_live ? load1_rt(p.bias, p.bias_dt, n) : 0.f;
+    if (pl.splits == 1) {
+      if (b_live) {
+#pragma unroll
+        for (int i = 0; i < T; ++i)
+          if (t0 + i < p.m)
+            store1_rt(p.out, p.out_dt, (t0 + i) * p.n + n, (i & 1 ? acc[i / 2].y : acc[i / 2].x) + bias);
+      }
+    } else {
+      // every copy has landed and been read: the stages take the sums
+      float* part = reinterpret_cast<float*>(smem);  // [T][128]
+#pragma unroll
+      for (int i = 0; i < T; ++i) part[i * kBlock + threadIdx.x] = i & 1 ? acc[i / 2].y : acc[i / 2].x;
+    }
+  }
+  // Tensor memory goes back before the CTAs of a cluster wait for one another: a peer that has
+  // none yet may wait for this CTA's SM.
+  __syncwarp();
+  tmem_fence_before_sync();
+  __syncthreads();
+  tmem_fence_after_sync();
+  if (warp == 5) tmem_dealloc_warp(tmem, F::kTmem);
+  if (pl.splits == 1) return;
+  cluster_sync_all();
+  if (warp < 4) {
+    const float bias = p.bias && n < p.n ? load1_rt(p.bias, p.bias_dt, n) : 0.f;
+    for (int i = rank; i < T && t0 + i < p.m; i += pl.splits) {
+      const uint32_t at = smem_u32(smem) + static_cast<uint32_t>(i * kBlock + threadIdx.x) * 4;
+      float sum = 0.f;
+      for (int r = 0; r < pl.splits; ++r) sum += ld_peer(map_peer(at, r));
+      if (n < p.n) store1_rt(p.out, p.out_dt, (t0 + i) * p.n + n, sum + bias);
+    }
+  }
+  cluster_sync_all();
+}
+
+// ---------------------------------------------------------------------------------------
+// An operand whose address or row stride is no multiple of 16, copied to where they are: 16
+// bytes a thread from the aligned words around them.
+// ---------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) repack_kernel(const unsigned char* src, int64_t src_row, int64_t rows, int32_t k,
+                                                     unsigned char* dst, int32_t pieces) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t row = i / pieces;
+  if (row >= rows) return;
+  const int at = static_cast<int>(i - row * pieces) * 16;
+  const unsigned char* s = src + row * src_row + at;
+  const int left = min(16, k - at);
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (left == 16) {
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(s)) & 3u;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(s - off);
+    uint32_t v[5];
+    // the first and last words hold bytes of other rows or of nothing: only those with bytes of
+    // this piece are read
+#pragma unroll
+    for (int j = 0; j < 5; ++j) v[j] = j < 4 || off ? words[j] : 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(v[j], v[j + 1], off * 8);
+  } else {
+    for (int j = 0; j < left; ++j) {
+      const uint32_t b = static_cast<uint32_t>(ld1(s + j)) << (8 * (j & 3));
+      if (j < 4) w[0] |= b;
+      else if (j < 8) w[1] |= b;
+      else if (j < 12) w[2] |= b;
+      else w[3] |= b;
+    }
+  }
+  uint4* to = reinterpret_cast<uint4*>(dst) + i;
+  if (RMSB_DBG_OK(to, 16, kDbgVecStore)) *to = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+}  // namespace rmsb200

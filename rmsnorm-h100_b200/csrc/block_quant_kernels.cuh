@@ -1,0 +1,245 @@
+// block_quant_kernels.cuh -- e4m3 values with a power of two as scale for 1 x 128 groups or
+// 128 x 128 blocks, of x and of x transposed.
+#pragma once
+
+#include "block_scale.cuh"
+
+namespace rmsb200 {
+
+struct BlockQuantParams {
+  const void* x;
+  int64_t x_row;
+  void* q;
+  int64_t q_row;
+  float* scales;
+  int64_t scale_row, scale_group;
+  void* q_t;
+  int64_t q_t_row;
+  float* scales_t;
+  float* sum_part;  // [tile rows][cols]
+  int64_t rows, cols;
+  bool vec_in, vec_q, vec_t;  // 8-element vectors of x, 8-byte stores of q, 16-byte stores of q_t
+};
+
+template <typename X>
+__device__ __forceinline__ float load_one(const void* base, int64_t e) {
+  const X* p = static_cast<const X*>(base) + e;
+  if (!RMSB_DBG_OK(p, sizeof(X), kDbgScalarLoad)) return 0.f;
+  if constexpr (sizeof(X) == 4) return *p;
+  else return static_cast<float>(*p);
+}
+
+// Columns col .. col + 7 of a row at element e0; zeros from `cols` on.
+template <typename X>
+__device__ __forceinline__ void load_octet(const BlockQuantParams& p, int64_t e0, int64_t col, float2 (&v)[4]) {
+  if (p.vec_in && col + 8 <= p.cols) {
+    Pair8<X>::load(static_cast<const X*>(p.x) + e0 + col, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i].x = col + 2 * i < p.cols ? load_one<X>(p.x, e0 + col + 2 * i) : 0.f;
+    v[i].y = col + 2 * i + 1 < p.cols ? load_one<X>(p.x, e0 + col + 2 * i + 1) : 0.f;
+  }
+}
+
+__device__ __forceinline__ uint2 pack_octet(const float2 (&v)[4], float inv) {
+  float2 t[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[i] = mul2(v[i], splat2(inv));
+  return make_uint2(E4M3::pack4(t[0], t[1]), E4M3::pack4(t[2], t[3]));
+}
+
+__device__ __forceinline__ void store_octet(const BlockQuantParams& p, int64_t row, int64_t col, uint2 b) {
+  unsigned char* dst = static_cast<unsigned char*>(p.q) + row * p.q_row + col;
+  if (p.vec_q && col + 8 <= p.cols) {
+    if (RMSB_DBG_OK(dst, 8, kDbgVecStore)) *reinterpret_cast<uint2*>(dst) = b;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (col + i < p.cols) st1(dst + i, static_cast<unsigned char>((i < 4 ? b.x : b.y) >> (8 * (i & 3))));
+}
+
+__device__ __forceinline__ uint32_t octet_magnitude(const float2 (&v)[4]) { return magnitude(largest8(0.f, v)); }
+
+// The largest of 16 neighbouring lanes.
+__device__ __forceinline__ uint32_t max16(uint32_t m) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+
+// Groups of a row, nothing else: 16 lanes a group, 8 columns a lane, kGroups groups in flight.
+template <typename X, int kGroups>
+__global__ void __launch_bounds__(256) quant_groups_kernel(const BlockQuantParams p, int64_t total, uint32_t groups) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int half = threadIdx.x >> 4, at = (threadIdx.x & 15) * 8;
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * 16 + half) * kGroups;
+  float2 v[kGroups][4];
+  int64_t row[kGroups], group[kGroups];
+#pragma unroll
+  for (int j = 0; j < kGroups; ++j) {
+    const int64_t g = first + j;
+    row[j] = g / groups;
+    group[j] = g - row[j] * groups;
+    if (g < total) {
+      load_octet<X>(p, row[j] * p.x_row, group[j] * kBlock + at, v[j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[j][i] = make_float2(0.f, 0.f);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kGroups; ++j) {
+    const uint32_t s = power_scale(max16(octet_magnitude(v[j])));
+    if (first + j >= total) continue;
+    if (at == 0) st1(p.scales + row[j] * p.scale_row + group[j] * p.scale_group, __uint_as_float(s));
+    store_octet(p, row[j], group[j] * kBlock + at, pack_octet(v[j], power_inverse(s)));
+  }
+}
+
+// One 128 x 128 tile a CTA, read once into registers: thread (warp w, lane l) holds rows
+// 16 w + 8 (l / 16) + 0 .. 7 and columns 8 (l % 16) + 0 .. 7. Rows' groups lie in 16 lanes of one
+// warp, columns' in all warps; the transposed bytes pass through shared memory, where the 8-byte
+// piece of rows 8 u .. 8 u + 7 of column c lies at place u ^ (c / 8) of the column, so that
+// neither side meets a bank twice.
+template <typename X, bool kBlocks>
+__global__ void __launch_bounds__(256, 2) quant_tiles_kernel(const BlockQuantParams p, uint32_t tiles_c) {
+  __shared__ __align__(16) unsigned char turned[kBlock * kBlock];
+  __shared__ uint32_t col_most[8][kBlock];
+  __shared__ float col_sum[8][kBlock];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c8 = lane & 15, half = lane >> 4;
+  const uint32_t tile_r = blockIdx.x / tiles_c, tile_c = blockIdx.x - tile_r * tiles_c;
+  const int64_t row0 = static_cast<int64_t>(tile_r) * kBlock + warp * 16 + half * 8;
+  const int64_t col0 = static_cast<int64_t>(tile_c) * kBlock, col = col0 + c8 * 8;
+  float2 v[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (row0 + i < p.rows) {
+      load_octet<X>(p, (row0 + i) * p.x_row, col, v[i]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[i][k] = make_float2(0.f, 0.f);
+    }
+  }
+  if (p.sum_part) {
+    float2 sum[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      sum[k] = v[0][k];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) sum[k] = add2(sum[k], v[i][k]);
+      sum[k].x += __shfl_xor_sync(0xffffffffu, sum[k].x, 16);
+      sum[k].y += __shfl_xor_sync(0xffffffffu, sum[k].y, 16);
+      if (half == 0) *reinterpret_cast<float2*>(&col_sum[warp][c8 * 8 + 2 * k]) = sum[k];
+    }
+  }
+  float inv_t[8];  // of this thread's columns
+  if (kBlocks) {
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = largest8(most, v[i]);
+    const uint32_t m = __reduce_max_sync(0xffffffffu, magnitude(most));
+    if (lane == 0) col_most[warp][0] = m;
+    __syncthreads();
+    uint32_t all = col_most[0][0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) all = max(all, col_most[w][0]);
+    const uint32_t s = power_scale(all);
+    const float inv = power_inverse(s);
+    if (threadIdx.x == 0) {
+      if (p.q) st1(p.scales + tile_r * p.scale_row + tile_c * p.scale_group, __uint_as_float(s));
+      if (p.q_t) {
+        const int64_t tiles_r = (p.rows + kBlock - 1) / kBlock;
+        st1(p.scales_t + tile_c * tiles_r + tile_r, __uint_as_float(s));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) inv_t[k] = inv;
+    if (p.q) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (row0 + i < p.rows) store_octet(p, row0 + i, col, pack_octet(v[i], inv));
+    }
+  } else {
+    if (p.q) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t s = power_scale(max16(octet_magnitude(v[i])));
+        if (row0 + i >= p.rows) continue;
+        if (c8 == 0) st1(p.scales + (row0 + i) * p.scale_row + tile_c * p.scale_group, __uint_as_float(s));
+        store_octet(p, row0 + i, col, pack_octet(v[i], power_inverse(s)));
+      }
+    }
+    if (p.q_t) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2)
+          most = max3_abs(most, k & 1 ? v[i][k >> 1].y : v[i][k >> 1].x, k & 1 ? v[i + 1][k >> 1].y : v[i + 1][k >> 1].x);
+        uint32_t m = magnitude(most);
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        if (half == 0) col_most[warp][c8 * 8 + k] = m;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t m = col_most[0][c8 * 8 + k];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) m = max(m, col_most[w][c8 * 8 + k]);
+        const uint32_t s = power_scale(m);
+        inv_t[k] = power_inverse(s);
+        if (warp == 0 && half == 0 && col + k < p.cols) {
+          const int64_t groups_t = (p.rows + kBlock - 1) / kBlock;
+          st1(p.scales_t + (col + k) * groups_t + tile_r, __uint_as_float(s));
+        }
+      }
+    }
+  }
+  if (p.q_t) {
+    const int u = warp * 2 + half;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float2 t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        t[i] = k & 1 ? make_float2(v[2 * i][k >> 1].y, v[2 * i + 1][k >> 1].y)
+                     : make_float2(v[2 * i][k >> 1].x, v[2 * i + 1][k >> 1].x);
+      *reinterpret_cast<uint2*>(turned + (c8 * 8 + k) * kBlock + ((u ^ c8) << 3)) = pack_octet(t, inv_t[k]);
+    }
+  }
+  __syncthreads();
+  if (p.sum_part && threadIdx.x < kBlock && col0 + threadIdx.x < p.cols) {
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) sum += col_sum[w][threadIdx.x];
+    st1(p.sum_part + static_cast<int64_t>(tile_r) * p.cols + col0 + threadIdx.x, sum);
+  }
+  if (!p.q_t) return;
+  // eight lanes a column, 16 rows a lane
+  const int64_t out0 = static_cast<int64_t>(tile_r) * kBlock + (threadIdx.x & 7) * 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = i * 32 + (threadIdx.x >> 3);
+    if (col0 + c >= p.cols || out0 >= p.rows) continue;
+    uint4 b = *reinterpret_cast<const uint4*>(turned + c * kBlock + (((threadIdx.x & 7) ^ (c >> 4)) << 4));
+    if ((c >> 3) & 1) b = make_uint4(b.z, b.w, b.x, b.y);
+    unsigned char* dst = static_cast<unsigned char*>(p.q_t) + (col0 + c) * p.q_t_row + out0;
+    if (p.vec_t && out0 + 16 <= p.rows) {
+      if (RMSB_DBG_OK(dst, 16, kDbgVecStore)) *reinterpret_cast<uint4*>(dst) = b;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const uint32_t word = j < 4 ? b.x : j < 8 ? b.y : j < 12 ? b.z : b.w;
+        if (out0 + j < p.rows) st1(dst + j, static_cast<unsigned char>(word >> (8 * (j & 3))));
+      }
+    }
+  }
+}
+
+}  // namespace rmsb200

@@ -269,6 +269,22 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
   return mbar_wait<kClusterScope>(bar, parity, where);
 }
 
+// The same without a call, for loops that hold nearly all registers there are.
+template <bool kClusterScope = false>
+__device__ __forceinline__ bool mbar_spin_warp(uint64_t* bar, uint32_t parity, int where) {
+  __syncwarp();
+  if (kClusterScope ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!(kClusterScope ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity))) {
+    if (abort_requested()) return false;
+    if (globaltimer_ns() - t0 > g_wait_timeout_ns) {
+      record_error(RMSNORM_B200_ERR_DEVICE_TIMEOUT, where);
+      return false;
+    }
+  }
+  return true;
+}
+
 // ---------------------------------------------------------------------------------------
 // TMA bulk copy (global -> this CTA's shared memory), completion counted in bytes on an
 // mbarrier. Source and destination 16-byte aligned, size a multiple of 16. No multicast.

@@ -1251,7 +1251,8 @@ int do_bwd(const rmsnorm_b200_bwd_args* a, void* ws, size_t ws_bytes, cudaStream
 
 // The library's other translation units (each has device-side state of its own).
 const rmsb_units::UnitHooks* const kUnitHooks[] = {&rmsb_units::fused_fwd_unit, &rmsb_units::fused_bwd_unit,
-                                                   &rmsb_units::rope_unit};
+                                                   &rmsb_units::rope_unit,      &rmsb_units::block_quant_unit,
+                                                   &rmsb_units::block_mm_unit,  &rmsb_units::kv_cache_unit};
 constexpr int kUnits = static_cast<int>(sizeof(kUnitHooks) / sizeof(kUnitHooks[0]));
 
 }  // namespace

@@ -31,6 +31,9 @@ struct UnitHooks {
 extern const UnitHooks fused_fwd_unit;
 extern const UnitHooks fused_bwd_unit;
 extern const UnitHooks rope_unit;
+extern const UnitHooks block_quant_unit;
+extern const UnitHooks block_mm_unit;
+extern const UnitHooks kv_cache_unit;
 
 // Bookkeeping of the main unit: rmsnorm_b200_launch_count and rmsnorm_b200_last_plan.
 void count_launches(uint64_t n);

@@ -2,7 +2,7 @@
 // main one: per-device properties, kernel attributes, the hooks of translation_units.h and
 // (bounds-checked build) the registration of a call's byte ranges.
 //
-// Include it after defining RMSB_UNIT (fused_fwd, fused_bwd, rope): the kernels and device
+// Include it after defining RMSB_UNIT (fused_fwd, fused_bwd, rope, block_quant, block_mm, kv_cache): the kernels and device
 // variables of the shared headers then live in a namespace of that unit, so that the units
 // link into one library.
 #pragma once

@@ -1,0 +1,256 @@
+# SPDX-License-Identifier: MIT
+"""8-bit products with a scale for every block of 128 (`rmsnorm.fused` offers them)."""
+
+from __future__ import annotations
+
+import ctypes
+import struct
+from typing import Optional, Tuple
+
+import torch
+from torch import Tensor
+
+from . import _host_fused as _host
+from . import _lib
+from ._autograd import first_order
+from .rmsnorm import _check_optional_dtype, _check_same_device, _check_tensor_dtype, _check_x_shape
+
+_CODE = _lib._DTYPE_CODES
+_BLOCK = 128
+_E4M3 = torch.float8_e4m3fn
+_is_compiling = torch.compiler.is_dynamo_compiling
+
+_QUANT = struct.Struct("2qQqQqQ2qQq2Q4i")
+_MM = struct.Struct("3qQqQqQ2qQ2q2Q4i")
+for _s, _c in ((_QUANT, _lib.BlockQuantArgs), (_MM, _lib.BlockMmArgs)):
+    assert _s.size == ctypes.sizeof(_c), _c.__name__
+
+_BYTES, _STREAM, _SIZE, _OUT = ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.POINTER(ctypes.c_size_t)
+
+
+def _rows_of(t: Tensor) -> Tensor:
+    """t as a matrix over its last dimension, whose values lie side by side: a view wherever
+    the strides allow one."""
+    if t.dim() != 2:
+        t = t.reshape(t.shape[:-1].numel(), t.shape[-1])
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    return t
+
+
+def _bytes_empty(shape, device) -> Tensor:
+    """e4m3 values whose rows begin at multiples of 16 bytes, as the product reads them."""
+    k = shape[-1]
+    pitch = -(-k // 16) * 16
+    if pitch == k:
+        return torch.empty(shape, dtype=_E4M3, device=device)
+    return torch.empty(*shape[:-1], pitch, dtype=_E4M3, device=device)[..., :k]
+
+
+def _quantize(x: Tensor, rows: int, want: bool, want_t: bool, column_major: bool = False, sums_dtype=None):
+    """(q, scales, q_t, scales_t, column sums) of a matrix, those that are wanted."""
+    n, k = x.shape
+    device = x.device
+    gn, gk = -(-n // rows), -(-k // _BLOCK)
+    q = scales = q_t = scales_t = sums = None
+    if not x.is_cuda:
+        if want:
+            q, scales = _host.block_quantize(x, rows)
+        if want_t:
+            q_t, scales_t = _host.block_quantize(x.t(), rows)
+        if sums_dtype is not None:
+            sums = x.float().sum(0).to(sums_dtype)
+        if column_major and want:
+            scales = scales.t().contiguous().t()
+        return q, scales, q_t, scales_t, sums
+    sr, sg = gk, 1
+    if want:
+        q = _bytes_empty((n, k), device)
+        if column_major:
+            scales = torch.empty(gk, gn, dtype=torch.float32, device=device).t()
+            sr, sg = 1, gn
+        else:
+            scales = torch.empty(gn, gk, dtype=torch.float32, device=device)
+    if want_t:
+        q_t = _bytes_empty((k, n), device)
+        scales_t = torch.empty(gk if rows > 1 else k, -(-n // _BLOCK), dtype=torch.float32, device=device)
+    if sums_dtype is not None:
+        sums = torch.empty(k, dtype=sums_dtype, device=device)
+    args = _QUANT.pack(
+        n, k, x.data_ptr(), x.stride(0), q.data_ptr() if want else 0, q.stride(0) if want else 0,
+        scales.data_ptr() if want else 0, sr, sg, q_t.data_ptr() if want_t else 0, q_t.stride(0) if want_t else 0,
+        scales_t.data_ptr() if want_t else 0, 0 if sums is None else sums.data_ptr(), _CODE[x.dtype], rows,
+        0 if sums is None else _CODE[sums_dtype], 0)
+    nbytes, ws = 0, None
+    if sums is not None:
+        name = "rmsnorm_b200_block_quant_workspace_size"
+        nbytes = _lib.workspace_bytes(_lib.packed_entry(name, _BYTES, _OUT), name, device.index, args)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    name = "rmsnorm_b200_block_quant"
+    _lib.enqueue(_lib.packed_entry(name, _BYTES, _STREAM, _SIZE, _STREAM), name, device.index, args,
+                 None if ws is None else ws.data_ptr(), nbytes)
+    return q, scales, q_t, scales_t, sums
+
+
+def block_quantize(x: Tensor, block_rows: int = 1, transposed: bool = False, scales_column_major: bool = False):
+    """(q, scales): x (..., K) held as q * scales, q in float8_e4m3fn and fp32 scales, one for
+    every 128 columns of a row (block_rows 1, scales x.shape[:-1] + (ceil(K / 128),)) or, of a
+    matrix, for every 128 x 128 block (block_rows 128, scales (ceil(N / 128), ceil(K / 128)));
+    the last ones may be shorter. With `transposed` (q, scales, q_t, scales_t): from the same
+    read also those of x transposed, the matrix (K, rows of x).
+
+    A scale is the smallest power of two that brings the largest |x| to 448 or below, at least
+    2^-126; q is x / scale, which is exact, rounded to nearest even. A NaN makes its scale NaN,
+    an infinity infinite. `scales_column_major` lays q's scales out column by column. q's rows
+    begin at multiples of 16 bytes: where K is none, q is a view of wider rows."""
+    if _is_compiling():
+        return _quantize_untraced(x, block_rows, transposed, scales_column_major)
+    if x.dtype not in _CODE:
+        raise AssertionError("Unsupported dtype")
+    if not x.shape or not x.shape[-1]:
+        _check_x_shape(x.shape)
+    if block_rows not in (1, _BLOCK):
+        raise ValueError(f"block_rows must be 1 or 128, got {block_rows}")
+    if block_rows > 1 and x.dim() != 2:
+        raise ValueError(f"128 x 128 blocks need a matrix, got shape {tuple(x.shape)}")
+    q, scales, q_t, scales_t, _ = _quantize(_rows_of(x), block_rows, True, transposed, scales_column_major)
+    if x.dim() != 2:
+        lead = x.shape[:-1]
+        q = q.view(*lead, x.shape[-1]) if q.is_contiguous() else q.unflatten(0, lead) if lead else q[0]
+        scales = scales.unflatten(0, lead) if lead else scales[0]
+    return (q, scales, q_t, scales_t) if transposed else (q, scales)
+
+
+def _mm(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, b_rows: int, bias: Optional[Tensor],
+        out_dtype: torch.dtype) -> Tensor:
+    """The product of matrices."""
+    m, k = a.shape
+    n = b.shape[0]
+    device = a.device
+    out = torch.empty(m, n, dtype=out_dtype, device=device)
+    args = _MM.pack(
+        m, n, k, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), a_scales.data_ptr(), *a_scales.stride(),
+        b_scales.data_ptr(), *b_scales.stride(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), b_rows,
+        0 if bias is None else _CODE[bias.dtype], _CODE[out_dtype], 0)
+    nbytes, ws = 0, None
+    if (a.data_ptr() | b.data_ptr() | a.stride(0) | b.stride(0)) & 15:
+        name = "rmsnorm_b200_block_mm_workspace_size"
+        nbytes = _lib.workspace_bytes(_lib.packed_entry(name, _BYTES, _OUT), name, device.index, args)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    name = "rmsnorm_b200_block_mm"
+    _lib.enqueue(_lib.packed_entry(name, _BYTES, _STREAM, _SIZE, _STREAM), name, device.index, args,
+                 None if ws is None else ws.data_ptr(), nbytes)
+    return out
+
+
+def _check_bias(bias: Optional[Tensor], n: int, device: torch.device) -> None:
+    if bias is None:
+        return
+    if bias.dtype not in _CODE:
+        _check_tensor_dtype("Bias", bias)
+    if bias.shape != (n,):
+        raise ValueError(f"bias shape must be (N,) with N={n}, got {tuple(bias.shape)}")
+    if bias.device != device:
+        _check_same_device("bias", bias, device)
+
+
+def block_mm(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, bias: Optional[Tensor] = None,
+             out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """The product of 8-bit matrices with scales, (a * a_scales) (b * b_scales)^T + bias, in
+    out_dtype: a (..., K) and b (N, K) in float8_e4m3fn, fp32 scales for groups of 128 columns,
+    a_scales a.shape[:-1] + (ceil(K / 128),) as `rmsnorm_quant_fwd` with group_size 128 and
+    `block_quantize` leave them, b_scales (N, ceil(K / 128)) or, a scale per 128 x 128 block,
+    (ceil(N / 128), ceil(K / 128)). Scales may have any strides. The sums are held in fp32 (and
+    so are products of two scales), rounded once at the end.
+
+    Operands whose rows begin at multiples of 16 bytes are read as they are, others copied by
+    every call. Outside autograd: `block_linear` has gradients."""
+    if _is_compiling():
+        return _mm_untraced(a, a_scales, b, b_scales, bias, out_dtype)
+    if a.dtype != _E4M3 or b.dtype != _E4M3:
+        raise AssertionError("a and b must be float8_e4m3fn")
+    if a_scales.dtype != torch.float32 or b_scales.dtype != torch.float32:
+        raise AssertionError("scales must be float32")
+    if out_dtype not in _CODE:
+        _check_optional_dtype("out_dtype", out_dtype)
+    if not a.shape or not a.shape[-1]:
+        _check_x_shape(a.shape)
+    k, device = a.shape[-1], a.device
+    if b.dim() != 2 or b.shape[1] != k or not b.shape[0]:
+        raise ValueError(f"b must be (N, K) with K={k} and at least one row, got {tuple(b.shape)}")
+    n, groups = b.shape[0], -(-k // _BLOCK)
+    if a_scales.shape != a.shape[:-1] + (groups,):
+        raise ValueError(f"a_scales must be {tuple(a.shape[:-1] + (groups,))}, got {tuple(a_scales.shape)}")
+    if b_scales.shape == (-(-n // _BLOCK), groups):
+        b_rows = _BLOCK
+    elif b_scales.shape == (n, groups):
+        b_rows = 1
+    else:
+        raise ValueError(f"b_scales must be {(n, groups)} or {(-(-n // _BLOCK), groups)}, got {tuple(b_scales.shape)}")
+    for name, t in (("a_scales", a_scales), ("b", b), ("b_scales", b_scales)):
+        if t.device != device:
+            _check_same_device(name, t, device)
+    _check_bias(bias, n, device)
+    a2, b2 = _rows_of(a), _rows_of(b)
+    s2 = a_scales if a_scales.dim() == 2 else a_scales.reshape(a2.shape[0], groups)
+    if a.is_cuda:
+        out = _mm(a2, s2, b2, b_scales, b_rows, None if bias is None else bias.contiguous(), out_dtype)
+    else:
+        with torch.no_grad():
+            out = _host.block_values(a2, s2, 1) @ _host.block_values(b2, b_scales, b_rows).t()
+            out = (out if bias is None else out + bias.float()).to(out_dtype)
+    return out if a.dim() == 2 else out.view(*a.shape[:-1], n)
+
+
+class BlockLinearFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        x2 = _rows_of(x)
+        q, s, x_t, x_ts, _ = _quantize(x2, 1, True, ctx.needs_input_grad[1], True)
+        w, ws, w_t, w_ts, _ = _quantize(_rows_of(weight), _BLOCK, True, ctx.needs_input_grad[0])
+        ctx.save_for_backward(x_t, x_ts, w_t, w_ts)
+        ctx.x_shape, ctx.dtypes = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
+        return block_mm(q, s, w, ws, bias, x.dtype).view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    def backward(ctx, dy):
+        x_t, x_ts, w_t, w_ts = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad
+        x_dtype, w_dtype, b_dtype = ctx.dtypes
+        dx = dw = db = None
+        q, s, d_t, d_ts, db = _quantize(_rows_of(dy), 1, need_x, need_w, True, b_dtype if need_b else None)
+        if need_x:
+            dx = block_mm(q, s, w_t, w_ts, None, x_dtype).view(ctx.x_shape)
+        if need_w:
+            if d_t.shape[1]:
+                dw = block_mm(d_t, d_ts, x_t, x_ts, None, w_dtype)
+            else:
+                dw = torch.zeros(d_t.shape[0], x_t.shape[0], dtype=w_dtype, device=dy.device)
+        return first_order("block_linear", (dx, dw, db))
+
+
+def block_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None) -> Tensor:
+    """x weight^T + bias in x's dtype by 8-bit products, with autograd: x (..., K) is quantised
+    per 128 columns of a row, weight (N, K) per 128 x 128 block (`block_quantize`), and in the
+    backward the gradient per 128 columns for x's and, like x, per 128 rows for weight's. Every
+    sum is held in fp32. What the backward needs of x and weight is kept in 8 bits. The
+    gradients are those of the product at the quantised values (rounding counts as the
+    identity); they cannot be differentiated again: that is an error."""
+    if _is_compiling():
+        return _linear_untraced(x, weight, bias)
+    for name, t in (("X", x), ("Weight", weight)):
+        if t.dtype not in _CODE:
+            _check_tensor_dtype(name, t)
+    if not x.shape or not x.shape[-1]:
+        _check_x_shape(x.shape)
+    if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or not weight.shape[0]:
+        raise ValueError(f"weight must be (N, K) with K={x.shape[-1]} and at least one row, got {tuple(weight.shape)}")
+    if weight.device != x.device:
+        _check_same_device("weight", weight, x.device)
+    _check_bias(bias, weight.shape[0], x.device)
+    return BlockLinearFunction.apply(x, weight, bias)
+
+
+_quantize_untraced = torch.compiler.disable(block_quantize)
+_mm_untraced = torch.compiler.disable(block_mm)
+_linear_untraced = torch.compiler.disable(block_linear)

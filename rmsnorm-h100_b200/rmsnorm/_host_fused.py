@@ -134,3 +134,42 @@ def qk_norm_rope_bwd(x, weight, dout, cos, sin, interleaved, norm, eps):
     if norm:
         g = (g - xhat * (g * xhat).mean(-1, keepdim=True)) * rstd
     return g.to(x.dtype), dw
+
+
+def power_scales(most: torch.Tensor) -> torch.Tensor:
+    """The smallest power of two, at least 2^-126, that brings each magnitude to 448 =
+    0.875 * 2^9 or below; infinity and NaN stay."""
+    part, exponent = torch.frexp(most)
+    exponent = exponent - 9 + (part > 0.875).to(torch.int32)
+    power = (exponent.clamp_min(-126) + 127 << 23).view(torch.float32)
+    return torch.where(most.isfinite(), power, most)
+
+
+def block_quantize(x, rows):
+    """(e4m3 values, scales) of a matrix, a scale per `rows` x 128 values."""
+    n, k = x.shape
+    gn, gk = -(-n // rows), -(-k // 128)
+    wide = torch.nn.functional.pad(x.float(), (0, gk * 128 - k, 0, gn * rows - n)).view(gn, rows, gk, 128)
+    scales = power_scales(wide.abs().amax((1, 3))) if n else wide.new_empty(gn, gk)
+    q = (wide / scales[:, None, :, None]).view(gn * rows, gk * 128)[:n, :k]
+    return q.to(torch.float8_e4m3fn), scales
+
+
+def block_values(q, scales, rows):
+    n, k = q.shape
+    return q.float() * scales.repeat_interleave(rows, 0)[:n].repeat_interleave(128, 1)[:, :k]
+
+
+def cache_write(x, cache, scales, page, place, top):
+    """x [tokens, heads, head_dim] into (page, place)."""
+    x = x.float()
+    s = (x.abs().amax(-1) / top).clamp_min(torch.finfo(torch.float32).tiny)
+    q = x / s[..., None]
+    if cache.dtype == torch.int8:
+        q = torch.where(q.isnan(), 0.0, q).round()
+    cache[page, place] = q.to(cache.dtype)
+    scales[page, place] = s
+
+
+def cache_read(cache, scales, page, place, dtype):
+    return (cache[page, place].float() * scales[page, place][..., None]).to(dtype)

@@ -233,7 +233,128 @@ class RopeGrads(ctypes.Structure):
     ]
 
 
+class BlockQuantArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("x", ctypes.c_void_p),
+        ("x_row_stride", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64),
+        ("scales", ctypes.c_void_p),
+        ("scale_row_stride", ctypes.c_int64),
+        ("scale_group_stride", ctypes.c_int64),
+        ("q_t", ctypes.c_void_p),
+        ("q_t_row_stride", ctypes.c_int64),
+        ("scales_t", ctypes.c_void_p),
+        ("column_sums", ctypes.c_void_p),
+        ("x_dtype", ctypes.c_int32),
+        ("block_rows", ctypes.c_int32),
+        ("column_sums_dtype", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
+class BlockMmArgs(ctypes.Structure):
+    _fields_ = [
+        ("m", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("a", ctypes.c_void_p),
+        ("a_row_stride", ctypes.c_int64),
+        ("b", ctypes.c_void_p),
+        ("b_row_stride", ctypes.c_int64),
+        ("a_scales", ctypes.c_void_p),
+        ("a_scale_row_stride", ctypes.c_int64),
+        ("a_scale_group_stride", ctypes.c_int64),
+        ("b_scales", ctypes.c_void_p),
+        ("b_scale_row_stride", ctypes.c_int64),
+        ("b_scale_group_stride", ctypes.c_int64),
+        ("bias", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("b_block_rows", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
+class CacheTensor(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("slot_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("scales", ctypes.c_void_p),
+        ("scale_page_stride", ctypes.c_int64),
+        ("scale_slot_stride", ctypes.c_int64),
+        ("scale_head_stride", ctypes.c_int64),
+    ]
+
+
+class CacheArgs(ctypes.Structure):
+    _fields_ = [
+        ("pages", ctypes.c_int64),
+        ("k", CacheTensor),
+        ("v", CacheTensor),
+        ("page_size", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("cache_dtype", ctypes.c_int32),
+    ]
+
+
+class CacheWriteArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("k", RopeTensor),
+        ("v", RopeTensor),
+        ("slots", ctypes.c_void_p),
+        ("slots_64bit", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class CacheReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("sequences", ctypes.c_int64),
+        ("table_width", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64),
+        ("page_table", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+        ("zero_rest", ctypes.c_int32),
+    ]
+
+
 SIGNATURES = {
+    "rmsnorm_b200_block_quant_workspace_size": (
+        ctypes.c_int,
+        [ctypes.POINTER(BlockQuantArgs), ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "rmsnorm_b200_block_quant": (
+        ctypes.c_int,
+        [ctypes.POINTER(BlockQuantArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "rmsnorm_b200_block_mm_workspace_size": (
+        ctypes.c_int,
+        [ctypes.POINTER(BlockMmArgs), ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "rmsnorm_b200_block_mm": (
+        ctypes.c_int,
+        [ctypes.POINTER(BlockMmArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "rmsnorm_b200_cache_write": (
+        ctypes.c_int,
+        [ctypes.POINTER(CacheArgs), ctypes.POINTER(CacheWriteArgs), ctypes.c_void_p],
+    ),
+    "rmsnorm_b200_cache_read": (
+        ctypes.c_int,
+        [ctypes.POINTER(CacheArgs), ctypes.POINTER(CacheReadArgs), ctypes.c_void_p],
+    ),
     "rmsnorm_b200_quant_fwd": (ctypes.c_int, [ctypes.POINTER(QuantArgs), ctypes.c_void_p]),
     "rmsnorm_b200_dropout_rmsnorm_fwd": (ctypes.c_int, [ctypes.POINTER(DropoutFwdArgs), ctypes.c_void_p]),
     "rmsnorm_b200_dropout_rmsnorm_bwd_workspace_size": (

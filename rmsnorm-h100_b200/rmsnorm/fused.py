@@ -5,7 +5,14 @@
 * `dropout_add_rmsnorm` (`_fwd`, `_bwd`) -- dropout from a counter-based generator, residual
   addition and RMSNorm; the mask is never stored;
 * `qk_norm_rope` (`_fwd`, `_bwd`) -- per-head RMSNorm of q and k with rotary positions on one
-  to four axes (`rope_table`, `rope_axes`).
+  to four axes (`rope_table`, `rope_axes`);
+
+and, on what these leave behind:
+
+* `block_mm` -- products of 8-bit matrices with a scale for every block of 128,
+  `block_quantize`, which makes their operands, and `block_linear`, a linear layer on both with
+  gradients;
+* `cache_write`, `cache_read` -- keys and values in the pages of an 8-bit cache.
 
 They follow the conventions of `rmsnorm.rmsnorm`: arguments are checked before anything
 runs, CUDA tensors go to the native library on the current stream of their device, tensors
@@ -26,6 +33,8 @@ from torch import Tensor
 from . import _host_fused as _host
 from . import _lib
 from ._autograd import first_order
+from ._block import BlockLinearFunction, block_linear, block_mm, block_quantize
+from ._cache import cache_read, cache_write
 from .rmsnorm import (
     _check_optional_dtype,
     _check_same_device,
@@ -35,8 +44,14 @@ from .rmsnorm import (
 )
 
 __all__ = [
+    "BlockLinearFunction",
     "DropoutAddRMSNormFunction",
     "QKNormRopeFunction",
+    "block_linear",
+    "block_mm",
+    "block_quantize",
+    "cache_read",
+    "cache_write",
     "dropout_add_rmsnorm",
     "dropout_add_rmsnorm_bwd",
     "dropout_add_rmsnorm_fwd",
