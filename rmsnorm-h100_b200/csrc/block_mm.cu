@@ -151,10 +151,13 @@ int launch_few(UnitDevice* ud, const void* a, int64_t a_row, const CUtensorMap& 
   FewPlan pl = {};
   pl.tiles_n = static_cast<int>((args->n + kBlock - 1) / kBlock);
   const int64_t tiles = (args->m + T - 1) / T * pl.tiles_n;
-  const int fit = T >= 128 ? 1 : 2;  // CTAs an SM
-  pl.splits = static_cast<int>(std::clamp<int64_t>(fit * ud->sm_count / tiles, 1, std::min(8, p.groups)));
+  constexpr int fit = T >= 128 ? 1 : 2;  // CTAs an SM
+  // as many CTAs as are resident together, of two groups at least: 1 x 4096 x 4096 in 1, 2, 4 and
+  // 8 parts 11.9, 8.8, 8.2 and 6.9 us, 64 x 8192 x 8192 38.7, 24.2, 17.8 and (512 CTAs) 25.2 us,
+  // 32 x 4096 x 1024 6.5, 5.6, 5.2 and (a group each) 6.3 us
+  pl.splits = static_cast<int>(std::clamp<int64_t>(fit * ud->sm_count / tiles, 1, std::clamp(p.groups / 2, 1, kFewMaxSplits)));
   const int each = (p.groups + pl.splits - 1) / pl.splits;
-  const int fixed = 1024 + static_cast<int>(sizeof(FewBars)) + 2 * T * 4;
+  const int fixed = 1024 + static_cast<int>(sizeof(FewBars)) + 2 * kFewChunk * T * 4;
   const int room = (fit == 2 ? kSmemOptIn / 2 - 1024 : kSmemOptIn) - fixed;
   pl.stages = std::min({kFewMaxStages, each, room / Few<T>::kStageBytes});
   pl.ring_bytes = std::max(pl.stages * Few<T>::kStageBytes, pl.splits > 1 ? T * kBlock * 4 : 0);
@@ -164,21 +167,21 @@ int launch_few(UnitDevice* ud, const void* a, int64_t a_row, const CUtensorMap& 
   return launch<FewKernel>(ud, block_mm_few_kernel<T>, map_a, map_b, p, pl, kFewThreads, smem, pl.splits, stream, l);
 }
 
-template <bool kPair>
 int launch_wide(UnitDevice* ud, const CUtensorMap& map_a, const CUtensorMap& map_b, const rmsnorm_b200_block_mm_args* a,
                 const BlockMmParams& p, cudaStream_t stream) {
-  using W = Wide<kPair>;
   WidePlan pl = {};
-  pl.tiles_m = static_cast<int>((a->m + W::kRows - 1) / W::kRows);
+  pl.tiles_m = static_cast<int>((a->m + kWideRows - 1) / kWideRows);
   pl.tiles_n = static_cast<int>((a->n + kWideN - 1) / kWideN);
-  pl.band = kPair ? 8 : 16;
+  pl.band = 8;
   const int64_t tiles = static_cast<int64_t>(pl.tiles_m) * pl.tiles_n;
-  const int per = kPair ? 2 : 1;
-  const int64_t units = std::min<int64_t>(tiles, ud->sm_count / per);
-  const int smem = 1024 + W::kStages * W::kStageBytes + static_cast<int>(sizeof(WideBars)) + 2 * kWideN * 4;
-  const MmLaunch l = {kPair ? "block_mm_pair" : "block_mm_wide", static_cast<unsigned>(units * per), kWideN, 1, W::kStages};
-  return launch<WideKernel>(ud, p.b_rows ? block_mm_wide_kernel<kPair, true> : block_mm_wide_kernel<kPair, false>, map_a,
-                            map_b, p, pl, kWideThreads, smem, per, stream, l);
+  const int64_t pairs = std::min<int64_t>(tiles, ud->sm_count / 2);
+  const int smem = 1024 + kWideStages * kWideStageBytes + static_cast<int>(sizeof(WideBars)) + 2 * kWideN * 4 +
+                   8 * kStagingBytes;
+  static_assert(1024 + kWideStages * kWideStageBytes + sizeof(WideBars) + 2 * kWideN * 4 + 8 * kStagingBytes <= kSmemOptIn,
+                "shared memory");
+  const MmLaunch l = {"block_mm_wide", static_cast<unsigned>(pairs * 2), kWideN, 1, kWideStages};
+  return launch<WideKernel>(ud, p.b_rows ? block_mm_wide_kernel<true> : block_mm_wide_kernel<false>, map_a, map_b, p, pl,
+                            kWideThreads, smem, 2, stream, l);
 }
 
 int run(const rmsnorm_b200_block_mm_args* a, void* ws, size_t ws_bytes, cudaStream_t stream) {
@@ -229,17 +232,21 @@ int run(const rmsnorm_b200_block_mm_args* a, void* ws, size_t ws_bytes, cudaStre
   p.bias = a->bias; p.bias_dt = a->bias_dtype;
   p.out = a->out; p.out_dt = a->out_dtype;
   p.b_rows = a->b_block_rows == 1;
-  p.vec_out = aligned_to(a->out, 16) && a->n * elem_bytes(a->out_dtype) % 16 == 0;
+  p.vec_out = aligned_to(a->out, 32) && a->n * elem_bytes(a->out_dtype) % 32 == 0;
   CUtensorMap map_a, map_b;
   st = make_map(&map_b, qb, a->n, a->k, b_row, kBlock);
   if (st) return st;
+  // Few rows, or more of them where two CTAs or more could share each 128 x 128 of the result:
+  // the kernel that splits k. K = 4096: 256 x 4096 14.9 against 21.8 us, 1024 x 1024 14.6 against
+  // 21.8 us, 512 x 4096 (128 tiles for 148 SMs) 25.2 against 22.0 us.
   if (a->m <= 16) return launch_few<16>(ud, qa, a_row, map_b, a, p, stream);
   if (a->m <= 32) return launch_few<32>(ud, qa, a_row, map_b, a, p, stream);
   if (a->m <= 64) return launch_few<64>(ud, qa, a_row, map_b, a, p, stream);
-  if (a->m <= 128) return launch_few<128>(ud, qa, a_row, map_b, a, p, stream);
+  const int64_t squares = (a->m + kBlock - 1) / kBlock * ((a->n + kBlock - 1) / kBlock);
+  if (a->m <= 128 || (2 * squares <= ud->sm_count && groups >= 4)) return launch_few<128>(ud, qa, a_row, map_b, a, p, stream);
   st = make_map(&map_a, qa, a->m, a->k, a_row, kBlock);
   if (st) return st;
-  return launch_wide<false>(ud, map_a, map_b, a, p, stream);
+  return launch_wide(ud, map_a, map_b, a, p, stream);
 }
 
 int workspace_size(const rmsnorm_b200_block_mm_args* a, size_t* bytes) {

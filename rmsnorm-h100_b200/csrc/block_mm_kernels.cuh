@@ -26,7 +26,7 @@ struct BlockMmParams {
   void* out;
   int32_t bias_dt, out_dt;
   bool b_rows;      // b's scales are per row
-  bool vec_out;     // 8-element vectors of out
+  bool vec_out;     // out's rows begin at multiples of 32 bytes
 };
 
 __device__ __forceinline__ const float* sb_of(const BlockMmParams& p, int64_t n) {
@@ -34,22 +34,22 @@ __device__ __forceinline__ const float* sb_of(const BlockMmParams& p, int64_t n)
 }
 
 // ---------------------------------------------------------------------------------------
-// Many rows: 128 x 256 of the result a CTA.
+// Many rows: 256 x 256 of the result a pair of CTAs, whose tensor cores work on one product: each
+// CTA holds 128 rows of a and of b and half of the result, so that what both need of b crosses
+// from L2 once.
 // ---------------------------------------------------------------------------------------
-constexpr int kWideN = 256;        // columns of a tile
+constexpr int kWideRows = 256, kWideN = 256;  // rows and columns of a pair's tile
 constexpr int kWideThreads = 384;  // warps 0 - 7 sum, 8 copies, 9 multiplies
-constexpr int kWideSums = 2;       // accumulators in tensor memory, 256 columns each
+constexpr int kWideHalf = kWideN / 2;
 constexpr int kTileBytes = kBlock * kTileK;  // 128 rows of an operand
 
-template <bool kPair>
-struct Wide {
-  static constexpr int kStages = kPair ? 6 : 4;
-  static constexpr int kStageBytes = kTileBytes * (kPair ? 2 : 3);
-  static constexpr int kRows = kPair ? 256 : 128;  // rows of a tile
-};
+constexpr int kWideStages = 6;
+constexpr int kWideStageBytes = 2 * kTileBytes;  // a CTA's rows of a and of b
+
+constexpr int kStagingBytes = 32 * 17 * 4;  // 32 rows of 16 columns, a word between them
 
 struct WideBars {
-  uint64_t full[6], empty[6], sum[kWideSums], sum_empty[kWideSums], done;
+  uint64_t full[kWideStages], empty[kWideStages], sum[2], sum_empty[2], done;
   uint32_t tmem;
 };
 
@@ -64,6 +64,14 @@ __device__ __forceinline__ void wide_tile(const WidePlan& pl, int64_t i, int* tm
   const int high = min(pl.band, pl.tiles_m - b * pl.band);
   *tn = static_cast<int>(at / high);
   *tm = b * pl.band + static_cast<int>(at - static_cast<int64_t>(*tn) * high);
+}
+
+// A whole 32-byte sector: a lane's neighbours write other rows.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  if (!RMSB_DBG_OK(p, 32, kDbgVecStore)) return;
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
 // acc += sums * scale, or acc += sums * (column scales) * scale.
@@ -82,42 +90,39 @@ __device__ __forceinline__ void add_scaled(float2* acc, const float2 (&v)[16], f
   }
 }
 
-template <bool kPair, bool kRowScales>
+template <bool kRowScales>
 __global__ void __launch_bounds__(kWideThreads, 1)
     block_mm_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                          const BlockMmParams p, const WidePlan pl) {
-  using W = Wide<kPair>;
   unsigned char* smem = rmsb_dyn_smem + ((1024u - (smem_u32(rmsb_dyn_smem) & 1023u)) & 1023u);
-  WideBars* bars = reinterpret_cast<WideBars*>(smem + W::kStages * W::kStageBytes);
+  WideBars* bars = reinterpret_cast<WideBars*>(smem + kWideStages * kWideStageBytes);
   float* col_scales = reinterpret_cast<float*>(bars + 1);  // [2][kWideN]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = kPair ? cluster_ctarank() : 0;
-  const int64_t unit = kPair ? blockIdx.x >> 1 : blockIdx.x, units = kPair ? gridDim.x >> 1 : gridDim.x;
+  unsigned char* staging = reinterpret_cast<unsigned char*>(col_scales + 2 * kWideN);  // kStagingBytes a warp
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int64_t unit = blockIdx.x >> 1, units = gridDim.x >> 1;
   const int64_t tiles = static_cast<int64_t>(pl.tiles_m) * pl.tiles_n;
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < W::kStages; ++i) {
+    for (int i = 0; i < kWideStages; ++i) {
       mbar_init(&bars->full[i], 1);
       mbar_init(&bars->empty[i], 1);
     }
-    for (int i = 0; i < kWideSums; ++i) {
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->sum[i], 1);
-      mbar_init(&bars->sum_empty[i], kPair ? 16 : 8);
+      mbar_init(&bars->sum_empty[i], 16);
     }
     mbar_init(&bars->done, 1);
     fence_mbar_init();
   }
-  if (warp == 9) {
-    if constexpr (kPair) tmem_alloc_pair(&bars->tmem, kWideSums * kWideN);
-    else tmem_alloc_warp(&bars->tmem, kWideSums * kWideN);
-  }
+  if (warp == 9) tmem_alloc_pair(&bars->tmem, 2 * kWideN);
   if (threadIdx.x == 256) {
     prefetch_map(&map_a);
     prefetch_map(&map_b);
   }
   tmem_fence_before_sync();
   __syncthreads();
-  if constexpr (kPair) cluster_sync_all();
+  cluster_sync_all();
   tmem_fence_after_sync();
   const uint32_t tmem = bars->tmem;
   pdl_wait();
@@ -131,21 +136,19 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       for (int64_t t = unit; ok && t < tiles; t += units) {
         int tm, tn;
         wide_tile(pl, t, &tm, &tn);
-        const int ya = tm * W::kRows + static_cast<int>(rank) * kBlock, yb = tn * kWideN + static_cast<int>(rank) * kBlock;
+        const int ya = tm * kWideRows + static_cast<int>(rank) * kBlock;
+        const int yb = tn * kWideN + static_cast<int>(rank) * kBlock;
         for (int g = 0; g < p.groups; ++g) {
-          ok = mbar_wait_warp<kPair>(&bars->empty[s], pass ^ 1u, kSiteMmEmpty);
-          ok = __all_sync(0xffffffffu, ok);
+          ok = __all_sync(0xffffffffu, mbar_spin_warp(&bars->empty[s], pass ^ 1u, kSiteMmEmpty));
           if (!ok) break;
-          if (lane == 0) {
-            unsigned char* at = smem + s * W::kStageBytes;
-            if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], W::kStageBytes * (kPair ? 2 : 1));
-            tile_load<kPair>(at, &map_a, g * kTileK, ya, &bars->full[s]);
-            tile_load<kPair>(at + kTileBytes, &map_b, g * kTileK, yb, &bars->full[s]);
-            if constexpr (!kPair)
-              tile_load<kPair>(at + 2 * kTileBytes, &map_b, g * kTileK, yb + kBlock, &bars->full[s]);
+          if (elect_one()) {
+            unsigned char* at = smem + s * kWideStageBytes;
+            if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * kWideStageBytes);
+            tile_load<true>(at, &map_a, g * kTileK, ya, &bars->full[s]);
+            tile_load<true>(at + kTileBytes, &map_b, g * kTileK, yb, &bars->full[s]);
           }
           __syncwarp();
-          if (++s == W::kStages) {
+          if (++s == kWideStages) {
             s = 0;
             pass ^= 1u;
           }
@@ -153,56 +156,54 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       }
       // Nobody leaves while copies may land in its memory or arrivals at its barriers.
       if (lane == 0 && rank == 0 && abort_requested())
-        for (int i = 0; i < W::kStages; ++i) mbar_wait(&bars->full[i], i < s ? pass : pass ^ 1u, kSiteDrain, false);
-      for (int i = 0; i < W::kStages; ++i)
-        mbar_wait_warp<kPair>(&bars->empty[i], i < s ? pass : pass ^ 1u, kSiteMmEmpty);
+        for (int i = 0; i < kWideStages; ++i) mbar_wait(&bars->full[i], i < s ? pass : pass ^ 1u, kSiteDrain, false);
+      for (int i = 0; i < kWideStages; ++i) mbar_spin_warp(&bars->empty[i], i < s ? pass : pass ^ 1u, kSiteMmEmpty);
     } else if (warp == 9 && rank == 0) {  // products
-      constexpr uint32_t idesc = product_desc(W::kRows, kWideN);
+      constexpr uint32_t idesc = product_desc(kWideRows, kWideN);
       int s = 0;
       uint32_t pass = 0, u = 0;
       bool ok = true;
       for (int64_t t = unit; ok && t < tiles; t += units)
         for (int g = 0; g < p.groups; ++g, ++u) {
           const uint32_t d = u & 1u;
-          ok = mbar_wait_warp<kPair>(&bars->sum_empty[d], ((u >> 1) & 1u) ^ 1u, kSiteMmSumEmpty);
-          ok = mbar_wait_warp<kPair>(&bars->full[s], pass, kSiteMmFull) && ok;
+          ok = mbar_spin_warp(&bars->full[s], pass, kSiteMmFull);
+          ok = mbar_spin_warp(&bars->sum_empty[d], ((u >> 1) & 1u) ^ 1u, kSiteMmSumEmpty) && ok;
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tmem_fence_after_sync();
-          if (lane == 0) {
-            const uint32_t at = smem_u32(smem + s * W::kStageBytes);
+          if (elect_one()) {
+            const uint32_t at = smem_u32(smem + s * kWideStageBytes);
             const uint64_t a = operand_desc(at), b = operand_desc(at + kTileBytes);
 #pragma unroll
-            for (int k = 0; k < kTileK / 32; ++k) mma_e4m3<kPair>(tmem + d * kWideN, a + 2 * k, b + 2 * k, idesc, k > 0);
-            mma_commit<kPair>(&bars->empty[s]);
-            mma_commit<kPair>(&bars->sum[d]);
+            for (int k = 0; k < kTileK / 32; ++k) mma_e4m3<true>(tmem + d * kWideN, a + 2 * k, b + 2 * k, idesc, k > 0);
+            mma_commit<true>(&bars->empty[s]);
+            mma_commit<true>(&bars->sum[d]);
           }
           __syncwarp();
-          if (++s == W::kStages) {
+          if (++s == kWideStages) {
             s = 0;
             pass ^= 1u;
           }
         }
       if (abort_requested()) {
         if (lane == 0) {
-          mma_commit<kPair>(&bars->done);
+          mma_commit<true>(&bars->done);
           mbar_wait(&bars->done, 0, kSiteDrain, false);
         }
         __syncwarp();
       }
-      for (int i = 0; i < kWideSums; ++i, ++u)
-        mbar_wait_warp<kPair>(&bars->sum_empty[u & 1u], ((u >> 1) & 1u) ^ 1u, kSiteMmSumEmpty);
+      for (int i = 0; i < 2; ++i, ++u) mbar_spin_warp(&bars->sum_empty[u & 1u], ((u >> 1) & 1u) ^ 1u, kSiteMmSumEmpty);
     }
   } else {  // sums: warp w has rows 32 (w % 4) .. + 31, the half w / 4 of the columns
     regs_up<232>();
     const int half = warp >> 2;
-    const uint32_t from = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * (kWideN / 2);
+    const uint32_t from = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * kWideHalf;
     uint32_t u = 0;
     for (int64_t t = unit; t < tiles; t += units) {
       int tm, tn;
       wide_tile(pl, t, &tm, &tn);
-      const int64_t row = static_cast<int64_t>(tm) * W::kRows + rank * kBlock + (warp & 3) * 32 + lane;
-      const int64_t col0 = static_cast<int64_t>(tn) * kWideN + half * (kWideN / 2);
+      const int64_t row = static_cast<int64_t>(tm) * kWideRows + rank * kBlock + (warp & 3) * 32 + lane;
+      const int64_t col0 = static_cast<int64_t>(tn) * kWideN + half * kWideHalf;
       const bool live = row < p.m;
       // scales two groups ahead; b's per row: thread i of the 256 brings column i's, else every
       // thread its half's
@@ -221,9 +222,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         return v;
       };
       float a0 = next_a(0), a1 = next_a(1), b0 = next_b(0), b1 = next_b(1);
-      float2 acc[kWideN / 4];
+      float2 acc[kWideHalf / 2];
 #pragma unroll
-      for (int i = 0; i < kWideN / 4; ++i) acc[i] = make_float2(0.f, 0.f);
+      for (int i = 0; i < kWideHalf / 2; ++i) acc[i] = make_float2(0.f, 0.f);
       for (int g = 0; g < p.groups; ++g, ++u) {
         const uint32_t d = u & 1u;
         float s = a0;
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           col_scales[d * kWideN + threadIdx.x] = b0;
           __syncwarp();
           named_barrier(1, 256);
-          cols += half * (kWideN / 2);
+          cols += half * kWideHalf;
         } else {
           s *= b0;
         }
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         b0 = b1;
         a1 = next_a(g + 2);
         b1 = next_b(g + 2);
-        mbar_spin_warp<kPair>(&bars->sum[d], (u >> 1) & 1u, kSiteMmSum);
+        mbar_spin_warp(&bars->sum[d], (u >> 1) & 1u, kSiteMmSum);
         __syncwarp();
         tmem_fence_after_sync();
         const uint32_t at = from + d * kWideN;
@@ -258,30 +259,57 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         tmem_landed(v1);
         tmem_fence_before_sync();
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (kPair) mbar_arrive_peer(&bars->sum_empty[d], 0);
-          else mbar_arrive(&bars->sum_empty[d]);
-        }
+        if (lane == 0) mbar_arrive_peer(&bars->sum_empty[d], 0);
         add_scaled<kRowScales>(acc + 48, v1, s, cols + 96);
       }
-      if (!live) continue;
+      const int64_t e = row * p.n + col0;
+      const int left = static_cast<int>(min(static_cast<int64_t>(kWideHalf), p.n - col0));
+      if (p.bias) {
 #pragma unroll
-      for (int i = 0; i < kWideN / 2; i += 8) {
-        const int64_t col = col0 + i;
-        if (col >= p.n) break;
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          v[k] = k & 1 ? acc[(i + k) / 2].y : acc[(i + k) / 2].x;
-          if (p.bias && col + k < p.n) v[k] += load1_rt(p.bias, p.bias_dt, col + k);
+        for (int i = 0; i < kWideHalf / 2; ++i) {
+          const float x = 2 * i < left ? load1_rt(p.bias, p.bias_dt, col0 + 2 * i) : 0.f;
+          const float y = 2 * i + 1 < left ? load1_rt(p.bias, p.bias_dt, col0 + 2 * i + 1) : 0.f;
+          acc[i] = add2(acc[i], make_float2(x, y));
         }
-        const int64_t e = row * p.n + col;
-        if (p.vec_out && col + 8 <= p.n) {
-          store8_rt(p.out, p.out_dt, e, v);
-        } else {
+      }
+      if (!p.vec_out || left < kWideHalf) {
+        // a lane's row begins anywhere: 16 columns at a time turned through shared memory, so that
+        // the warp stores a row's neighbours side by side (1000 x 4100 with K = 1008: 50 us when
+        // every lane stored its own row's values one by one)
+        float* mine = reinterpret_cast<float*>(staging + warp * kStagingBytes);
+        const int64_t row0 = row - lane;
+        const int rows = static_cast<int>(max(int64_t{0}, min(int64_t{32}, p.m - row0)));
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (col + k < p.n) store1_rt(p.out, p.out_dt, e + k, v[k]);
+        for (int c = 0; c < kWideHalf; c += 16) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mine[lane * 17 + i] = i & 1 ? acc[(c + i) / 2].y : acc[(c + i) / 2].x;
+          __syncwarp();
+          const int col = c + (lane & 15);
+          if (col < left)
+            for (int r = lane >> 4; r < rows; r += 2)
+              store1_rt(p.out, p.out_dt, (row0 + r) * p.n + col0 + col, mine[r * 17 + (lane & 15)]);
+        }
+      } else if (!live) {
+        continue;
+      } else if (p.out_dt == RMSNORM_B200_F32) {
+        float* out = static_cast<float*>(p.out) + e;
+#pragma unroll
+        for (int i = 0; i < kWideHalf; i += 8) {
+          uint32_t w[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(k & 1 ? acc[(i + k) / 2].y : acc[(i + k) / 2].x);
+          store32(out + i, w);
+        }
+      } else {
+        uint16_t* out = static_cast<uint16_t*>(p.out) + e;
+        const bool bf16 = p.out_dt == RMSNORM_B200_BF16;
+#pragma unroll
+        for (int i = 0; i < kWideHalf; i += 16) {
+          uint32_t w[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w[k] = bf16 ? pack_bf16x2_pair(acc[i / 2 + k]) : pack_f16x2_pair(acc[i / 2 + k]);
+          store32(out + i, w);
         }
       }
     }
@@ -289,12 +317,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   __syncwarp();
   tmem_fence_before_sync();
   __syncthreads();
-  if constexpr (kPair) cluster_sync_all();
+  cluster_sync_all();
   tmem_fence_after_sync();
-  if (warp == 9) {
-    if constexpr (kPair) tmem_dealloc_pair(tmem, kWideSums * kWideN);
-    else tmem_dealloc_warp(tmem, kWideSums * kWideN);
-  }
+  if (warp == 9) tmem_dealloc_pair(tmem, 2 * kWideN);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -303,7 +328,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 // which then adds up some rows of the result.
 // ---------------------------------------------------------------------------------------
 constexpr int kFewThreads = 192;  // warps 0 - 3 sum, 4 copies, 5 multiplies
-constexpr int kFewMaxStages = 16;
+constexpr int kFewMaxStages = 16, kFewMaxSplits = 8, kFewChunk = 16;
 
 template <int T>
 struct Few {
@@ -330,8 +355,8 @@ __global__ void __launch_bounds__(kFewThreads, T >= 128 ? 1 : 2)
   constexpr int kChunk = T < 32 ? 16 : 32;
   unsigned char* smem = rmsb_dyn_smem + ((1024u - (smem_u32(rmsb_dyn_smem) & 1023u)) & 1023u);
   FewBars* bars = reinterpret_cast<FewBars*>(smem + pl.ring_bytes);
-  float* row_scales = reinterpret_cast<float*>(bars + 1);  // [2][T]: of the rows of a
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* row_scales = reinterpret_cast<float*>(bars + 1);  // [2][kFewChunk][T]: of the rows of a
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = static_cast<int>(blockIdx.x % pl.splits);
   const int64_t tile = blockIdx.x / pl.splits;
   const int tn = static_cast<int>(tile % pl.tiles_n);
@@ -365,48 +390,50 @@ __global__ void __launch_bounds__(kFewThreads, T >= 128 ? 1 : 2)
   float2 acc[T / 2];
   const int64_t n = static_cast<int64_t>(tn) * kBlock + threadIdx.x;  // warps 0 - 3: this thread's row of b
   if (warp == 4) {
-    int u = 0;
-    bool ok = true;
-    for (int g = g0; ok && g < g1; ++g, ++u) {
-      const int s = u % pl.stages;
-      if (u >= pl.stages)
-        ok = __all_sync(0xffffffffu, mbar_wait_warp(&bars->empty[s], static_cast<uint32_t>(u / pl.stages - 1) & 1u,
-                                                    kSiteMmEmpty));
+    int st = 0;
+    uint32_t pass = 0;
+    for (int g = g0; g < g1; ++g) {
+      const bool ok = __all_sync(0xffffffffu, mbar_spin_warp(&bars->empty[st], pass ^ 1u, kSiteMmEmpty));
       if (!ok) break;
-      if (lane == 0) {
-        unsigned char* at = smem + s * F::kStageBytes;
-        mbar_arrive_expect_tx(&bars->full[s], F::kStageBytes);
-        tile_load<false>(at, &map_b, g * kTileK, tn * kBlock, &bars->full[s]);
-        tile_load<false>(at + kTileBytes, &map_a, g * kTileK, static_cast<int>(t0), &bars->full[s]);
+      if (elect_one()) {
+        unsigned char* at = smem + st * F::kStageBytes;
+        mbar_arrive_expect_tx(&bars->full[st], F::kStageBytes);
+        tile_load<false>(at, &map_b, g * kTileK, tn * kBlock, &bars->full[st]);
+        tile_load<false>(at + kTileBytes, &map_a, g * kTileK, static_cast<int>(t0), &bars->full[st]);
       }
       __syncwarp();
+      if (++st == pl.stages) {
+        st = 0;
+        pass ^= 1u;
+      }
     }
     if (lane == 0 && abort_requested())
-      for (int j = max(0, u - pl.stages); j < u; ++j)
-        mbar_wait(&bars->full[j % pl.stages], static_cast<uint32_t>(j / pl.stages) & 1u, kSiteDrain, false);
-    for (int j = max(0, u - pl.stages); j < u; ++j)
-      mbar_wait_warp(&bars->empty[j % pl.stages], static_cast<uint32_t>(j / pl.stages) & 1u, kSiteMmEmpty);
+      for (int i = 0; i < pl.stages; ++i) mbar_wait(&bars->full[i], i < st ? pass : pass ^ 1u, kSiteDrain, false);
+    for (int i = 0; i < pl.stages; ++i) mbar_spin_warp(&bars->empty[i], i < st ? pass : pass ^ 1u, kSiteMmEmpty);
   } else if (warp == 5) {
     constexpr uint32_t idesc = product_desc(kBlock, T);
-    int u = 0;
-    bool ok = true;
-    for (int g = g0; ok && g < g1; ++g, ++u) {
-      const int s = u % pl.stages, d = u % F::kSums;
-      if (u >= F::kSums)
-        ok = mbar_wait_warp(&bars->sum_empty[d], static_cast<uint32_t>(u / F::kSums - 1) & 1u, kSiteMmSumEmpty);
-      ok = mbar_wait_warp(&bars->full[s], static_cast<uint32_t>(u / pl.stages) & 1u, kSiteMmFull) && ok;
+    int st = 0;
+    uint32_t pass = 0, u = 0;
+    for (int g = g0; g < g1; ++g, ++u) {
+      const uint32_t d = u % F::kSums;
+      bool ok = mbar_spin_warp(&bars->full[st], pass, kSiteMmFull);
+      ok = mbar_spin_warp(&bars->sum_empty[d], ((u / F::kSums) & 1u) ^ 1u, kSiteMmSumEmpty) && ok;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tmem_fence_after_sync();
-      if (lane == 0) {
-        const uint32_t at = smem_u32(smem + s * F::kStageBytes);
+      if (elect_one()) {
+        const uint32_t at = smem_u32(smem + st * F::kStageBytes);
         const uint64_t a = operand_desc(at), b = operand_desc(at + kTileBytes);
 #pragma unroll
         for (int k = 0; k < kTileK / 32; ++k) mma_e4m3<false>(tmem + d * T, a + 2 * k, b + 2 * k, idesc, k > 0);
-        mma_commit<false>(&bars->empty[s]);
+        mma_commit<false>(&bars->empty[st]);
         mma_commit<false>(&bars->sum[d]);
       }
       __syncwarp();
+      if (++st == pl.stages) {
+        st = 0;
+        pass ^= 1u;
+      }
     }
     if (abort_requested()) {
       if (lane == 0) {
@@ -417,45 +444,76 @@ __global__ void __launch_bounds__(kFewThreads, T >= 128 ? 1 : 2)
     }
   } else {
     const uint32_t from = tmem + (static_cast<uint32_t>(warp) << 21);
-    const int64_t t = t0 + threadIdx.x;
-    const bool b_live = n < p.n, a_live = threadIdx.x < T && t < p.m;
-    const float* sa = p.sa + t * p.sa_row;
-    const float* sb = sb_of(p, n);
-    auto load_a = [&](int g) { return a_live && g < g1 ? ld1(sa + g * p.sa_group) : 0.f; };
-    auto load_b = [&](int g) { return b_live && g < g1 ? ld1(sb + g * p.sb_group) : 0.f; };
-    float a0 = load_a(g0), a1 = load_a(g0 + 1), b0 = load_b(g0), b1 = load_b(g0 + 1);
+    const bool b_live = n < p.n;
+    const float* sb = sb_of(p, n) + g0 * p.sb_group;
+    auto next_b = [&](int g) {
+      const float v = b_live && g < g1 ? ld1(sb) : 0.f;
+      sb += p.sb_group;
+      return v;
+    };
+    float b0 = next_b(g0), b1 = next_b(g0 + 1);  // two groups ahead
 #pragma unroll
     for (int i = 0; i < T / 2; ++i) acc[i] = make_float2(0.f, 0.f);
-    int u = 0;
-    for (int g = g0; g < g1; ++g, ++u) {
-      const int d = u % F::kSums;
-      const float s = b0;
-      float* rows = row_scales + (u & 1) * T;
-      if (threadIdx.x < T) rows[threadIdx.x] = a0;
-      a0 = a1;
-      b0 = b1;
-      a1 = load_a(g + 2);
-      b1 = load_b(g + 2);
+    // a's scales, kFewChunk groups of T rows at a time, a chunk ahead in registers: thread i has
+    // row i % T of groups i / T, i / T + 128 / T, ...
+    float ahead[kFewChunk * T / 128];
+    auto fetch = [&](int c0) {
+#pragma unroll
+      for (int j = 0; j < kFewChunk * T / 128; ++j) {
+        const int i = threadIdx.x + j * 128, g = c0 + i / T;
+        const int64_t t = t0 + i % T;
+        ahead[j] = g < g1 && t < p.m ? ld1(p.sa + t * p.sa_row + g * p.sa_group) : 0.f;
+      }
+    };
+    fetch(g0);
+    int d = 0, buffer = 0;
+    uint32_t pass = 0;
+    for (int c0 = g0; c0 < g1; c0 += kFewChunk, buffer ^= 1) {
+      const int c1 = min(c0 + kFewChunk, g1);
+      float* scales = row_scales + buffer * (kFewChunk * T);
+#pragma unroll
+      for (int j = 0; j < kFewChunk * T / 128; ++j) scales[threadIdx.x + j * 128] = ahead[j];
+      fetch(c0 + kFewChunk);
       __syncwarp();
       named_barrier(1, 128);
-      mbar_wait_warp(&bars->sum[d], static_cast<uint32_t>(u / F::kSums) & 1u, kSiteMmSum);
-      __syncwarp();
-      tmem_fence_after_sync();
+      for (int g = c0; g < c1; ++g) {
+        const float s = b0;
+        const float* rows = scales + (g - c0) * T;
+        b0 = b1;
+        b1 = next_b(g + 2);
+        mbar_spin_warp(&bars->sum[d], pass, kSiteMmSum);
+        __syncwarp();
+        tmem_fence_after_sync();
+        float2 v[T > 64 ? 1 : T / kChunk][kChunk / 2];
+        if constexpr (T <= 64) {
 #pragma unroll
-      for (int c = 0; c < T; c += kChunk) {
-        float2 v[kChunk / 2];
-        tmem_ld(from + d * T + c, v);
-        tmem_landed(v);
-        if (c + kChunk == T) {
-          tmem_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->sum_empty[d]);
+          for (int c = 0; c < T / kChunk; ++c) tmem_ld(from + d * T + c * kChunk, v[c]);
+#pragma unroll
+          for (int c = 0; c < T / kChunk; ++c) tmem_landed(v[c]);
         }
 #pragma unroll
-        for (int i = 0; i < kChunk / 2; i += 2) {
-          const float4 r = *reinterpret_cast<const float4*>(rows + c + 2 * i);
-          acc[c / 2 + i] = fma2(mul2(v[i], make_float2(r.x, r.y)), splat2(s), acc[c / 2 + i]);
-          acc[c / 2 + i + 1] = fma2(mul2(v[i + 1], make_float2(r.z, r.w)), splat2(s), acc[c / 2 + i + 1]);
+        for (int c = 0; c < T / kChunk; ++c) {
+          float2(&x)[kChunk / 2] = v[T > 64 ? 0 : c];
+          if constexpr (T > 64) {
+            tmem_ld(from + d * T + c * kChunk, x);
+            tmem_landed(x);
+          }
+          if (c == (T > 64 ? T / kChunk - 1 : 0)) {
+            tmem_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->sum_empty[d]);
+          }
+#pragma unroll
+          for (int i = 0; i < kChunk / 2; i += 2) {
+            const float4 r = *reinterpret_cast<const float4*>(rows + c * kChunk + 2 * i);
+            float2* to = acc + c * (kChunk / 2) + i;
+            to[0] = fma2(mul2(x[i], make_float2(r.x, r.y)), splat2(s), to[0]);
+            to[1] = fma2(mul2(x[i + 1], make_float2(r.z, r.w)), splat2(s), to[1]);
+          }
+        }
+        if (++d == F::kSums) {
+          d = 0;
+          pass ^= 1u;
         }
       }
     }
@@ -483,14 +541,24 @@ __global__ void __launch_bounds__(kFewThreads, T >= 128 ? 1 : 2)
   if (warp == 5) tmem_dealloc_warp(tmem, F::kTmem);
   if (pl.splits == 1) return;
   cluster_sync_all();
-  if (warp < 4) {
-    const float bias = p.bias && n < p.n ? load1_rt(p.bias, p.bias_dt, n) : 0.f;
-    for (int i = rank; i < T && t0 + i < p.m; i += pl.splits) {
-      const uint32_t at = smem_u32(smem) + static_cast<uint32_t>(i * kBlock + threadIdx.x) * 4;
-      float sum = 0.f;
-      for (int r = 0; r < pl.splits; ++r) sum += ld_peer(map_peer(at, r));
-      if (n < p.n) store1_rt(p.out, p.out_dt, (t0 + i) * p.n + n, sum + bias);
+  // Row i of the result is CTA i % splits's, a warp a row, four columns a lane; the partial sums
+  // are added in the order of the CTAs.
+  for (int i = rank + warp * pl.splits; i < T && t0 + i < p.m; i += kFewThreads / 32 * pl.splits) {
+    const uint32_t at = smem_u32(smem) + static_cast<uint32_t>(i * kBlock + lane * 4) * 4;
+    float4 part[kFewMaxSplits];
+#pragma unroll
+    for (int r = 0; r < kFewMaxSplits; ++r) part[r] = r < pl.splits ? ld_peer4(map_peer(at, r)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 sum = part[0];
+#pragma unroll
+    for (int r = 1; r < kFewMaxSplits; ++r) {
+      sum.x += part[r].x; sum.y += part[r].y; sum.z += part[r].z; sum.w += part[r].w;
     }
+    const int64_t col = static_cast<int64_t>(tn) * kBlock + lane * 4;
+    const float out[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (col + k < p.n)
+        store1_rt(p.out, p.out_dt, (t0 + i) * p.n + col + k, out[k] + (p.bias ? load1_rt(p.bias, p.bias_dt, col + k) : 0.f));
   }
   cluster_sync_all();
 }

@@ -16,9 +16,9 @@ int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
 int check(const rmsnorm_b200_block_quant_args* a) {
   if (!a || a->rows < 0 || a->cols < 1 || !valid_dt(a->x_dtype)) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
   if (a->block_rows != 1 && a->block_rows != kBlock) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
-  if (!a->q && !a->q_t && !a->column_sums) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
   if (a->column_sums && !valid_dt(a->column_sums_dtype)) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
   if (a->rows == 0) return RMSNORM_B200_OK;
+  if (!a->q && !a->q_t && !a->column_sums) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
   if (!a->x || (a->q && !a->scales) || (a->q_t && !a->scales_t)) return RMSNORM_B200_ERR_INVALID_ARGUMENT;
   if (a->x_row_stride < 0 || (a->q && a->q_row_stride < a->cols) || (a->q_t && a->q_t_row_stride < a->rows) ||
       a->scale_row_stride < 0 || a->scale_group_stride < 0)

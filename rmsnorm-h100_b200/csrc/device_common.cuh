@@ -269,20 +269,28 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
   return mbar_wait<kClusterScope>(bar, parity, where);
 }
 
-// The same without a call, for loops that hold nearly all registers there are.
-template <bool kClusterScope = false>
-__device__ __forceinline__ bool mbar_spin_warp(uint64_t* bar, uint32_t parity, int where) {
-  __syncwarp();
-  if (kClusterScope ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  while (!(kClusterScope ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity))) {
+// The same without a call, and with the status word and the clock looked at after every 64
+// probes only (a look at the status word is a load from L2): for waits that end within some
+// hundred cycles again and again. mbar_spin_one is for a role that one lane of a warp plays from
+// its first wait to its last, while the others stay at the warp's next barrier.
+__device__ __forceinline__ bool mbar_spin_one(uint64_t* bar, uint32_t parity, int where) {
+  uint64_t t0 = 0;
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
     if (abort_requested()) return false;
-    if (globaltimer_ns() - t0 > g_wait_timeout_ns) {
+    const uint64_t now = globaltimer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > g_wait_timeout_ns) {
       record_error(RMSNORM_B200_ERR_DEVICE_TIMEOUT, where);
       return false;
     }
   }
-  return true;
+}
+__device__ __forceinline__ bool mbar_spin_warp(uint64_t* bar, uint32_t parity, int where) {
+  __syncwarp();
+  return mbar_spin_one(bar, parity, where);
 }
 
 // ---------------------------------------------------------------------------------------

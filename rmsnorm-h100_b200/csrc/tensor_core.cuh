@@ -27,6 +27,14 @@ __host__ __device__ constexpr uint32_t product_desc(int m, int n) {
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// One lane of a whole warp, always the same. Unlike a test of the lane's number it tells the
+// compiler that a single thread follows, whose operands can lie in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
+}
+
 // One thread of the CTA (of the pair): D (+)= A B^T over 32 values of k.
 template <bool kPair>
 __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
@@ -83,13 +91,16 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
 
 // One arrival at the barrier of CTA `rank` of the cluster.
 __device__ __forceinline__ void mbar_arrive_peer(uint64_t* bar, uint32_t rank) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_peer(smem_u32(bar), rank))
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(map_peer(smem_u32(bar), rank))
                : "memory");
 }
 
-__device__ __forceinline__ float ld_peer(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_peer4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 

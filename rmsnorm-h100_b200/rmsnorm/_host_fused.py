@@ -140,7 +140,7 @@ def power_scales(most: torch.Tensor) -> torch.Tensor:
     """The smallest power of two, at least 2^-126, that brings each magnitude to 448 =
     0.875 * 2^9 or below; infinity and NaN stay."""
     part, exponent = torch.frexp(most)
-    exponent = exponent - 9 + (part > 0.875).to(torch.int32)
+    exponent = torch.where(most == 0, -126, exponent - 9 + (part > 0.875).to(torch.int32))
     power = (exponent.clamp_min(-126) + 127 << 23).view(torch.float32)
     return torch.where(most.isfinite(), power, most)
 
