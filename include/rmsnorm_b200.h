@@ -511,8 +511,8 @@ typedef struct rmsnorm_b200_cache_args {
 } rmsnorm_b200_cache_args;
 
 /* Writes token t's heads into slot slots[t] = page * page_size + place in the page:
- *   scale = max(max |x| / Q, 2^-126), Q = 448 (E4M3) or 127 (I8); q = x / scale rounded to
- *   nearest, ties to even. NaN and infinities as in rmsnorm_b200_quant_fwd.
+ *   scale = max(max |x| / Q, 2^-126), Q = 448 (E4M3) or 127 (I8); q = Q x / max |x| (or
+ *   x 2^126) rounded to nearest, ties to even. NaN and infinities as in rmsnorm_b200_quant_fwd.
  * A negative slot leaves its token out. A slot beyond the cache leaves it out too and records
  * RMSNORM_B200_ERR_INVALID_ARGUMENT (site 11) for rmsnorm_b200_device_status. Slots named more
  * than once hold bytes of any of their tokens. */

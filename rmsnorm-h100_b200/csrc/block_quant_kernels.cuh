@@ -2,6 +2,8 @@
 // 128 x 128 blocks, of x and of x transposed.
 #pragma once
 
+#include <type_traits>
+
 #include "block_scale.cuh"
 
 namespace rmsb200 {
@@ -100,15 +102,93 @@ __global__ void __launch_bounds__(256) quant_groups_kernel(const BlockQuantParam
   }
 }
 
+// Eight values of a row as they are loaded: 4 registers, 8 for fp32. Magnitudes of 16-bit values
+// are compared as they are, two at a time: without the sign their bits order as unsigned integers,
+// infinity above the numbers and NaN above it.
+template <typename X>
+struct Held {
+  uint32_t w[4];
+  __device__ __forceinline__ float2 pair(int k) const {
+    if constexpr (std::is_same<X, __half>::value) return unpack_f16x2_pair(w[k]);
+    else return unpack_bf16x2_pair(w[k]);
+  }
+  __device__ __forceinline__ static uint32_t widen(uint32_t m) {  // a magnitude's bits in fp32
+    if constexpr (std::is_same<X, __half>::value)
+      return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+    else return m << 16;
+  }
+};
+template <>
+struct Held<float> {
+  float2 v[4];
+  __device__ __forceinline__ float2 pair(int k) const { return v[k]; }
+};
+
+template <typename X>
+__device__ __forceinline__ void load_held(const BlockQuantParams& p, int64_t row, int64_t col, Held<X>& h) {
+  const int64_t e = row * p.x_row + col;
+  const X* src = static_cast<const X*>(p.x) + e;
+  if (row < p.rows && p.vec_in && col + 8 <= p.cols) {
+    if constexpr (sizeof(X) == 4) {
+      Pair8<X>::load(src, h.v);
+    } else {
+      const uint4 u = RMSB_DBG_OK(src, 16, kDbgVecLoad) ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+      h.w[0] = u.x; h.w[1] = u.y; h.w[2] = u.z; h.w[3] = u.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const bool first = row < p.rows && col + 2 * k < p.cols, second = row < p.rows && col + 2 * k + 1 < p.cols;
+    if constexpr (sizeof(X) == 4) {
+      h.v[k] = make_float2(first ? ld1(src + 2 * k) : 0.f, second ? ld1(src + 2 * k + 1) : 0.f);
+    } else {
+      const uint16_t* bits = reinterpret_cast<const uint16_t*>(src);
+      h.w[k] = (first ? ld1(bits + 2 * k) : 0u) | (second ? static_cast<uint32_t>(ld1(bits + 2 * k + 1)) << 16 : 0u);
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {  // of both halves
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// The largest magnitude (fp32 bits) of each of the thread's rows, over the 16 lanes they lie in.
+template <typename X>
+__device__ __forceinline__ void rows_most(const Held<X> (&h)[8], uint32_t (&most)[8]) {
+  if constexpr (sizeof(X) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most[i] = max16(octet_magnitude(h[i].v));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      uint32_t m[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t(&w)[4] = h[i + k].w;
+        m[k] = larger2(larger2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), larger2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+      }
+      // row i's in the low half, the next one's in the high half
+      uint32_t both = larger2(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) both = larger2(both, __shfl_xor_sync(0xffffffffu, both, o));
+      most[i] = Held<X>::widen(both & 0xffffu);
+      most[i + 1] = Held<X>::widen(both >> 16);
+    }
+  }
+}
+
 // One 128 x 128 tile a CTA, read once into registers: thread (warp w, lane l) holds rows
 // 16 w + 8 (l / 16) + 0 .. 7 and columns 8 (l % 16) + 0 .. 7. Rows' groups lie in 16 lanes of one
 // warp, columns' in all warps; the transposed bytes pass through shared memory, where the 8-byte
 // piece of rows 8 u .. 8 u + 7 of column c lies at place u ^ (c / 8) of the column, so that
 // neither side meets a bank twice.
 template <typename X, bool kBlocks>
-__global__ void __launch_bounds__(256, 2) quant_tiles_kernel(const BlockQuantParams p, uint32_t tiles_c) {
+__global__ void __launch_bounds__(256, sizeof(X) == 4 ? 2 : 3) quant_tiles_kernel(const BlockQuantParams p, uint32_t tiles_c) {
   __shared__ __align__(16) unsigned char turned[kBlock * kBlock];
-  __shared__ uint32_t col_most[8][kBlock];
+  __shared__ __align__(16) uint32_t col_most[8][kBlock];  // 16-bit values: two columns a word
   __shared__ float col_sum[8][kBlock];
   pdl_launch_dependents();
   pdl_wait();
@@ -116,34 +196,28 @@ __global__ void __launch_bounds__(256, 2) quant_tiles_kernel(const BlockQuantPar
   const uint32_t tile_r = blockIdx.x / tiles_c, tile_c = blockIdx.x - tile_r * tiles_c;
   const int64_t row0 = static_cast<int64_t>(tile_r) * kBlock + warp * 16 + half * 8;
   const int64_t col0 = static_cast<int64_t>(tile_c) * kBlock, col = col0 + c8 * 8;
-  float2 v[8][4];
+  Held<X> h[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (row0 + i < p.rows) {
-      load_octet<X>(p, (row0 + i) * p.x_row, col, v[i]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[i][k] = make_float2(0.f, 0.f);
-    }
-  }
+  for (int i = 0; i < 8; ++i) load_held<X>(p, row0 + i, col, h[i]);
   if (p.sum_part) {
-    float2 sum[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      sum[k] = v[0][k];
+      float2 sum = h[0].pair(k);
 #pragma unroll
-      for (int i = 1; i < 8; ++i) sum[k] = add2(sum[k], v[i][k]);
-      sum[k].x += __shfl_xor_sync(0xffffffffu, sum[k].x, 16);
-      sum[k].y += __shfl_xor_sync(0xffffffffu, sum[k].y, 16);
-      if (half == 0) *reinterpret_cast<float2*>(&col_sum[warp][c8 * 8 + 2 * k]) = sum[k];
+      for (int i = 1; i < 8; ++i) sum = add2(sum, h[i].pair(k));
+      sum.x += __shfl_xor_sync(0xffffffffu, sum.x, 16);
+      sum.y += __shfl_xor_sync(0xffffffffu, sum.y, 16);
+      if (half == 0) *reinterpret_cast<float2*>(&col_sum[warp][c8 * 8 + 2 * k]) = sum;
     }
   }
   float inv_t[8];  // of this thread's columns
+  uint32_t most[8];
+  if (kBlocks || p.q) rows_most<X>(h, most);
   if (kBlocks) {
-    float most = 0.f;
+    uint32_t m = most[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) most = largest8(most, v[i]);
-    const uint32_t m = __reduce_max_sync(0xffffffffu, magnitude(most));
+    for (int i = 1; i < 8; ++i) m = max(m, most[i]);
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
     if (lane == 0) col_most[warp][0] = m;
     __syncthreads();
     uint32_t all = col_most[0][0];
@@ -160,44 +234,71 @@ __global__ void __launch_bounds__(256, 2) quant_tiles_kernel(const BlockQuantPar
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) inv_t[k] = inv;
-    if (p.q) {
+  }
+  if (p.q) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (row0 + i < p.rows) store_octet(p, row0 + i, col, pack_octet(v[i], inv));
-    }
-  } else {
-    if (p.q) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t s = power_scale(max16(octet_magnitude(v[i])));
-        if (row0 + i >= p.rows) continue;
+    for (int i = 0; i < 8; ++i) {
+      if (row0 + i >= p.rows) continue;
+      float inv = inv_t[0];
+      if (!kBlocks) {
+        const uint32_t s = power_scale(most[i]);
+        inv = power_inverse(s);
         if (c8 == 0) st1(p.scales + (row0 + i) * p.scale_row + tile_c * p.scale_group, __uint_as_float(s));
-        store_octet(p, row0 + i, col, pack_octet(v[i], power_inverse(s)));
       }
+      const float2 v[4] = {h[i].pair(0), h[i].pair(1), h[i].pair(2), h[i].pair(3)};
+      store_octet(p, row0 + i, col, pack_octet(v, inv));
     }
-    if (p.q_t) {
+  }
+  if (!kBlocks && p.q_t) {
+    if constexpr (sizeof(X) == 4) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        float most = 0.f;
+        float top = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i += 2)
-          most = max3_abs(most, k & 1 ? v[i][k >> 1].y : v[i][k >> 1].x, k & 1 ? v[i + 1][k >> 1].y : v[i + 1][k >> 1].x);
-        uint32_t m = magnitude(most);
+          top = max3_abs(top, k & 1 ? h[i].v[k >> 1].y : h[i].v[k >> 1].x, k & 1 ? h[i + 1].v[k >> 1].y : h[i + 1].v[k >> 1].x);
+        uint32_t m = magnitude(top);
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
         if (half == 0) col_most[warp][c8 * 8 + k] = m;
       }
-      __syncthreads();
+    } else {
+      uint32_t m[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        m[k] = h[0].w[k] & 0x7fff7fffu;
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m[k] = larger2(m[k], h[i].w[k] & 0x7fff7fffu);
+        m[k] = larger2(m[k], __shfl_xor_sync(0xffffffffu, m[k], 16));
+      }
+      if (half == 0) *reinterpret_cast<uint4*>(&col_most[warp][c8 * 4]) = make_uint4(m[0], m[1], m[2], m[3]);
+    }
+    __syncthreads();
+    uint32_t m[8];
+    if constexpr (sizeof(X) == 4) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        uint32_t m = col_most[0][c8 * 8 + k];
+        m[k] = col_most[0][c8 * 8 + k];
 #pragma unroll
-        for (int w = 1; w < 8; ++w) m = max(m, col_most[w][c8 * 8 + k]);
-        const uint32_t s = power_scale(m);
-        inv_t[k] = power_inverse(s);
-        if (warp == 0 && half == 0 && col + k < p.cols) {
-          const int64_t groups_t = (p.rows + kBlock - 1) / kBlock;
-          st1(p.scales_t + (col + k) * groups_t + tile_r, __uint_as_float(s));
-        }
+        for (int w = 1; w < 8; ++w) m[k] = max(m[k], col_most[w][c8 * 8 + k]);
+      }
+    } else {
+      uint4 t = *reinterpret_cast<const uint4*>(&col_most[0][c8 * 4]);
+#pragma unroll
+      for (int w = 1; w < 8; ++w) {
+        const uint4 o = *reinterpret_cast<const uint4*>(&col_most[w][c8 * 4]);
+        t = make_uint4(larger2(t.x, o.x), larger2(t.y, o.y), larger2(t.z, o.z), larger2(t.w, o.w));
+      }
+      const uint32_t two[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m[k] = Held<X>::widen(k & 1 ? two[k / 2] >> 16 : two[k / 2] & 0xffffu);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t s = power_scale(m[k]);
+      inv_t[k] = power_inverse(s);
+      if (warp == 0 && half == 0 && col + k < p.cols) {
+        const int64_t groups_t = (p.rows + kBlock - 1) / kBlock;
+        st1(p.scales_t + (col + k) * groups_t + tile_r, __uint_as_float(s));
       }
     }
   }
@@ -207,9 +308,10 @@ __global__ void __launch_bounds__(256, 2) quant_tiles_kernel(const BlockQuantPar
     for (int k = 0; k < 8; ++k) {
       float2 t[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        t[i] = k & 1 ? make_float2(v[2 * i][k >> 1].y, v[2 * i + 1][k >> 1].y)
-                     : make_float2(v[2 * i][k >> 1].x, v[2 * i + 1][k >> 1].x);
+      for (int i = 0; i < 4; ++i) {
+        const float2 a = h[2 * i].pair(k >> 1), b = h[2 * i + 1].pair(k >> 1);
+        t[i] = k & 1 ? make_float2(a.y, b.y) : make_float2(a.x, b.x);
+      }
       *reinterpret_cast<uint2*>(turned + (c8 * 8 + k) * kBlock + ((u ^ c8) << 3)) = pack_octet(t, inv_t[k]);
     }
   }

@@ -45,6 +45,16 @@ void add_ranges(Ranges* r, const rmsnorm_b200_cache_args* c, const CacheSide& s,
   r->add(s.x, ((tokens - 1) * s.x_token + (c->heads - 1) * s.x_head + c->head_dim) * x_bytes);
 }
 
+void set_sizes(CacheParams* p, const rmsnorm_b200_cache_args* c) {
+  constexpr int64_t kMost = int64_t{1} << 31;
+  p->page_size = c->page_size;
+  p->heads = c->heads;
+  p->head_dim = c->head_dim;
+  p->by_heads = divisor_of(static_cast<uint32_t>(c->heads));
+  p->by_page = divisor_of(static_cast<uint32_t>(c->page_size));
+  p->small = p->tokens < kMost / c->heads && c->pages < kMost / c->page_size;
+}
+
 template <bool kWrite, typename X, typename Q, int kItems>
 CacheKernel pick_lanes(int lanes) {
   if constexpr (kWrite)
@@ -126,7 +136,7 @@ int write(const rmsnorm_b200_cache_args* c, const rmsnorm_b200_cache_write_args*
   p.side[1] = side_of(c, c->v, a->v.data, a->v.token_stride, a->v.head_stride, xb);
   p.pages = c->pages; p.tokens = a->tokens;
   p.slots = a->slots; p.slots_64bit = a->slots_64bit != 0;
-  p.page_size = c->page_size; p.heads = c->heads; p.head_dim = c->head_dim;
+  set_sizes(&p, c);
   Ranges ranges;
   for (const CacheSide& s : p.side) add_ranges(&ranges, c, s, a->tokens, xb);
   ranges.add(a->slots, a->tokens * (p.slots_64bit ? 8 : 4));
@@ -161,7 +171,7 @@ int read(const rmsnorm_b200_cache_args* c, const rmsnorm_b200_cache_read_args* a
   p.table_width = a->table_width; p.table_stride = a->table_stride;
   p.sequences = static_cast<int32_t>(a->sequences);
   p.zero_rest = a->zero_rest != 0;
-  p.page_size = c->page_size; p.heads = c->heads; p.head_dim = c->head_dim;
+  set_sizes(&p, c);
   Ranges ranges;
   for (const CacheSide& s : p.side) add_ranges(&ranges, c, s, a->tokens, xb);
   ranges.add(a->starts, (a->sequences + 1) * 4);

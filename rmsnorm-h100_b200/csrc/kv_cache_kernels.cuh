@@ -11,6 +11,22 @@ namespace rmsb200 {
 constexpr int kSiteCacheSlot = 11;  // a slot beyond the cache
 constexpr int kSiteCachePage = 12;  // a row whose page the cache or the table does not have
 
+// Division of numbers below 2^31 by a divisor known on the host: n / d = n m >> (31 + l) with
+// l = ceil(log2 d) and m = ceil(2^(31 + l) / d) (Granlund and Montgomery: Division by invariant
+// integers using multiplication, 1994). The compiler's own take 20 instructions in 32 bits and
+// over 100 in 64, of which every lane of a head makes two: half the time of a write.
+struct Divisor {
+  uint32_t m, shift, d;
+};
+inline Divisor divisor_of(uint32_t d) {
+  uint32_t l = 0;
+  while ((uint64_t{1} << l) < d) ++l;
+  return {static_cast<uint32_t>(((uint64_t{1} << (31 + l)) + d - 1) / d), 31 + l, d};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t n, const Divisor& d) {
+  return static_cast<uint32_t>((static_cast<uint64_t>(n) * d.m) >> d.shift);
+}
+
 struct CacheSide {  // k or v
   unsigned char* data;
   int64_t page, slot, head;
@@ -28,8 +44,10 @@ struct CacheParams {
   const int32_t* table;
   const int32_t* starts;
   int64_t table_width, table_stride;
+  Divisor by_heads, by_page;
   int32_t sequences, page_size, heads, head_dim;
   bool slots_64bit, zero_rest;
+  bool small;  // heads of all tokens, and slots of the cache, are fewer than 2^31
 };
 
 constexpr int kCacheThreads = 256;
@@ -41,24 +59,27 @@ __device__ __forceinline__ float cache_load1(const void* base, int64_t e) {
   return static_cast<float>(*p);
 }
 
-// Item i of `items` is head i % heads of token i / heads.
-__device__ __forceinline__ void cache_item(int64_t i, int32_t heads, bool small, int64_t* token, int32_t* head) {
-  if (small) {
-    const uint32_t t = static_cast<uint32_t>(i) / static_cast<uint32_t>(heads);
+// Item i is head i % heads of token i / heads.
+__device__ __forceinline__ void cache_item(const CacheParams& p, int64_t i, int64_t* token, int32_t* head) {
+  if (p.small) {
+    const uint32_t t = divide(static_cast<uint32_t>(i), p.by_heads);
     *token = t;
-    *head = static_cast<int32_t>(static_cast<uint32_t>(i) - t * static_cast<uint32_t>(heads));
+    *head = static_cast<int32_t>(static_cast<uint32_t>(i) - t * p.by_heads.d);
   } else {
-    *token = i / heads;
-    *head = static_cast<int32_t>(i - *token * heads);
+    *token = i / p.heads;
+    *head = static_cast<int32_t>(i - *token * p.heads);
   }
 }
 
 // A head takes kLanes lanes of 8 values each; every one of them has kItems heads of k or of v
 // (blockIdx.y) in flight.
-//   scale = max(max |x| / Q, 2^-126), q = round(x / scale)
-// x / scale is divided, not multiplied by an inverse: 16-bit x lie on ties of q far more often
-// than chance has it (where max |x| is a power of two times Q, on every one), and the quotient's
-// own rounding decides them the same way everywhere.
+//   scale = max(max |x| / Q, 2^-126), q = round(Q x / max |x|)
+// Q x is exact for 16-bit x, and so is the quotient wherever it is a tie of q: 16-bit x lie on
+// ties far more often than chance has it (one in 700 of normal bf16 values), which x / scale, or x
+// times an inverse, would decide by the rounding of the scale. The quotient is the product with
+// the inverse and one correction by its remainder (Markstein: Computation of elementary functions
+// on the IBM RISC System/6000 processor, 1990), of numbers brought to max |x| in [1, 8) by a power
+// of two, so that the remainder is exact. A head whose scale is 2^-126 takes x 2^126.
 template <typename X, typename Q, int kLanes, int kItems>
 __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid_constant__ CacheParams p) {
   pdl_launch_dependents();
@@ -67,7 +88,6 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid
   constexpr int kGroups = kCacheThreads / kLanes;
   const int lane = threadIdx.x % kLanes, col = lane * 8;
   const int64_t items = p.tokens * p.heads;
-  const bool small = items < (int64_t{1} << 32);
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (kGroups * kItems) + threadIdx.x / kLanes;
   float2 v[kItems][4];
   int64_t slot[kItems];
@@ -80,7 +100,7 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid
     for (int k = 0; k < 4; ++k) v[j][k] = make_float2(0.f, 0.f);
     if (i >= items) continue;
     int64_t token;
-    cache_item(i, p.heads, small, &token, &head[j]);
+    cache_item(p, i, &token, &head[j]);
     slot[j] = p.slots_64bit ? ld1(static_cast<const int64_t*>(p.slots) + token)
                             : ld1(static_cast<const int32_t*>(p.slots) + token);
     const int64_t e = token * side.x_token + head[j] * side.x_head + col;
@@ -100,18 +120,28 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     if (slot[j] < 0) continue;
-    const int64_t page = slot[j] / p.page_size;
-    if (page >= p.pages) {
+    if (slot[j] >= p.pages * p.page_size) {
       if (lane == 0) record_data_error(RMSNORM_B200_ERR_INVALID_ARGUMENT, kSiteCacheSlot);
       continue;
     }
+    const int64_t page = p.small ? divide(static_cast<uint32_t>(slot[j]), p.by_page) : slot[j] / p.page_size;
     const int64_t place = slot[j] - page * p.page_size;
-    const float s0 = __fdiv_rn(__uint_as_float(most), std::is_same<Q, I8>::value ? 127.f : 448.f);
-    const float s = s0 < 1.17549435e-38f ? 1.17549435e-38f : s0;  // NaN stays
-    if (lane == 0) st1(side.scales + page * side.s_page + place * side.s_slot + head[j] * side.s_head, s);
+    constexpr float kTop = std::is_same<Q, I8>::value ? 127.f : 448.f;
+    const float largest = __uint_as_float(most), s0 = __fdiv_rn(largest, kTop);
+    const bool least = s0 < 1.17549435e-38f;  // NaN is not
+    if (lane == 0)
+      st1(side.scales + page * side.s_page + place * side.s_slot + head[j] * side.s_head, least ? 1.17549435e-38f : s0);
     if (col >= p.head_dim) continue;
+    const int e = static_cast<int>(most >> 23);
+    const float power = __uint_as_float(static_cast<uint32_t>(max(254 - e, 1)) << 23);
+    const float times = least ? 8.5070592e37f : kTop * power;  // 2^126
+    const float by = least ? 1.f : e < 255 ? largest * power : 0.f;  // infinity: no remainder
+    const float inv = __frcp_rn(!least && e == 255 ? largest : by);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[j][k] = make_float2(__fdiv_rn(v[j][k].x, s), __fdiv_rn(v[j][k].y, s));
+    for (int k = 0; k < 4; ++k) {
+      const float2 n = mul2(v[j][k], splat2(times)), q = mul2(n, splat2(inv));
+      v[j][k] = fma2(fma2(q, splat2(-by), n), splat2(inv), q);
+    }
     const uint2 b = make_uint2(Q::pack4(v[j][0], v[j][1]), Q::pack4(v[j][2], v[j][3]));
     unsigned char* dst = side.data + page * side.page + place * side.slot + head[j] * side.head + col;
     if (side.vec_q) {
@@ -160,11 +190,12 @@ __device__ __forceinline__ int2 cache_place(const CacheParams& p, int64_t token)
     if (token >= ld1(p.starts + mid)) lo = mid;
     else hi = mid;
   }
-  const int64_t at = token - ld1(p.starts + lo), column = at / p.page_size;
-  if (column >= p.table_width) return make_int2(kNowhere, 0);
+  // starts are 32 bits, and so are rows that lie before the last
+  const uint32_t at = static_cast<uint32_t>(token - ld1(p.starts + lo)), column = at / static_cast<uint32_t>(p.page_size);
+  if (static_cast<int64_t>(column) >= p.table_width) return make_int2(kNowhere, 0);
   const int32_t page = ld1(p.table + lo * p.table_stride + column);
   if (page < 0 || page >= p.pages) return make_int2(kNowhere, 0);
-  return make_int2(page, static_cast<int32_t>(at - column * p.page_size));
+  return make_int2(page, static_cast<int32_t>(at - column * static_cast<uint32_t>(p.page_size)));
 }
 
 // A head takes kLanes lanes of 8 values; every one of them has kItems heads of k and as many of v
@@ -177,11 +208,10 @@ __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const __grid_
   pdl_wait();
   const int lane = threadIdx.x % kLanes, col = lane * 8;
   const int64_t items = p.tokens * p.heads, begin = static_cast<int64_t>(blockIdx.x) * kPer;
-  const bool small = items < (int64_t{1} << 32);
   int64_t token0, token1;
   int32_t unused;
-  cache_item(begin, p.heads, small, &token0, &unused);
-  cache_item(min(begin + kPer, items) - 1, p.heads, small, &token1, &unused);
+  cache_item(p, begin, &token0, &unused);
+  cache_item(p, min(begin + kPer, items) - 1, &token1, &unused);
   if (token0 + threadIdx.x <= token1) {
     const int2 at = cache_place(p, token0 + threadIdx.x);
     if (at.x == kNowhere) record_data_error(RMSNORM_B200_ERR_INVALID_ARGUMENT, kSiteCachePage);
@@ -201,7 +231,7 @@ __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const __grid_
     if (i >= items || col >= p.head_dim) continue;
     int64_t token;
     int32_t head;
-    cache_item(i, p.heads, small, &token, &head);
+    cache_item(p, i, &token, &head);
     const int2 at = places[token - token0];
     if (at.x < 0) {
       s[j][0] = s[j][1] = at.x == kNowhere ? __int_as_float(0x7fc00000) : 0.f;
@@ -231,7 +261,7 @@ __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const __grid_
     if (i >= items || col >= p.head_dim) continue;
     int64_t token;
     int32_t head;
-    cache_item(i, p.heads, small, &token, &head);
+    cache_item(p, i, &token, &head);
     if (places[token - token0].x == kRest && !p.zero_rest) continue;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {

@@ -80,8 +80,8 @@ def cache_write(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, k_scales
     caches' dtype (float8_e4m3fn or int8; (pages, page_size, heads, head_dim), any strides but
     the last) and an fp32 scale for every head (k_scales, v_scales: (pages, page_size, heads)).
 
-    A scale is max |x| / 448 (e4m3) or / 127 (int8), at least 2^-126; q is x / scale rounded to
-    nearest even. A NaN makes its head's scale NaN, an infinity infinite.
+    A scale is max |x| / 448 (e4m3) or / 127 (int8), at least 2^-126; q is x over that quotient as
+    it is before it is rounded to fp32, rounded to nearest even. A NaN makes its head's scale NaN, an infinity infinite.
 
     slots (int32 or int64, k's leading shape) has each token's place, page * page_size + place
     in the page. A negative slot leaves its token out. One beyond the cache does too and, on

@@ -163,8 +163,11 @@ def block_values(q, scales, rows):
 def cache_write(x, cache, scales, page, place, top):
     """x [tokens, heads, head_dim] into (page, place)."""
     x = x.float()
-    s = (x.abs().amax(-1) / top).clamp_min(torch.finfo(torch.float32).tiny)
-    q = x / s[..., None]
+    most = x.abs().amax(-1, keepdim=True)
+    s = most / top
+    down = torch.where(most > 2.0**100, 2.0**-30, 1.0)
+    q = torch.where(s < 2.0**-126, x * 2.0**126, x * (top * down) / (most * down))
+    s = s.clamp_min(2.0**-126).squeeze(-1)
     if cache.dtype == torch.int8:
         q = torch.where(q.isnan(), 0.0, q).round()
     cache[page, place] = q.to(cache.dtype)

@@ -136,6 +136,31 @@ def test_write_slots_beyond_the_cache_are_left_out_and_told():
 
 
 @pytest.mark.parametrize("kept", [E4M3, I8])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_write_ties_go_to_even(kept, dtype):
+    """16-bit x: q is the number nearest to Q x / max |x| in exact arithmetic, ties to even."""
+    k = rand(4000, 2, 128, dtype=dtype, seed=5)
+    k[:1000] = k[:1000] * torch.exp2(torch.arange(1000, device=DEV) % 20 - 10.0)[:, None, None]
+    cache = new_cache(4000, 1, 2, 128, kept)
+    fused.cache_write(k, k, *cache, torch.arange(4000, device=DEV))
+    x = k.double()
+    most = x.abs().amax(-1, keepdim=True)
+    v = x * TOP[kept] / most  # a tie has few bits: 53 give it exactly, and keep what is none apart
+    want = v.round() if kept == I8 else ref.nearest_e4m3(v)
+    assert torch.equal(cache[0].view(4000, 2, 128).double(), want)
+
+
+@pytest.mark.parametrize("kept", [E4M3, I8])
+@pytest.mark.parametrize("power", [-135, -118, -100, 0, 100, 120])
+def test_write_at_the_ends_of_the_range(kept, power):
+    k = (rand(50, 1, 64, seed=6).double() * 2.0**power).float()
+    k[0, 0, 0], k[1, 0, 5] = torch.finfo(F32).max, -torch.finfo(F32).max
+    cache = new_cache(50, 1, 1, 64, kept)
+    fused.cache_write(k, k, *cache, torch.arange(50, device=DEV))
+    ref.check_cached(cache[0].view(50, 1, 64), cache[2].view(50, 1), k, TOP[kept])
+
+
+@pytest.mark.parametrize("kept", [E4M3, I8])
 def test_write_zeros_nan_and_infinity(kept):
     cache = new_cache(1, 8, 1, 64, kept)
     k = torch.zeros(5, 1, 64, device=DEV)
