@@ -50,9 +50,8 @@ void set_sizes(CacheParams* p, const rmsnorm_b200_cache_args* c) {
   p->page_size = c->page_size;
   p->heads = c->heads;
   p->head_dim = c->head_dim;
-  p->by_heads = divisor_of(static_cast<uint32_t>(c->heads));
   p->by_page = divisor_of(static_cast<uint32_t>(c->page_size));
-  p->small = p->tokens < kMost / c->heads && c->pages < kMost / c->page_size;
+  p->small = p->tokens < kMost / c->heads && c->pages < kMost / c->page_size;  // there are no more rounds than heads
 }
 
 template <bool kWrite, typename X, typename Q, int kItems>
@@ -88,12 +87,14 @@ std::string describe(const void* data) {
 }
 
 template <bool kWrite>
-int launch(UnitDevice* ud, const rmsnorm_b200_cache_args* c, const CacheParams& p, int dtype, cudaStream_t stream) {
+int launch(UnitDevice* ud, const rmsnorm_b200_cache_args* c, CacheParams& p, int dtype, cudaStream_t stream) {
   const int lanes = c->head_dim <= 64 ? 8 : c->head_dim <= 128 ? 16 : 32;
-  const int64_t items = p.tokens * p.heads;
-  // four heads in flight a lane, where that leaves two CTAs for every SM
-  const int each = items * lanes >= int64_t{8} * kCacheThreads * ud->sm_count ? 4 : 1;
-  const int64_t per = kCacheThreads / lanes * each, grid = (items + per - 1) / per;
+  // four heads of a token in flight a lane, where it has that many and that leaves two CTAs for
+  // every SM
+  const int each = c->heads >= 3 && p.tokens * p.heads * lanes >= int64_t{8} * kCacheThreads * ud->sm_count ? 4 : 1;
+  p.rounds = (c->heads + each - 1) / each;
+  p.by_rounds = divisor_of(static_cast<uint32_t>(p.rounds));
+  const int64_t per = kCacheThreads / lanes, grid = (p.tokens * p.rounds + per - 1) / per;
   if (grid >= int64_t{1} << 31) return RMSNORM_B200_ERR_UNSUPPORTED;
   const CacheKernel kernel = dtype == RMSNORM_B200_F32    ? pick<kWrite, float>(c->cache_dtype, lanes, each)
                              : dtype == RMSNORM_B200_BF16 ? pick<kWrite, __nv_bfloat16>(c->cache_dtype, lanes, each)

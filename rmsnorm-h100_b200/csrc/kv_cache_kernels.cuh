@@ -44,10 +44,11 @@ struct CacheParams {
   const int32_t* table;
   const int32_t* starts;
   int64_t table_width, table_stride;
-  Divisor by_heads, by_page;
+  Divisor by_rounds, by_page;  // rounds: of kItems heads, of a token
   int32_t sequences, page_size, heads, head_dim;
   bool slots_64bit, zero_rest;
-  bool small;  // heads of all tokens, and slots of the cache, are fewer than 2^31
+  int32_t rounds;
+  bool small;  // rounds of all tokens, and slots of the cache, are fewer than 2^31
 };
 
 constexpr int kCacheThreads = 256;
@@ -59,20 +60,21 @@ __device__ __forceinline__ float cache_load1(const void* base, int64_t e) {
   return static_cast<float>(*p);
 }
 
-// Item i is head i % heads of token i / heads.
-__device__ __forceinline__ void cache_item(const CacheParams& p, int64_t i, int64_t* token, int32_t* head) {
+// Unit i is round i % rounds of token i / rounds.
+__device__ __forceinline__ void cache_unit(const CacheParams& p, int64_t i, int64_t* token, int32_t* round) {
   if (p.small) {
-    const uint32_t t = divide(static_cast<uint32_t>(i), p.by_heads);
+    const uint32_t t = divide(static_cast<uint32_t>(i), p.by_rounds);
     *token = t;
-    *head = static_cast<int32_t>(static_cast<uint32_t>(i) - t * p.by_heads.d);
+    *round = static_cast<int32_t>(static_cast<uint32_t>(i) - t * p.by_rounds.d);
   } else {
-    *token = i / p.heads;
-    *head = static_cast<int32_t>(i - *token * p.heads);
+    *token = i / p.rounds;
+    *round = static_cast<int32_t>(i - *token * p.rounds);
   }
 }
 
-// A head takes kLanes lanes of 8 values each; every one of them has kItems heads of k or of v
-// (blockIdx.y) in flight.
+// A head takes kLanes lanes of 8 values each; every one of them has kItems heads of a token's k or
+// v (blockIdx.y) in flight, which share the work on its place (a head by itself takes 235
+// instructions for 8 values, 110 of them its place).
 //   scale = max(max |x| / Q, 2^-126), q = round(Q x / max |x|)
 // Q x is exact for 16-bit x, and so is the quotient wherever it is a tie of q: 16-bit x lie on
 // ties far more often than chance has it (one in 700 of normal bf16 values), which x / scale, or x
@@ -87,69 +89,72 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid
   const CacheSide& side = blockIdx.y == 0 ? p.side[0] : p.side[1];
   constexpr int kGroups = kCacheThreads / kLanes;
   const int lane = threadIdx.x % kLanes, col = lane * 8;
-  const int64_t items = p.tokens * p.heads;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kGroups * kItems) + threadIdx.x / kLanes;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / kLanes;
   float2 v[kItems][4];
-  int64_t slot[kItems];
-  int32_t head[kItems];
+  int64_t slot = -1, token = 0;
+  int32_t round = 0;
+  if (unit < p.tokens * p.rounds) {
+    cache_unit(p, unit, &token, &round);
+    slot = p.slots_64bit ? ld1(static_cast<const int64_t*>(p.slots) + token)
+                         : ld1(static_cast<const int32_t*>(p.slots) + token);
+  }
+  const int32_t head0 = round * kItems, heads = unit < p.tokens * p.rounds ? min(kItems, p.heads - head0) : 0;
+  const X* src = static_cast<const X*>(side.x) + token * side.x_token + head0 * side.x_head + col;
 #pragma unroll
-  for (int j = 0; j < kItems; ++j) {
-    const int64_t i = first + j * kGroups;
-    slot[j] = -1;
+  for (int j = 0; j < kItems; ++j, src += side.x_head) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[j][k] = make_float2(0.f, 0.f);
-    if (i >= items) continue;
-    int64_t token;
-    cache_item(p, i, &token, &head[j]);
-    slot[j] = p.slots_64bit ? ld1(static_cast<const int64_t*>(p.slots) + token)
-                            : ld1(static_cast<const int32_t*>(p.slots) + token);
-    const int64_t e = token * side.x_token + head[j] * side.x_head + col;
+    if (j >= heads) continue;
     if (side.vec_x) {
-      if (col < p.head_dim) Pair8<X>::load(static_cast<const X*>(side.x) + e, v[j]);
+      if (col < p.head_dim) Pair8<X>::load(src, v[j]);
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (col + 2 * k < p.head_dim) v[j][k].x = cache_load1<X>(side.x, e + 2 * k);
-        if (col + 2 * k + 1 < p.head_dim) v[j][k].y = cache_load1<X>(side.x, e + 2 * k + 1);
+        if (col + 2 * k < p.head_dim) v[j][k].x = cache_load1<X>(src, 2 * k);
+        if (col + 2 * k + 1 < p.head_dim) v[j][k].y = cache_load1<X>(src, 2 * k + 1);
       }
     }
   }
+  // no lane leaves before the last shuffle: its slot may differ from its neighbours'
+  const bool beyond = slot >= p.pages * p.page_size;
+  if (beyond && lane == 0 && head0 == 0) record_data_error(RMSNORM_B200_ERR_INVALID_ARGUMENT, kSiteCacheSlot);
+  const bool kept = slot >= 0 && !beyond;
+  const int64_t page = !kept ? 0 : p.small ? divide(static_cast<uint32_t>(slot), p.by_page) : slot / p.page_size;
+  const int64_t place = kept ? slot - page * p.page_size : 0;
+  float* scale = side.scales + page * side.s_page + place * side.s_slot + head0 * side.s_head;
+  unsigned char* dst = side.data + page * side.page + place * side.slot + head0 * side.head + col;
 #pragma unroll
   for (int j = 0; j < kItems; ++j) {
     uint32_t most = magnitude(largest8(0.f, v[j]));
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (slot[j] < 0) continue;
-    if (slot[j] >= p.pages * p.page_size) {
-      if (lane == 0) record_data_error(RMSNORM_B200_ERR_INVALID_ARGUMENT, kSiteCacheSlot);
-      continue;
-    }
-    const int64_t page = p.small ? divide(static_cast<uint32_t>(slot[j]), p.by_page) : slot[j] / p.page_size;
-    const int64_t place = slot[j] - page * p.page_size;
-    constexpr float kTop = std::is_same<Q, I8>::value ? 127.f : 448.f;
-    const float largest = __uint_as_float(most), s0 = __fdiv_rn(largest, kTop);
-    const bool least = s0 < 1.17549435e-38f;  // NaN is not
-    if (lane == 0)
-      st1(side.scales + page * side.s_page + place * side.s_slot + head[j] * side.s_head, least ? 1.17549435e-38f : s0);
-    if (col >= p.head_dim) continue;
+    if (!kept || j >= heads) continue;
+    constexpr float kTop = std::is_same<Q, I8>::value ? 127.f : 448.f, kInvTop = 1.f / kTop;
+    const float largest = __uint_as_float(most);
     const int e = static_cast<int>(most >> 23);
+    // max |x| / Q by the same correction, which infinity does not survive
+    float s0 = largest * kInvTop;
+    s0 = e == 255 ? largest : fmaf(fmaf(-s0, kTop, largest), kInvTop, s0);
+    const bool least = s0 < 1.17549435e-38f;  // NaN is not
+    if (lane == 0) st1(scale + j * side.s_head, least ? 1.17549435e-38f : s0);
+    if (col >= p.head_dim) continue;
     const float power = __uint_as_float(static_cast<uint32_t>(max(254 - e, 1)) << 23);
     const float times = least ? 8.5070592e37f : kTop * power;  // 2^126
     const float by = least ? 1.f : e < 255 ? largest * power : 0.f;  // infinity: no remainder
-    const float inv = __frcp_rn(!least && e == 255 ? largest : by);
+    const float inv = inverse(!least && e == 255 ? largest : by);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float2 n = mul2(v[j][k], splat2(times)), q = mul2(n, splat2(inv));
       v[j][k] = fma2(fma2(q, splat2(-by), n), splat2(inv), q);
     }
     const uint2 b = make_uint2(Q::pack4(v[j][0], v[j][1]), Q::pack4(v[j][2], v[j][3]));
-    unsigned char* dst = side.data + page * side.page + place * side.slot + head[j] * side.head + col;
+    unsigned char* to = dst + j * side.head;
     if (side.vec_q) {
-      if (RMSB_DBG_OK(dst, 8, kDbgVecStore)) *reinterpret_cast<uint2*>(dst) = b;
+      if (RMSB_DBG_OK(to, 8, kDbgVecStore)) *reinterpret_cast<uint2*>(to) = b;
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (col + k < p.head_dim) st1(dst + k, static_cast<unsigned char>((k < 4 ? b.x : b.y) >> (8 * (k & 3))));
+        if (col + k < p.head_dim) st1(to + k, static_cast<unsigned char>((k < 4 ? b.x : b.y) >> (8 * (k & 3))));
     }
   }
 }
@@ -198,76 +203,68 @@ __device__ __forceinline__ int2 cache_place(const CacheParams& p, int64_t token)
   return make_int2(page, static_cast<int32_t>(at - column * static_cast<uint32_t>(p.page_size)));
 }
 
-// A head takes kLanes lanes of 8 values; every one of them has kItems heads of k and as many of v
-// in flight. The CTA's tokens are looked up first, a thread each.
+// A head takes kLanes lanes of 8 values; every one of them has kItems heads of a token's k and as
+// many of its v in flight. The CTA's tokens are looked up first, a thread each.
 template <typename X, typename Q, int kLanes, int kItems>
 __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const __grid_constant__ CacheParams p) {
-  constexpr int kGroups = kCacheThreads / kLanes, kPer = kGroups * kItems;
-  __shared__ int2 places[kPer];  // of the CTA's tokens: one at least for every head of the items
+  constexpr int kGroups = kCacheThreads / kLanes;
+  __shared__ int2 places[kGroups];  // of the CTA's tokens: no more than its units
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x % kLanes, col = lane * 8;
-  const int64_t items = p.tokens * p.heads, begin = static_cast<int64_t>(blockIdx.x) * kPer;
-  int64_t token0, token1;
-  int32_t unused;
-  cache_item(p, begin, &token0, &unused);
-  cache_item(p, min(begin + kPer, items) - 1, &token1, &unused);
+  const int64_t units = p.tokens * p.rounds, begin = static_cast<int64_t>(blockIdx.x) * kGroups;
+  const int64_t unit = min(begin + threadIdx.x / kLanes, units - 1);
+  int64_t token0, token1, token;
+  int32_t round;
+  cache_unit(p, begin, &token0, &round);
+  cache_unit(p, min(begin + kGroups, units) - 1, &token1, &round);
   if (token0 + threadIdx.x <= token1) {
     const int2 at = cache_place(p, token0 + threadIdx.x);
     if (at.x == kNowhere) record_data_error(RMSNORM_B200_ERR_INVALID_ARGUMENT, kSiteCachePage);
     places[threadIdx.x] = at;
   }
+  cache_unit(p, unit, &token, &round);
   __syncthreads();
-  uint2 b[kItems][2];
-  float s[kItems][2];
+  if (begin + threadIdx.x / kLanes >= units || col >= p.head_dim) return;
+  const int2 at = places[token - token0];
+  if (at.x == kRest && !p.zero_rest) return;
+  const int32_t head0 = round * kItems, heads = min(kItems, p.heads - head0);
+  uint2 b[2][kItems];
+  float s[2][kItems];
 #pragma unroll
-  for (int j = 0; j < kItems; ++j) {
-    const int64_t i = begin + j * kGroups + threadIdx.x / kLanes;
+  for (int k = 0; k < 2; ++k) {
+    const CacheSide& side = p.side[k];
+    const int64_t page = max(at.x, 0), place = at.y;
+    const unsigned char* src = side.data + page * side.page + place * side.slot + head0 * side.head + col;
+    const float* scale = side.scales + page * side.s_page + place * side.s_slot + head0 * side.s_head;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      b[j][k] = make_uint2(0, 0);
-      s[j][k] = 0.f;
-    }
-    if (i >= items || col >= p.head_dim) continue;
-    int64_t token;
-    int32_t head;
-    cache_item(p, i, &token, &head);
-    const int2 at = places[token - token0];
-    if (at.x < 0) {
-      s[j][0] = s[j][1] = at.x == kNowhere ? __int_as_float(0x7fc00000) : 0.f;
-      continue;
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const CacheSide& side = p.side[k];
-      const unsigned char* src = side.data + at.x * side.page + at.y * side.slot + head * side.head + col;
-      s[j][k] = ld1(side.scales + at.x * side.s_page + at.y * side.s_slot + head * side.s_head);
+    for (int j = 0; j < kItems; ++j, src += side.head) {
+      b[k][j] = make_uint2(0, 0);
+      s[k][j] = at.x == kNowhere ? __int_as_float(0x7fc00000) : 0.f;
+      if (at.x < 0 || j >= heads) continue;
+      s[k][j] = ld1(scale + j * side.s_head);
       if (side.vec_q) {
-        if (RMSB_DBG_OK(src, 8, kDbgVecLoad)) b[j][k] = *reinterpret_cast<const uint2*>(src);
+        if (RMSB_DBG_OK(src, 8, kDbgVecLoad)) b[k][j] = *reinterpret_cast<const uint2*>(src);
       } else {
 #pragma unroll
         for (int m = 0; m < 8; ++m)
           if (col + m < p.head_dim) {
             const uint32_t one = static_cast<uint32_t>(ld1(src + m)) << (8 * (m & 3));
-            if (m < 4) b[j][k].x |= one;
-            else b[j][k].y |= one;
+            if (m < 4) b[k][j].x |= one;
+            else b[k][j].y |= one;
           }
       }
     }
   }
+  const int64_t e = token * p.side[0].x_token + head0 * p.head_dim + col;  // both outputs are contiguous
 #pragma unroll
-  for (int j = 0; j < kItems; ++j) {
-    const int64_t i = begin + j * kGroups + threadIdx.x / kLanes;
-    if (i >= items || col >= p.head_dim) continue;
-    int64_t token;
-    int32_t head;
-    cache_item(p, i, &token, &head);
-    if (places[token - token0].x == kRest && !p.zero_rest) continue;
+  for (int k = 0; k < 2; ++k) {
+    X* dst = static_cast<X*>(p.side[k].x) + e;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int j = 0; j < kItems; ++j, dst += p.head_dim) {
+      if (j >= heads) continue;
       float2 v[4];
-      unpack_octet<Q>(b[j][k], s[j][k], v);
-      X* dst = static_cast<X*>(p.side[k].x) + i * p.head_dim + col;
+      unpack_octet<Q>(b[k][j], s[k][j], v);
       if (p.side[k].vec_x) {
         Pair8<X>::store(dst, v);
       } else {
