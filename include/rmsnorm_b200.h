@@ -475,7 +475,9 @@ typedef struct rmsnorm_b200_block_mm_args {
   int32_t b_block_rows;       /* 1 or 128 */
   int32_t bias_dtype;
   int32_t out_dtype;
-  int32_t reserved0;
+  int32_t power_of_two;       /* nonzero: every scale is a power of two, 2^-126 at least (or NaN, and
+                               * infinity counts as NaN), as rmsnorm_b200_block_quant leaves them;
+                               * of other scales only the exponent may be used */
 } rmsnorm_b200_block_mm_args;
 
 /* Bytes of device workspace (16-byte aligned): copies of operands whose address or row stride

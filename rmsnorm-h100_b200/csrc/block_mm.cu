@@ -167,21 +167,59 @@ int launch_few(UnitDevice* ud, const void* a, int64_t a_row, const CUtensorMap& 
   return launch<FewKernel>(ud, block_mm_few_kernel<T>, map_a, map_b, p, pl, kFewThreads, smem, pl.splits, stream, l);
 }
 
-int launch_wide(UnitDevice* ud, const CUtensorMap& map_a, const CUtensorMap& map_b, const rmsnorm_b200_block_mm_args* a,
-                const BlockMmParams& p, cudaStream_t stream) {
+// Pairs of CTAs, one tile after the other.
+int launch_pairs(UnitDevice* ud, const char* kind, WideKernel kernel, int threads, int tile_n, int stages, int smem,
+                 const CUtensorMap& map_a, const CUtensorMap& map_b, const rmsnorm_b200_block_mm_args* a,
+                 const BlockMmParams& p, cudaStream_t stream) {
   WidePlan pl = {};
   pl.tiles_m = static_cast<int>((a->m + kWideRows - 1) / kWideRows);
-  pl.tiles_n = static_cast<int>((a->n + kWideN - 1) / kWideN);
+  pl.tiles_n = static_cast<int>((a->n + tile_n - 1) / tile_n);
   pl.band = 8;
   const int64_t tiles = static_cast<int64_t>(pl.tiles_m) * pl.tiles_n;
   const int64_t pairs = std::min<int64_t>(tiles, ud->sm_count / 2);
-  const int smem = 1024 + kWideStages * kWideStageBytes + static_cast<int>(sizeof(WideBars)) + 2 * kWideN * 4 +
-                   8 * kStagingBytes;
-  static_assert(1024 + kWideStages * kWideStageBytes + sizeof(WideBars) + 2 * kWideN * 4 + 8 * kStagingBytes <= kSmemOptIn,
-                "shared memory");
-  const MmLaunch l = {"block_mm_wide", static_cast<unsigned>(pairs * 2), kWideN, 1, kWideStages};
-  return launch<WideKernel>(ud, p.b_rows ? block_mm_wide_kernel<true> : block_mm_wide_kernel<false>, map_a, map_b, p, pl,
-                            kWideThreads, smem, 2, stream, l);
+  const MmLaunch l = {kind, static_cast<unsigned>(pairs * 2), tile_n, 1, stages};
+  return launch<WideKernel>(ud, kernel, map_a, map_b, p, pl, threads, smem, 2, stream, l);
+}
+
+template <int N>
+int launch_scaled(UnitDevice* ud, const CUtensorMap& map_a, const void* b, int64_t b_row,
+                  const rmsnorm_b200_block_mm_args* args, const BlockMmParams& p, cudaStream_t stream) {
+  constexpr int kSmem = 1024 + kScaledStages * (ScaledTile<N>::kStageBytes + kExpBytes) + static_cast<int>(sizeof(ScaledBars)) +
+                        8 * kStagingBytes;
+  static_assert(kSmem <= kSmemOptIn, "shared memory");
+  CUtensorMap map_b;
+  const int st = make_map(&map_b, b, args->n, args->k, b_row, N / 2);
+  if (st) return st;
+  return launch_pairs(ud, "block_mm_scaled", block_mm_scaled_kernel<N>, kScaledThreads, N, kScaledStages, kSmem, map_a, map_b,
+                      args, p, stream);
+}
+
+int launch_wide(UnitDevice* ud, const void* a, int64_t a_row, const void* b, int64_t b_row,
+                const rmsnorm_b200_block_mm_args* args, const BlockMmParams& p, cudaStream_t stream) {
+  constexpr int kSmem = 1024 + kWideStages * kWideStageBytes + static_cast<int>(sizeof(WideBars)) + 2 * kWideN * 4 +
+                        8 * kStagingBytes;
+  static_assert(kSmem <= kSmemOptIn, "shared memory");
+  CUtensorMap map_a, map_b;
+  int st = make_map(&map_a, a, args->m, args->k, a_row, kBlock);
+  if (st) return st;
+  if (args->power_of_two && args->out_dtype != RMSNORM_B200_F32) {
+    // The width of a tile that leaves the least to do one after the other: rounds of tiles, each of
+    // N columns a group, and for the widest the time its results take to come out (about 1600
+    // cycles, of which a column takes two a group). fp32 results keep the sum of the groups' sums
+    // in registers, whose additions round to nearest.
+    const int64_t pairs = ud->sm_count / 2, tiles_m = (args->m + kWideRows - 1) / kWideRows;
+    auto cost = [&](int64_t n, int64_t alone) {
+      return (tiles_m * ((args->n + n - 1) / n) + pairs - 1) / pairs * (p.groups * n + alone);
+    };
+    const int64_t c256 = cost(256, 800), c224 = cost(224, 0), c192 = cost(192, 0);
+    if (c224 <= c256 && c224 <= c192) return launch_scaled<224>(ud, map_a, b, b_row, args, p, stream);
+    if (c192 <= c256) return launch_scaled<192>(ud, map_a, b, b_row, args, p, stream);
+    return launch_scaled<256>(ud, map_a, b, b_row, args, p, stream);
+  }
+  st = make_map(&map_b, b, args->n, args->k, b_row, kBlock);
+  if (st) return st;
+  return launch_pairs(ud, "block_mm_wide", p.b_rows ? block_mm_wide_kernel<true> : block_mm_wide_kernel<false>, kWideThreads,
+                      kWideN, kWideStages, kSmem, map_a, map_b, args, p, stream);
 }
 
 int run(const rmsnorm_b200_block_mm_args* a, void* ws, size_t ws_bytes, cudaStream_t stream) {
@@ -233,20 +271,18 @@ int run(const rmsnorm_b200_block_mm_args* a, void* ws, size_t ws_bytes, cudaStre
   p.out = a->out; p.out_dt = a->out_dtype;
   p.b_rows = a->b_block_rows == 1;
   p.vec_out = aligned_to(a->out, 32) && a->n * elem_bytes(a->out_dtype) % 32 == 0;
-  CUtensorMap map_a, map_b;
-  st = make_map(&map_b, qb, a->n, a->k, b_row, kBlock);
-  if (st) return st;
   // Few rows, or more of them where two CTAs or more could share each 128 x 128 of the result:
   // the kernel that splits k. K = 4096: 256 x 4096 14.9 against 21.8 us, 1024 x 1024 14.6 against
   // 21.8 us, 512 x 4096 (128 tiles for 148 SMs) 25.2 against 22.0 us.
+  const int64_t squares = (a->m + kBlock - 1) / kBlock * ((a->n + kBlock - 1) / kBlock);
+  if (a->m > 128 && (2 * squares > ud->sm_count || groups < 4)) return launch_wide(ud, qa, a_row, qb, b_row, a, p, stream);
+  CUtensorMap map_b;
+  st = make_map(&map_b, qb, a->n, a->k, b_row, kBlock);
+  if (st) return st;
   if (a->m <= 16) return launch_few<16>(ud, qa, a_row, map_b, a, p, stream);
   if (a->m <= 32) return launch_few<32>(ud, qa, a_row, map_b, a, p, stream);
   if (a->m <= 64) return launch_few<64>(ud, qa, a_row, map_b, a, p, stream);
-  const int64_t squares = (a->m + kBlock - 1) / kBlock * ((a->n + kBlock - 1) / kBlock);
-  if (a->m <= 128 || (2 * squares <= ud->sm_count && groups >= 4)) return launch_few<128>(ud, qa, a_row, map_b, a, p, stream);
-  st = make_map(&map_a, qa, a->m, a->k, a_row, kBlock);
-  if (st) return st;
-  return launch_wide(ud, map_a, map_b, a, p, stream);
+  return launch_few<128>(ud, qa, a_row, map_b, a, p, stream);
 }
 
 int workspace_size(const rmsnorm_b200_block_mm_args* a, size_t* bytes) {

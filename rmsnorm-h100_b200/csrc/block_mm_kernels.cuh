@@ -46,7 +46,7 @@ constexpr int kTileBytes = kBlock * kTileK;  // 128 rows of an operand
 constexpr int kWideStages = 6;
 constexpr int kWideStageBytes = 2 * kTileBytes;  // a CTA's rows of a and of b
 
-constexpr int kStagingBytes = 32 * 17 * 4;  // 32 rows of 16 columns, a word between them
+constexpr int kStagingBytes = 32 * 17 * 4;  // store_turned's: 32 rows of 16 columns, a word between them
 
 struct WideBars {
   uint64_t full[kWideStages], empty[kWideStages], sum[2], sum_empty[2], done;
@@ -72,6 +72,22 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
+}
+
+// A warp's 32 rows of 16 columns, a row a lane, where rows begin anywhere: turned through shared
+// memory, so that the warp stores a row's neighbours side by side (1000 x 4100 with K = 1008: 50 us
+// when every lane stored its own row's values one by one, 22 us so).
+__device__ __forceinline__ void store_turned(float* mine, const float2 (&v)[8], const BlockMmParams& p, int64_t row0,
+                                             int64_t col0, int left) {
+  const int rows = static_cast<int>(max(int64_t{0}, min(int64_t{32}, p.m - row0)));
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) mine[lane * 17 + i] = i & 1 ? v[i / 2].y : v[i / 2].x;
+  __syncwarp();
+  const int col = lane & 15;
+  if (col < left)
+    for (int r = lane >> 4; r < rows; r += 2) store1_rt(p.out, p.out_dt, (row0 + r) * p.n + col0 + col, mine[r * 17 + col]);
 }
 
 // acc += sums * scale, or acc += sums * (column scales) * scale.
@@ -273,22 +289,13 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         }
       }
       if (!p.vec_out || left < kWideHalf) {
-        // a lane's row begins anywhere: 16 columns at a time turned through shared memory, so that
-        // the warp stores a row's neighbours side by side (1000 x 4100 with K = 1008: 50 us when
-        // every lane stored its own row's values one by one)
         float* mine = reinterpret_cast<float*>(staging + warp * kStagingBytes);
-        const int64_t row0 = row - lane;
-        const int rows = static_cast<int>(max(int64_t{0}, min(int64_t{32}, p.m - row0)));
 #pragma unroll
         for (int c = 0; c < kWideHalf; c += 16) {
-          __syncwarp();
+          float2 v[8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) mine[lane * 17 + i] = i & 1 ? acc[(c + i) / 2].y : acc[(c + i) / 2].x;
-          __syncwarp();
-          const int col = c + (lane & 15);
-          if (col < left)
-            for (int r = lane >> 4; r < rows; r += 2)
-              store1_rt(p.out, p.out_dt, (row0 + r) * p.n + col0 + col, mine[r * 17 + (lane & 15)]);
+          for (int i = 0; i < 8; ++i) v[i] = acc[c / 2 + i];
+          if (c < left) store_turned(mine, v, p, row - lane, col0 + c, left - c);
         }
       } else if (!live) {
         continue;
@@ -320,6 +327,246 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   cluster_sync_all();
   tmem_fence_after_sync();
   if (warp == 9) tmem_dealloc_pair(tmem, 2 * kWideN);
+}
+
+// ---------------------------------------------------------------------------------------
+// Many rows, scales that are powers of two, 16-bit results: the tensor cores apply the scales.
+// Warps 10 to 13 turn a group's scales into exponents, one for every 32 values of k, which a copy
+// in the products' order brings to tensor memory; the sum over all of k stays there, and the eight
+// summing warps only bring results out. Tiles of 224 or 192 columns leave tensor memory for two of
+// them, so that one comes out while the next is summed, and for the exponents; one of 256 comes out
+// before the next begins, for pairs that have a single tile or two.
+// Measured: 8192 x 16384 x 4096 410 us (2680 TFLOP/s, at the card's power limit), scaled in
+// registers 514 us.
+// ---------------------------------------------------------------------------------------
+constexpr int kScaledThreads = 448;
+constexpr int kScaledStages = 6;
+constexpr int kExpBytes = 3 * 512;  // exponents of a stage: of 128 rows of a, 256 of b
+constexpr int kExpAhead = 4;        // groups whose scales are on their way
+
+template <int N>
+struct ScaledTile {
+  static constexpr int kSums = N > 224 ? 1 : 2;
+  static constexpr int kStageBytes = kTileBytes + N / 2 * kTileK;  // a CTA's rows of a and of b
+  static constexpr int kExpColumns = kSums * N;                    // in tensor memory, 16 columns for each of four groups
+};
+
+struct ScaledBars {
+  uint64_t full[kScaledStages], empty[kScaledStages], sum[2], sum_empty[2], done;
+  uint32_t tmem;
+};
+
+template <int N>
+__global__ void __launch_bounds__(kScaledThreads, 1)
+    block_mm_scaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                           const BlockMmParams p, const WidePlan pl) {
+  using S = ScaledTile<N>;
+  unsigned char* smem = rmsb_dyn_smem + ((1024u - (smem_u32(rmsb_dyn_smem) & 1023u)) & 1023u);
+  unsigned char* exponents = smem + kScaledStages * S::kStageBytes;
+  ScaledBars* bars = reinterpret_cast<ScaledBars*>(exponents + kScaledStages * kExpBytes);
+  unsigned char* staging = reinterpret_cast<unsigned char*>(bars + 1);  // kStagingBytes a warp
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int64_t unit = blockIdx.x >> 1, units = gridDim.x >> 1;
+  const int64_t tiles = static_cast<int64_t>(pl.tiles_m) * pl.tiles_n;
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kScaledStages; ++i) {
+      mbar_init(&bars->full[i], 9);  // the copies, and four warps' exponents in each CTA
+      mbar_init(&bars->empty[i], 1);
+    }
+    for (int i = 0; i < S::kSums; ++i) {
+      mbar_init(&bars->sum[i], 1);
+      mbar_init(&bars->sum_empty[i], 16);
+    }
+    mbar_init(&bars->done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc_pair(&bars->tmem, 512);
+  if (threadIdx.x == 256) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_b);
+  }
+  tmem_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();
+  tmem_fence_after_sync();
+  const uint32_t tmem = bars->tmem;
+  pdl_wait();
+
+  if (warp == 8) {  // copies
+    int s = 0;
+    uint32_t pass = 0;
+    bool ok = true;
+    for (int64_t t = unit; ok && t < tiles; t += units) {
+      int tm, tn;
+      wide_tile(pl, t, &tm, &tn);
+      const int ya = tm * kWideRows + static_cast<int>(rank) * kBlock;
+      const int yb = tn * N + static_cast<int>(rank) * (N / 2);
+      for (int g = 0; g < p.groups; ++g) {
+        ok = __all_sync(0xffffffffu, mbar_spin_warp(&bars->empty[s], pass ^ 1u, kSiteMmEmpty));
+        if (!ok) break;
+        if (elect_one()) {
+          unsigned char* at = smem + s * S::kStageBytes;
+          if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * S::kStageBytes);
+          tile_load<true>(at, &map_a, g * kTileK, ya, &bars->full[s]);
+          tile_load<true>(at + kTileBytes, &map_b, g * kTileK, yb, &bars->full[s]);
+        }
+        __syncwarp();
+        if (++s == kScaledStages) {
+          s = 0;
+          pass ^= 1u;
+        }
+      }
+    }
+    // Nobody leaves while copies may land in its memory or arrivals at its barriers.
+    if (lane == 0 && rank == 0 && abort_requested())
+      for (int i = 0; i < kScaledStages; ++i) mbar_wait(&bars->full[i], i < s ? pass : pass ^ 1u, kSiteDrain, false);
+    for (int i = 0; i < kScaledStages; ++i) mbar_spin_warp(&bars->empty[i], i < s ? pass : pass ^ 1u, kSiteMmEmpty);
+  } else if (warp == 9 && rank == 0) {  // products
+    constexpr uint32_t idesc = scaled_product_desc(kWideRows, N);
+    int s = 0;
+    uint32_t pass = 0, u = 0, n = 0;  // rounds of the stages, tiles, groups
+    bool ok = true;
+    for (int64_t t = unit; ok && t < tiles; t += units, ++u) {
+      const uint32_t d = u % S::kSums;
+      ok = __all_sync(0xffffffffu, mbar_spin_warp(&bars->sum_empty[d], ((u / S::kSums) & 1u) ^ 1u, kSiteMmSumEmpty));
+      for (int g = 0; ok && g < p.groups; ++g, ++n) {
+        ok = __all_sync(0xffffffffu, mbar_spin_warp(&bars->full[s], pass, kSiteMmFull));
+        if (!ok) break;
+        tmem_fence_after_sync();
+        if (elect_one()) {
+          const uint32_t at = smem_u32(smem + s * S::kStageBytes), exps = smem_u32(exponents + s * kExpBytes);
+          const uint32_t sa = tmem + S::kExpColumns + (n & 3u) * 16, sb = sa + 4;
+          scales_to_tmem(sa, exps);
+          scales_to_tmem(sb, exps + 512);
+          scales_to_tmem(sb + 4, exps + 1024);
+          const uint64_t a = operand_desc(at), b = operand_desc(at + kTileBytes);
+#pragma unroll
+          for (int k = 0; k < kTileK / 32; ++k)
+            mma_e4m3_scaled(tmem + d * N, a + 2 * k, b + 2 * k, idesc, sa, sb, g > 0 || k > 0);
+          mma_commit<true>(&bars->empty[s]);
+          if (g == p.groups - 1) mma_commit<true>(&bars->sum[d]);
+        }
+        __syncwarp();
+        if (++s == kScaledStages) {
+          s = 0;
+          pass ^= 1u;
+        }
+      }
+    }
+    if (abort_requested()) {
+      if (lane == 0) {
+        mma_commit<true>(&bars->done);
+        mbar_wait(&bars->done, 0, kSiteDrain, false);
+      }
+      __syncwarp();
+    }
+    for (int i = 0; i < S::kSums; ++i, ++u)
+      mbar_spin_warp(&bars->sum_empty[u % S::kSums], ((u / S::kSums) & 1u) ^ 1u, kSiteMmSumEmpty);
+  } else if (warp >= 10) {  // exponents: thread i has row i of a, rows i and i + 128 of b
+    const int i = threadIdx.x - 320;
+    int s = 0;
+    uint32_t pass = 0;
+    for (int64_t t = unit; t < tiles; t += units) {
+      int tm, tn;
+      wide_tile(pl, t, &tm, &tn);
+      const int64_t rows[3] = {static_cast<int64_t>(tm) * kWideRows + rank * kBlock + i, static_cast<int64_t>(tn) * N + i,
+                               static_cast<int64_t>(tn) * N + i + 128};
+      const bool live[3] = {rows[0] < p.m, rows[1] < p.n, rows[2] < p.n && i + 128 < N};
+      const float* src[3] = {p.sa + rows[0] * p.sa_row, sb_of(p, rows[1]), sb_of(p, rows[2])};
+      int ahead = 0;
+      auto fetch = [&](uint32_t (&e)[3]) {
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          e[j] = live[j] && ahead < p.groups ? __float_as_uint(ld1(src[j])) : 0x3f800000u;
+          src[j] += j < 1 ? p.sa_group : p.sb_group;
+        }
+        ++ahead;
+      };
+      uint32_t e[kExpAhead][3];
+#pragma unroll
+      for (int k = 0; k < kExpAhead; ++k) fetch(e[k]);
+      for (int g = 0; g < p.groups; ++g) {
+        uint32_t word[3];
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          word[j] = (e[0][j] >> 23 & 255u) * 0x01010101u;
+#pragma unroll
+          for (int k = 1; k < kExpAhead; ++k) e[k - 1][j] = e[k][j];
+        }
+        fetch(e[kExpAhead - 1]);
+        mbar_spin_warp(&bars->empty[s], pass ^ 1u, kSiteMmEmpty);
+        uint32_t* to = reinterpret_cast<uint32_t*>(exponents + s * kExpBytes) + (i & 31) * 4 + (i >> 5);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) to[128 * j] = word[j];
+        // The bytes are in place for this SM's tensor core before the arrival leaves; the pair's
+        // first CTA makes it read them. (Release at the cluster's scope would wait for the loads in
+        // flight: 1058 instead of 460 us at 8192 x 16384 x 4096.)
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_peer(&bars->full[s], 0);
+        if (++s == kScaledStages) {
+          s = 0;
+          pass ^= 1u;
+        }
+      }
+    }
+  } else if (warp < 8) {  // results: warp w has rows 32 (w % 4) .. + 31, the half w / 4 of the columns
+    constexpr int kHalf = N / 2;
+    const int half = warp >> 2;
+    const uint32_t from = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * kHalf;
+    uint32_t u = 0;
+    for (int64_t t = unit; t < tiles; t += units, ++u) {
+      int tm, tn;
+      wide_tile(pl, t, &tm, &tn);
+      const uint32_t d = u % S::kSums;
+      const int64_t row = static_cast<int64_t>(tm) * kWideRows + rank * kBlock + (warp & 3) * 32 + lane;
+      const int64_t col0 = static_cast<int64_t>(tn) * N + half * kHalf;
+      const int left = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(kHalf), p.n - col0)));
+      const bool whole = p.vec_out && left == kHalf, bf16 = p.out_dt == RMSNORM_B200_BF16;
+      mbar_spin_warp(&bars->sum[d], (u / S::kSums) & 1u, kSiteMmSum);
+      __syncwarp();
+      tmem_fence_after_sync();
+#pragma unroll
+      for (int c = 0; c < kHalf; c += 16) {
+        float2 v[8];
+        tmem_ld(from + d * N + c, v);
+        tmem_landed(v);
+        if (c + 16 == kHalf) {
+          tmem_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_peer(&bars->sum_empty[d], 0);
+        }
+        if (c >= left) continue;
+        if (p.bias) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int at = c + 2 * i;
+            const float x = at < left ? load1_rt(p.bias, p.bias_dt, col0 + at) : 0.f;
+            const float y = at + 1 < left ? load1_rt(p.bias, p.bias_dt, col0 + at + 1) : 0.f;
+            v[i] = add2(v[i], make_float2(x, y));
+          }
+        }
+        if (whole) {
+          if (row < p.m) {
+            uint32_t w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = bf16 ? pack_bf16x2_pair(v[k]) : pack_f16x2_pair(v[k]);
+            store32(static_cast<uint16_t*>(p.out) + row * p.n + col0 + c, w);
+          }
+        } else {
+          store_turned(reinterpret_cast<float*>(staging + warp * kStagingBytes), v, p, row - lane, col0 + c, left - c);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tmem_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();
+  tmem_fence_after_sync();
+  if (warp == 9) tmem_dealloc_pair(tmem, 512);
 }
 
 // ---------------------------------------------------------------------------------------

@@ -52,6 +52,31 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uin
         : "memory");
 }
 
+// The same for block-scaled operands: an exponent (8 bits, as a power of two in fp32 has it) for
+// every 32 values of k of every row, in tensor memory; the tensor cores apply them.
+__host__ __device__ constexpr uint32_t scaled_product_desc(int m, int n) {
+  return (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// By a pair. Every 32 rows of a CTA's a take a column at scale_a (lane: row % 32), of all of b at
+// scale_b, in both CTAs; byte 0 of a cell is read.
+__device__ __forceinline__ void mma_e4m3_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scale_a,
+                                                uint32_t scale_b, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add)), "r"(scale_a), "r"(scale_b)
+      : "memory");
+}
+
+// 32 rows of 16 bytes, one behind the other in shared memory, into four columns of 32 lanes and
+// their copies in the other 96; in both CTAs of a pair, each from its own shared memory.
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t smem_addr) {
+  const uint64_t desc = static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4) | (uint64_t{1} << 16) | (uint64_t{128 >> 4} << 32) |
+                        (uint64_t{1} << 46);
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
 // `bar` gets one arrival when this thread's products so far are complete; of a pair, both CTAs'.
 template <bool kPair>
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {

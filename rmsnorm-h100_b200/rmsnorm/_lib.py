@@ -275,7 +275,7 @@ class BlockMmArgs(ctypes.Structure):
         ("b_block_rows", ctypes.c_int32),
         ("bias_dtype", ctypes.c_int32),
         ("out_dtype", ctypes.c_int32),
-        ("reserved0", ctypes.c_int32),
+        ("power_of_two", ctypes.c_int32),
     ]
 
 
