@@ -58,14 +58,15 @@ def values(q, scales):
     return q.double() * scales.double().repeat_interleave(128, 1)[:, :k].repeat_interleave(rows, 0)[:n]
 
 
-def check_product(got, a, b, bias, what):
+def check_product(got, a, b, bias, what, in_cores=False):
     """got against a b^T + bias for 64-bit a and b."""
     want, size = a @ b.t(), a.abs() @ b.abs().t()
     if bias is not None:
         want, size = want + bias.double(), size + bias.double().abs()
     groups = -(-a.shape[1] // 128)
     off = (got.double() - want).abs()
-    allowed = UNIT[got.dtype] * want.abs() + (128 + groups + 4) * 2.0**-23 * size + TINY[got.dtype]
+    # where the tensor cores add all of k, 32 products at a time, there are 4 additions a group
+    allowed = UNIT[got.dtype] * want.abs() + (128 + (4 if in_cores else 1) * groups + 4) * 2.0**-23 * size + TINY[got.dtype]
     bad = ~(off <= allowed)
     assert got.shape == want.shape, (what, got.shape, want.shape)
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((off - allowed)[bad].max())} beyond"

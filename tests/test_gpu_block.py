@@ -247,6 +247,85 @@ def test_product_on_streams_and_in_graphs():
         assert all(torch.equal(r, w) for r, w in zip(results, want))
 
 
+# ------------------------------------------------------------------ scales left to the tensor cores
+def power_case(m, n, k, block_rows, out_dtype, bias=True, column_major=False):
+    """Scales over many octaves, that differ from row to row and from group to group."""
+    a, _ = operand(m, k, 1, 1)
+    b, _ = operand(n, k, block_rows, 2)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    groups = -(-k // 128)
+    sa = torch.exp2(torch.randint(-14, -5, (m, groups), device=DEV, generator=g).float())
+    sb = torch.exp2(torch.randint(-14, -5, (-(-n // block_rows), groups), device=DEV, generator=g).float())
+    if column_major:
+        sa, sb = sa.t().contiguous().t(), sb.t().contiguous().t()
+    bias = rand(n, seed=3) if bias else None
+    out = fused.block_mm(a, sa, b, sb, bias, out_dtype, power_of_two=True)
+    assert out.dtype == out_dtype and out.shape == (m, n)
+    ref.check_product(out, ref.values(a, sa), ref.values(b, sb), bias, f"{m}x{n}x{k}", True)
+
+
+# tiles of 256, 224 and 192 columns: one round of them, two, several; ragged ones; one group to many
+@pytest.mark.parametrize("m,n,k", [(129, 9600, 100), (200, 20000, 128), (300, 12345, 700), (1000, 4096, 2048), (1024, 4100, 512),
+                                   (600, 4096, 1001), (2300, 5000, 1280), (4096, 1024, 640), (5000, 3000, 300), (257, 19000, 130)])
+@pytest.mark.parametrize("out_dtype", [BF16, F16, F32])
+def test_powers_of_two(m, n, k, out_dtype):
+    power_case(m, n, k, 128, out_dtype, False)
+    power_case(m, n, k, 1, out_dtype, True, True)
+
+
+@pytest.mark.parametrize("m", [1, 16, 40, 100, 200])
+def test_powers_of_two_of_few_rows(m):
+    power_case(m, 1000, 1024, 128, BF16)
+    power_case(m, 130, 2000, 1, F16)
+
+
+def test_powers_of_two_tiles_are_what_the_test_means_them_to_be():
+    tiles = set()
+    for m, n, k in [(1000, 4096, 2048), (2300, 5000, 1280), (600, 4096, 1001)]:
+        power_case(m, n, k, 128, BF16)
+        plan = _lib.last_plan()
+        assert plan.startswith("block_mm_scaled"), plan
+        tiles.add(plan.split("tile=")[1].split()[0])
+    assert tiles == {"192", "224", "256"}, tiles
+
+
+def test_powers_of_two_at_the_ends_of_the_range():
+    a, b = (torch.full((300, 128), v, device=DEV).to(E4M3) for v in (448.0, 1.0))
+    b = b.repeat(40, 1)
+    low, high = (torch.full((300, 1), 2.0**e, device=DEV) for e in (-126, 120))
+    sb = torch.ones(94, 1, device=DEV)
+    out = fused.block_mm(a, high * 2.0**-110, b, sb * 2.0**-10, None, BF16, power_of_two=True)
+    assert (out == 448 * 128).all()
+    out = fused.block_mm(a, low, b, sb * 2.0**100, None, BF16, power_of_two=True)
+    assert (out.double() == 448 * 128 * 2.0**-26).all()
+    out = fused.block_mm(a, high, b, sb * 2.0**-126, None, BF16, power_of_two=True)
+    assert (out.double() == 448 * 128 * 2.0**-6).all()
+    sa = torch.ones(300, 1, device=DEV)
+    sa[7], sb[3] = float("nan"), float("inf")
+    nan = fused.block_mm(a, sa, b, sb, None, BF16, power_of_two=True).isnan()
+    assert nan[7].all() and nan[:, 384:512].all() and int(nan.sum()) == 12000 + 299 * 128
+
+
+def test_powers_of_two_do_not_depend_on_the_run_and_replay():
+    x, w = rand(1500, 1024, dtype=BF16), rand(5000, 1024, dtype=BF16, seed=1)
+    a, sa = fused.block_quantize(x)
+    b, sb = fused.block_quantize(w, 128)
+    first = fused.block_mm(a, sa, b, sb, power_of_two=True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = fused.block_mm(a, sa, b, sb, power_of_two=True)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(3):
+        outs = []
+        for st in streams:
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                outs.append(fused.block_mm(a, sa, b, sb, power_of_two=True))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, first) for o in (*outs, out))
+
+
 # ------------------------------------------------------------------ linear layer
 def linear_reference(x, w, b, dy):
     """y, dx, dw as pairs of 64-bit factors, db."""
@@ -255,7 +334,8 @@ def linear_reference(x, w, b, dy):
     return (val(x, 1), wv), (val(dy, 1), wv.t()), (val(dy.t(), 1), val(x.t(), 1))
 
 
-@pytest.mark.parametrize("t,n,k", [(1, 8, 16), (7, 100, 300), (128, 256, 384), (333, 520, 1001), (1500, 1300, 640)])
+@pytest.mark.parametrize("t,n,k", [(1, 8, 16), (7, 100, 300), (128, 256, 384), (333, 520, 1001), (1500, 1300, 640),
+                                   (3000, 2500, 2304)])
 @pytest.mark.parametrize("dtype,w_dtype", [(BF16, BF16), (F16, F16), (F32, F32), (BF16, F32)])
 def test_linear(t, n, k, dtype, w_dtype):
     x = rand(t, k, dtype=dtype, seed=1).requires_grad_(True)
@@ -266,9 +346,9 @@ def test_linear(t, n, k, dtype, w_dtype):
     dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
     fy, fdx, fdw = linear_reference(x.detach(), w.detach(), b.detach(), dy)
     assert y.dtype == dtype and dx.dtype == dtype and dw.dtype == w_dtype and db.dtype == F32
-    ref.check_product(y.detach(), *fy, b.detach(), "y")
-    ref.check_product(dx, *fdx, None, "dx")
-    ref.check_product(dw, *fdw, None, "dw")
+    ref.check_product(y.detach(), *fy, b.detach(), "y", True)
+    ref.check_product(dx, *fdx, None, "dx", True)
+    ref.check_product(dw, *fdw, None, "dw", True)
     off = (db.double() - dy.double().sum(0)).abs()
     assert (off <= (t + 8) * 2.0**-24 * dy.double().abs().sum(0) + 2.0**-140).all()
 
