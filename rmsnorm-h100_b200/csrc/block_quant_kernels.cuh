@@ -2,8 +2,6 @@
 // 128 x 128 blocks, of x and of x transposed.
 #pragma once
 
-#include <type_traits>
-
 #include "block_scale.cuh"
 
 namespace rmsb200 {
@@ -63,15 +61,6 @@ __device__ __forceinline__ void store_octet(const BlockQuantParams& p, int64_t r
     if (col + i < p.cols) st1(dst + i, static_cast<unsigned char>((i < 4 ? b.x : b.y) >> (8 * (i & 3))));
 }
 
-__device__ __forceinline__ uint32_t octet_magnitude(const float2 (&v)[4]) { return magnitude(largest8(0.f, v)); }
-
-// The largest of 16 neighbouring lanes.
-__device__ __forceinline__ uint32_t max16(uint32_t m) {
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m;
-}
-
 // Groups of a row, nothing else: 16 lanes a group, 8 columns a lane, kGroups groups in flight.
 template <typename X, int kGroups>
 __global__ void __launch_bounds__(256) quant_groups_kernel(const BlockQuantParams p, int64_t total, uint32_t groups) {
@@ -95,89 +84,18 @@ __global__ void __launch_bounds__(256) quant_groups_kernel(const BlockQuantParam
   }
 #pragma unroll
   for (int j = 0; j < kGroups; ++j) {
-    const uint32_t s = power_scale(max16(octet_magnitude(v[j])));
+    const uint32_t s = power_scale(largest_of<16>(octet_magnitude(v[j])));
     if (first + j >= total) continue;
     if (at == 0) st1(p.scales + row[j] * p.scale_row + group[j] * p.scale_group, __uint_as_float(s));
     store_octet(p, row[j], group[j] * kBlock + at, pack_octet(v[j], power_inverse(s)));
   }
 }
 
-// Eight values of a row as they are loaded: 4 registers, 8 for fp32. Magnitudes of 16-bit values
-// are compared as they are, two at a time: without the sign their bits order as unsigned integers,
-// infinity above the numbers and NaN above it.
-template <typename X>
-struct Held {
-  uint32_t w[4];
-  __device__ __forceinline__ float2 pair(int k) const {
-    if constexpr (std::is_same<X, __half>::value) return unpack_f16x2_pair(w[k]);
-    else return unpack_bf16x2_pair(w[k]);
-  }
-  __device__ __forceinline__ static uint32_t widen(uint32_t m) {  // a magnitude's bits in fp32
-    if constexpr (std::is_same<X, __half>::value)
-      return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
-    else return m << 16;
-  }
-};
-template <>
-struct Held<float> {
-  float2 v[4];
-  __device__ __forceinline__ float2 pair(int k) const { return v[k]; }
-};
-
 template <typename X>
 __device__ __forceinline__ void load_held(const BlockQuantParams& p, int64_t row, int64_t col, Held<X>& h) {
-  const int64_t e = row * p.x_row + col;
-  const X* src = static_cast<const X*>(p.x) + e;
-  if (row < p.rows && p.vec_in && col + 8 <= p.cols) {
-    if constexpr (sizeof(X) == 4) {
-      Pair8<X>::load(src, h.v);
-    } else {
-      const uint4 u = RMSB_DBG_OK(src, 16, kDbgVecLoad) ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
-      h.w[0] = u.x; h.w[1] = u.y; h.w[2] = u.z; h.w[3] = u.w;
-    }
-    return;
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const bool first = row < p.rows && col + 2 * k < p.cols, second = row < p.rows && col + 2 * k + 1 < p.cols;
-    if constexpr (sizeof(X) == 4) {
-      h.v[k] = make_float2(first ? ld1(src + 2 * k) : 0.f, second ? ld1(src + 2 * k + 1) : 0.f);
-    } else {
-      const uint16_t* bits = reinterpret_cast<const uint16_t*>(src);
-      h.w[k] = (first ? ld1(bits + 2 * k) : 0u) | (second ? static_cast<uint32_t>(ld1(bits + 2 * k + 1)) << 16 : 0u);
-    }
-  }
-}
-
-__device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {  // of both halves
-  uint32_t r;
-  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-
-// The largest magnitude (fp32 bits) of each of the thread's rows, over the 16 lanes they lie in.
-template <typename X>
-__device__ __forceinline__ void rows_most(const Held<X> (&h)[8], uint32_t (&most)[8]) {
-  if constexpr (sizeof(X) == 4) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) most[i] = max16(octet_magnitude(h[i].v));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      uint32_t m[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t(&w)[4] = h[i + k].w;
-        m[k] = larger2(larger2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), larger2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-      }
-      // row i's in the low half, the next one's in the high half
-      uint32_t both = larger2(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) both = larger2(both, __shfl_xor_sync(0xffffffffu, both, o));
-      most[i] = Held<X>::widen(both & 0xffffu);
-      most[i + 1] = Held<X>::widen(both >> 16);
-    }
-  }
+  const X* src = static_cast<const X*>(p.x) + row * p.x_row + col;
+  if (row < p.rows && p.vec_in && col + 8 <= p.cols) h.load(src);
+  else h.load(src, row < p.rows ? p.cols - col : 0);
 }
 
 // One 128 x 128 tile a CTA, read once into registers: thread (warp w, lane l) holds rows
@@ -212,7 +130,7 @@ __global__ void __launch_bounds__(256, sizeof(X) == 4 ? 2 : 3) quant_tiles_kerne
   }
   float inv_t[8];  // of this thread's columns
   uint32_t most[8];
-  if (kBlocks || p.q) rows_most<X>(h, most);
+  if (kBlocks || p.q) most_of<X, 16, 8>(h, most);
   if (kBlocks) {
     uint32_t m = most[0];
 #pragma unroll

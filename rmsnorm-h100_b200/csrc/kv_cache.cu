@@ -68,9 +68,14 @@ CacheKernel pick_lanes(int lanes) {
 
 template <bool kWrite, typename X>
 CacheKernel pick(int cache_dtype, int lanes, int items) {
+  constexpr int kMost = kWrite && sizeof(X) == 2 ? 8 : 4;
   if (cache_dtype == RMSNORM_B200_E4M3)
-    return items == 1 ? pick_lanes<kWrite, X, E4M3, 1>(lanes) : pick_lanes<kWrite, X, E4M3, 4>(lanes);
-  return items == 1 ? pick_lanes<kWrite, X, I8, 1>(lanes) : pick_lanes<kWrite, X, I8, 4>(lanes);
+    return items == 1   ? pick_lanes<kWrite, X, E4M3, 1>(lanes)
+           : items == 4 ? pick_lanes<kWrite, X, E4M3, 4>(lanes)
+                        : pick_lanes<kWrite, X, E4M3, kMost>(lanes);
+  return items == 1   ? pick_lanes<kWrite, X, I8, 1>(lanes)
+         : items == 4 ? pick_lanes<kWrite, X, I8, 4>(lanes)
+                      : pick_lanes<kWrite, X, I8, kMost>(lanes);
 }
 
 struct CacheLaunch {
@@ -89,9 +94,10 @@ std::string describe(const void* data) {
 template <bool kWrite>
 int launch(UnitDevice* ud, const rmsnorm_b200_cache_args* c, CacheParams& p, int dtype, cudaStream_t stream) {
   const int lanes = c->head_dim <= 64 ? 8 : c->head_dim <= 128 ? 16 : 32;
-  // four heads of a token in flight a lane, where it has that many and that leaves two CTAs for
-  // every SM
-  const int each = c->heads >= 3 && p.tokens * p.heads * lanes >= int64_t{8} * kCacheThreads * ud->sm_count ? 4 : 1;
+  // four heads of a token in flight a lane, eight when 16-bit values are written (4 registers each),
+  // where it has that many and that leaves two CTAs for every SM
+  const auto enough = [&](int n) { return p.tokens * p.heads * lanes >= int64_t{2} * n * kCacheThreads * ud->sm_count; };
+  const int each = kWrite && dtype != RMSNORM_B200_F32 && c->heads >= 5 && enough(8) ? 8 : c->heads >= 3 && enough(4) ? 4 : 1;
   p.rounds = (c->heads + each - 1) / each;
   p.by_rounds = divisor_of(static_cast<uint32_t>(p.rounds));
   const int64_t per = kCacheThreads / lanes, grid = (p.tokens * p.rounds + per - 1) / per;

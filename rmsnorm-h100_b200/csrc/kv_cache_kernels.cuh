@@ -2,8 +2,6 @@
 // head of a token, and read back.
 #pragma once
 
-#include <type_traits>
-
 #include "block_scale.cuh"
 
 namespace rmsb200 {
@@ -53,13 +51,6 @@ struct CacheParams {
 
 constexpr int kCacheThreads = 256;
 
-template <typename X>
-__device__ __forceinline__ float cache_load1(const void* base, int64_t e) {
-  const X* p = static_cast<const X*>(base) + e;
-  if (!RMSB_DBG_OK(p, sizeof(X), kDbgScalarLoad)) return 0.f;
-  return static_cast<float>(*p);
-}
-
 // Unit i is round i % rounds of token i / rounds.
 __device__ __forceinline__ void cache_unit(const CacheParams& p, int64_t i, int64_t* token, int32_t* round) {
   if (p.small) {
@@ -90,7 +81,7 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid
   constexpr int kGroups = kCacheThreads / kLanes;
   const int lane = threadIdx.x % kLanes, col = lane * 8;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / kLanes;
-  float2 v[kItems][4];
+  Held<X> held[kItems];
   int64_t slot = -1, token = 0;
   int32_t round = 0;
   if (unit < p.tokens * p.rounds) {
@@ -102,18 +93,10 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid
   const X* src = static_cast<const X*>(side.x) + token * side.x_token + head0 * side.x_head + col;
 #pragma unroll
   for (int j = 0; j < kItems; ++j, src += side.x_head) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[j][k] = make_float2(0.f, 0.f);
-    if (j >= heads) continue;
-    if (side.vec_x) {
-      if (col < p.head_dim) Pair8<X>::load(src, v[j]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (col + 2 * k < p.head_dim) v[j][k].x = cache_load1<X>(src, 2 * k);
-        if (col + 2 * k + 1 < p.head_dim) v[j][k].y = cache_load1<X>(src, 2 * k + 1);
-      }
-    }
+    held[j].zero();
+    if (j >= heads || col >= p.head_dim) continue;
+    if (side.vec_x) held[j].load(src);
+    else held[j].load(src, p.head_dim - col);
   }
   // no lane leaves before the last shuffle: its slot may differ from its neighbours'
   const bool beyond = slot >= p.pages * p.page_size;
@@ -123,15 +106,15 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid
   const int64_t place = kept ? slot - page * p.page_size : 0;
   float* scale = side.scales + page * side.s_page + place * side.s_slot + head0 * side.s_head;
   unsigned char* dst = side.data + page * side.page + place * side.slot + head0 * side.head + col;
+  uint32_t largest_bits[kItems];
+  most_of<X, kLanes, kItems>(held, largest_bits);
+  if (!kept) return;
 #pragma unroll
   for (int j = 0; j < kItems; ++j) {
-    uint32_t most = magnitude(largest8(0.f, v[j]));
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (!kept || j >= heads) continue;
+    if (j >= heads) break;
     constexpr float kTop = std::is_same<Q, I8>::value ? 127.f : 448.f, kInvTop = 1.f / kTop;
-    const float largest = __uint_as_float(most);
-    const int e = static_cast<int>(most >> 23);
+    const float largest = __uint_as_float(largest_bits[j]);
+    const int e = static_cast<int>(largest_bits[j] >> 23);
     // max |x| / Q by the same correction, which infinity does not survive
     float s0 = largest * kInvTop;
     s0 = e == 255 ? largest : fmaf(fmaf(-s0, kTop, largest), kInvTop, s0);
@@ -142,12 +125,13 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid
     const float times = least ? 8.5070592e37f : kTop * power;  // 2^126
     const float by = least ? 1.f : e < 255 ? largest * power : 0.f;  // infinity: no remainder
     const float inv = inverse(!least && e == 255 ? largest : by);
+    float2 v[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float2 n = mul2(v[j][k], splat2(times)), q = mul2(n, splat2(inv));
-      v[j][k] = fma2(fma2(q, splat2(-by), n), splat2(inv), q);
+      const float2 n = mul2(held[j].pair(k), splat2(times)), q = mul2(n, splat2(inv));
+      v[k] = fma2(fma2(q, splat2(-by), n), splat2(inv), q);
     }
-    const uint2 b = make_uint2(Q::pack4(v[j][0], v[j][1]), Q::pack4(v[j][2], v[j][3]));
+    const uint2 b = make_uint2(Q::pack4(v[0], v[1]), Q::pack4(v[2], v[3]));
     unsigned char* to = dst + j * side.head;
     if (side.vec_q) {
       if (RMSB_DBG_OK(to, 8, kDbgVecStore)) *reinterpret_cast<uint2*>(to) = b;
