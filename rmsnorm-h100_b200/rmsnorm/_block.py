@@ -77,10 +77,9 @@ def _quantize(x: Tensor, rows: int, want: bool, want_t: bool, column_major: bool
     if sums_dtype is not None:
         sums = torch.empty(k, dtype=sums_dtype, device=device)
     args = _QUANT.pack(
-        n, k, x.data_ptr(), x.stride(0), q.data_ptr() if want else 0, q.stride(0) if want else 0,
-        scales.data_ptr() if want else 0, sr, sg, q_t.data_ptr() if want_t else 0, q_t.stride(0) if want_t else 0,
-        scales_t.data_ptr() if want_t else 0, 0 if sums is None else sums.data_ptr(), _CODE[x.dtype], rows,
-        0 if sums is None else _CODE[sums_dtype], 0)
+        n, k, x.data_ptr(), x.stride(0), q.data_ptr() if want else 0, -(-k // 16) * 16, scales.data_ptr() if want else 0, sr, sg,
+        q_t.data_ptr() if want_t else 0, -(-n // 16) * 16, scales_t.data_ptr() if want_t else 0,
+        0 if sums is None else sums.data_ptr(), _CODE[x.dtype], rows, 0 if sums is None else _CODE[sums_dtype], 0)
     nbytes, ws = 0, None
     if sums is not None:
         name = "rmsnorm_b200_block_quant_workspace_size"
@@ -121,37 +120,18 @@ def block_quantize(x: Tensor, block_rows: int = 1, transposed: bool = False, sca
     return (q, scales, q_t, scales_t) if transposed else (q, scales)
 
 
-def _mm(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, b_rows: int, bias: Optional[Tensor],
-        out_dtype: torch.dtype, power_of_two: bool) -> Tensor:
-    """The product of matrices."""
-    m, k = a.shape
-    n = b.shape[0]
-    device = a.device
-    out = torch.empty(m, n, dtype=out_dtype, device=device)
-    args = _MM.pack(
-        m, n, k, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), a_scales.data_ptr(), *a_scales.stride(),
-        b_scales.data_ptr(), *b_scales.stride(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), b_rows,
-        0 if bias is None else _CODE[bias.dtype], _CODE[out_dtype], power_of_two)
-    nbytes, ws = 0, None
-    if (a.data_ptr() | b.data_ptr() | a.stride(0) | b.stride(0)) & 15:
-        name = "rmsnorm_b200_block_mm_workspace_size"
-        nbytes = _lib.workspace_bytes(_lib.packed_entry(name, _BYTES, _OUT), name, device.index, args)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    name = "rmsnorm_b200_block_mm"
-    _lib.enqueue(_lib.packed_entry(name, _BYTES, _STREAM, _SIZE, _STREAM), name, device.index, args,
-                 None if ws is None else ws.data_ptr(), nbytes)
-    return out
-
-
-def _check_bias(bias: Optional[Tensor], n: int, device: torch.device) -> None:
+def _check_bias(bias: Optional[Tensor], n: int, device: torch.device) -> int:
+    """Its dtype code."""
     if bias is None:
-        return
-    if bias.dtype not in _CODE:
+        return 0
+    code = _CODE.get(bias.dtype)
+    if code is None:
         _check_tensor_dtype("Bias", bias)
     if bias.shape != (n,):
         raise ValueError(f"bias shape must be (N,) with N={n}, got {tuple(bias.shape)}")
     if bias.device != device:
         _check_same_device("bias", bias, device)
+    return code
 
 
 def block_mm(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, bias: Optional[Tensor] = None,
@@ -175,35 +155,65 @@ def block_mm(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, bias: Opt
         raise AssertionError("a and b must be float8_e4m3fn")
     if a_scales.dtype != torch.float32 or b_scales.dtype != torch.float32:
         raise AssertionError("scales must be float32")
-    if out_dtype not in _CODE:
+    oc = _CODE.get(out_dtype)
+    if oc is None:
         _check_optional_dtype("out_dtype", out_dtype)
-    if not a.shape or not a.shape[-1]:
-        _check_x_shape(a.shape)
-    k, device = a.shape[-1], a.device
-    if b.dim() != 2 or b.shape[1] != k or not b.shape[0]:
-        raise ValueError(f"b must be (N, K) with K={k} and at least one row, got {tuple(b.shape)}")
-    n, groups = b.shape[0], -(-k // _BLOCK)
-    if a_scales.shape != a.shape[:-1] + (groups,):
-        raise ValueError(f"a_scales must be {tuple(a.shape[:-1] + (groups,))}, got {tuple(a_scales.shape)}")
-    if b_scales.shape == (-(-n // _BLOCK), groups):
+    shape, b_shape = a.shape, b.shape
+    if not shape or not shape[-1]:
+        _check_x_shape(shape)
+    k, device = shape[-1], a.device
+    if len(b_shape) != 2 or b_shape[1] != k or not b_shape[0]:
+        raise ValueError(f"b must be (N, K) with K={k} and at least one row, got {tuple(b_shape)}")
+    n, groups = b_shape[0], -(-k // _BLOCK)
+    matrix = len(shape) == 2
+    s_shape = a_scales.shape
+    if len(s_shape) != len(shape) or s_shape[-1] != groups or s_shape[:-1] != shape[:-1]:
+        raise ValueError(f"a_scales must be {tuple(shape[:-1] + (groups,))}, got {tuple(s_shape)}")
+    bs_rows = b_scales.shape[0] if b_scales.dim() == 2 and b_scales.shape[1] == groups else -1
+    if bs_rows == -(-n // _BLOCK):
         b_rows = _BLOCK
-    elif b_scales.shape == (n, groups):
+    elif bs_rows == n:
         b_rows = 1
     else:
         raise ValueError(f"b_scales must be {(n, groups)} or {(-(-n // _BLOCK), groups)}, got {tuple(b_scales.shape)}")
-    for name, t in (("a_scales", a_scales), ("b", b), ("b_scales", b_scales)):
-        if t.device != device:
+    if a_scales.device != device or b.device != device or b_scales.device != device:
+        for name, t in (("a_scales", a_scales), ("b", b), ("b_scales", b_scales)):
             _check_same_device(name, t, device)
-    _check_bias(bias, n, device)
-    a2, b2 = _rows_of(a), _rows_of(b)
-    s2 = a_scales if a_scales.dim() == 2 else a_scales.reshape(a2.shape[0], groups)
-    if a.is_cuda:
-        out = _mm(a2, s2, b2, b_scales, b_rows, None if bias is None else bias.contiguous(), out_dtype, bool(power_of_two))
-    else:
+    bias_code = 0
+    if bias is not None:
+        bias_code = _check_bias(bias, n, device)
+        bias = bias.contiguous()
+    if not matrix:
+        a = a.reshape(shape[:-1].numel(), k)
+        a_scales = a_scales.reshape(a.shape[0], groups)
+    a_row, a_step = a.stride()
+    if a_step != 1 and k > 1:
+        a = a.contiguous()
+        a_row = k
+    b_row, b_step = b.stride()
+    if b_step != 1 and k > 1:
+        b = b.contiguous()
+        b_row = k
+    if not a.is_cuda:
         with torch.no_grad():
-            out = _host.block_values(a2, s2, 1) @ _host.block_values(b2, b_scales, b_rows).t()
+            out = _host.block_values(a, a_scales, 1) @ _host.block_values(b, b_scales, b_rows).t()
             out = (out if bias is None else out + bias.float()).to(out_dtype)
-    return out if a.dim() == 2 else out.view(*a.shape[:-1], n)
+        return out if matrix else out.view(*shape[:-1], n)
+    m = a.shape[0]
+    out = torch.empty(m, n, dtype=out_dtype, device=device)
+    a_ptr, b_ptr = a.data_ptr(), b.data_ptr()
+    args = _MM.pack(
+        m, n, k, a_ptr, a_row, b_ptr, b_row, a_scales.data_ptr(), *a_scales.stride(), b_scales.data_ptr(),
+        *b_scales.stride(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), b_rows, bias_code, oc, bool(power_of_two))
+    nbytes = ws = None
+    if (a_ptr | b_ptr | a_row | b_row) & 15:
+        name = "rmsnorm_b200_block_mm_workspace_size"
+        nbytes = _lib.workspace_bytes(_lib.packed_entry(name, _BYTES, _OUT), name, device.index, args)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    name = "rmsnorm_b200_block_mm"
+    _lib.enqueue(_lib.packed_entry(name, _BYTES, _STREAM, _SIZE, _STREAM), name, device.index, args,
+                 None if ws is None else ws.data_ptr(), nbytes or 0)
+    return out if matrix else out.view(*shape[:-1], n)
 
 
 class BlockLinearFunction(torch.autograd.Function):

@@ -42,13 +42,13 @@ def _check_cache(k_cache: Tensor, v_cache: Tensor, k_scales: Tensor, v_scales: T
     if not 1 <= heads <= _MAX_HEADS or not 1 <= d <= _MAX_HEAD_DIM or page_size < 1:
         raise ValueError(f"a cache has 1 to {_MAX_HEADS} heads of 1 to {_MAX_HEAD_DIM} columns and pages of at least one "
                          f"slot, got {tuple(shape)}")
-    device = k_cache.device
-    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
-        if t.dtype != torch.float32 or t.shape != shape[:3]:
-            raise ValueError(f"{name} must be float32 {tuple(shape[:3])}, got {t.dtype} {tuple(t.shape)}")
-    for name, t in (("v_cache", v_cache), ("k_scales", k_scales), ("v_scales", v_scales)):
-        if t.device != device:
-            raise ValueError(f"{name} must be on the same device as k_cache")
+    f32, lead, device = torch.float32, shape[:3], k_cache.device
+    if k_scales.dtype != f32 or v_scales.dtype != f32 or k_scales.shape != lead or v_scales.shape != lead:
+        for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+            if t.dtype != f32 or t.shape != lead:
+                raise ValueError(f"{name} must be float32 {tuple(lead)}, got {t.dtype} {tuple(t.shape)}")
+    if v_cache.device != device or k_scales.device != device or v_scales.device != device:
+        raise ValueError("v_cache, k_scales and v_scales must be on the same device as k_cache")
     ks, vs = k_cache.stride(), v_cache.stride()
     if d > 1 and (ks[3] != 1 or vs[3] != 1):
         raise ValueError("a cache's heads must be contiguous")
@@ -62,15 +62,21 @@ def _repeats(t: Tensor) -> bool:
     return 0 in stride and any(s == 0 and n > 1 for s, n in zip(stride, t.shape))
 
 
-def _heads_of(name: str, t: Tensor, lead, cache: Tensor) -> Tensor:
-    """t as [tokens, heads, head_dim], a view wherever the strides allow one."""
-    if t.shape != (*lead, *cache.shape[2:]):
-        raise ValueError(f"{name} must be {(*lead, *cache.shape[2:])}, got {tuple(t.shape)}")
-    if t.device != cache.device:
+def _heads_of(name: str, t: Tensor, shape: torch.Size, device: torch.device) -> Tuple[Tensor, Tuple[int, int, int]]:
+    """t as [tokens, heads, head_dim], a view wherever the strides allow one; its address, token
+    stride and head stride."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
         raise ValueError(f"{name} must be on the same device as k_cache")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    stride = t.stride()
+    if stride[-1] != 1 and shape[-1] > 1:
         t = t.contiguous()
-    return t if t.dim() == 3 else t.reshape(lead.numel(), *cache.shape[2:])
+        stride = t.stride()
+    if len(stride) != 3:
+        t = t.reshape(shape[:-2].numel(), *shape[-2:])
+        stride = t.stride()
+    return t, (t.data_ptr(), stride[0], stride[1])
 
 
 def cache_write(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, k_scales: Tensor, v_scales: Tensor,
@@ -102,14 +108,17 @@ def cache_write(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, k_scales
         raise ValueError(f"slots must have k's leading shape {tuple(lead)}, got {tuple(slots.shape)}")
     if slots.device != k_cache.device:
         raise ValueError("slots must be on the same device as k_cache")
-    kf, vf = _heads_of("k", k, lead, k_cache), _heads_of("v", v, lead, k_cache)
+    shape = lead + k_cache.shape[2:]
+    kf, k_place = _heads_of("k", k, shape, k_cache.device)
+    vf, v_place = _heads_of("v", v, shape, k_cache.device)
     written = (k_cache, v_cache, k_scales, v_scales)
     for t in written:
         if _repeats(t):
             raise ValueError("caches and scales must have places of their own, not be expanded views")
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError("cache_write is outside autograd: caches and scales must not require gradients")
-    slots = slots.reshape(-1)
+    if len(lead) != 1:
+        slots = slots.reshape(-1)
     if not k_cache.is_cuda:
         keep = slots >= 0
         at = slots[keep].long()
@@ -121,8 +130,7 @@ def cache_write(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, k_scales
             _host.cache_write(vf[keep], v_cache, v_scales, page, place, _TOP[k_cache.dtype])
         return
     slots = slots.contiguous()
-    args = _WRITE.pack(slots.numel(), kf.data_ptr(), *kf.stride()[:2], vf.data_ptr(), *vf.stride()[:2], slots.data_ptr(),
-                       slots.dtype == torch.int64, code)
+    args = _WRITE.pack(slots.shape[0], *k_place, *v_place, slots.data_ptr(), slots.dtype == torch.int64, code)
     name = "rmsnorm_b200_cache_write"
     _lib.enqueue(_lib.packed_entry(name, _BYTES, _BYTES, _STREAM), name, k_cache.device.index, cache, args)
     torch.autograd.graph.increment_version(written)
