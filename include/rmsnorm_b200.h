@@ -442,7 +442,8 @@ typedef struct rmsnorm_b200_block_quant_args {
   int64_t scale_group_stride;
   void* q_t;                  /* nullable, [cols, rows] */
   int64_t q_t_row_stride;
-  float* scales_t;            /* [cols or blocks of columns][groups of rows], contiguous */
+  float* scales_t;            /* column by column, as products read them: of (column or block of columns j,
+                               * group of rows g) at g * (columns or blocks of columns) + j */
   void* column_sums;          /* nullable, [cols] */
   int32_t x_dtype;
   int32_t block_rows;         /* 1 or 128, for x and for x transposed */

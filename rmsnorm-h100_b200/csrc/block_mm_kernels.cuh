@@ -92,9 +92,9 @@ __device__ __forceinline__ void store_turned(float* mine, const float2 (&v)[8], 
 
 // acc += sums * scale, or acc += sums * (column scales) * scale.
 template <bool kRowScales>
-__device__ __forceinline__ void add_scaled(float2* acc, const float2 (&v)[16], float s, const float* col) {
+__device__ __forceinline__ void add_scaled(float2* acc, const float2 (&v)[8], float s, const float* col) {
 #pragma unroll
-  for (int i = 0; i < 16; i += 2) {
+  for (int i = 0; i < 8; i += 2) {
     if constexpr (kRowScales) {
       const float4 c = *reinterpret_cast<const float4*>(col + 2 * i);
       acc[i] = fma2(mul2(v[i], make_float2(c.x, c.y)), splat2(s), acc[i]);
@@ -261,22 +261,20 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         __syncwarp();
         tmem_fence_after_sync();
         const uint32_t at = from + d * kWideN;
-        float2 v0[16], v1[16];
-        tmem_ld(at, v0);
-        tmem_landed(v0);
-        tmem_ld(at + 32, v1);
-        add_scaled<kRowScales>(acc, v0, s, cols);
-        tmem_landed(v1);
-        tmem_ld(at + 64, v0);
-        add_scaled<kRowScales>(acc + 16, v1, s, cols + 32);
-        tmem_landed(v0);
-        tmem_ld(at + 96, v1);
-        add_scaled<kRowScales>(acc + 32, v0, s, cols + 64);
-        tmem_landed(v1);
-        tmem_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_peer(&bars->sum_empty[d], 0);
-        add_scaled<kRowScales>(acc + 48, v1, s, cols + 96);
+        float2 v[2][8];
+        tmem_ld(at, v[0]);
+        tmem_landed(v[0]);
+#pragma unroll
+        for (int c = 0; c < kWideHalf / 16; ++c) {
+          if (c + 1 < kWideHalf / 16) tmem_ld(at + (c + 1) * 16, v[(c + 1) & 1]);
+          add_scaled<kRowScales>(acc + 8 * c, v[c & 1], s, cols + 16 * c);
+          if (c + 1 < kWideHalf / 16) tmem_landed(v[(c + 1) & 1]);
+          if (c + 2 == kWideHalf / 16) {
+            tmem_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_peer(&bars->sum_empty[d], 0);
+          }
+        }
       }
       const int64_t e = row * p.n + col0;
       const int left = static_cast<int>(min(static_cast<int64_t>(kWideHalf), p.n - col0));

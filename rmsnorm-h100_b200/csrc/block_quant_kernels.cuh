@@ -146,8 +146,7 @@ __global__ void __launch_bounds__(256, sizeof(X) == 4 ? 2 : 3) quant_tiles_kerne
     if (threadIdx.x == 0) {
       if (p.q) st1(p.scales + tile_r * p.scale_row + tile_c * p.scale_group, __uint_as_float(s));
       if (p.q_t) {
-        const int64_t tiles_r = (p.rows + kBlock - 1) / kBlock;
-        st1(p.scales_t + tile_c * tiles_r + tile_r, __uint_as_float(s));
+        st1(p.scales_t + static_cast<int64_t>(tile_r) * tiles_c + tile_c, __uint_as_float(s));
       }
     }
 #pragma unroll
@@ -214,10 +213,7 @@ __global__ void __launch_bounds__(256, sizeof(X) == 4 ? 2 : 3) quant_tiles_kerne
     for (int k = 0; k < 8; ++k) {
       const uint32_t s = power_scale(m[k]);
       inv_t[k] = power_inverse(s);
-      if (warp == 0 && half == 0 && col + k < p.cols) {
-        const int64_t groups_t = (p.rows + kBlock - 1) / kBlock;
-        st1(p.scales_t + (col + k) * groups_t + tile_r, __uint_as_float(s));
-      }
+      if (warp == 0 && half == 0 && col + k < p.cols) st1(p.scales_t + tile_r * p.cols + col + k, __uint_as_float(s));
     }
   }
   if (p.q_t) {

@@ -73,7 +73,7 @@ def _quantize(x: Tensor, rows: int, want: bool, want_t: bool, column_major: bool
             scales = torch.empty(gn, gk, dtype=torch.float32, device=device)
     if want_t:
         q_t = _bytes_empty((k, n), device)
-        scales_t = torch.empty(gk if rows > 1 else k, -(-n // _BLOCK), dtype=torch.float32, device=device)
+        scales_t = torch.empty(-(-n // _BLOCK), gk if rows > 1 else k, dtype=torch.float32, device=device).t()
     if sums_dtype is not None:
         sums = torch.empty(k, dtype=sums_dtype, device=device)
     args = _QUANT.pack(
@@ -100,8 +100,9 @@ def block_quantize(x: Tensor, block_rows: int = 1, transposed: bool = False, sca
 
     A scale is the smallest power of two that brings the largest |x| to 448 or below, at least
     2^-126; q is x / scale, which is exact, rounded to nearest even. A NaN makes its scale NaN,
-    an infinity infinite. `scales_column_major` lays q's scales out column by column. q's rows
-    begin at multiples of 16 bytes: where K is none, q is a view of wider rows."""
+    an infinity infinite. `scales_column_major` lays q's scales out column by column, as scales_t
+    are: large products read them faster so. The rows of q and q_t begin at multiples of 16 bytes:
+    where their length is none, they are views of wider rows."""
     if _is_compiling():
         return _quantize_untraced(x, block_rows, transposed, scales_column_major)
     if x.dtype not in _CODE:
@@ -187,44 +188,54 @@ def block_mm(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, bias: Opt
         a = a.reshape(shape[:-1].numel(), k)
         a_scales = a_scales.reshape(a.shape[0], groups)
     a_row, a_step = a.stride()
-    if a_step != 1 and k > 1:
+    if a_step != 1 and k > 1 or a_row < k:  # a column by column, or rows that overlap
         a = a.contiguous()
         a_row = k
     b_row, b_step = b.stride()
-    if b_step != 1 and k > 1:
+    if b_step != 1 and k > 1 or b_row < k:
         b = b.contiguous()
         b_row = k
+    out = _product(a, a_row, a_scales, b, b_row, b_scales, b_rows, bias, bias_code, out_dtype, oc, bool(power_of_two))
+    return out if matrix else out.view(*shape[:-1], n)
+
+
+def _product(a, a_row, a_scales, b, b_row, b_scales, b_rows, bias, bias_code, out_dtype, oc, power_of_two) -> Tensor:
+    """The product of checked matrices with rows a_row and b_row apart."""
     if not a.is_cuda:
         with torch.no_grad():
             out = _host.block_values(a, a_scales, 1) @ _host.block_values(b, b_scales, b_rows).t()
-            out = (out if bias is None else out + bias.float()).to(out_dtype)
-        return out if matrix else out.view(*shape[:-1], n)
-    m = a.shape[0]
+            return (out if bias is None else out + bias.float()).to(out_dtype)
+    m, k = a.shape
+    n, device = b.shape[0], a.device
     out = torch.empty(m, n, dtype=out_dtype, device=device)
     a_ptr, b_ptr = a.data_ptr(), b.data_ptr()
     args = _MM.pack(
         m, n, k, a_ptr, a_row, b_ptr, b_row, a_scales.data_ptr(), *a_scales.stride(), b_scales.data_ptr(),
-        *b_scales.stride(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), b_rows, bias_code, oc, bool(power_of_two))
-    nbytes = ws = None
+        *b_scales.stride(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), b_rows, bias_code, oc, power_of_two)
+    nbytes, ws = 0, None
     if (a_ptr | b_ptr | a_row | b_row) & 15:
         name = "rmsnorm_b200_block_mm_workspace_size"
         nbytes = _lib.workspace_bytes(_lib.packed_entry(name, _BYTES, _OUT), name, device.index, args)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     name = "rmsnorm_b200_block_mm"
     _lib.enqueue(_lib.packed_entry(name, _BYTES, _STREAM, _SIZE, _STREAM), name, device.index, args,
-                 None if ws is None else ws.data_ptr(), nbytes or 0)
-    return out if matrix else out.view(*shape[:-1], n)
+                 None if ws is None else ws.data_ptr(), nbytes)
+    return out
 
 
 class BlockLinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        x2 = _rows_of(x)
-        q, s, x_t, x_ts, _ = _quantize(x2, 1, True, ctx.needs_input_grad[1], True)
-        w, ws, w_t, w_ts, _ = _quantize(_rows_of(weight), _BLOCK, True, ctx.needs_input_grad[0])
+        x2, need = _rows_of(x), ctx.needs_input_grad
+        q, s, x_t, x_ts, _ = _quantize(x2, 1, True, need[1], True)
+        w, ws, w_t, w_ts, _ = _quantize(_rows_of(weight), _BLOCK, True, need[0])
         ctx.save_for_backward(x_t, x_ts, w_t, w_ts)
         ctx.x_shape, ctx.dtypes = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
-        return block_mm(q, s, w, ws, bias, x.dtype, True).view(*x.shape[:-1], weight.shape[0])
+        code = 0
+        if bias is not None:
+            bias, code = bias.contiguous(), _CODE[bias.dtype]
+        y = _product(q, _pitch(q), s, w, _pitch(w), ws, _BLOCK, bias, code, x.dtype, _CODE[x.dtype], True)
+        return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     def backward(ctx, dy):
@@ -234,13 +245,19 @@ class BlockLinearFunction(torch.autograd.Function):
         dx = dw = db = None
         q, s, d_t, d_ts, db = _quantize(_rows_of(dy), 1, need_x, need_w, True, b_dtype if need_b else None)
         if need_x:
-            dx = block_mm(q, s, w_t, w_ts, None, x_dtype, True).view(ctx.x_shape)
+            dx = _product(q, _pitch(q), s, w_t, _pitch(w_t), w_ts, _BLOCK, None, 0, x_dtype, _CODE[x_dtype], True)
+            dx = dx.view(ctx.x_shape)
         if need_w:
             if d_t.shape[1]:
-                dw = block_mm(d_t, d_ts, x_t, x_ts, None, w_dtype, True)
+                dw = _product(d_t, _pitch(d_t), d_ts, x_t, _pitch(x_t), x_ts, 1, None, 0, w_dtype, _CODE[w_dtype], True)
             else:
                 dw = torch.zeros(d_t.shape[0], x_t.shape[0], dtype=w_dtype, device=dy.device)
         return first_order("block_linear", (dx, dw, db))
+
+
+def _pitch(q: Tensor) -> int:
+    """How far apart the rows of `_quantize`'s matrices are."""
+    return -(-q.shape[1] // 16) * 16
 
 
 def block_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None) -> Tensor:

@@ -112,6 +112,8 @@ def cache_write(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, k_scales
     kf, k_place = _heads_of("k", k, shape, k_cache.device)
     vf, v_place = _heads_of("v", v, shape, k_cache.device)
     written = (k_cache, v_cache, k_scales, v_scales)
+    if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel() and slots.numel():
+        raise ValueError("k_cache and v_cache must be different tensors")
     for t in written:
         if _repeats(t):
             raise ValueError("caches and scales must have places of their own, not be expanded views")
@@ -170,6 +172,8 @@ def cache_read(k_cache: Tensor, v_cache: Tensor, k_scales: Tensor, v_scales: Ten
         k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
     else:
         k, v = out
+        if k is v or k.data_ptr() == v.data_ptr() and k.numel():
+            raise ValueError("out must be two different tensors")
         for t in out:
             if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
                 raise ValueError(f"out must be two contiguous {dtype} tensors of shape {shape} on {device}")

@@ -183,6 +183,8 @@ def test_cache_refusals():
     for error, match, args in bad:
         with pytest.raises(error, match=match):
             fused.cache_write(*args)
+    with pytest.raises(ValueError, match="different"):
+        fused.cache_write(k, k, c[0], c[0], c[2], c[3], slots)
     grad = [*c[:3], c[3].clone().requires_grad_(True)]
     with pytest.raises(ValueError, match="autograd"):
         fused.cache_write(k, k, *grad, slots)
@@ -194,8 +196,9 @@ def test_cache_refusals():
         ("starts", (*c, table, starts.long(), 5)),
         ("starts", (*c, table, starts[:2], 5)),
         ("negative", (*c, table, starts, -1)),
-        ("out must be", (*c, table, starts, 5, torch.bfloat16, (k, k))),
-        ("out must be", (*c, table, starts, 5, torch.float32, (k[:4], k))),
+        ("out must be", (*c, table, starts, 5, torch.bfloat16, (k, k.clone()))),
+        ("out must be", (*c, table, starts, 5, torch.float32, (k[:4], k.clone()))),
+        ("different", (*c, table, starts, 5, torch.float32, (k, k))),
         ("same device", (*c, table.to("meta"), starts, 5)),
     ]
     for match, args in bad:
@@ -283,3 +286,27 @@ def test_c_entries_check_their_arguments():
                    dict(v=0), dict(page_table=0), dict(dtype=4)):
         assert make(read=change)[1] == 1, change
     assert make(write=dict(tokens=0), read=dict(tokens=0)) == (0, 0)
+
+
+def test_untraced_under_compile():
+    """A graph break each, as the other fused operators."""
+    x, w = torch.randn(6, 200), torch.randn(5, 200)
+    k, slots = torch.randn(5, 2, 16), torch.arange(5)
+
+    def f(x):
+        q, s = fused.block_quantize(x + 0)
+        b, sb = fused.block_quantize(w, 128)
+        c = _cache()
+        fused.cache_write(k, k, *c, slots)
+        r = fused.cache_read(*c, torch.arange(3, dtype=torch.int32)[None], torch.tensor([0, 5], dtype=torch.int32), 5)
+        return fused.block_mm(q, s, b, sb) + 1, fused.block_linear(x, w) * 2, r[0]
+
+    for got, want in zip(torch.compile(f, backend="eager")(x), f(x)):
+        assert torch.equal(got, want)
+
+
+def test_product_of_expanded_and_overlapping_rows():
+    a, sa = fused.block_quantize(torch.randn(1, 128))
+    b, sb = fused.block_quantize(torch.randn(6, 128))
+    out = fused.block_mm(a.expand(4, 128), sa.expand(4, 1), b, sb, out_dtype=torch.float32)
+    assert torch.equal(out, fused.block_mm(a, sa, b, sb, out_dtype=torch.float32).expand(4, 6))

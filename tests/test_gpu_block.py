@@ -183,6 +183,17 @@ def test_product_of_norm_outputs_and_leading_dimensions():
     assert fused.block_mm(q[:0], s[:0], wq, ws).shape == (0, 50, 200)
 
 
+def test_product_of_expanded_and_overlapping_rows():
+    a, sa = operand(1, 256, 1, 1)
+    b, sb = operand(300, 256, 1, 2)
+    out = fused.block_mm(a.expand(40, 256), sa.expand(40, 2), b, sb[:1].expand(300, 2), out_dtype=F32)
+    ref.check_product(out, ref.values(a, sa).expand(40, 256), ref.values(b, sb[:1].expand(300, 2)), None, "expanded")
+    long, _ = operand(1, 400, 1, 3)
+    windows = long.as_strided((20, 256), (7, 1))
+    out = fused.block_mm(windows, sa.expand(20, 2), b, sb, out_dtype=F32)
+    ref.check_product(out, ref.values(windows.contiguous(), sa.expand(20, 2)), ref.values(b, sb), None, "windows")
+
+
 def test_product_bias_types():
     a, sa = operand(200, 256, 1, 1)
     b, sb = operand(333, 256, 128, 2)
