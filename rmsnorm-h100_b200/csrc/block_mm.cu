@@ -88,17 +88,24 @@ std::string describe(const void* data) {
   return buf;
 }
 
+// Called with the device's lock held.
+template <typename Kernel>
+int prepare(UnitDevice* ud, Kernel kernel) {
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  if (ud->attrs_done.count(fn)) return RMSNORM_B200_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemOptIn) != cudaSuccess)
+    return RMSNORM_B200_ERR_CUDA;
+  ud->attrs_done.insert(fn);
+  return RMSNORM_B200_OK;
+}
+
 template <typename Kernel, typename KernelPlan>
 int launch(UnitDevice* ud, Kernel kernel, const CUtensorMap& ma, const CUtensorMap& mb, const BlockMmParams& p,
            const KernelPlan& kp, int threads, int smem, int cluster, cudaStream_t stream, const MmLaunch& l) {
   {
-    const void* fn = reinterpret_cast<const void*>(kernel);
     std::lock_guard<std::mutex> lock(ud->mu);
-    if (!ud->attrs_done.count(fn)) {
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemOptIn) != cudaSuccess)
-        return RMSNORM_B200_ERR_CUDA;
-      ud->attrs_done.insert(fn);
-    }
+    const int st = prepare(ud, kernel);
+    if (st) return st;
   }
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -121,47 +128,91 @@ int launch(UnitDevice* ud, Kernel kernel, const CUtensorMap& ma, const CUtensorM
   return launched(describe, l);
 }
 
-int repack(const void* src, int64_t row_stride, int64_t rows, int64_t k, void* dst, int64_t pitch, cudaStream_t stream) {
-  const int64_t pieces = pitch / 16, total = rows * pieces;
-  if (total > (int64_t{1} << 31) * 255) return RMSNORM_B200_ERR_UNSUPPORTED;
+int repack(const RepackJob* jobs, int count, int64_t k, int64_t pitch, cudaStream_t stream) {
+  RepackParams p = {};
+  int64_t rows = 0;
+  for (int i = 0; i < count; ++i) {
+    p.job[i] = jobs[i];
+    rows = std::max(rows, jobs[i].rows);
+  }
+  p.k = static_cast<int32_t>(k);
+  p.pieces = static_cast<int32_t>(pitch / 16);
+  if (rows > (int64_t{1} << 38) / p.pieces) return RMSNORM_B200_ERR_UNSUPPORTED;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((total + 255) / 256));
+  cfg.gridDim = dim3(static_cast<unsigned>((rows * p.pieces + 255) / 256), count);
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, repack_kernel, static_cast<const unsigned char*>(src), row_stride, rows,
-                         static_cast<int32_t>(k), static_cast<unsigned char*>(dst), static_cast<int32_t>(pieces)) !=
-      cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, repack_kernel, p) != cudaSuccess) {
     cudaGetLastError();
     return RMSNORM_B200_ERR_CUDA;
   }
   return launched("");
 }
 
+// Clusters of the kernel with `cluster` CTAs that are resident together, a CTA an SM.
+template <typename Kernel>
+int resident(UnitDevice* ud, Kernel kernel, int threads, int cluster, int smem, int* clusters) {
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  std::lock_guard<std::mutex> lock(ud->mu);
+  const auto key = std::make_tuple(fn, cluster, smem);
+  const auto it = ud->clusters.find(key);
+  if (it != ud->clusters.end()) {
+    *clusters = it->second;
+    return RMSNORM_B200_OK;
+  }
+  const int st = prepare(ud, kernel);
+  if (st) return st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster * ud->sm_count);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(clusters, kernel, &cfg) != cudaSuccess) *clusters = 0;
+  cudaGetLastError();
+  ud->clusters[key] = *clusters;
+  return RMSNORM_B200_OK;
+}
+
 template <int T>
 int launch_few(UnitDevice* ud, const void* a, int64_t a_row, const CUtensorMap& map_b, const rmsnorm_b200_block_mm_args* args,
                const BlockMmParams& p, cudaStream_t stream) {
   CUtensorMap map_a;
-  const int st = make_map(&map_a, a, args->m, args->k, a_row, T);
+  int st = make_map(&map_a, a, args->m, args->k, a_row, T);
   if (st) return st;
   FewPlan pl = {};
   pl.tiles_n = static_cast<int>((args->n + kBlock - 1) / kBlock);
   const int64_t tiles = (args->m + T - 1) / T * pl.tiles_n;
   constexpr int fit = T >= 128 ? 1 : 2;  // CTAs an SM
-  // as many CTAs as are resident together, of two groups at least: 1 x 4096 x 4096 in 1, 2, 4 and
-  // 8 parts 11.9, 8.8, 8.2 and 6.9 us, 64 x 8192 x 8192 38.7, 24.2, 17.8 and (512 CTAs) 25.2 us,
-  // 32 x 4096 x 1024 6.5, 5.6, 5.2 and (a group each) 6.3 us
+  // As many parts as are resident together, of two groups at least: 1 x 4096 x 4096 in 1, 2, 4, 6
+  // and 8 parts 11.5, 8.6, 7.7, 7.0 and 6.7 us, 64 x 8192 x 8192 38, 24, 17.3, 24 and 25 us,
+  // 32 x 4096 x 1024 6.8, 5.1, 5.2, -- and (a group each) 6.2 us, 256 x 1024 x 4096 22.6, 12.9, 9.2,
+  // 8.6 and 14.2 us (16 clusters of 8: 15 fit at once).
   pl.splits = static_cast<int>(std::clamp<int64_t>(fit * ud->sm_count / tiles, 1, std::clamp(p.groups / 2, 1, kFewMaxSplits)));
-  const int each = (p.groups + pl.splits - 1) / pl.splits;
-  const int fixed = 1024 + static_cast<int>(sizeof(FewBars)) + 2 * kFewChunk * T * 4;
-  const int room = (fit == 2 ? kSmemOptIn / 2 - 1024 : kSmemOptIn) - fixed;
-  pl.stages = std::min({kFewMaxStages, each, room / Few<T>::kStageBytes});
-  pl.ring_bytes = std::max(pl.stages * Few<T>::kStageBytes, pl.splits > 1 ? T * kBlock * 4 : 0);
-  const int smem = pl.ring_bytes + fixed;
+  int smem = 0;
+  for (;; --pl.splits) {
+    const int each = (p.groups + pl.splits - 1) / pl.splits;
+    const int fixed = 1024 + static_cast<int>(sizeof(FewBars)) + 2 * kFewChunk * T * 4;
+    const int room = (fit == 2 ? kSmemOptIn / 2 - 1024 : kSmemOptIn) - fixed;
+    pl.stages = std::min({kFewMaxStages, each, room / Few<T>::kStageBytes});
+    pl.ring_bytes = std::max(pl.stages * Few<T>::kStageBytes, pl.splits > 1 ? T * kBlock * 4 : 0);
+    smem = pl.ring_bytes + fixed;
+    if (pl.splits == 1) break;
+    int clusters = 0;
+    st = resident<FewKernel>(ud, block_mm_few_kernel<T>, kFewThreads, pl.splits, smem, &clusters);
+    if (st) return st;
+    if (clusters * fit >= tiles) break;
+  }
   if (tiles * pl.splits >= int64_t{1} << 31) return RMSNORM_B200_ERR_UNSUPPORTED;
   const MmLaunch l = {"block_mm_few", static_cast<unsigned>(tiles * pl.splits), T, pl.splits, pl.stages};
   return launch<FewKernel>(ud, block_mm_few_kernel<T>, map_a, map_b, p, pl, kFewThreads, smem, pl.splits, stream, l);
@@ -250,18 +301,22 @@ int run(const rmsnorm_b200_block_mm_args* a, void* ws, size_t ws_bytes, cudaStre
 
   const void *qa = a->a, *qb = a->b;
   int64_t a_row = a->m == 1 ? pl.pitch : a->a_row_stride, b_row = a->n == 1 ? pl.pitch : a->b_row_stride;
+  RepackJob jobs[2];
+  int copies = 0;
   if (pl.copy_a) {
-    st = repack(a->a, a->a_row_stride, a->m, a->k, ws, pl.pitch, stream);
-    if (st) return st;
+    jobs[copies++] = {static_cast<const unsigned char*>(a->a), a->a_row_stride, a->m, static_cast<unsigned char*>(ws)};
     qa = ws;
     a_row = pl.pitch;
   }
   if (pl.copy_b) {
-    void* to = static_cast<unsigned char*>(ws) + pl.copy_a;
-    st = repack(a->b, a->b_row_stride, a->n, a->k, to, pl.pitch, stream);
-    if (st) return st;
+    unsigned char* to = static_cast<unsigned char*>(ws) + pl.copy_a;
+    jobs[copies++] = {static_cast<const unsigned char*>(a->b), a->b_row_stride, a->n, to};
     qb = to;
     b_row = pl.pitch;
+  }
+  if (copies) {
+    st = repack(jobs, copies, a->k, pl.pitch, stream);
+    if (st) return st;
   }
   BlockMmParams p = {};
   p.m = a->m; p.n = static_cast<int32_t>(a->n); p.groups = static_cast<int32_t>(groups);
@@ -270,10 +325,11 @@ int run(const rmsnorm_b200_block_mm_args* a, void* ws, size_t ws_bytes, cudaStre
   p.bias = a->bias; p.bias_dt = a->bias_dtype;
   p.out = a->out; p.out_dt = a->out_dtype;
   p.b_rows = a->b_block_rows == 1;
+  p.vec_bias = aligned_to(a->bias, 16);
   p.vec_out = aligned_to(a->out, 32) && a->n * elem_bytes(a->out_dtype) % 32 == 0;
   // Few rows, or more of them where two CTAs or more could share each 128 x 128 of the result:
-  // the kernel that splits k. K = 4096: 256 x 4096 14.9 against 21.8 us, 1024 x 1024 14.6 against
-  // 21.8 us, 512 x 4096 (128 tiles for 148 SMs) 25.2 against 22.0 us.
+  // the kernel that splits k. K = 4096: 256 x 4096 14.4 against 20.1 us, 1024 x 1024 14.2 against
+  // 20.0 us, 512 x 4096 (128 tiles for 148 SMs) 24.8 against 20.3 us.
   const int64_t squares = (a->m + kBlock - 1) / kBlock * ((a->n + kBlock - 1) / kBlock);
   if (a->m > 128 && (2 * squares > ud->sm_count || groups < 4)) return launch_wide(ud, qa, a_row, qb, b_row, a, p, stream);
   CUtensorMap map_b;

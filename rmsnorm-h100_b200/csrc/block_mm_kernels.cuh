@@ -27,6 +27,7 @@ struct BlockMmParams {
   int32_t bias_dt, out_dt;
   bool b_rows;      // b's scales are per row
   bool vec_out;     // out's rows begin at multiples of 32 bytes
+  bool vec_bias;    // bias begins at one of 16
 };
 
 __device__ __forceinline__ const float* sb_of(const BlockMmParams& p, int64_t n) {
@@ -76,7 +77,7 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
 
 // A warp's 32 rows of 16 columns, a row a lane, where rows begin anywhere: turned through shared
 // memory, so that the warp stores a row's neighbours side by side (1000 x 4100 with K = 1008: 50 us
-// when every lane stored its own row's values one by one, 22 us so).
+// when every lane stored its own row's values one by one, 14 us so).
 __device__ __forceinline__ void store_turned(float* mine, const float2 (&v)[8], const BlockMmParams& p, int64_t row0,
                                              int64_t col0, int left) {
   const int rows = static_cast<int>(max(int64_t{0}, min(int64_t{32}, p.m - row0)));
@@ -86,8 +87,27 @@ __device__ __forceinline__ void store_turned(float* mine, const float2 (&v)[8], 
   for (int i = 0; i < 16; ++i) mine[lane * 17 + i] = i & 1 ? v[i / 2].y : v[i / 2].x;
   __syncwarp();
   const int col = lane & 15;
-  if (col < left)
-    for (int r = lane >> 4; r < rows; r += 2) store1_rt(p.out, p.out_dt, (row0 + r) * p.n + col0 + col, mine[r * 17 + col]);
+  if (col >= left) return;
+  const float bias = p.bias ? load1_rt(p.bias, p.bias_dt, col0 + col) : 0.f;
+  for (int r = lane >> 4; r < rows; r += 2)
+    store1_rt(p.out, p.out_dt, (row0 + r) * p.n + col0 + col, mine[r * 17 + col] + bias);
+}
+
+// Adds bias to 16 columns from col on, a multiple of 16.
+__device__ __forceinline__ void add_bias16(const BlockMmParams& p, int64_t col, float2* v) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float2 b[4];
+    if (p.vec_bias) {
+      load8p_rt(p.bias, p.bias_dt, col + 8 * k, b);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        b[i] = make_float2(load1_rt(p.bias, p.bias_dt, col + 8 * k + 2 * i), load1_rt(p.bias, p.bias_dt, col + 8 * k + 2 * i + 1));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[4 * k + i] = add2(v[4 * k + i], b[i]);
+  }
 }
 
 // acc += sums * scale, or acc += sums * (column scales) * scale.
@@ -221,7 +241,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       const int64_t row = static_cast<int64_t>(tm) * kWideRows + rank * kBlock + (warp & 3) * 32 + lane;
       const int64_t col0 = static_cast<int64_t>(tn) * kWideN + half * kWideHalf;
       const bool live = row < p.m;
-      // scales two groups ahead; b's per row: thread i of the 256 brings column i's, else every
+      // scales kAhead groups ahead; b's per row: thread i of the 256 brings column i's, else every
       // thread its half's
       const int64_t own = kRowScales ? static_cast<int64_t>(tn) * kWideN + threadIdx.x : col0;
       const bool own_live = own < p.n;
@@ -237,26 +257,35 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         sb += p.sb_group;
         return v;
       };
-      float a0 = next_a(0), a1 = next_a(1), b0 = next_b(0), b1 = next_b(1);
+      constexpr int kAhead = 2;
+      float a[kAhead], b[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        a[i] = next_a(i);
+        b[i] = next_b(i);
+      }
       float2 acc[kWideHalf / 2];
 #pragma unroll
       for (int i = 0; i < kWideHalf / 2; ++i) acc[i] = make_float2(0.f, 0.f);
       for (int g = 0; g < p.groups; ++g, ++u) {
         const uint32_t d = u & 1u;
-        float s = a0;
+        float s = a[0];
         const float* cols = col_scales + d * kWideN;
         if constexpr (kRowScales) {
-          col_scales[d * kWideN + threadIdx.x] = b0;
+          col_scales[d * kWideN + threadIdx.x] = b[0];
           __syncwarp();
           named_barrier(1, 256);
           cols += half * kWideHalf;
         } else {
-          s *= b0;
+          s *= b[0];
         }
-        a0 = a1;
-        b0 = b1;
-        a1 = next_a(g + 2);
-        b1 = next_b(g + 2);
+#pragma unroll
+        for (int i = 0; i + 1 < kAhead; ++i) {
+          a[i] = a[i + 1];
+          b[i] = b[i + 1];
+        }
+        a[kAhead - 1] = next_a(g + kAhead);
+        b[kAhead - 1] = next_b(g + kAhead);
         mbar_spin_warp(&bars->sum[d], (u >> 1) & 1u, kSiteMmSum);
         __syncwarp();
         tmem_fence_after_sync();
@@ -278,14 +307,6 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       }
       const int64_t e = row * p.n + col0;
       const int left = static_cast<int>(min(static_cast<int64_t>(kWideHalf), p.n - col0));
-      if (p.bias) {
-#pragma unroll
-        for (int i = 0; i < kWideHalf / 2; ++i) {
-          const float x = 2 * i < left ? load1_rt(p.bias, p.bias_dt, col0 + 2 * i) : 0.f;
-          const float y = 2 * i + 1 < left ? load1_rt(p.bias, p.bias_dt, col0 + 2 * i + 1) : 0.f;
-          acc[i] = add2(acc[i], make_float2(x, y));
-        }
-      }
       if (!p.vec_out || left < kWideHalf) {
         float* mine = reinterpret_cast<float*>(staging + warp * kStagingBytes);
 #pragma unroll
@@ -295,9 +316,14 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           for (int i = 0; i < 8; ++i) v[i] = acc[c / 2 + i];
           if (c < left) store_turned(mine, v, p, row - lane, col0 + c, left - c);
         }
-      } else if (!live) {
         continue;
-      } else if (p.out_dt == RMSNORM_B200_F32) {
+      }
+      if (!live) continue;
+      if (p.bias) {
+#pragma unroll
+        for (int c = 0; c < kWideHalf; c += 16) add_bias16(p, col0 + c, acc + c / 2);
+      }
+      if (p.out_dt == RMSNORM_B200_F32) {
         float* out = static_cast<float*>(p.out) + e;
 #pragma unroll
         for (int i = 0; i < kWideHalf; i += 8) {
@@ -334,13 +360,13 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 // summing warps only bring results out. Tiles of 224 or 192 columns leave tensor memory for two of
 // them, so that one comes out while the next is summed, and for the exponents; one of 256 comes out
 // before the next begins, for pairs that have a single tile or two.
-// Measured: 8192 x 16384 x 4096 410 us (2680 TFLOP/s, at the card's power limit), scaled in
-// registers 514 us.
+// Measured: 8192 x 16384 x 4096 409 us (2690 TFLOP/s, at the card's power limit), scaled in
+// registers 495 us.
 // ---------------------------------------------------------------------------------------
 constexpr int kScaledThreads = 448;
 constexpr int kScaledStages = 6;
 constexpr int kExpBytes = 3 * 512;  // exponents of a stage: of 128 rows of a, 256 of b
-constexpr int kExpAhead = 4;        // groups whose scales are on their way
+constexpr int kExpAhead = 8;        // groups whose scales are on their way
 
 template <int N>
 struct ScaledTile {
@@ -537,16 +563,8 @@ __global__ void __launch_bounds__(kScaledThreads, 1)
           if (lane == 0) mbar_arrive_peer(&bars->sum_empty[d], 0);
         }
         if (c >= left) continue;
-        if (p.bias) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int at = c + 2 * i;
-            const float x = at < left ? load1_rt(p.bias, p.bias_dt, col0 + at) : 0.f;
-            const float y = at + 1 < left ? load1_rt(p.bias, p.bias_dt, col0 + at + 1) : 0.f;
-            v[i] = add2(v[i], make_float2(x, y));
-          }
-        }
         if (whole) {
+          if (p.bias) add_bias16(p, col0 + c, v);
           if (row < p.m) {
             uint32_t w[8];
 #pragma unroll
@@ -809,18 +827,29 @@ __global__ void __launch_bounds__(kFewThreads, T >= 128 ? 1 : 2)
 }
 
 // ---------------------------------------------------------------------------------------
-// An operand whose address or row stride is no multiple of 16, copied to where they are: 16
+// Operands whose address or row stride is no multiple of 16 (blockIdx.y: one or both), copied to where they are: 16
 // bytes a thread from the aligned words around them.
 // ---------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) repack_kernel(const unsigned char* src, int64_t src_row, int64_t rows, int32_t k,
-                                                     unsigned char* dst, int32_t pieces) {
+struct RepackJob {
+  const unsigned char* src;
+  int64_t src_row, rows;
+  unsigned char* dst;
+};
+struct RepackParams {
+  RepackJob job[2];
+  int32_t k, pieces;  // bytes of a row; pieces of 16 bytes of a row of the copy
+};
+
+__global__ void __launch_bounds__(256) repack_kernel(const RepackParams p) {
   pdl_launch_dependents();
   pdl_wait();
+  const RepackJob& jb = blockIdx.y == 0 ? p.job[0] : p.job[1];
+  const int32_t k = p.k, pieces = p.pieces;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   const int64_t row = i / pieces;
-  if (row >= rows) return;
+  if (row >= jb.rows) return;
   const int at = static_cast<int>(i - row * pieces) * 16;
-  const unsigned char* s = src + row * src_row + at;
+  const unsigned char* s = jb.src + row * jb.src_row + at;
   const int left = min(16, k - at);
   uint32_t w[4] = {0, 0, 0, 0};
   if (left == 16) {
@@ -842,7 +871,7 @@ __global__ void __launch_bounds__(256) repack_kernel(const unsigned char* src, i
       else w[3] |= b;
     }
   }
-  uint4* to = reinterpret_cast<uint4*>(dst) + i;
+  uint4* to = reinterpret_cast<uint4*>(jb.dst) + i;
   if (RMSB_DBG_OK(to, 16, kDbgVecStore)) *to = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
