@@ -109,9 +109,15 @@ int run(const rmsnorm_b200_block_quant_args* a, void* ws, size_t ws_bytes, cudaS
   p.vec_in = aligned_to(a->x, 16) && a->x_row_stride * xb % 16 == 0;
   p.vec_q = aligned_to(a->q, 8) && a->q_row_stride % 8 == 0;
   p.vec_t = aligned_to(a->q_t, 16) && a->q_t_row_stride % 16 == 0;
+  p.vec_all = p.vec_in && (!a->q || p.vec_q) && (!a->q_t || p.vec_t);
   if (a->rows > 0) {
     QuantLaunch l = {};
-    if (tiled(a)) {
+    // Row groups alone go by tiles where 16-bit values fill three CTAs on every SM: bf16, 8192 x
+    // 4096 takes 19.2 us by tiles and 26.1 by groups, 2048 x 4096 6.4 and 7.2, 1024 x 4096 4.5 and
+    // 4.2. fp32 gains nothing (2048 x 4096: 9.0 and 7.9, 8192 x 4096: 28.2 and 28.2), and neither
+    // do rows without vectors (8192 x 4097: 50.3 and 32.7).
+    const bool wide = xb == 2 && p.vec_all && rb * cb >= int64_t{3} * ud->sm_count;
+    if (tiled(a) || wide) {
       TileKernel kernel = a->x_dtype == RMSNORM_B200_F32    ? tiles<float>(a->block_rows)
                           : a->x_dtype == RMSNORM_B200_BF16 ? tiles<__nv_bfloat16>(a->block_rows)
                                                             : tiles<__half>(a->block_rows);
@@ -119,16 +125,10 @@ int run(const rmsnorm_b200_block_quant_args* a, void* ws, size_t ws_bytes, cudaS
       st = launch(kernel, dim3(l.grid), 256, stream, p, static_cast<uint32_t>(cb));
     } else {
       const int64_t total = a->rows * cb;
-      // four groups in flight a lane, where that leaves a CTA for every SM
-      const int each = total >= int64_t{64} * ud->sm_count ? 4 : 1;
-      GroupKernel kernel = nullptr;
-      if (a->x_dtype == RMSNORM_B200_F32)
-        kernel = each == 4 ? quant_groups_kernel<float, 4> : quant_groups_kernel<float, 1>;
-      else if (a->x_dtype == RMSNORM_B200_BF16)
-        kernel = each == 4 ? quant_groups_kernel<__nv_bfloat16, 4> : quant_groups_kernel<__nv_bfloat16, 1>;
-      else
-        kernel = each == 4 ? quant_groups_kernel<__half, 4> : quant_groups_kernel<__half, 1>;
-      l = {"quant_groups", static_cast<unsigned>((total + 16 * each - 1) / (16 * each))};
+      GroupKernel kernel = a->x_dtype == RMSNORM_B200_F32    ? quant_groups_kernel<float>
+                           : a->x_dtype == RMSNORM_B200_BF16 ? quant_groups_kernel<__nv_bfloat16>
+                                                             : quant_groups_kernel<__half>;
+      l = {"quant_groups", static_cast<unsigned>((total + 15) / 16)};
       st = launch(kernel, dim3(l.grid), 256, stream, p, total, static_cast<uint32_t>(cb));
     }
     if (!st) st = launched(describe, l);

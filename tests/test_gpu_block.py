@@ -44,6 +44,14 @@ def test_quantize(rows, cols, dtype, block_rows):
     assert all(t.stride(0) % 16 == 0 or t.shape[0] == 1 for t in (q, q_t))
 
 
+@pytest.mark.parametrize("rows,cols,pitch,at", [(3000, 4096, 4096, 0), (3001, 4200, 4208, 8), (3001, 4201, 4201, 0), (3001, 4096, 4104, 4)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_quantize_many_groups(rows, cols, pitch, at, dtype):
+    """Enough of them for whole tiles: aligned, ragged, without vectors, from rows that start off a vector."""
+    x = rand(rows * pitch + at, dtype=dtype, seed=cols)[at:].view(rows, pitch)[:, :cols]
+    ref.check_quantized(*fused.block_quantize(x), x, 1)
+
+
 def test_quantize_ends_of_the_range():
     """Zeros, the largest and smallest numbers, a maximum that is a power of two times 448."""
     x = torch.zeros(6, 256, device=DEV)
