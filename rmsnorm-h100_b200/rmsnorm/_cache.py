@@ -114,6 +114,8 @@ def cache_write(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, k_scales
     written = (k_cache, v_cache, k_scales, v_scales)
     if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel() and slots.numel():
         raise ValueError("k_cache and v_cache must be different tensors")
+    if k_scales.data_ptr() == v_scales.data_ptr() and k_scales.numel() and slots.numel():
+        raise ValueError("k_scales and v_scales must be different tensors")
     for t in written:
         if _repeats(t):
             raise ValueError("caches and scales must have places of their own, not be expanded views")

@@ -310,3 +310,10 @@ def test_product_of_expanded_and_overlapping_rows():
     b, sb = fused.block_quantize(torch.randn(6, 128))
     out = fused.block_mm(a.expand(4, 128), sa.expand(4, 1), b, sb, out_dtype=torch.float32)
     assert torch.equal(out, fused.block_mm(a, sa, b, sb, out_dtype=torch.float32).expand(4, 6))
+
+
+def test_cache_write_refuses_one_tensor_for_both_scales():
+    k_cache, v_cache, scales, _ = _cache()
+    x = torch.randn(3, *k_cache.shape[2:])
+    with pytest.raises(ValueError, match="k_scales and v_scales must be different"):
+        fused.cache_write(x, x, k_cache, v_cache, scales, scales, torch.arange(3))
