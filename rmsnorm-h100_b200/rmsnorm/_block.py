@@ -102,7 +102,7 @@ def block_quantize(x: Tensor, block_rows: int = 1, transposed: bool = False, sca
     2^-126; q is x / scale, which is exact, rounded to nearest even. A NaN makes its scale NaN,
     an infinity infinite. `scales_column_major` lays q's scales out column by column, as scales_t
     are: large products read them faster so. The rows of q and q_t begin at multiples of 16 bytes:
-    where their length is none, they are views of wider rows."""
+    where their length is none, they are views of wider rows. Outside autograd."""
     if _is_compiling():
         return _quantize_untraced(x, block_rows, transposed, scales_column_major)
     if x.dtype not in _CODE:
@@ -113,6 +113,8 @@ def block_quantize(x: Tensor, block_rows: int = 1, transposed: bool = False, sca
         raise ValueError(f"block_rows must be 1 or 128, got {block_rows}")
     if block_rows > 1 and x.dim() != 2:
         raise ValueError(f"128 x 128 blocks need a matrix, got shape {tuple(x.shape)}")
+    if x.requires_grad:
+        x = x.detach()
     q, scales, q_t, scales_t, _ = _quantize(_rows_of(x), block_rows, True, transposed, scales_column_major)
     if x.dim() != 2:
         lead = x.shape[:-1]

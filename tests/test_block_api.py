@@ -317,3 +317,7 @@ def test_cache_write_refuses_one_tensor_for_both_scales():
     x = torch.randn(3, *k_cache.shape[2:])
     with pytest.raises(ValueError, match="k_scales and v_scales must be different"):
         fused.cache_write(x, x, k_cache, v_cache, scales, scales, torch.arange(3))
+
+
+def test_quantised_values_are_outside_autograd():
+    assert not any(t.requires_grad for t in fused.block_quantize(torch.randn(5, 130, requires_grad=True), transposed=True))
