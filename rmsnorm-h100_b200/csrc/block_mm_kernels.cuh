@@ -146,7 +146,6 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   const uint32_t rank = cluster_ctarank();
   const int64_t unit = blockIdx.x >> 1, units = gridDim.x >> 1;
   const int64_t tiles = static_cast<int64_t>(pl.tiles_m) * pl.tiles_n;
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kWideStages; ++i) {
       mbar_init(&bars->full[i], 1);
@@ -169,6 +168,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   cluster_sync_all();
   tmem_fence_after_sync();
   const uint32_t tmem = bars->tmem;
+  pdl_launch_dependents();  // they may take tensor memory and wait: this grid has all of its own by now
   pdl_wait();
 
   if (warp >= 8) {
@@ -400,7 +400,6 @@ __global__ void __launch_bounds__(kScaledThreads, 1)
   const uint32_t rank = cluster_ctarank();
   const int64_t unit = blockIdx.x >> 1, units = gridDim.x >> 1;
   const int64_t tiles = static_cast<int64_t>(pl.tiles_m) * pl.tiles_n;
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kScaledStages; ++i) {
       mbar_init(&bars->full[i], 9);  // the copies, and four warps' exponents in each CTA
@@ -423,6 +422,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1)
   cluster_sync_all();
   tmem_fence_after_sync();
   const uint32_t tmem = bars->tmem;
+  pdl_launch_dependents();  // they may take tensor memory and wait: this grid has all of its own by now
   pdl_wait();
 
   if (warp == 8) {  // copies
@@ -635,7 +635,6 @@ __global__ void __launch_bounds__(kFewThreads, T >= 128 ? 1 : 2)
   const int64_t t0 = tile / pl.tiles_n * T;  // first row of a
   const int g0 = static_cast<int>(static_cast<int64_t>(p.groups) * rank / pl.splits);
   const int g1 = static_cast<int>(static_cast<int64_t>(p.groups) * (rank + 1) / pl.splits);
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < pl.stages; ++i) {
       mbar_init(&bars->full[i], 1);
@@ -657,6 +656,7 @@ __global__ void __launch_bounds__(kFewThreads, T >= 128 ? 1 : 2)
   __syncthreads();
   tmem_fence_after_sync();
   const uint32_t tmem = bars->tmem;
+  pdl_launch_dependents();  // they may take tensor memory and wait: this grid has all of its own by now
   pdl_wait();
 
   float2 acc[T / 2];

@@ -407,6 +407,19 @@ def test_linear_second_derivatives_are_refused():
         dx.sum().backward()
 
 
+def test_products_one_behind_the_other_share_tensor_memory():
+    """Each may start before the one before it has ended; small ones of a single group fit beside a
+    large one on an SM, whose tensor memory they cannot share."""
+    a, sa = operand(2000, 128, 1, 1)
+    b, sb = operand(3000, 128, 128, 2)
+    (a2, sa2), (b2, sb2) = fused.block_quantize(rand(2000, 256, seed=3)), fused.block_quantize(rand(3000, 256, seed=4), 128)
+    want = fused.block_mm(a[:8], sa[:8], b, sb), fused.block_mm(a2, sa2, b2, sb2, power_of_two=True), fused.block_mm(a2, sa2, b2, sb2)
+    for _ in range(40):
+        got = (fused.block_mm(a[:8], sa[:8], b, sb), fused.block_mm(a2, sa2, b2, sb2, power_of_two=True),
+               fused.block_mm(a[:8], sa[:8], b, sb), fused.block_mm(a2, sa2, b2, sb2))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[0]) and torch.equal(got[3], want[2])
+
+
 def test_linear_captured_and_replayed():
     x, w = rand(200, 512, dtype=BF16).requires_grad_(True), rand(384, 512, dtype=BF16, seed=1).requires_grad_(True)
     dy = rand(200, 384, dtype=BF16, seed=2)
