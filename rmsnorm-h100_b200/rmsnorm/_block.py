@@ -227,8 +227,9 @@ def _product(a, a_row, a_scales, b, b_row, b_scales, b_rows, bias, bias_code, ou
 
 class BlockLinearFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias):
-        x2, need = _rows_of(x), ctx.needs_input_grad
+    def forward(ctx, x, weight, bias, grad):
+        x2 = _rows_of(x)
+        need = ctx.needs_input_grad if grad else (False, False)  # they are what the inputs want, whatever the mode
         q, s, x_t, x_ts, _ = _quantize(x2, 1, True, need[1], True)
         w, ws, w_t, w_ts, _ = _quantize(_rows_of(weight), _BLOCK, True, need[0])
         ctx.save_for_backward(x_t, x_ts, w_t, w_ts)
@@ -242,7 +243,7 @@ class BlockLinearFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         x_t, x_ts, w_t, w_ts = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
         x_dtype, w_dtype, b_dtype = ctx.dtypes
         dx = dw = db = None
         q, s, d_t, d_ts, db = _quantize(_rows_of(dy), 1, need_x, need_w, True, b_dtype if need_b else None)
@@ -254,7 +255,7 @@ class BlockLinearFunction(torch.autograd.Function):
                 dw = _product(d_t, _pitch(d_t), d_ts, x_t, _pitch(x_t), x_ts, 1, None, 0, w_dtype, _CODE[w_dtype], True)
             else:
                 dw = torch.zeros(d_t.shape[0], x_t.shape[0], dtype=w_dtype, device=dy.device)
-        return first_order("block_linear", (dx, dw, db))
+        return (*first_order("block_linear", (dx, dw, db)), None)
 
 
 def _pitch(q: Tensor) -> int:
@@ -281,7 +282,7 @@ def block_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None) -> Te
     if weight.device != x.device:
         _check_same_device("weight", weight, x.device)
     _check_bias(bias, weight.shape[0], x.device)
-    return BlockLinearFunction.apply(x, weight, bias)
+    return BlockLinearFunction.apply(x, weight, bias, torch.is_grad_enabled())
 
 
 _quantize_untraced = torch.compiler.disable(block_quantize)

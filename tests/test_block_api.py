@@ -326,3 +326,15 @@ def test_cache_write_refuses_one_tensor_for_both_scales():
 
 def test_quantised_values_are_outside_autograd():
     assert not any(t.requires_grad for t in fused.block_quantize(torch.randn(5, 130, requires_grad=True), transposed=True))
+
+
+def test_linear_without_gradients_quantises_nothing_for_them(monkeypatch):
+    from rmsnorm import _block
+
+    wanted, quantize = [], _block._quantize
+    monkeypatch.setattr(_block, "_quantize", lambda x, rows, want, want_t, *a: wanted.append(want_t) or quantize(x, rows, want, want_t, *a))
+    x, w = torch.randn(3, 130, requires_grad=True), torch.randn(7, 130, requires_grad=True)
+    y = fused.block_linear(x, w)
+    with torch.no_grad():
+        assert torch.equal(fused.block_linear(x, w), y)
+    assert wanted == [True, True, False, False]
