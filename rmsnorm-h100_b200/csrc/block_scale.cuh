@@ -87,22 +87,31 @@ __device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {  // of bot
   return r;
 }
 
-// The largest magnitude (fp32 bits) of each of kCount octets, over the kLanes lanes that share it.
-template <typename X, int kLanes, int kCount>
-__device__ __forceinline__ void most_of(const Held<X> (&h)[kCount], uint32_t (&most)[kCount]) {
+// The largest magnitude (fp32 bits) of each of kCount rows of kOctets octets a lane, over the
+// kLanes lanes that share it.
+template <typename X, int kLanes, int kCount, int kOctets = 1>
+__device__ __forceinline__ void most_of(const Held<X> (&h)[kCount * kOctets], uint32_t (&most)[kCount]) {
   if constexpr (sizeof(X) == 4) {
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) most[i] = largest_of<kLanes>(octet_magnitude(h[i].v));
+    for (int i = 0; i < kCount; ++i) {
+      uint32_t m = octet_magnitude(h[i * kOctets].v);
+#pragma unroll
+      for (int o = 1; o < kOctets; ++o) m = max(m, octet_magnitude(h[i * kOctets + o].v));
+      most[i] = largest_of<kLanes>(m);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < kCount; i += 2) {
       uint32_t m[2] = {0, 0};
 #pragma unroll
-      for (int k = 0; k < 2 && i + k < kCount; ++k) {
-        const uint32_t(&w)[4] = h[i + k].w;
-        m[k] = larger2(larger2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), larger2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-      }
-      // octet i's in the low half, the next one's in the high half
+      for (int k = 0; k < 2 && i + k < kCount; ++k)
+#pragma unroll
+        for (int o = 0; o < kOctets; ++o) {
+          const uint32_t(&w)[4] = h[(i + k) * kOctets + o].w;
+          const uint32_t one = larger2(larger2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), larger2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+          m[k] = o ? larger2(m[k], one) : one;
+        }
+      // row i's in the low half, the next one's in the high half
       uint32_t both = larger2(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) both = larger2(both, __shfl_xor_sync(0xffffffffu, both, o));

@@ -54,12 +54,13 @@ void set_sizes(CacheParams* p, const rmsnorm_b200_cache_args* c) {
   p->small = p->tokens < kMost / c->heads && c->pages < kMost / c->page_size;  // there are no more rounds than heads
 }
 
-template <bool kWrite, typename X, typename Q, int kItems>
+// Lanes of a head with one octet of columns each; where a lane has two, a head takes half of them.
+template <bool kWrite, typename X, typename Q, int kItems, int kOctets>
 CacheKernel pick_lanes(int lanes) {
   if constexpr (kWrite)
-    return lanes == 8    ? cache_write_kernel<X, Q, 8, kItems>
-           : lanes == 16 ? cache_write_kernel<X, Q, 16, kItems>
-                         : cache_write_kernel<X, Q, 32, kItems>;
+    return lanes == 8    ? cache_write_kernel<X, Q, 8 / kOctets, kItems, kOctets>
+           : lanes == 16 ? cache_write_kernel<X, Q, 16 / kOctets, kItems, kOctets>
+                         : cache_write_kernel<X, Q, 32 / kOctets, kItems, kOctets>;
   else
     return lanes == 8    ? cache_read_kernel<X, Q, 8, kItems>
            : lanes == 16 ? cache_read_kernel<X, Q, 16, kItems>
@@ -67,15 +68,15 @@ CacheKernel pick_lanes(int lanes) {
 }
 
 template <bool kWrite, typename X>
-CacheKernel pick(int cache_dtype, int lanes, int items) {
-  constexpr int kMost = kWrite && sizeof(X) == 2 ? 8 : 4;
+CacheKernel pick(int cache_dtype, int lanes, int items, int octets) {
+  constexpr int kMost = kWrite && sizeof(X) == 2 ? 2 : 1;
   if (cache_dtype == RMSNORM_B200_E4M3)
-    return items == 1   ? pick_lanes<kWrite, X, E4M3, 1>(lanes)
-           : items == 4 ? pick_lanes<kWrite, X, E4M3, 4>(lanes)
-                        : pick_lanes<kWrite, X, E4M3, kMost>(lanes);
-  return items == 1   ? pick_lanes<kWrite, X, I8, 1>(lanes)
-         : items == 4 ? pick_lanes<kWrite, X, I8, 4>(lanes)
-                      : pick_lanes<kWrite, X, I8, kMost>(lanes);
+    return items == 1    ? pick_lanes<kWrite, X, E4M3, 1, 1>(lanes)
+           : octets == 1 ? pick_lanes<kWrite, X, E4M3, 4, 1>(lanes)
+                         : pick_lanes<kWrite, X, E4M3, 4, kMost>(lanes);
+  return items == 1    ? pick_lanes<kWrite, X, I8, 1, 1>(lanes)
+         : octets == 1 ? pick_lanes<kWrite, X, I8, 4, 1>(lanes)
+                       : pick_lanes<kWrite, X, I8, 4, kMost>(lanes);
 }
 
 struct CacheLaunch {
@@ -94,17 +95,18 @@ std::string describe(const void* data) {
 template <bool kWrite>
 int launch(UnitDevice* ud, const rmsnorm_b200_cache_args* c, CacheParams& p, int dtype, cudaStream_t stream) {
   const int lanes = c->head_dim <= 64 ? 8 : c->head_dim <= 128 ? 16 : 32;
-  // four heads of a token in flight a lane, eight when 16-bit values are written (4 registers each),
-  // where it has that many and that leaves two CTAs for every SM
+  // Four heads of a token in flight a lane, and two octets of each when 16-bit values are written
+  // (4 registers an octet), where it has that many and that leaves two CTAs for every SM.
   const auto enough = [&](int n) { return p.tokens * p.heads * lanes >= int64_t{2} * n * kCacheThreads * ud->sm_count; };
-  const int each = kWrite && dtype != RMSNORM_B200_F32 && c->heads >= 5 && enough(8) ? 8 : c->heads >= 3 && enough(4) ? 4 : 1;
+  const int octets = kWrite && dtype != RMSNORM_B200_F32 && c->heads >= 3 && enough(8) ? 2 : 1;
+  const int each = c->heads >= 3 && enough(4) ? 4 : 1;
   p.rounds = (c->heads + each - 1) / each;
   p.by_rounds = divisor_of(static_cast<uint32_t>(p.rounds));
-  const int64_t per = kCacheThreads / lanes, grid = (p.tokens * p.rounds + per - 1) / per;
+  const int64_t per = kCacheThreads / (lanes / octets), grid = (p.tokens * p.rounds + per - 1) / per;
   if (grid >= int64_t{1} << 31) return RMSNORM_B200_ERR_UNSUPPORTED;
-  const CacheKernel kernel = dtype == RMSNORM_B200_F32    ? pick<kWrite, float>(c->cache_dtype, lanes, each)
-                             : dtype == RMSNORM_B200_BF16 ? pick<kWrite, __nv_bfloat16>(c->cache_dtype, lanes, each)
-                                                          : pick<kWrite, __half>(c->cache_dtype, lanes, each);
+  const CacheKernel kernel = dtype == RMSNORM_B200_F32    ? pick<kWrite, float>(c->cache_dtype, lanes, each, octets)
+                             : dtype == RMSNORM_B200_BF16 ? pick<kWrite, __nv_bfloat16>(c->cache_dtype, lanes, each, octets)
+                                                          : pick<kWrite, __half>(c->cache_dtype, lanes, each, octets);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -118,7 +120,7 @@ int launch(UnitDevice* ud, const rmsnorm_b200_cache_args* c, CacheParams& p, int
     cudaGetLastError();
     return RMSNORM_B200_ERR_CUDA;
   }
-  const CacheLaunch l = {kWrite ? "cache_write" : "cache_read", static_cast<unsigned>(grid), lanes, each};
+  const CacheLaunch l = {kWrite ? "cache_write" : "cache_read", static_cast<unsigned>(grid), lanes / octets, each};
   return launched(describe, l);
 }
 

@@ -63,9 +63,11 @@ __device__ __forceinline__ void cache_unit(const CacheParams& p, int64_t i, int6
   }
 }
 
-// A head takes kLanes lanes of 8 values each; every one of them has kItems heads of a token's k or
-// v (blockIdx.y) in flight, which share the work on its place (a head by itself takes 235
-// instructions for 8 values, 110 of them its place).
+// A head takes kLanes lanes of kOctets times 8 values each; every one of them has kItems heads of a
+// token's k or v (blockIdx.y) in flight, which share the work on its place (a head by itself takes
+// 235 instructions for 8 values, 110 of them its place). Two octets a lane share the work on a
+// head's scale as well: bf16, 16384 tokens of 8 heads of 128 19.9 us, with eight heads of one octet
+// 23.8. Four CTAs an SM leave 64 registers; five (48, some in local memory) took 20.3 us.
 //   scale = max(max |x| / Q, 2^-126), q = round(Q x / max |x|)
 // Q x is exact for 16-bit x, and so is the quotient wherever it is a tie of q: 16-bit x lie on
 // ties far more often than chance has it (one in 700 of normal bf16 values), which x / scale, or x
@@ -73,15 +75,15 @@ __device__ __forceinline__ void cache_unit(const CacheParams& p, int64_t i, int6
 // the inverse and one correction by its remainder (Markstein: Computation of elementary functions
 // on the IBM RISC System/6000 processor, 1990), of numbers brought to max |x| in [1, 8) by a power
 // of two, so that the remainder is exact. A head whose scale is 2^-126 takes x 2^126.
-template <typename X, typename Q, int kLanes, int kItems>
-__global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid_constant__ CacheParams p) {
+template <typename X, typename Q, int kLanes, int kItems, int kOctets>
+__global__ void __launch_bounds__(kCacheThreads, kOctets == 2 ? 4 : 1) cache_write_kernel(const __grid_constant__ CacheParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const CacheSide& side = blockIdx.y == 0 ? p.side[0] : p.side[1];
   constexpr int kGroups = kCacheThreads / kLanes;
   const int lane = threadIdx.x % kLanes, col = lane * 8;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / kLanes;
-  Held<X> held[kItems];
+  Held<X> held[kItems * kOctets];
   int64_t slot = -1, token = 0;
   int32_t round = 0;
   if (unit < p.tokens * p.rounds) {
@@ -93,10 +95,15 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid
   const X* src = static_cast<const X*>(side.x) + token * side.x_token + head0 * side.x_head + col;
 #pragma unroll
   for (int j = 0; j < kItems; ++j, src += side.x_head) {
-    held[j].zero();
-    if (j >= heads || col >= p.head_dim) continue;
-    if (side.vec_x) held[j].load(src);
-    else held[j].load(src, p.head_dim - col);
+#pragma unroll
+    for (int o = 0; o < kOctets; ++o) {
+      Held<X>& h = held[j * kOctets + o];
+      const int at = o * kLanes * 8;
+      h.zero();
+      if (j >= heads || col + at >= p.head_dim) continue;
+      if (side.vec_x) h.load(src + at);
+      else h.load(src + at, p.head_dim - col - at);
+    }
   }
   // no lane leaves before the last shuffle: its slot may differ from its neighbours'
   const bool beyond = slot >= p.pages * p.page_size;
@@ -107,7 +114,7 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid
   float* scale = side.scales + page * side.s_page + place * side.s_slot + head0 * side.s_head;
   unsigned char* dst = side.data + page * side.page + place * side.slot + head0 * side.head + col;
   uint32_t largest_bits[kItems];
-  most_of<X, kLanes, kItems>(held, largest_bits);
+  most_of<X, kLanes, kItems, kOctets>(held, largest_bits);
   if (!kept) return;
 #pragma unroll
   for (int j = 0; j < kItems; ++j) {
@@ -120,25 +127,29 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const __grid
     s0 = e == 255 ? largest : fmaf(fmaf(-s0, kTop, largest), kInvTop, s0);
     const bool least = s0 < 1.17549435e-38f;  // NaN is not
     if (lane == 0) st1(scale + j * side.s_head, least ? 1.17549435e-38f : s0);
-    if (col >= p.head_dim) continue;
     const float power = __uint_as_float(static_cast<uint32_t>(max(254 - e, 1)) << 23);
     const float times = least ? 8.5070592e37f : kTop * power;  // 2^126
     const float by = least ? 1.f : e < 255 ? largest * power : 0.f;  // infinity: no remainder
     const float inv = inverse(!least && e == 255 ? largest : by);
-    float2 v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 n = mul2(held[j].pair(k), splat2(times)), q = mul2(n, splat2(inv));
-      v[k] = fma2(fma2(q, splat2(-by), n), splat2(inv), q);
-    }
-    const uint2 b = make_uint2(Q::pack4(v[0], v[1]), Q::pack4(v[2], v[3]));
-    unsigned char* to = dst + j * side.head;
-    if (side.vec_q) {
-      if (RMSB_DBG_OK(to, 8, kDbgVecStore)) *reinterpret_cast<uint2*>(to) = b;
-    } else {
+    for (int o = 0; o < kOctets; ++o) {
+      const int at = o * kLanes * 8;
+      if (col + at >= p.head_dim) continue;
+      float2 v[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (col + k < p.head_dim) st1(to + k, static_cast<unsigned char>((k < 4 ? b.x : b.y) >> (8 * (k & 3))));
+      for (int k = 0; k < 4; ++k) {
+        const float2 n = mul2(held[j * kOctets + o].pair(k), splat2(times)), q = mul2(n, splat2(inv));
+        v[k] = fma2(fma2(q, splat2(-by), n), splat2(inv), q);
+      }
+      const uint2 b = make_uint2(Q::pack4(v[0], v[1]), Q::pack4(v[2], v[3]));
+      unsigned char* to = dst + j * side.head + at;
+      if (side.vec_q) {
+        if (RMSB_DBG_OK(to, 8, kDbgVecStore)) *reinterpret_cast<uint2*>(to) = b;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (col + at + k < p.head_dim) st1(to + k, static_cast<unsigned char>((k < 4 ? b.x : b.y) >> (8 * (k & 3))));
+      }
     }
   }
 }

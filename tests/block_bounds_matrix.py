@@ -47,6 +47,8 @@ def cases():
         for kept in (E4M3, I8):
             yield f"cache write {d}", lambda d=d, q=kept: c.write_case(700, 5, d, 16, BF16, q)
             yield f"cache read {d}", lambda d=d, q=kept: c.read_case([5, 0, 333, 1], 5, d, 17, q, F16, 3)
+    for d in (7, 72, 128, 200):
+        yield f"cache write of many {d}", lambda d=d: c.write_case(16001, 5, d, 16, BF16, E4M3)
     yield "cache strides", c.test_write_strided_inputs_and_caches
     yield "cache far", c.test_write_leading_dimensions_and_none
     yield "cache one", lambda: c.write_case(1, 1, 128, 64, F32, E4M3)

@@ -81,6 +81,23 @@ def test_write_types_and_pages(dtype, slot_dtype, page_size):
     write_case(3000, 8, 128, page_size, dtype, E4M3, slot_dtype)
 
 
+@pytest.mark.parametrize("d", [1, 7, 64, 65, 72, 128, 129, 136, 200, 256])
+@pytest.mark.parametrize("dtype,kept", [(BF16, E4M3), (F16, E4M3), (BF16, I8)])
+def test_write_of_many_tokens(d, dtype, kept):
+    """So many that a lane takes two octets of a head; bits as when they are written few at a time."""
+    tokens, heads = 16001, 5
+    write_case(tokens, heads, d, 16, dtype, kept)
+    k, v = rand(tokens, heads, d, dtype=dtype, seed=4), rand(tokens, heads, d, dtype=dtype, seed=5)
+    k[3, 1, d // 2], k[4, 2, d - 1], v[5, 0, 0], v[6] = float("nan"), float("inf"), float("-inf"), 0
+    k[100:200] *= 2.0 ** (-130 if dtype == BF16 else -20)
+    slots = torch.randperm(16 * 1001, device=DEV)[:tokens]
+    one, other = new_cache(1001, 16, heads, d, kept), new_cache(1001, 16, heads, d, kept)
+    fused.cache_write(k, v, *one, slots)
+    for at in range(0, tokens, 1000):
+        fused.cache_write(k[at: at + 1000], v[at: at + 1000], *other, slots[at: at + 1000])
+    assert all(torch.equal(bits(x), bits(y)) for x, y in zip(one, other))
+
+
 def test_write_strided_inputs_and_caches():
     odd = lambda t: torch.cat([t, t], -1)[..., 1: 1 + t.shape[-1]]  # noqa: E731 -- off any 16 bytes
     for d in (64, 128):
