@@ -284,7 +284,8 @@ def _room(rows: int, k: int, scales: int, device: torch.device) -> Tuple[Tensor,
     return buf, at, at + size
 
 
-def _enqueue_product(m, n, k, a, a_scales, sa_row, sa_group, b, b_scales, sb_row, sb_group, b_rows, bias, bias_code, out) -> None:
+def _enqueue_product(m, n, k, a, a_scales, sa_row, sa_group, b, b_scales, sb_row, sb_group, b_rows, bias, bias_code,
+                     out) -> None:
     """Of what lies at these addresses, rows at multiples of 16 bytes, with powers of two as scales."""
     pitch = -(-k // 16) * 16
     args = _MM.pack(m, n, k, a, pitch, b, pitch, a_scales, sa_row, sa_group, b_scales, sb_row, sb_group,
