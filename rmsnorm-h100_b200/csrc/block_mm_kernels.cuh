@@ -118,18 +118,18 @@ __device__ __forceinline__ void add_bias16(const BlockMmParams& p, int64_t col, 
   }
 }
 
-// acc += sums * scale, or acc += sums * (column scales) * scale.
+// What a chunk's sums are multiplied by: scale, or (column scales) * scale. The two scales first, as
+// wherever they are multiplied, so that only their product has to be a number of fp32.
 template <bool kRowScales>
-__device__ __forceinline__ void add_scaled(float2* acc, const float2 (&v)[8], float s, const float* col) {
+__device__ __forceinline__ void chunk_scales(float2 (&to)[8], float s, const float* col) {
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     if constexpr (kRowScales) {
       const float4 c = *reinterpret_cast<const float4*>(col + 2 * i);
-      acc[i] = fma2(mul2(v[i], make_float2(c.x, c.y)), splat2(s), acc[i]);
-      acc[i + 1] = fma2(mul2(v[i + 1], make_float2(c.z, c.w)), splat2(s), acc[i + 1]);
+      to[i] = mul2(make_float2(c.x, c.y), splat2(s));
+      to[i + 1] = mul2(make_float2(c.z, c.w), splat2(s));
     } else {
-      acc[i] = fma2(v[i], splat2(s), acc[i]);
-      acc[i + 1] = fma2(v[i + 1], splat2(s), acc[i + 1]);
+      to[i] = to[i + 1] = splat2(s);
     }
   }
 }
@@ -297,13 +297,16 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         __syncwarp();
         tmem_fence_after_sync();
         const uint32_t at = from + d * kWideN;
-        float2 v[2][8];
+        float2 v[2][8], scale[8];
         tmem_ld(at, v[0]);
+        chunk_scales<kRowScales>(scale, s, cols);  // a chunk's while its sums are on their way
         tmem_landed(v[0]);
 #pragma unroll
         for (int c = 0; c < kWideHalf / 16; ++c) {
           if (c + 1 < kWideHalf / 16) tmem_ld(at + (c + 1) * 16, v[(c + 1) & 1]);
-          add_scaled<kRowScales>(acc + 8 * c, v[c & 1], s, cols + 16 * c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[8 * c + i] = fma2(v[c & 1][i], scale[i], acc[8 * c + i]);
+          if (c + 1 < kWideHalf / 16) chunk_scales<kRowScales>(scale, s, cols + 16 * (c + 1));
           if (c + 1 < kWideHalf / 16) tmem_landed(v[(c + 1) & 1]);
           if (c + 2 == kWideHalf / 16) {
             tmem_fence_before_sync();
@@ -778,8 +781,8 @@ __global__ void __launch_bounds__(kFewThreads, T >= 128 ? 1 : 2)
           for (int i = 0; i < kChunk / 2; i += 2) {
             const float4 r = *reinterpret_cast<const float4*>(rows + c * kChunk + 2 * i);
             float2* to = acc + c * (kChunk / 2) + i;
-            to[0] = fma2(mul2(x[i], make_float2(r.x, r.y)), splat2(s), to[0]);
-            to[1] = fma2(mul2(x[i + 1], make_float2(r.z, r.w)), splat2(s), to[1]);
+            to[0] = fma2(x[i], mul2(make_float2(r.x, r.y), splat2(s)), to[0]);
+            to[1] = fma2(x[i + 1], mul2(make_float2(r.z, r.w), splat2(s)), to[1]);
           }
         }
         if (++d == F::kSums) {

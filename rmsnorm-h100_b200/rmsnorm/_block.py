@@ -150,8 +150,9 @@ def block_mm(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, bias: Opt
     out_dtype: a (..., K) and b (N, K) in float8_e4m3fn, fp32 scales for groups of 128 columns,
     a_scales a.shape[:-1] + (ceil(K / 128),) as `rmsnorm_quant_fwd` with group_size 128 and
     `block_quantize` leave them, b_scales (N, ceil(K / 128)) or, a scale per 128 x 128 block,
-    (ceil(N / 128), ceil(K / 128)). Scales may have any strides. The sums are held in fp32 (and
-    so are products of two scales), rounded once at the end.
+    (ceil(N / 128), ceil(K / 128)). Scales may have any strides. The sums are held in fp32,
+    rounded once at the end; on CUDA so is the product of a's and b's scale for a group, which has
+    to be a normal number there.
 
     `power_of_two` tells that every scale is a power of two, as `block_quantize` makes them: large
     products with 16-bit results then leave the scales to the tensor cores, which is a fifth to a

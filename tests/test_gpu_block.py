@@ -467,3 +467,21 @@ def test_host_and_device_agree():
         for d, h in zip(fused.block_quantize(x, rows, True), fused.block_quantize(x.cpu(), rows, True)):
             assert torch.equal(d.cpu().float(), h.float())
     assert torch.allclose(fused.block_linear(x, w, b).cpu(), fused.block_linear(x.cpu(), w.cpu(), b.cpu()), rtol=1e-5, atol=1e-4)
+
+
+# ------------------------------------------------------------------ what the tests above leave out
+@pytest.mark.parametrize("m", [5, 40, 100, 300])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("far", [100, 119])
+def test_product_of_far_scales_whose_product_is_near(m, block_rows, far):
+    """Scales far up and far down: their product is a number, and so are the sums times it, wherever
+    the sums times one of them are not."""
+    a, _ = operand(m, 384, 1, 1)
+    b, _ = operand(2000, 384, block_rows, 2)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    near_a = 1 + torch.rand(m, 3, device=DEV, generator=g)
+    near_b = 1 + torch.rand(-(-2000 // block_rows), 3, device=DEV, generator=g)
+    for up in (2.0**far, 2.0**-far):
+        sa, sb = near_a * up, near_b / up
+        out = fused.block_mm(a, sa, b, sb, out_dtype=F32)
+        ref.check_product(out, ref.values(a, sa), ref.values(b, sb), None, f"{m} rows, {up}")
