@@ -212,7 +212,7 @@ def block_mm(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, bias: Opt
 def _product(a, a_row, a_scales, b, b_row, b_scales, b_rows, bias, bias_code, out_dtype, oc, power_of_two) -> Tensor:
     """The product of checked matrices with rows a_row and b_row apart."""
     if not a.is_cuda:
-        with torch.no_grad():
+        with torch.no_grad(), torch.autocast("cpu", enabled=False):  # the sums are fp32 in any mode
             out = _host.block_values(a, a_scales, 1) @ _host.block_values(b, b_scales, b_rows).t()
             return (out if bias is None else out + bias.float()).to(out_dtype)
     m, k = a.shape

@@ -338,3 +338,23 @@ def test_linear_without_gradients_quantises_nothing_for_them(monkeypatch):
     with torch.no_grad():
         assert torch.equal(fused.block_linear(x, w), y)
     assert wanted == [True, True, False, False]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_products_do_not_depend_on_autocast(dtype):
+    """Their sums are fp32 whatever mode another part of the program has set, as they are on CUDA."""
+    g = torch.Generator().manual_seed(0)
+    x, w, dy = (torch.randn(*s, generator=g) for s in ((8, 256), (4, 256), (8, 4)))
+    a, sa = fused.block_quantize(x)
+    b, sb = fused.block_quantize(w)
+
+    def results():
+        out = [fused.block_mm(a, sa * f, b, sb * f, out_dtype=torch.float32) for f in (1.0, 1.1)]  # powers of two and none
+        leaves = [x.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+        y = fused.block_linear(*leaves)
+        return [*out, y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    want = results()
+    with torch.autocast("cpu", dtype=dtype):
+        got = results()
+    assert all(i.dtype == j.dtype and torch.equal(i, j) for i, j in zip(got, want))
