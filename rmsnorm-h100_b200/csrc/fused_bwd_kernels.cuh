@@ -69,9 +69,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fused_bwd_kernel(const FusedBw
   constexpr int kH = Vec8<H>::kBytes / 8, kDy = Vec8<DY>::kBytes / 8;
   RowCtx c = row_begin(pl, p.N);
   const int G = kTmem ? kG : pl.G, KC = kTmem ? bwd_unit_steps(kG) : pl.KC, R = kTmem ? 1 : pl.R;
-  pdl_launch_dependents();
   if constexpr (kTmem) {
-    if (c.warp == 0) tmem_alloc_warp(&c.bars->tmem, kTmemCols);
+    if (c.warp == 0) {
+      tmem_alloc_warp(&c.bars->tmem, kTmemCols);
+      pdl_launch_dependents();  // for the CTA, and not before: they may take tensor memory and wait for this grid
+    }
+  } else {
+    pdl_launch_dependents();
   }
   pdl_wait();
   const void* src[kStreams];

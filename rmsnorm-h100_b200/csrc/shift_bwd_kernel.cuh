@@ -19,8 +19,10 @@ __global__ void __launch_bounds__(kShiftThreads, 1) shift_bwd_kernel(const Fused
   constexpr int kH = sizeof(H), kDy = sizeof(DY);
   RowCtx c = row_begin(pl, p.N);
   const RowShift sh = shift_begin(pl, c, p.rows, p.N);
-  pdl_launch_dependents();
-  if (c.warp == 0) tmem_alloc_warp(&c.bars->tmem, kTmemCols);
+  if (c.warp == 0) {
+    tmem_alloc_warp(&c.bars->tmem, kTmemCols);
+    pdl_launch_dependents();  // for the CTA, and not before: they may take tensor memory and wait for this grid
+  }
   pdl_wait();
   const void* src[3] = {p.h, p.dy, p.dro};
   const int bytes[3] = {kH, kDy, p.dro ? kH : 0};

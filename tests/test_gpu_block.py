@@ -485,3 +485,33 @@ def test_product_of_far_scales_whose_product_is_near(m, block_rows, far):
         sa, sb = near_a * up, near_b / up
         out = fused.block_mm(a, sa, b, sb, out_dtype=F32)
         ref.check_product(out, ref.values(a, sa), ref.values(b, sb), None, f"{m} rows, {up}")
+
+
+@pytest.mark.parametrize("rows,width", [(4, 1001), (300, 1001), (8, 4096), (2000, 4096)])
+def test_products_behind_and_beside_dropout_backwards_share_tensor_memory(rows, width):
+    """The dropout's backward holds its columns' sums in tensor memory, on shifted vectors or whole ones,
+    and with no weight no reduction stands between it and what follows it on its stream: a product,
+    directly or behind a quantisation. Products of few rows run on another stream meanwhile."""
+    x, dy = rand(rows, width, dtype=BF16, seed=1), rand(rows, width, dtype=BF16, seed=2)
+    _, h, rstd = fused.dropout_add_rmsnorm_fwd(x, None, p=0.1, rng=(1, 2), store_rstd=True)
+    a, sa = operand(2000, 256, 1, 1)
+    b, sb = operand(3000, 256, 128, 2)
+    (a2, sa2), (b2, sb2) = fused.block_quantize(rand(2000, 256, seed=3)), fused.block_quantize(rand(3000, 256, seed=4), 128)
+
+    def chain():
+        return (fused.dropout_add_rmsnorm_bwd(h, None, dy, rstd, p=0.1, rng=(1, 2))[0], fused.block_mm(a, sa, b, sb),
+                fused.dropout_add_rmsnorm_bwd(h, None, dy, rstd, p=0.1, rng=(1, 2))[0], *fused.block_quantize(x),
+                fused.block_mm(a2, sa2, b2, sb2, power_of_two=True), fused.block_mm(a[:8], sa[:8], b, sb))
+
+    bits = lambda ts: [t.view(torch.uint8).clone() for t in ts]  # noqa: E731
+    want = bits(chain())
+    few = fused.block_mm(a[:40], sa[:40], b, sb)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        with torch.cuda.stream(streams[0]):
+            got = chain()
+        with torch.cuda.stream(streams[1]):
+            beside = [fused.block_mm(a[:40], sa[:40], b, sb) for _ in range(4)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(i, j) for i, j in zip(bits(got), want)) and all(torch.equal(t, few) for t in beside)
