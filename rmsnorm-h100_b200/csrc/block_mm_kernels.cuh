@@ -564,6 +564,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1)
 #pragma unroll
       for (int c = 0; c < kHalf; c += 16) {
         float2 v[8];
+        __syncwarp();  // of the chunk before, lanes stored or did not
         tmem_ld(from + d * N + c, v);
         tmem_landed(v);
         if (c + 16 == kHalf) {

@@ -54,3 +54,18 @@ def test_dependents_start_once_tensor_memory_is_held(name, body):
         between = body[taken[0]: at]
         # a barrier of the CTA, or the warp that took it, in the same block
         assert "__syncthreads" in between or "init_barriers(" in between or "}" not in between
+
+
+def test_warps_come_together_before_they_read_tensor_memory():
+    """tcgen05.ld takes a whole warp, converged. In a loop that a warp leaves some of its lanes behind
+    in (stores of rows inside the matrix, returns of columns outside it), it comes together first."""
+    found = 0
+    for name, body in TAKING:
+        for m in re.finditer(r"\bfor\s*\([^{;]*;[^{;]*;[^{;]*\)\s*\{", body):
+            loop = body_at(body, m.end() - 1)
+            read = loop.find("tmem_ld(")
+            if read < 0 or not re.search(r"store_turned\(|if \(row < p\.m\)", loop) or re.search(r"\bfor\s*\([^{]*\)\s*\{[^}]*tmem_ld\(", loop):
+                continue
+            found += 1
+            assert "__syncwarp();" in loop[:read], f"{name}: {loop[:read]}"
+    assert found == 1
