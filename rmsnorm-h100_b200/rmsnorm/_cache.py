@@ -150,8 +150,9 @@ def cache_read(k_cache: Tensor, v_cache: Tensor, k_scales: Tensor, v_scales: Ten
     sequence's last page are not read.
 
     Rows from starts[-1] on are zeros, or left as they are in `out`, a pair of contiguous
-    tensors to write into. Rows whose page lies outside the table or the cache are NaN and, on
-    CUDA, the device status tells of an invalid argument (on the host it is an IndexError)."""
+    tensors to write into. Rows before starts[0], and rows whose page lies outside the table or the
+    cache, are NaN and, on CUDA, the device status tells of an invalid argument (on the host it is
+    an IndexError)."""
     if _is_compiling():
         return _read_untraced(k_cache, v_cache, k_scales, v_scales, page_table, starts, tokens, dtype, out)
     cache = _check_cache(k_cache, v_cache, k_scales, v_scales)
@@ -186,6 +187,8 @@ def cache_read(k_cache: Tensor, v_cache: Tensor, k_scales: Tensor, v_scales: Ten
             k.zero_()
             v.zero_()
         at = starts.tolist()
+        if tokens and at[0] != 0 and at[-1] > 0:
+            raise IndexError(f"the first sequence must begin at row 0, got starts[0] = {at[0]}")
         page_size = k_cache.shape[1]
         with torch.no_grad():
             for s in range(sequences):

@@ -358,3 +358,15 @@ def test_products_do_not_depend_on_autocast(dtype):
     with torch.autocast("cpu", dtype=dtype):
         got = results()
     assert all(i.dtype == j.dtype and torch.equal(i, j) for i, j in zip(got, want))
+
+
+@pytest.mark.parametrize("starts,sequences", [([1, 10], 1), ([3, 3, 9], 2), ([2], 0)])
+def test_cache_read_refuses_rows_before_the_first_sequence(starts, sequences):
+    """On CUDA they are NaN and the device status tells; on the host, like a page outside the table, an error."""
+    c = _cache()
+    table = torch.zeros(sequences, 3, dtype=torch.int32)
+    with pytest.raises(IndexError, match="first"):
+        fused.cache_read(*c, table, torch.tensor(starts, dtype=torch.int32), 12)
+    assert fused.cache_read(*c, table, torch.tensor(starts, dtype=torch.int32), 0)[0].shape == (0, 2, 16)
+    nothing = torch.zeros(sequences + 1, dtype=torch.int32)
+    assert (fused.cache_read(*c, table, nothing, 12)[0] == 0).all()
