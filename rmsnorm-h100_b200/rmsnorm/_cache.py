@@ -62,6 +62,34 @@ def _repeats(t: Tensor) -> bool:
     return 0 in stride and any(s == 0 and n > 1 for s, n in zip(stride, t.shape))
 
 
+def _meet(apart: int, dims, width: int) -> bool:
+    """Whether two places of one layout, `apart` from each other, share some of `width` elements:
+    dims has (stride, most steps), the largest stride first. Where places do not overlap by
+    themselves at most two numbers of steps of a stride bring them near enough to look further."""
+    if not dims:
+        return -width < apart < width
+    (stride, most), rest = dims[0], dims[1:]
+    reach = sum(s * n for s, n in rest) + width - 1
+    low, high = max(-(-(apart - reach) // stride), -most), min((apart + reach) // stride, most)
+    return any(_meet(apart - i * stride, rest, width) for i in range(low, high + 1))
+
+
+def _overlap(t: Tensor, u: Tensor, lead: Tuple[int, int, int], width: int) -> bool:
+    """Whether tensors of one layout (`lead` places of `width` elements) share memory. Of tensors
+    with other strides than one another nothing is told but that they begin at the same place."""
+    stride, size = t.stride(), t.element_size()
+    apart = t.data_ptr() - u.data_ptr()
+    a, b, c = lead
+    if abs(apart) >= size * ((a - 1) * stride[0] + (b - 1) * stride[1] + (c - 1) * stride[2] + width) or not a:
+        return False
+    if apart == 0:
+        return True
+    if stride != u.stride() or apart % size:
+        return False
+    dims = sorted(((s, n - 1) for s, n in zip(stride, lead) if n > 1), reverse=True)
+    return _meet(apart // size, dims, width)
+
+
 def _heads_of(name: str, t: Tensor, shape: torch.Size, device: torch.device) -> Tuple[Tensor, Tuple[int, int, int]]:
     """t as [tokens, heads, head_dim], a view wherever the strides allow one; its address, token
     stride and head stride."""
@@ -85,6 +113,8 @@ def cache_write(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, k_scales
     may be strided views such as slices of a packed projection, as q * scale with q in the
     caches' dtype (float8_e4m3fn or int8; (pages, page_size, heads, head_dim), any strides but
     the last) and an fp32 scale for every head (k_scales, v_scales: (pages, page_size, heads)).
+    The four may share a buffer, but no bytes: of two of one kind with the same strides that is an
+    error, of others it is not looked at.
 
     A scale is max |x| / 448 (e4m3) or / 127 (int8), at least 2^-126; q is x over that quotient as
     it is before it is rounded to fp32, rounded to nearest even. A NaN makes its head's scale NaN, an infinity infinite.
@@ -112,15 +142,16 @@ def cache_write(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, k_scales
     kf, k_place = _heads_of("k", k, shape, k_cache.device)
     vf, v_place = _heads_of("v", v, shape, k_cache.device)
     written = (k_cache, v_cache, k_scales, v_scales)
-    if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel() and slots.numel():
-        raise ValueError("k_cache and v_cache must be different tensors")
-    if k_scales.data_ptr() == v_scales.data_ptr() and k_scales.numel() and slots.numel():
-        raise ValueError("k_scales and v_scales must be different tensors")
     for t in written:
         if _repeats(t):
             raise ValueError("caches and scales must have places of their own, not be expanded views")
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError("cache_write is outside autograd: caches and scales must not require gradients")
+    *places, d = k_cache.shape
+    if _overlap(k_cache, v_cache, places, d) and slots.numel():
+        raise ValueError("k_cache and v_cache must be different tensors that do not overlap")
+    if _overlap(k_scales, v_scales, places, 1) and slots.numel():
+        raise ValueError("k_scales and v_scales must be different tensors that do not overlap")
     if len(lead) != 1:
         slots = slots.reshape(-1)
     if not k_cache.is_cuda:

@@ -370,3 +370,44 @@ def test_cache_read_refuses_rows_before_the_first_sequence(starts, sequences):
     assert fused.cache_read(*c, table, torch.tensor(starts, dtype=torch.int32), 0)[0].shape == (0, 2, 16)
     nothing = torch.zeros(sequences + 1, dtype=torch.int32)
     assert (fused.cache_read(*c, table, nothing, 12)[0] == 0).all()
+
+
+def _halves(shape, *axes, dtype=torch.float32):
+    """k's and v's part of one buffer, in every place that the axis of both can have."""
+    for axis in axes:
+        both = torch.zeros(*shape[:axis], 2, *shape[axis:]).to(dtype)
+        yield both.select(axis, 0), both.select(axis, 1)
+
+
+def test_cache_write_takes_caches_that_share_a_buffer():
+    shape, slots = (3, 4, 2, 16), torch.tensor([0, 5, 11, 7, 2])
+    k, v = torch.randn(5, 2, 16), torch.randn(5, 2, 16)
+    want = _cache()
+    fused.cache_write(k, v, *want, slots)
+    wide = torch.zeros(3, 4, 2, 32).to(E4M3)
+    across = torch.zeros(2, 4, 3, 2, 16).to(E4M3).transpose(1, 2)  # slots before pages
+    for kc, vc in [*_halves(shape, 0, 1, 2, 3, dtype=E4M3), wide.split(16, -1), across]:
+        for ks, vs in [(torch.zeros(3, 4, 2), torch.zeros(3, 4, 2)), *_halves(shape[:3], 0, 1, 2, 3)]:
+            fused.cache_write(k, v, kc, vc, ks, vs, slots)
+            got = (kc, vc, ks, vs)
+            assert all(torch.equal(i.float(), j.float()) for i, j in zip(got, want))
+
+
+def test_cache_write_refuses_caches_that_overlap():
+    k, slots = torch.randn(5, 2, 16), torch.arange(5)
+    c = _cache()
+    pages = torch.zeros(5, 4, 2, 16).to(E4M3)
+    slots_apart = torch.zeros(4, 8, 2, 16).to(E4M3)
+    columns = torch.zeros(3, 4, 2, 31).to(E4M3)
+    across = torch.zeros(4, 4, 2, 16).to(E4M3).transpose(0, 1)[:, 1:]
+    for kc, vc in [(pages[:3], pages[1:4]), (pages[:3], pages[2:]), (slots_apart[:3, :4], slots_apart[:3, 3:7]),
+                   (slots_apart[:3, 4:], slots_apart[1:, 4:]), (columns[..., :16], columns[..., 15:]),
+                   (across, torch.as_strided(across, across.shape, across.stride(), 0))]:
+        c2, c3 = (torch.zeros(kc.shape[:3]) for _ in range(2))
+        for one, other in ((kc, vc), (vc, kc)):
+            with pytest.raises(ValueError, match="k_cache and v_cache must"):
+                fused.cache_write(k, k, one, other, c2, c3, slots)
+    scales = torch.zeros(5, 4, 2)
+    for ks, vs in [(scales[:3], scales[1:4]), (scales[:3], scales[2:])]:
+        with pytest.raises(ValueError, match="k_scales and v_scales must"):
+            fused.cache_write(k, k, *c[:2], ks, vs, slots)
