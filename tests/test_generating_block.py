@@ -85,3 +85,80 @@ def test_training_with_block_scaled_products(device):
     for plain, eight in zip(*grads):
         # the error of up to eight products in a row, 0.037 each
         assert (plain - eight).norm() <= 0.3 * plain.norm()
+
+
+def peaked(device):
+    """A block whose branch is that of its attention alone (its MLP gives zeros), with logits twice as
+    wide as random heads' own, so that what a token reads depends on which keys it has."""
+    (block,), dtype = blocks(device)
+    with torch.no_grad():
+        block.down.zero_()
+        block.q_norm.fill_(2**0.5)
+        block.k_norm.fill_(2**0.5)
+    return block, dtype
+
+
+def attention_off(block, x, prompt):
+    """How far the generated attention branches are off the unquantised ones."""
+    table = fused.rope_table(x.shape[1], 64, device=x.device)
+    got = generate([block], x, prompt, table) - x.float()
+    with torch.no_grad():
+        want = torch.stack([sum(t.float() for t in block(s, None, torch.arange(x.shape[1], device=x.device), table)) for s in x])
+    want = want - x.float()
+    return float((got - want).norm() / want.norm())
+
+
+# The branch is off by its two products' operands, 0.037 each, by the values' 0.026 and by its softmax:
+# q and k are off by 0.037, k by 0.026 more, so a logit (0.06 of sqrt(2) sqrt(2) times a normal
+# number each way) by 0.12 to 0.17, and what is read with such weights by as much. Added up: 0.27.
+ATTENTION = 0.3
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("prompt,tokens", [(1, 24), (17, 40)])
+def test_generated_attention_matches_the_whole_sequence(device, prompt, tokens):
+    block, dtype = peaked(device)
+    x = torch.randn(3, tokens, 256, device=device, generator=torch.Generator(device=device).manual_seed(3)).to(dtype)
+    assert attention_off(block, x, prompt) <= ATTENTION
+
+
+@pytest.mark.parametrize("mistake", ["no keys", "no values", "keys of the token before", "values of the token before",
+                                     "keys of the other head", "keys turned to one position"])
+def test_generated_attention_tells_mistakes(mistake, monkeypatch):
+    """What the bound above is good for: each of these exceeds it."""
+    from rmsnorm.examples import prenorm_block
+
+    read, turn = fused.cache_read, fused.qk_norm_rope_fwd
+
+    def wrong_read(*args, **kw):
+        k, v = read(*args, **kw)
+        if mistake == "no keys":
+            k = torch.zeros_like(k)
+        elif mistake == "no values":
+            v = torch.zeros_like(v)
+        elif mistake == "keys of the token before":
+            k = k.roll(1, 0)
+        elif mistake == "values of the token before":
+            v = v.roll(1, 0)
+        elif mistake == "keys of the other head":
+            k = k.flip(1)
+        return k, v
+
+    def wrong_turn(q, k, positions, *args, **kw):
+        if mistake == "keys turned to one position":
+            turn(q, k.clone(), positions, *args, **kw)
+            positions = positions * 0
+            return turn(q.clone(), k, positions, *args, **kw)
+        return turn(q, k, positions, *args, **kw)
+
+    block, dtype = peaked("cpu")
+    x = torch.randn(3, 24, 256, generator=torch.Generator().manual_seed(3)).to(dtype)
+    wrong = type("wrong", (), {n: staticmethod(getattr(fused, n)) for n in fused.__all__})
+    wrong.cache_read, wrong.qk_norm_rope_fwd = staticmethod(wrong_read), staticmethod(wrong_turn)
+    monkeypatch.setattr(prenorm_block, "fused", wrong)
+    table = fused.rope_table(24, 64)
+    got = generate([block], x, 7, table) - x
+    monkeypatch.undo()
+    with torch.no_grad():
+        want = torch.stack([sum(t.float() for t in block(s, None, torch.arange(24), table)) for s in x]) - x
+    assert (got - want).norm() > ATTENTION * want.norm()
