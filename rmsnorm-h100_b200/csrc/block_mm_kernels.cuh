@@ -369,7 +369,10 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 // in the products' order brings to tensor memory; the sum over all of k stays there, and the eight
 // summing warps only bring results out. Tiles of 224 or 192 columns leave tensor memory for two of
 // them, so that one comes out while the next is summed, and for the exponents; one of 256 comes out
-// before the next begins, for pairs that have a single tile or two.
+// before the next begins, for pairs that have a single tile or two. Each addition of 32 products
+// rounds towards zero: where all values are positive, sums are low by 9.1e-6, 3.9e-5 and 3.3e-4 of
+// themselves at 4096, 16384 and 131072 columns (scaled in registers: 1e-7 to 5e-7), of random signs by
+// less than 16 bits show.
 // Measured: 8192 x 16384 x 4096 409 us (2690 TFLOP/s, at the card's power limit), scaled in
 // registers 495 us.
 // ---------------------------------------------------------------------------------------

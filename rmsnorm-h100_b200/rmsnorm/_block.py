@@ -156,7 +156,10 @@ def block_mm(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, bias: Opt
 
     `power_of_two` tells that every scale is a power of two, as `block_quantize` makes them: large
     products with 16-bit results then leave the scales to the tensor cores, which is a fifth to a
-    half faster. Of scales that are none only the exponent may be used; an infinite one counts as NaN.
+    half faster. They add all of K themselves then, in fp32 but not rounded to nearest: a sum may lose
+    up to 2^-23 of its magnitudes with each of K / 32 additions (in registers the groups' sums are
+    added rounded to nearest). Of scales that are none only the exponent may be used; an infinite one
+    counts as NaN.
 
     Operands whose rows begin at multiples of 16 bytes are read as they are, others copied by
     every call. Outside autograd: `block_linear` has gradients."""
@@ -342,9 +345,11 @@ def block_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None) -> Te
     """x weight^T + bias in x's dtype by 8-bit products, with autograd: x (..., K) is quantised
     per 128 columns of a row, weight (N, K) per 128 x 128 block (`block_quantize`), and in the
     backward the gradient per 128 columns for x's and, like x, per 128 rows for weight's. Every
-    sum is held in fp32. What the backward needs of x and weight is kept in 8 bits. The
-    gradients are those of the product at the quantised values (rounding counts as the
-    identity); they cannot be differentiated again: that is an error."""
+    sum is held in fp32, those of large products with 16-bit results in the tensor cores (`block_mm`
+    with `power_of_two`: weight's gradient adds up as many products as x has rows). What the
+    backward needs of x and weight is kept in 8 bits. The gradients are those of the product at the
+    quantised values (rounding counts as the identity); they cannot be differentiated again: that is
+    an error."""
     if _is_compiling():
         return _linear_untraced(x, weight, bias)
     for name, t in (("X", x), ("Weight", weight)):

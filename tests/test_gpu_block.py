@@ -515,3 +515,21 @@ def test_products_behind_and_beside_dropout_backwards_share_tensor_memory(rows, 
             beside = [fused.block_mm(a[:40], sa[:40], b, sb) for _ in range(4)]
         torch.cuda.synchronize()
         assert all(torch.equal(i, j) for i, j in zip(bits(got), want)) and all(torch.equal(t, few) for t in beside)
+
+
+@pytest.mark.parametrize("k", [16384, 131072])
+@pytest.mark.parametrize("positive", [False, True])
+@pytest.mark.parametrize("out_dtype", [BF16, F16])
+def test_powers_of_two_of_long_sums(k, positive, out_dtype):
+    """All of k is added in the tensor cores, 32 products at a time: what every addition may lose
+    adds up where no value is negative."""
+    m, n = 256, 4864
+    a, b = operand(m, k, 1, 1)[0], operand(n, k, 128, 2)[0]
+    if positive:
+        a, b = (t.view(torch.uint8).bitwise_and(127).view(E4M3) for t in (a, b))
+    g = torch.Generator(device=DEV).manual_seed(5)
+    sa = torch.exp2(torch.randint(-12, -9, (m, k // 128), device=DEV, generator=g).float())
+    sb = torch.exp2(torch.randint(-12, -9, (n // 128, k // 128), device=DEV, generator=g).float())
+    out = fused.block_mm(a, sa, b, sb, out_dtype=out_dtype, power_of_two=True)
+    assert _lib.last_plan().startswith("block_mm_scaled")
+    ref.check_product(out, ref.values(a, sa), ref.values(b, sb), None, f"k = {k}", True)
