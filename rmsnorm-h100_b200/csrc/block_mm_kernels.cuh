@@ -14,7 +14,7 @@
 
 namespace rmsb200 {
 
-constexpr int kSiteMmFull = 12, kSiteMmEmpty = 13, kSiteMmSum = 14, kSiteMmSumEmpty = 15;
+constexpr int kSiteMmFull = 13, kSiteMmEmpty = 14, kSiteMmSum = 15, kSiteMmSumEmpty = 16;  // waits that gave up
 
 struct BlockMmParams {
   int64_t m;
@@ -371,8 +371,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 // them, so that one comes out while the next is summed, and for the exponents; one of 256 comes out
 // before the next begins, for pairs that have a single tile or two. Each addition of 32 products
 // rounds towards zero: where all values are positive, sums are low by 9.1e-6, 3.9e-5 and 3.3e-4 of
-// themselves at 4096, 16384 and 131072 columns (scaled in registers: 1e-7 to 5e-7), of random signs by
-// less than 16 bits show.
+// themselves at 4096, 16384 and 131072 columns (scaled in registers: 1e-7 to 5e-7).
 // Measured: 8192 x 16384 x 4096 409 us (2690 TFLOP/s, at the card's power limit), scaled in
 // registers 495 us.
 // ---------------------------------------------------------------------------------------

@@ -20,3 +20,11 @@ def test_plain_waits_are_for_single_threads(path):
     for m in re.finditer(r"\bmbar_(?:try_)?wait(?:_cluster|_slow)?(?:<\w+>)?\s*\(", code):
         call = code[m.start():code.index(";", m.start())]
         assert "kSiteDrain" in call or path.name == "generic_kernels.cuh", f"{path.name}: {call}"
+
+
+def test_every_site_has_a_number_of_its_own():
+    """rmsnorm_b200_device_status tells where something went wrong by a site's number."""
+    found = re.findall(r"\b(kSite\w+) = (\d+)", "\n".join(p.read_text() for p in [*SOURCES, CSRC / "device_common.cuh"]))
+    assert len(found) > 12
+    numbers = [n for _, n in found]
+    assert len(set(numbers)) == len(numbers), found
