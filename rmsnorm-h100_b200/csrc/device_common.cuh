@@ -271,9 +271,9 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
 
 // The same without a call, and with the status word and the clock looked at after every 64
 // probes only (a look at the status word is a load from L2): for waits that end within some
-// hundred cycles again and again. mbar_spin_one is for a role that one lane of a warp plays from
-// its first wait to its last, while the others stay at the warp's next barrier.
-__device__ __forceinline__ bool mbar_spin_one(uint64_t* bar, uint32_t parity, int where) {
+// hundred cycles again and again.
+__device__ __forceinline__ bool mbar_spin_warp(uint64_t* bar, uint32_t parity, int where) {
+  __syncwarp();
   uint64_t t0 = 0;
   while (true) {
 #pragma unroll 1
@@ -287,10 +287,6 @@ __device__ __forceinline__ bool mbar_spin_one(uint64_t* bar, uint32_t parity, in
       return false;
     }
   }
-}
-__device__ __forceinline__ bool mbar_spin_warp(uint64_t* bar, uint32_t parity, int where) {
-  __syncwarp();
-  return mbar_spin_one(bar, parity, where);
 }
 
 // ---------------------------------------------------------------------------------------

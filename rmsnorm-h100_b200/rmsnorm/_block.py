@@ -47,38 +47,31 @@ def _bytes_empty(shape, device) -> Tensor:
     return torch.empty(*shape[:-1], pitch, dtype=_E4M3, device=device)[..., :k]
 
 
-def _quantize(x: Tensor, rows: int, want: bool, want_t: bool, column_major: bool = False, sums_dtype=None):
-    """(q, scales, q_t, scales_t, column sums) of a matrix, those that are wanted."""
+def _quantize(x: Tensor, rows: int, want: bool, want_t: bool, sums_dtype=None):
+    """On the host, (q, scales, q_t, scales_t, column sums) of a matrix, those that are wanted."""
+    none = (None, None)
+    sums = None if sums_dtype is None else x.float().sum(0).to(sums_dtype)
+    return (*(_host.block_quantize(x, rows) if want else none), *(_host.block_quantize(x.t(), rows) if want_t else none), sums)
+
+
+def _quantize_cuda(x: Tensor, rows: int, want_t: bool, column_major: bool):
+    """(q, scales, q_t, scales_t) of a matrix, the last two where they are wanted."""
     n, k = x.shape
     device = x.device
     gn, gk = -(-n // rows), -(-k // _BLOCK)
-    q = scales = q_t = scales_t = sums = None
-    if not x.is_cuda:
-        if want:
-            q, scales = _host.block_quantize(x, rows)
-        if want_t:
-            q_t, scales_t = _host.block_quantize(x.t(), rows)
-        if sums_dtype is not None:
-            sums = x.float().sum(0).to(sums_dtype)
-        if column_major and want:
-            scales = scales.t().contiguous().t()
-        return q, scales, q_t, scales_t, sums
-    sr, sg = gk, 1
-    if want:
-        q = _bytes_empty((n, k), device)
-        if column_major:
-            scales = torch.empty(gk, gn, dtype=torch.float32, device=device).t()
-            sr, sg = 1, gn
-        else:
-            scales = torch.empty(gn, gk, dtype=torch.float32, device=device)
+    q, q_t, scales_t = _bytes_empty((n, k), device), None, None
+    if column_major:
+        scales = torch.empty(gk, gn, dtype=torch.float32, device=device).t()
+        sr, sg = 1, gn
+    else:
+        scales = torch.empty(gn, gk, dtype=torch.float32, device=device)
+        sr, sg = gk, 1
     if want_t:
         q_t = _bytes_empty((k, n), device)
         scales_t = torch.empty(-(-n // _BLOCK), gk if rows > 1 else k, dtype=torch.float32, device=device).t()
-    if sums_dtype is not None:
-        sums = torch.empty(k, dtype=sums_dtype, device=device)
-    _enqueue_quantize(x, rows, q.data_ptr() if want else 0, scales.data_ptr() if want else 0, sr, sg,
-                      q_t.data_ptr() if want_t else 0, scales_t.data_ptr() if want_t else 0, sums)
-    return q, scales, q_t, scales_t, sums
+    _enqueue_quantize(x, rows, q.data_ptr(), scales.data_ptr(), sr, sg, q_t.data_ptr() if want_t else 0,
+                      scales_t.data_ptr() if want_t else 0, None)
+    return q, scales, q_t, scales_t
 
 
 def _enqueue_quantize(x: Tensor, rows: int, q: int, scales: int, sr: int, sg: int, q_t: int, scales_t: int, sums) -> None:
@@ -122,7 +115,12 @@ def block_quantize(x: Tensor, block_rows: int = 1, transposed: bool = False, sca
         raise ValueError(f"128 x 128 blocks need a matrix, got shape {tuple(x.shape)}")
     if x.requires_grad:
         x = x.detach()
-    q, scales, q_t, scales_t, _ = _quantize(_rows_of(x), block_rows, True, transposed, scales_column_major)
+    if x.is_cuda:
+        q, scales, q_t, scales_t = _quantize_cuda(_rows_of(x), block_rows, transposed, scales_column_major)
+    else:
+        q, scales, q_t, scales_t, _ = _quantize(_rows_of(x), block_rows, True, transposed)
+        if scales_column_major:
+            scales = scales.t().contiguous().t()
     if x.dim() != 2:
         lead = x.shape[:-1]
         q = q.view(*lead, x.shape[-1]) if q.is_contiguous() else q.unflatten(0, lead) if lead else q[0]
@@ -200,6 +198,9 @@ def block_mm(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, bias: Opt
     if not matrix:
         a = a.reshape(shape[:-1].numel(), k)
         a_scales = a_scales.reshape(a.shape[0], groups)
+    if not a.is_cuda:
+        out = _host_product(a, a_scales, b, b_scales, b_rows, bias, out_dtype)
+        return out if matrix else out.view(*shape[:-1], n)
     a_row, a_step = a.stride()
     if a_step != 1 and k > 1 or a_row < k:  # a column by column, or rows that overlap
         a = a.contiguous()
@@ -212,12 +213,14 @@ def block_mm(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, bias: Opt
     return out if matrix else out.view(*shape[:-1], n)
 
 
+def _host_product(a, a_scales, b, b_scales, b_rows, bias, out_dtype) -> Tensor:
+    with torch.no_grad(), torch.autocast("cpu", enabled=False):  # the sums are fp32 in any mode
+        out = _host.block_values(a, a_scales, 1) @ _host.block_values(b, b_scales, b_rows).t()
+        return (out if bias is None else out + bias.float()).to(out_dtype)
+
+
 def _product(a, a_row, a_scales, b, b_row, b_scales, b_rows, bias, bias_code, out_dtype, oc, power_of_two) -> Tensor:
-    """The product of checked matrices with rows a_row and b_row apart."""
-    if not a.is_cuda:
-        with torch.no_grad(), torch.autocast("cpu", enabled=False):  # the sums are fp32 in any mode
-            out = _host.block_values(a, a_scales, 1) @ _host.block_values(b, b_scales, b_rows).t()
-            return (out if bias is None else out + bias.float()).to(out_dtype)
+    """The product of checked matrices on CUDA with rows a_row and b_row apart."""
     m, k = a.shape
     n, device = b.shape[0], a.device
     out = torch.empty(m, n, dtype=out_dtype, device=device)
@@ -242,16 +245,16 @@ class BlockLinearFunction(torch.autograd.Function):
         x2 = _rows_of(x)
         need = ctx.needs_input_grad if grad else (False, False)  # they are what the inputs want, whatever the mode
         ctx.x_shape, ctx.dtypes = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
-        code = 0
-        if bias is not None:
-            bias, code = bias.contiguous(), _CODE[bias.dtype]
         if x.is_cuda:
+            code = 0
+            if bias is not None:
+                bias, code = bias.contiguous(), _CODE[bias.dtype]
             y, kept = _linear_forward(x2, _rows_of(weight), bias, code, need[0], need[1])
         else:
-            q, s, x_t, x_ts, _ = _quantize(x2, 1, True, need[1], True)
+            q, s, x_t, x_ts, _ = _quantize(x2, 1, True, need[1])
             w, ws, w_t, w_ts, _ = _quantize(_rows_of(weight), _BLOCK, True, need[0])
             kept = x_t, x_ts, w_t, w_ts
-            y = _product(q, _pitch(q), s, w, _pitch(w), ws, _BLOCK, bias, code, x.dtype, _CODE[x.dtype], True)
+            y = _host_product(q, s, w, ws, _BLOCK, bias, x.dtype)
         ctx.save_for_backward(*kept)
         return y.view(*x.shape[:-1], weight.shape[0])
 
@@ -267,11 +270,11 @@ class BlockLinearFunction(torch.autograd.Function):
         else:
             x_t, x_ts, w_t, w_ts = ctx.saved_tensors
             dx = dw = None
-            q, s, d_t, d_ts, db = _quantize(_rows_of(dy), 1, need_x, need_w, True, b_dtype)
+            q, s, d_t, d_ts, db = _quantize(_rows_of(dy), 1, need_x, need_w, b_dtype)
             if need_x:
-                dx = _product(q, _pitch(q), s, w_t, _pitch(w_t), w_ts, _BLOCK, None, 0, x_dtype, _CODE[x_dtype], True)
+                dx = _host_product(q, s, w_t, w_ts, _BLOCK, None, x_dtype)
             if need_w:
-                dw = _product(d_t, _pitch(d_t), d_ts, x_t, _pitch(x_t), x_ts, 1, None, 0, w_dtype, _CODE[w_dtype], True)
+                dw = _host_product(d_t, d_ts, x_t, x_ts, 1, None, w_dtype)
         if need_x:
             dx = dx.view(ctx.x_shape)
         return (*first_order("block_linear", (dx, dw, db)), None)
@@ -334,11 +337,6 @@ def _linear_backward(dy: Tensor, x_t, w_t, k: int, x_dtype, w_dtype, b_dtype):
     elif w_dtype:
         dw = torch.zeros(n, k, dtype=w_dtype, device=device)
     return dx, dw, db
-
-
-def _pitch(q: Tensor) -> int:
-    """How far apart the rows of `_quantize`'s matrices are."""
-    return -(-q.shape[1] // 16) * 16
 
 
 def block_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None) -> Tensor:

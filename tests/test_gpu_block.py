@@ -533,3 +533,17 @@ def test_powers_of_two_of_long_sums(k, positive, out_dtype):
     out = fused.block_mm(a, sa, b, sb, out_dtype=out_dtype, power_of_two=True)
     assert _lib.last_plan().startswith("block_mm_scaled")
     ref.check_product(out, ref.values(a, sa), ref.values(b, sb), None, f"k = {k}", True)
+
+
+def test_linear_without_gradients_quantises_nothing_for_them(monkeypatch):
+    """What the host's test of that name says, of the kernels' calls."""
+    from rmsnorm import _block
+
+    wanted, enqueue = [], _block._enqueue_quantize
+    monkeypatch.setattr(_block, "_enqueue_quantize", lambda *a: wanted.append(a[6] != 0) or enqueue(*a))
+    x, w = rand(30, 130).requires_grad_(True), rand(7, 130, seed=1).requires_grad_(True)
+    y = fused.block_linear(x, w)
+    with torch.no_grad():
+        assert torch.equal(fused.block_linear(x, w), y)
+    assert torch.equal(fused.block_linear(x.detach(), w), y) and torch.equal(fused.block_linear(x, w.detach()), y)
+    assert wanted == [True, True, False, False, True, False, False, True]
