@@ -206,13 +206,13 @@ def cache_read(k_cache: Tensor, v_cache: Tensor, k_scales: Tensor, v_scales: Ten
         k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
     else:
         k, v = out
-        if k is v or k.data_ptr() == v.data_ptr() and k.numel():
-            raise ValueError("out must be two different tensors")
         for t in out:
             if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
                 raise ValueError(f"out must be two contiguous {dtype} tensors of shape {shape} on {device}")
             if t.requires_grad and torch.is_grad_enabled():
                 raise ValueError("cache_read is outside autograd: out must not require gradients")
+        if abs(k.data_ptr() - v.data_ptr()) < k.numel() * k.element_size():
+            raise ValueError("out must be two different tensors that do not overlap")
     if not k_cache.is_cuda:
         if out is None:
             k.zero_()

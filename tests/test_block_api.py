@@ -411,3 +411,13 @@ def test_cache_write_refuses_caches_that_overlap():
     for ks, vs in [(scales[:3], scales[1:4]), (scales[:3], scales[2:])]:
         with pytest.raises(ValueError, match="k_scales and v_scales must"):
             fused.cache_write(k, k, *c[:2], ks, vs, slots)
+
+
+def test_cache_read_refuses_outputs_that_overlap():
+    c = _cache()
+    table, starts = torch.zeros(1, 3, dtype=torch.int32), torch.tensor([0, 5], dtype=torch.int32)
+    both = torch.zeros(10, 2, 16)
+    for k, v in ((both[:5], both[1:6]), (both[4:9], both[:5])):
+        with pytest.raises(ValueError, match="overlap"):
+            fused.cache_read(*c, table, starts, 5, torch.float32, (k, v))
+    fused.cache_read(*c, table, starts, 5, torch.float32, (both[5:], both[:5]))
