@@ -144,7 +144,7 @@ class PagedSequences:
             at += range(first, last)
             slots += [self.pages[s][t // self.page_size] * self.page_size + t % self.page_size for t in range(first, last)]
             self.lengths[s] = last
-        return torch.tensor(at, device=self.device), torch.tensor(slots, device=self.device)
+        return tuple(torch.tensor(t, dtype=torch.int64, device=self.device) for t in (at, slots))
 
     def table(self) -> Tuple[Tensor, Tensor]:
         """(page table, starts) as `cache_read` takes them."""

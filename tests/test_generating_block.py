@@ -162,3 +162,25 @@ def test_generated_attention_tells_mistakes(mistake, monkeypatch):
     with torch.no_grad():
         want = torch.stack([sum(t.float() for t in block(s, None, torch.arange(24), table)) for s in x]) - x
     assert (got - want).norm() > ATTENTION * want.norm()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sequences_without_new_tokens(device):
+    """Some, or all, have none in a step: the others' results are what they are alone."""
+    (block,), dtype = blocks(device)
+    table = fused.rope_table(16, 64, device=device)
+    x = torch.randn(5, 256, device=device, generator=torch.Generator(device=device).manual_seed(4)).to(dtype)
+
+    def step(layer, sequences, new, x):
+        positions, slots = sequences.extend(new)
+        assert positions.dtype == slots.dtype == torch.int64
+        branch, residual = layer(x, None, new, slots, positions, table)
+        return branch.float() + residual
+
+    alone, among = (PagedSequences(n, 8, 4, device) for n in (1, 3))
+    one, three = block.prepare_generating(alone), block.prepare_generating(among)
+    want = step(one, alone, [3], x[:3]), step(one, alone, [2], x[3:])
+    got = step(three, among, [0, 3, 0], x[:3]), step(three, among, [0, 2, 0], x[3:])
+    # the same sums in the same order, but for the library's attention
+    assert all((a - b).norm() <= 0.05 * a.norm() for a, b in zip(want, got))
+    assert step(three, among, [0, 0, 0], x[:0]).shape == (0, 256)
