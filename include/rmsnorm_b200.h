@@ -458,7 +458,8 @@ int rmsnorm_b200_block_quant(const rmsnorm_b200_block_quant_args* args, void* wo
 
 /* out[m][n] = sum over groups g of a_scale[m][g] * b_scale[n or n / 128][g] *
  *             (sum over the columns k of g of a[m][k] * b[n][k])  (+ bias[n])
- * The sums are held in fp32, the result rounded once. */
+ * The sums are held in fp32, the result rounded once. The product of a's and b's scale for a group has
+ * to be a normal number of fp32; it is what the group's sum is multiplied by. */
 typedef struct rmsnorm_b200_block_mm_args {
   int64_t m, n, k;            /* m >= 0, n and k >= 1, below 2^31 */
   const void* a;              /* [m, k] E4M3 */

@@ -40,8 +40,9 @@ __device__ __forceinline__ const float* sb_of(const BlockMmParams& p, int64_t n)
 // CTA holds 128 rows of a and of b and half of the result, so that what both need of b crosses
 // from L2 once. Tensor memory holds two groups' sums (all of it), so a group's have to be taken out
 // within the time of the next one's products.
-// Measured (bf16 results): 8192 x 16384 x 4096 495 us, 2220 TFLOP/s; with a scale a row of b
-// 8192 x 4096 x 8192 345 to 395 us (blocks: 239 us). The products alone run at 3950 TFLOP/s, with
+// Measured (bf16 results, in a burst): 8192 x 16384 x 4096 495 to 510 us, 2160 to 2220 TFLOP/s; with
+// a scale a row of b, whose exchange has the summing warps meet once a group, 8192 x 4096 x 8192 345
+// to 395 us (blocks: 243 us). The products alone run at 3950 TFLOP/s, with
 // their copies at 2860 (the card's power limit), with the sums' hand-over as well at 2460, with
 // tensor memory read at 2270: the scaling shares its time with none of these completely.
 // What was tried: accumulators of 128 columns, four of them, 575 us and more; 16 summing warps of
@@ -372,8 +373,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 // before the next begins, for pairs that have a single tile or two. Each addition of 32 products
 // rounds towards zero: where all values are positive, sums are low by 9.1e-6, 3.9e-5 and 3.3e-4 of
 // themselves at 4096, 16384 and 131072 columns (scaled in registers: 1e-7 to 5e-7).
-// Measured: 8192 x 16384 x 4096 409 us (2690 TFLOP/s, at the card's power limit), scaled in
-// registers 495 us.
+// Measured in a burst: 8192 x 16384 x 4096 409 us (2690 TFLOP/s, at the card's power limit), scaled
+// in registers 495 to 510 us.
 // ---------------------------------------------------------------------------------------
 constexpr int kScaledThreads = 448;
 constexpr int kScaledStages = 6;
@@ -602,7 +603,7 @@ __global__ void __launch_bounds__(kScaledThreads, 1)
 // that b streams through once. The groups of k are split over the CTAs of a cluster, each of
 // which then adds up some rows of the result.
 // Measured: 1 x 16384 x 16384 46 us (5.8 TB/s), 8 x 16384 x 4096 14.7 us (4.6), 64 x 8192 x 8192
-// 17.3 us (4.0), 1 x 4096 x 4096 6.5 to 7 us: start, the way of the first copies and the joining of
+// 17.3 us (4.0), 1 x 4096 x 4096 5.9 to 7 us: start, the way of the first copies and the joining of
 // the parts take 5 to 6 us of each.
 // ---------------------------------------------------------------------------------------
 constexpr int kFewThreads = 192;  // warps 0 - 3 sum, 4 copies, 5 multiplies
