@@ -547,3 +547,37 @@ def test_linear_without_gradients_quantises_nothing_for_them(monkeypatch):
         assert torch.equal(fused.block_linear(x, w), y)
     assert torch.equal(fused.block_linear(x.detach(), w), y) and torch.equal(fused.block_linear(x, w.detach()), y)
     assert wanted == [True, True, False, False, True, False, False, True]
+
+
+@pytest.mark.parametrize("case", ["quantize", "many rows", "powers of two", "few rows"])
+def test_offsets_beyond_32_bits(case):
+    """More than 2^31 elements; the ends are what they are by themselves."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GiB")
+    same = lambda x, y: torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8))  # noqa: E731
+    if case == "quantize":
+        rows, cols, last = 128 * 8192 + 77, 2056, 128 * 8190
+        x = torch.empty(rows, cols, dtype=BF16, device=DEV).normal_()
+        q, s, q_t, s_t = fused.block_quantize(x, transposed=True)
+        e, es, e_t, es_t = fused.block_quantize(x[last:], transposed=True)
+        assert same(q[last:], e) and torch.equal(s[last:], es) and same(q_t[:, last:], e_t) and torch.equal(s_t[:, last // 128:], es_t)
+        ref.check_quantized(q[last:], s[last:], x[last:], 1)
+        q, s = fused.block_quantize(x, 128)
+        e, es = fused.block_quantize(x[last:], 128)
+        assert same(q[last:], e) and torch.equal(s[last // 128:], es)
+        return
+    few = case == "few rows"
+    m, n, k = (100, (1 << 25) + 40, 16) if few else (70000, 33000, 64)
+    a, b = operand(m, k, 1, 1)[0], operand(n, k, 1, 2)[0]
+    sa, sb = torch.ones(m, 1, device=DEV) / 512, torch.ones(-(-n // 128), 1, device=DEV) / 512
+    out = fused.block_mm(a, sa, b, sb, power_of_two=case == "powers of two")
+    if few:
+        last = 128 * ((n - 5000) // 128)
+        end, got = fused.block_mm(a, sa, b[last:], sb[last // 128:]), out[:, last:]
+        factors = (a, sa), (b[last:], sb[last // 128:])
+    else:
+        last = 256 * 272
+        end, got = fused.block_mm(a[last:], sa[last:], b, sb, power_of_two=case == "powers of two"), out[last:]
+        factors = (a[last:], sa[last:]), (b, sb)
+    assert same(got, end)
+    ref.check_product(end, ref.values(*factors[0]), ref.values(*factors[1]), None, case, True)
